@@ -1,5 +1,5 @@
 """ctypes binding of libesda.so (the C ABI declared in include/esda.h,
-include/esda_cache.h and include/esda_prefill.h).
+include/esda_cache.h, include/esda_prefill.h and include/esda_rope.h).
 
 The library is loaded from the package directory only (built in-tree by
 ``apertura_amd/build.py``); a missing library raises instead of falling back.
@@ -37,6 +37,8 @@ EXPORTS = (
     # include/esda_prefill.h
     "esda_prefill_workspace_size", "esda_prefill", "esda_prefill_stages", "esda_raw_prefill_kv",
     "esda_raw_q8_prefill_kv", "esda_cache_prefill", "esda_cache_prefill_raw", "esda_lds_read",
+    # include/esda_rope.h
+    "esda_rope", "esda_rope_frequencies",
 )
 _VOID = ("esda_cache_destroy", "esda_cache_mark_step", "esda_cache_reset", "esda_cache_clear_rewind_mark")
 
@@ -129,6 +131,32 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class RopeDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("num_k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32), ("attn_factor", ctypes.c_float),
+        ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("q_out_row_stride", ctypes.c_int64), ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_row_stride", ctypes.c_int64), ("k_out_head_stride", ctypes.c_int64),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+    ]
+
+
+class RopeScalingDesc(ctypes.Structure):
+    _fields_ = [
+        ("kind", ctypes.c_int32), ("trained_len", ctypes.c_int32), ("base", ctypes.c_double),
+        ("factor", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+    ]
+
+
 class Q8View(ctypes.Structure):
     """esda_q8_view: u8 rows q [kv_heads, pitch, 512], f32 scale / bias [kv_heads, pitch]."""
     _fields_ = [
@@ -212,6 +240,9 @@ def lib() -> ctypes.CDLL:
         L.esda_cache_prefill_raw.argtypes = [P, i32, P, i32, i32, P, i32, P, f32, P, i32, i32, f32, i32, P, P]
         L.esda_raw_prefill_kv.argtypes = [P, i64, i32, i32, i32, P, f32, P, i32, P, P, i64, P]
         L.esda_raw_q8_prefill_kv.argtypes = [P, i64, P, P, i64, i32, i32, P, f32, P, i32, P, P, i64, P]
+        L.esda_rope.argtypes = [ctypes.POINTER(RopeDesc), ctypes.POINTER(RopeArgs), P]
+        L.esda_rope_frequencies.argtypes = [ctypes.POINTER(RopeScalingDesc), i32, ctypes.POINTER(f32),
+                                            ctypes.POINTER(f32)]
         for name in EXPORTS:
             if name in _VOID:
                 getattr(L, name).restype = None

@@ -22,6 +22,7 @@ CXX = os.environ.get("CXX", "g++")
 SOURCES = [
     "esda_decode.hip",
     "esda_prefill.hip",
+    "esda_rope.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",

@@ -190,15 +190,9 @@ constexpr float kPio2Hi = 1.57079637050628662109375f;         // fp32(pi/2)
 constexpr float kPio2Mid = -4.37113882867379300296306610107421875e-8f;
 constexpr float kPio2Lo = -1.715124510005881916757519826222e-15f;
 
-// cos and sin of an fp32 angle |a| < 2^20.  Reduction a = n*pi/2 + r in three FMA
-// steps (the first is exact: n*hi is a multiple of 2^-23 within 1 of a), then Taylor
-// polynomials on |r| <= pi/4 (truncation error < 2e-9), then the quadrant n mod 4.
-// Absolute error is a few 1e-8, far inside the bf16 rounding applied to the results.
-__device__ __forceinline__ void sincos_f32(float a, float &s, float &c) {
-    const float n = __builtin_rintf(a * kTwoOverPi);
-    float r = __builtin_fmaf(-n, kPio2Hi, a);
-    r = __builtin_fmaf(-n, kPio2Mid, r);
-    r = __builtin_fmaf(-n, kPio2Lo, r);
+// cos and sin of r + q pi/2, |r| <= pi/4: Taylor polynomials (truncation error < 2e-9), then
+// the quadrant q mod 4.
+__device__ __forceinline__ void sincos_quadrant(float r, int q, float &s, float &c) {
     const float r2 = r * r;
     float ps = __builtin_fmaf(r2, 1.0f / 362880.0f, -1.0f / 5040.0f);
     ps = __builtin_fmaf(r2, ps, 1.0f / 120.0f);
@@ -209,11 +203,22 @@ __device__ __forceinline__ void sincos_f32(float a, float &s, float &c) {
     pc = __builtin_fmaf(r2, pc, 1.0f / 24.0f);
     pc = __builtin_fmaf(r2, pc, -0.5f);
     const float cr = __builtin_fmaf(r2, pc, 1.0f);
-    const int q = (int) n & 3;
+    q &= 3;
     s = (q & 1) ? cr : sr;
     c = (q & 1) ? sr : cr;
     if (q & 2) s = -s;
     if ((q + 1) & 2) c = -c;
+}
+
+// cos and sin of an fp32 angle |a| < 2^20.  Reduction a = n*pi/2 + r in three FMA
+// steps (the first is exact: n*hi is a multiple of 2^-23 within 1 of a), then the polynomials
+// above.  Absolute error is a few 1e-8, far inside the bf16 rounding applied to the results.
+__device__ __forceinline__ void sincos_f32(float a, float &s, float &c) {
+    const float n = __builtin_rintf(a * kTwoOverPi);
+    float r = __builtin_fmaf(-n, kPio2Hi, a);
+    r = __builtin_fmaf(-n, kPio2Mid, r);
+    r = __builtin_fmaf(-n, kPio2Lo, r);
+    sincos_quadrant(r, (int) n, s, c);
 }
 
 __device__ __forceinline__ float bf16_lo(unsigned w) { return __builtin_bit_cast(float, w << 16); }
