@@ -10,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -55,9 +56,9 @@ def sources() -> list[str]:
 
 def build(verbose: bool = False) -> str:
     """Compile every source and link libesda.so; always recompiles."""
-    objs = []
     inc = ["-I", os.path.join(ROOT, "include"), "-I", CSRC]
-    for src in sources():
+
+    def compile_one(src: str) -> str:
         obj = os.path.join(CSRC, os.path.basename(src) + ".o")
         # ES* C++ layer: host code only (HIP runtime API and the esda C ABI), built by
         # the host compiler so no device code is generated for it.
@@ -68,7 +69,10 @@ def build(verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-        objs.append(obj)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, sources()))
     tmp = LIB + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp] + objs
     subprocess.run(cmd, check=True)
