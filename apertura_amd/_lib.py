@@ -1,5 +1,5 @@
 """ctypes binding of libesda.so (the C ABI declared in include/esda.h,
-include/esda_cache.h, include/esda_prefill.h and include/esda_rope.h).
+include/esda_cache.h, include/esda_prefill.h, include/esda_rope.h and include/esda_scored.h).
 
 The library is loaded from the package directory only (built in-tree by
 ``apertura_amd/build.py``); a missing library raises instead of falling back.
@@ -39,6 +39,8 @@ EXPORTS = (
     "esda_raw_q8_prefill_kv", "esda_cache_prefill", "esda_cache_prefill_raw", "esda_lds_read",
     # include/esda_rope.h
     "esda_rope", "esda_rope_frequencies",
+    # include/esda_scored.h
+    "esda_scored_prefill_workspace_size", "esda_scored_prefill", "esda_scored_decode",
 )
 _VOID = ("esda_cache_destroy", "esda_cache_mark_step", "esda_cache_reset", "esda_cache_clear_rewind_mark")
 
@@ -157,6 +159,19 @@ class RopeScalingDesc(ctypes.Structure):
     ]
 
 
+class ScoreDesc(ctypes.Structure):
+    """esda_score"""
+    _fields_ = [("softcap", ctypes.c_float), ("prefix", ctypes.c_int32), ("slopes", ctypes.c_void_p)]
+
+
+class ScoredPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("q_doc", ctypes.c_void_p), ("k_doc", ctypes.c_void_p),
+    ]
+
+
 class Q8View(ctypes.Structure):
     """esda_q8_view: u8 rows q [kv_heads, pitch, 512], f32 scale / bias [kv_heads, pitch]."""
     _fields_ = [
@@ -243,6 +258,10 @@ def lib() -> ctypes.CDLL:
         L.esda_rope.argtypes = [ctypes.POINTER(RopeDesc), ctypes.POINTER(RopeArgs), P]
         L.esda_rope_frequencies.argtypes = [ctypes.POINTER(RopeScalingDesc), i32, ctypes.POINTER(f32),
                                             ctypes.POINTER(f32)]
+        SP = ctypes.POINTER(ScoreDesc)
+        L.esda_scored_prefill_workspace_size.argtypes = [PD, SP, ctypes.POINTER(sz)]
+        L.esda_scored_prefill.argtypes = [PD, SP, ctypes.POINTER(ScoredPrefillArgs), P]
+        L.esda_scored_decode.argtypes = [ctypes.POINTER(DecodeDesc), SP, ctypes.POINTER(DecodeArgs), P]
         for name in EXPORTS:
             if name in _VOID:
                 getattr(L, name).restype = None

@@ -24,6 +24,8 @@ SOURCES = [
     "esda_decode.hip",
     "esda_prefill.hip",
     "esda_rope.hip",
+    "esda_scored_decode.hip",
+    "esda_scored_prefill.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",
@@ -47,6 +49,8 @@ HIP_FLAGS = [
 # accumulation registers an AGPR result, which would cost four copies per product.
 EXTRA_FLAGS = {
     "esda_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+    # the decode kernel's other forms, compiled as esda_decode.hip's
+    "esda_scored_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -68,6 +68,13 @@ struct AttendParams {
 
 
 
+// A step with modified scores (esda_scored.h): score (log2 units) = cap_out tanh(cap_in raw /
+// (2 log2 e)) where cap_out is not 0, less slopes[head] log2 e per position of distance.
+struct ScoredAttendParams : AttendParams {
+    float cap_in, cap_out;
+    const float *slopes;
+};
+
 // ---------------------------------------------------------------- LDS ring layout
 //
 // A workgroup streams its rows through a ring of NS stages of 16 rows in LDS.  Rows
@@ -272,13 +279,17 @@ __device__ __forceinline__ void walk_segments(const AttendParams &p, Seg &&segme
 // The new token's row is copied from k_new/v_new into the cache by the workgroup whose
 // split ends at it (bit-exact copy); that workgroup's own loads read the row from
 // k_new/v_new and no other workgroup reads it, so the copy needs no ordering.
-template <int D, bool SHARED, int NW, int OCC = 1>
+//
+// P = ScoredAttendParams: the four scores a lane holds of a stage are capped and biased before
+// the softmax; row j of the visible ones lies nvis - 1 - j positions behind the token.
+template <int D, bool SHARED, int NW, int OCC = 1, class P = AttendParams>
 // The LDS ring allows OCC workgroups per CU, i.e. OCC * NW/4 waves per SIMD: telling the
 // compiler so lifts the register limit it would otherwise keep for higher occupancy,
 // which it meets by serialising LDS reads behind their uses.  (Plans may still place one
 // workgroup per CU on a kernel built with OCC = 2: its shallower ring is what they want.)
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * NW, 64 * NW), amdgpu_waves_per_eu(OCC * NW / 4, OCC * NW / 4)))
-void attend_kernel(AttendParams p) {
+void attend_kernel(P p) {
+    constexpr bool SCORED = std::is_same<P, ScoredAttendParams>::value;
     using R = Ring<D, SHARED, NW, 160 * 1024 / OCC>;
     // D = 512 exchanges only the live heads' partial scores (the padding columns are zero)
     constexpr bool kLiveX = D == 512;
@@ -350,6 +361,10 @@ void attend_kernel(AttendParams p) {
             const u32x4 t = qok ? *reinterpret_cast<const u32x4 *>(qrow + 32 * qk_chunk(kk)) : u32x4{0u, 0u, 0u, 0u};
             qv[kk] = __builtin_bit_cast(bf16x8, t);
         }
+    }
+    float slope = 0.0f;  // of this lane's head, log2 units
+    if constexpr (SCORED) {
+        if (p.slopes && li < p.G) slope = p.slopes[kvh * p.G + li] * kLog2e;
     }
     ESDA_WAIT_VM(0);  // operands are in registers before the ring starts counting its own loads
 
@@ -480,7 +495,16 @@ void attend_kernel(AttendParams p) {
         // end (last stage only) and rows of another kv head of the group are masked.
         const int jt = j0 + st * RPP + jl;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[r] = hmatch && (jt + r) < j1 ? sc[r] * p.scale_log2e : -INFINITY;
+        for (int r = 0; r < 4; ++r) {
+            float x = sc[r] * p.scale_log2e;
+            if constexpr (SCORED) {
+                // tanh(y) = 1 - 2 / (1 + e^2y)
+                if (p.cap_out != 0.0f)
+                    x = p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[r] * p.cap_in)), 1.0f);
+                x = __builtin_fmaf(-slope, (float) (sv.nvis - 1 - jt - r), x);
+            }
+            sc[r] = hmatch && (jt + r) < j1 ? x : -INFINITY;
+        }
         const float tmax = wave_max_across_groups(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
         if (__any(tmax > m + kRescaleSlack)) {
             const float mnew = fmaxf(m, tmax);
@@ -887,10 +911,10 @@ int make_plan(const esda_decode_desc *d, Plan *pl, bool raw = false) {
 template <int D>
 constexpr int ring_waves() { return D == 256 ? kWaves256 : 4; }
 
-template <int D, bool SHARED, int OCC = 1>
-hipError_t launch_attend(const AttendParams &ap, dim3 grid, hipStream_t st) {
+template <int D, bool SHARED, int OCC, class P>
+hipError_t launch_attend(const P &ap, dim3 grid, hipStream_t st) {
     constexpr int NW = ring_waves<D>();
-    hipLaunchKernelGGL((attend_kernel<D, SHARED, NW, OCC>), grid, dim3(64 * NW), 0, st, ap);
+    hipLaunchKernelGGL((attend_kernel<D, SHARED, NW, OCC, P>), grid, dim3(64 * NW), 0, st, ap);
     return hipGetLastError();
 }
 
@@ -902,17 +926,137 @@ hipError_t launch_attend(const AttendParams &ap, dim3 grid, hipStream_t st) {
 // workgroups two stages each keep ~8.4 MB in flight, enough to saturate HBM (a read probe reads
 // 7.1-7.3 TB/s with 6-15 MB in flight, less with ~30 MB), where 9 stages keep ~29 MB.  A
 // separate 512-dim V needs the whole LDS for 4 stages; D = 128 stages are 4 KB.
-hipError_t dispatch_attend(int D, bool shared, const AttendParams &ap, dim3 grid, hipStream_t st) {
+template <class P>
+hipError_t dispatch_attend(int D, bool shared, const P &ap, dim3 grid, hipStream_t st) {
     constexpr int O256 = kOcc256, O512 = kOcc512Shared;
     switch (D) {
-        case 128: return shared ? launch_attend<128, true>(ap, grid, st) : launch_attend<128, false>(ap, grid, st);
+        case 128: return shared ? launch_attend<128, true, 1>(ap, grid, st) : launch_attend<128, false, 1>(ap, grid, st);
         case 256:
             return shared ? launch_attend<256, true, O256>(ap, grid, st)
                           : launch_attend<256, false, O256>(ap, grid, st);
         default:
             return shared ? launch_attend<512, true, O512>(ap, grid, st)
-                          : launch_attend<512, false>(ap, grid, st);
+                          : launch_attend<512, false, 1>(ap, grid, st);
     }
+}
+
+// The step's shape, plan and workspace in a kernel's parameters.
+struct DecodeSpace {
+    long long *table;
+    float *part_ml, *part_acc;
+};
+DecodeSpace space_of(const Plan &pl, void *workspace) {
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    return {reinterpret_cast<long long *>(ws + pl.off_table), reinterpret_cast<float *>(ws + pl.off_ml),
+            reinterpret_cast<float *>(ws + pl.off_acc)};
+}
+void fill_attend(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp, int *status, uint16_t *out,
+                 AttendParams &ap) {
+    ap.part_acc = sp.part_acc;
+    ap.part_ml = sp.part_ml;
+    ap.status = status;
+    ap.table = sp.table;
+    ap.out = out;
+    ap.seq_stride = d->seq_stride;
+    ap.head_stride = d->head_stride;
+    ap.B = d->batch;
+    ap.Hq = d->num_q_heads;
+    ap.Hkv = d->num_kv_heads / pl.pk;
+    ap.G = pl.G * pl.pk;
+    ap.pk = pl.pk;
+    ap.gk = pl.G;
+    ap.cap = d->cap;
+    ap.window = d->window;
+    ap.ring = d->ring;
+    ap.balanced = pl.balanced;
+    ap.W = pl.W;
+    ap.S = pl.S;
+    ap.chunk = pl.chunk;
+    ap.scale_log2e = d->scale * kLog2e;
+}
+dim3 attend_grid(const esda_decode_desc *d, const Plan &pl) {
+    return pl.balanced ? dim3(pl.W) : dim3(pl.S, d->num_kv_heads / pl.pk, d->batch);
+}
+
+// The split merge of a step.  pad: rows a pair counted beside its own (walk_segments' PAD).
+int launch_merge(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp, const int *pos, const int *row_base,
+                 int pad, uint16_t *out, hipStream_t st) {
+    // One split per pair: the attend workgroups wrote every output themselves.
+    if (!pl.balanced && pl.S == 1) return ESDA_OK;
+    MergeParams mp;
+    mp.part_acc = sp.part_acc;
+    mp.part_ml = sp.part_ml;
+    mp.table = sp.table;
+    mp.pos = pos;
+    mp.row_base = row_base;
+    mp.out = out;
+    mp.B = d->batch;
+    mp.Hq = d->num_q_heads;
+    mp.Hkv = d->num_kv_heads / pl.pk;
+    mp.G = pl.G * pl.pk;
+    mp.D = d->head_dim;
+    mp.cap = d->cap;
+    mp.window = d->window;
+    mp.ring = d->ring;
+    mp.balanced = pl.balanced;
+    mp.W = pl.W;
+    mp.S = pl.S;
+    mp.chunk = pl.chunk;
+    mp.pad = pad;
+    // Partials per pair: a grid's S, or about W / pairs + 1 of the balanced shares.
+    const long long pairs = (long long) d->batch * d->num_kv_heads / pl.pk;
+    if (pl.balanced ? pl.W < kMergeShares * pairs : pl.S <= kMergeRowsChunk) {
+        // A few splits per pair: the thread-per-output merge, one memory round trip per
+        // kMergeRowsChunk of them (C5's global layers, 128 pairs of 3 partials: 11 -> 4.4
+        // us).  With more, merge_kernel's workgroups reduce 16 split groups side by side:
+        // at C1's 16 splits over 8 pairs the rows kernel takes two round trips (9.0 ->
+        // 11.8 us a step), and on balanced shares (step us, rows / merge_kernel): 8 pairs of
+        // 32 partials 46.1 / 30.0, 16 of 16 47.7 / 38.4, 32 of 8 41.6 / 38.7, 40 of 6.4
+        // 50.4 / 49.6, 48 of 5.3 51.0 / 50.8, 64 of 4 39.5 / 42.5.
+        const int threads = d->num_q_heads * (d->head_dim / 4);
+        dim3 grid((threads + kMergeRowsThreads - 1) / kMergeRowsThreads, d->batch);
+        hipLaunchKernelGGL(merge_rows_kernel, grid, dim3(kMergeRowsThreads), 0, st, mp);
+    } else {
+        dim3 grid(d->head_dim / kMergeDims, d->num_q_heads, d->batch);
+        // (balanced: room for a pair of twice the average partials; longer ones are looped over)
+        if (pl.balanced ? 2LL * pl.W <= kMergeGroups * 4 * pairs : pl.S <= kMergeGroups * 4)
+            hipLaunchKernelGGL(merge_kernel<4>, grid, dim3(kMergeThreads), 0, st, mp);
+        else
+            hipLaunchKernelGGL(merge_kernel<16>, grid, dim3(kMergeThreads), 0, st, mp);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return hip_fail(e, "merge_kernel launch");
+    return ESDA_OK;
+}
+
+// Argument checks shared by the decode entry points over a bf16 cache (everything but the
+// workspace).
+int check_decode_args(const esda_decode_desc *d, const esda_decode_args *a) {
+    if (!a) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: null arguments");
+    if (!a->q || !a->k_new || !a->k_cache || !a->v_cache || !a->pos || !a->out)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: null device pointer");
+    if (!d->kv_shared && !a->v_new)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: v_new is required unless kv_shared");
+    if (d->kv_shared && a->v_cache != a->k_cache)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: kv_shared needs v_cache == k_cache");
+    if (!d->kv_shared && a->v_cache == a->k_cache)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: separate K/V need distinct caches");
+    if (!aligned16(a->q) || !aligned16(a->k_new) || (a->v_new && !aligned16(a->v_new)) ||
+        !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out))
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: tensors must be 16-byte aligned");
+    return ESDA_OK;
+}
+
+AttendParams decode_params(const esda_decode_desc *d, const esda_decode_args *a) {
+    AttendParams ap{};
+    ap.q = static_cast<const uint16_t *>(a->q);
+    ap.k_new = static_cast<const uint16_t *>(a->k_new);
+    ap.v_new = static_cast<const uint16_t *>(d->kv_shared ? a->k_new : a->v_new);
+    ap.k_cache = static_cast<uint16_t *>(a->k_cache);
+    ap.v_cache = static_cast<uint16_t *>(a->v_cache);
+    ap.pos = a->pos;
+    ap.row_base = a->row_base;
+    return ap;
 }
 
 }  // namespace

@@ -889,34 +889,11 @@ int raw_as_decode(const esda_raw_desc *r, esda_decode_desc *d) {
 // the workspace's first word).
 int run_stages(const esda_decode_desc *d, const Plan &pl, const AttendParams &ap_in, uint16_t *out,
                void *workspace, int stages, int mode, hipStream_t st, int *status = nullptr) {
-    unsigned char *ws = static_cast<unsigned char *>(workspace);
-    long long *table = reinterpret_cast<long long *>(ws + pl.off_table);
-    float *part_ml = reinterpret_cast<float *>(ws + pl.off_ml);
-    float *part_acc = reinterpret_cast<float *>(ws + pl.off_acc);
+    const DecodeSpace sp = space_of(pl, workspace);
     if (stages & ESDA_STAGE_ATTEND) {
         AttendParams ap = ap_in;
-        ap.part_acc = part_acc;
-        ap.part_ml = part_ml;
-        ap.status = status ? status : reinterpret_cast<int *>(ws);
-        ap.seq_stride = d->seq_stride;
-        ap.head_stride = d->head_stride;
-        ap.B = d->batch;
-        ap.Hq = d->num_q_heads;
-        ap.Hkv = d->num_kv_heads / pl.pk;
-        ap.G = pl.G * pl.pk;
-        ap.pk = pl.pk;
-        ap.gk = pl.G;
-        ap.cap = d->cap;
-        ap.window = d->window;
-        ap.ring = d->ring;
-        ap.balanced = pl.balanced;
-        ap.W = pl.W;
-        ap.S = pl.S;
-        ap.chunk = pl.chunk;
-        ap.table = table;
-        ap.scale_log2e = d->scale * kLog2e;
-        ap.out = out;
-        const dim3 grid = pl.balanced ? dim3(pl.W) : dim3(pl.S, d->num_kv_heads / pl.pk, d->batch);
+        fill_attend(d, pl, sp, status ? status : static_cast<int *>(workspace), out, ap);
+        const dim3 grid = attend_grid(d, pl);
         hipError_t e;
         if (mode == 0) {
             e = dispatch_attend(d->head_dim, d->kv_shared != 0, ap, grid, st);
@@ -930,83 +907,9 @@ int run_stages(const esda_decode_desc *d, const Plan &pl, const AttendParams &ap
         }
         if (e != hipSuccess) return hip_fail(e, "attend_kernel launch");
     }
-    // One split per pair: the attend workgroups wrote every output themselves.
-    if ((stages & ESDA_STAGE_MERGE) && !(!pl.balanced && pl.S == 1)) {
-        MergeParams mp;
-        mp.part_acc = part_acc;
-        mp.part_ml = part_ml;
-        mp.table = table;
-        mp.pos = ap_in.pos;
-        mp.row_base = ap_in.row_base;
-        mp.out = out;
-        mp.B = d->batch;
-        mp.Hq = d->num_q_heads;
-        mp.Hkv = d->num_kv_heads / pl.pk;
-        mp.G = pl.G * pl.pk;
-        mp.D = d->head_dim;
-        mp.cap = d->cap;
-        mp.window = d->window;
-        mp.ring = d->ring;
-        mp.balanced = pl.balanced;
-        mp.W = pl.W;
-        mp.S = pl.S;
-        mp.chunk = pl.chunk;
-        mp.pad = mode != 0 && !ap_in.rope_tab ? kOwnTablePad : 0;
-        // Partials per pair: a grid's S, or about W / pairs + 1 of the balanced shares.
-        const long long pairs = (long long) d->batch * d->num_kv_heads / pl.pk;
-        if (pl.balanced ? pl.W < kMergeShares * pairs : pl.S <= kMergeRowsChunk) {
-            // A few splits per pair: the thread-per-output merge, one memory round trip per
-            // kMergeRowsChunk of them (C5's global layers, 128 pairs of 3 partials: 11 -> 4.4
-            // us).  With more, merge_kernel's workgroups reduce 16 split groups side by side:
-            // at C1's 16 splits over 8 pairs the rows kernel takes two round trips (9.0 ->
-            // 11.8 us a step), and on balanced shares (step us, rows / merge_kernel): 8 pairs of
-            // 32 partials 46.1 / 30.0, 16 of 16 47.7 / 38.4, 32 of 8 41.6 / 38.7, 40 of 6.4
-            // 50.4 / 49.6, 48 of 5.3 51.0 / 50.8, 64 of 4 39.5 / 42.5.
-            const int threads = d->num_q_heads * (d->head_dim / 4);
-            dim3 grid((threads + kMergeRowsThreads - 1) / kMergeRowsThreads, d->batch);
-            hipLaunchKernelGGL(merge_rows_kernel, grid, dim3(kMergeRowsThreads), 0, st, mp);
-        } else {
-            dim3 grid(d->head_dim / kMergeDims, d->num_q_heads, d->batch);
-            // (balanced: room for a pair of twice the average partials; longer ones are looped over)
-            if (pl.balanced ? 2LL * pl.W <= kMergeGroups * 4 * pairs : pl.S <= kMergeGroups * 4)
-                hipLaunchKernelGGL(merge_kernel<4>, grid, dim3(kMergeThreads), 0, st, mp);
-            else
-                hipLaunchKernelGGL(merge_kernel<16>, grid, dim3(kMergeThreads), 0, st, mp);
-        }
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return hip_fail(e, "merge_kernel launch");
-    }
+    if (stages & ESDA_STAGE_MERGE)
+        return launch_merge(d, pl, sp, ap_in.pos, ap_in.row_base, mode != 0 && !ap_in.rope_tab ? kOwnTablePad : 0, out, st);
     return ESDA_OK;
-}
-
-// Argument checks shared by esda_decode_stages and esda_decode_noalloc (everything but
-// the workspace).
-int check_decode_args(const esda_decode_desc *d, const esda_decode_args *a) {
-    if (!a) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: null arguments");
-    if (!a->q || !a->k_new || !a->k_cache || !a->v_cache || !a->pos || !a->out)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: null device pointer");
-    if (!d->kv_shared && !a->v_new)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: v_new is required unless kv_shared");
-    if (d->kv_shared && a->v_cache != a->k_cache)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: kv_shared needs v_cache == k_cache");
-    if (!d->kv_shared && a->v_cache == a->k_cache)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: separate K/V need distinct caches");
-    if (!aligned16(a->q) || !aligned16(a->k_new) || (a->v_new && !aligned16(a->v_new)) ||
-        !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out))
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_decode: tensors must be 16-byte aligned");
-    return ESDA_OK;
-}
-
-AttendParams decode_params(const esda_decode_desc *d, const esda_decode_args *a) {
-    AttendParams ap{};
-    ap.q = static_cast<const uint16_t *>(a->q);
-    ap.k_new = static_cast<const uint16_t *>(a->k_new);
-    ap.v_new = static_cast<const uint16_t *>(d->kv_shared ? a->k_new : a->v_new);
-    ap.k_cache = static_cast<uint16_t *>(a->k_cache);
-    ap.v_cache = static_cast<uint16_t *>(a->v_cache);
-    ap.pos = a->pos;
-    ap.row_base = a->row_base;
-    return ap;
 }
 
 }  // namespace

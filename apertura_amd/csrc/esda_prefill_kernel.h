@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -21,6 +23,7 @@ constexpr int kRingBudget = 136 * 1024;    // LDS bytes for the K / V ring
 // K / V stream loads without the non-temporal hint: the tiles of one kv head read the
 // same keys, and the L2 keeping them for the next tile was measured 2-12% faster.
 constexpr bool kStreamNT = false;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // LDS ring geometry for head dim D: a 16-key half stage is NI DMA blocks of kBlk bytes,
 // block b holding keys b + NI*q (q < 512/D) at +2D*q; a stage is the K halves then the V
@@ -70,8 +73,18 @@ struct PRing {
 // parity only after reading its partner's next flag, which the partner writes after reading
 // this stage's P^T.  Used by the K = V kernel at D = 512 (p512gs 436 -> 422 us on one box);
 // with separate K and V -- one stage per barrier -- it measured 1-3% slower and is not used.
-template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves>
-__global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
+//
+// P = ScoredParams (esda_scored.h): scores s become cap_out tanh(.) and lose slope * distance, and
+// three more masks apply.  A prefix opens keys ahead of a query.  Document ids (equal, not
+// negative) close the others: each wave reads the ids of 64 stages at a time and keeps which of
+// them hold an id of the tile's range (the others are never loaded) and which hold nothing but
+// the tile's one id (those need no mask); the ids of the stages loaded come with their keys by
+// DMA.  A row that sees nothing gives 0.  In masked stages a value that is not finite reaches
+// only the rows that see its key: 0 x inf in the product would be NaN in every row of the tile.
+template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves,
+          class P = PrefillParams>
+__global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
+    constexpr bool SCORED = std::is_same<P, ScoredParams>::value;
     static_assert(!S2 || !KH, "two stages per iteration: all waves on both");
     static_assert(!PS || (QB == 1 && !KH), "pair split: one block per wave, every wave on every stage");
     constexpr int NQW = KH ? NW / 2 : NW;  // waves with distinct query blocks
@@ -89,6 +102,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
     constexpr int XP = 64 * 16 + 64 * 4;
     constexpr int XPAR = NW * XP + NW * 4;
     __shared__ __attribute__((aligned(16))) unsigned char xch[PS ? 2 * XPAR + NW * 16 * 4 : 16];
+    __shared__ __attribute__((aligned(16))) int dids[SCORED ? NSL : 1][kStageKeys];  // the slots' document ids
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, lg = lane >> 4;
@@ -133,12 +147,25 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
                         f32x2{-INFINITY, 0.0f};
                 }
         }
+        if constexpr (SCORED) {  // unsplit: a tile whose rows see nothing is 0
+            if (p.splits == 1) {
+                for (int r = wave; r < QT; r += NW) {
+                    const long long gr = (long long) tile * QT + r;
+                    if (gr >= nq) break;
+                    const unsigned qi = position_of(gr, p.G);
+                    uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.o_hs;
+                    for (int d = 4 * lane; d < D; d += 256) *reinterpret_cast<u32x2 *>(o + d) = u32x2{0u, 0u};
+                }
+            }
+        }
         return;
     }
 
     // Q^T B operands: lane (li, lg) holds dims 32ks + 8lg .. +8 of its query row.
     bf16x8 qreg[QB][KS];
     int qabs[QB];  // absolute position of this lane's query in block qb
+    float slope[SCORED ? QB : 1];  // its bias per position of distance (log2 units)
+    int qdoc[SCORED ? QB : 1];     // its document
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const long long gr = qrow(qb);
@@ -146,6 +173,10 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         const uint16_t *qr = p.q + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.q_hs +
                              (size_t) qi * p.q_rs + lg * 8;
         qabs[qb] = p.q_pos0 + (int) qi;
+        if constexpr (SCORED) {
+            slope[qb] = p.slopes ? p.slopes[kvh * p.G + (int) ((unsigned) gr - qi * p.G)] * kLog2e : 0.0f;
+            qdoc[qb] = p.q_doc ? p.q_doc[qi] : 0;
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 w = qvalid(qb) ? *reinterpret_cast<const u32x4 *>(qr + ks * 32) : u32x4{0u, 0u, 0u, 0u};
@@ -197,6 +228,15 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
 
     const int qk_off = R::off(li) + lg * 16;                    // + 64 ks (+ HB: keys 16..31)
     const int tr_off = R::off(4 * lg + li / 4) + (li % 4) * 8;  // + 32 dt (+ HB)
+    // V^T of dims 16 dt .. of a stage's slot (PS: from its half), the PV A operand
+    auto vtile_of = [&](const unsigned char *vbh, int dt) {
+        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4v *) (vbh + tr_off + 32 * dt));
+        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4v *) (vbh + R::HB + tr_off + 32 * dt));
+        const short8v a8 = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+        return __builtin_bit_cast(bf16x8, a8);
+    };
 
     float m[QB], l[QB];
     f32x4 acc[NB][DW];
@@ -245,18 +285,172 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         return sc;
     };
 
-    issue(kvb, 0, kslot(0));  // nst >= 1 here
-    if (!SH) issue(vvb, 0, vslot(0));
-    if ((KH || S2) && nst > 1) {
-        issue(kvb, 1, kslot(1));
-        if (!SH) issue(vvb, 1, vslot(1));
+    // Scored: the stages to compute, in order.  cur[i] / ahead[i] are the key stages of this and of
+    // the next iteration (nst past the last), and whether their documents need no mask.  The i-th
+    // stage computed takes ring slot i % NSL.
+    struct Stage {
+        int st;
+        bool pure;
+    };
+    Stage cur[SPI], ahead[SPI];
+    int window = -1;                             // the 64 stages that live / pure describe
+    unsigned long long live = 0ull, pure = 0ull;
+    int qlo = 0, qhi = 0;                        // the tile's documents
+    bool one_doc = true;                         // all of its rows in one
+    auto load_window = [&](int w) {
+        if constexpr (SCORED) {
+            window = w;
+            live = pure = 0ull;
+#pragma unroll 1
+            for (int u = 0; u < 8; ++u) {  // 8 stages at a time, 8 lanes of 4 keys each
+                const long long j = (long long) j0 + w * 2048LL + u * 256 + 4 * lane;
+                int lo = INT_MAX, hi = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // past the last key: its id again
+                    const int d = p.k_doc[min(j + e, (long long) p.Sk - 1)];
+                    lo = min(lo, d);
+                    hi = max(hi, d);
+                }
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) {
+                    lo = min(lo, __shfl_xor(lo, o));
+                    hi = max(hi, __shfl_xor(hi, o));
+                }
+                // bit 8i of the ballot (lane 8i: stage i of the eight) -> bit i
+                auto stages = [&](bool b) {
+                    const unsigned long long x = __builtin_amdgcn_ballot_w64(b) & 0x0101010101010101ull;
+                    return (x * 0x0102040810204080ull) >> 56 << (8 * u);
+                };
+                live |= stages(hi >= qlo && lo <= qhi);
+                pure |= stages(one_doc && lo == qlo && hi == qhi);
+            }
+        }
+    };
+    // to[0 .. SPI-1]: the first SPI stages to compute from stage s on
+    auto next_stages = [&](int s, auto &to) {
+        if constexpr (SCORED) {
+            if (!p.k_doc) {
+#pragma unroll
+                for (int i = 0; i < SPI; ++i) to[i] = {min(s + i, nst), true};
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < SPI; ++i) to[i] = {nst, true};
+            int n = 0;
+#pragma unroll 1
+            while (s < nst && n < SPI) {
+                if ((s >> 6) != window) load_window(s >> 6);
+                const unsigned long long m = live >> (s & 63);
+                if (m == 0ull) {
+                    s = (s | 63) + 1;
+                    continue;
+                }
+                s += __builtin_ctzll(m);
+                if (s >= nst) break;
+                to[n == 0 ? 0 : SPI - 1] = {s, ((pure >> (s & 63)) & 1) != 0};
+                ++n;
+                ++s;
+            }
+        }
+    };
+    if constexpr (SCORED) {
+        if (p.k_doc) {
+            // lowest and highest document of the tile's positions; negative ids are nobody's
+            qlo = INT_MAX;
+            qhi = -1;
+            const int i0 = qa_min - p.q_pos0, i1 = qa_max - p.q_pos0;
+            for (int i = i0 + lane; i <= i1; i += 64) {
+                const int d = p.q_doc[i];
+                if (d < 0) one_doc = false;
+                else {
+                    qlo = min(qlo, d);
+                    qhi = max(qhi, d);
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                qlo = min(qlo, __shfl_xor(qlo, o));
+                qhi = max(qhi, __shfl_xor(qhi, o));
+            }
+            qlo = __builtin_amdgcn_readfirstlane(qlo);
+            qhi = __builtin_amdgcn_readfirstlane(qhi);
+            one_doc = __builtin_amdgcn_ballot_w64(!one_doc) == 0ull && qlo == qhi;
+        }
+        next_stages(0, cur);
+    }
+    auto issue_docs = [&](int st, int s) {
+        if constexpr (SCORED) {
+            if (p.k_doc && wave == 0 && lane < kStageKeys)
+                lds_dma4(p.k_doc + min(j0 + st * kStageKeys + lane, j1 - 1), lds_addr(dids[s & (NSL - 1)]));
+        }
+    };
+
+    if constexpr (!SCORED) {
+        issue(kvb, 0, kslot(0));  // nst >= 1 here
+        if (!SH) issue(vvb, 0, vslot(0));
+        if ((KH || S2) && nst > 1) {
+            issue(kvb, 1, kslot(1));
+            if (!SH) issue(vvb, 1, vslot(1));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < SPI; ++i)
+            if (cur[i].st < nst) {
+                issue(kvb, cur[i].st, kslot(i));
+                if (!SH) issue(vvb, cur[i].st, vslot(i));
+                issue_docs(cur[i].st, i);
+            }
     }
 
-    for (int s0 = 0; s0 < nst; s0 += SPI) {
+    auto shift = [&]() {
+        if constexpr (SCORED) {
+#pragma unroll
+            for (int i = 0; i < SPI; ++i) cur[i] = ahead[i];
+        }
+    };
+    auto scored_full = [&](int jb, int ka_first, int ka_last, bool pure) {
+        if constexpr (SCORED)
+            return jb + kStageKeys <= j1 && (ka_last <= qa_min || ka_last < p.prefix) &&
+                   (p.window == 0 || ka_first > qa_max - p.window) && pure;
+        else return false;
+    };
+    // Scored: whether a masked stage holds a value that is not finite (V^T . 0 is NaN then; rare).
+    auto odd_values = [&](int s, int st, bool pure) {
+        const int jb = j0 + st * kStageKeys, ka_first = p.k_pos0 + jb, ka_last = ka_first + kStageKeys - 1;
+        if (st >= nst || scored_full(jb, ka_first, ka_last, pure)) return false;
+        const unsigned char *const vbh = vslot(s) + 32 * DW * hd;
+        f32x4 chk = {0.0f, 0.0f, 0.0f, 0.0f};
+        const bf16x8 zero = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+        for (int dt = 0; dt < DW; ++dt) {
+            chk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vtile_of(vbh, dt), zero, chk, 0, 0, 0);
+            if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        const float c = chk[0] + chk[1] + chk[2] + chk[3];
+        return __builtin_amdgcn_ballot_w64(c != c) != 0ull;
+    };
+
+    bool odd = false;  // a masked stage held such a value
+    for (int s0 = 0; SCORED ? cur[0].st < nst : s0 < nst; s0 += SPI, shift()) {
+        // the key stage of the i-th stage from s0 on
+        auto at = [&](int i) -> int {
+            if constexpr (!SCORED) return s0 + i;
+            else if (i < SPI) return i == 0 ? cur[0].st : cur[SPI - 1].st;
+            else return i == SPI ? ahead[0].st : ahead[SPI - 1].st;
+        };
         // The iteration's stages s0 .. s0+SPI-1 landed (this wave's loads; the barrier covers
         // the other waves') and every wave is done with the previous iteration
         ESDA_WAIT_VM(0);
         lds_barrier();
+        if constexpr (SCORED) {
+            next_stages(cur[SPI - 1].st + 1, ahead);
+            if constexpr (KH) {
+                odd |= odd_values(s0 + kh, kh ? cur[1].st : cur[0].st, kh ? cur[1].pure : cur[0].pure);
+            } else {
+                odd |= odd_values(s0, cur[0].st, cur[0].pure);
+                if constexpr (S2) odd |= odd_values(s0 + 1, cur[1].st, cur[1].pure);
+            }
+        }
         // The next iteration's DMAs, spread over this iteration so that the workgroup's loads
         // do not all queue at the barrier (each slot is free once the barrier has passed):
         //  - separate K and V (plain, S2): K of the next stage at the barrier, its V after
@@ -266,15 +460,19 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         //  - KH: all at the barrier (spreading measured slower there).
         constexpr bool kVLate = !SH && !KH;
         auto issue_k = [&]() {
-            if (s0 + SPI < nst) issue(kvb, s0 + SPI, kslot(s0 + SPI));
+            if (at(SPI) < nst) {
+                issue(kvb, at(SPI), kslot(s0 + SPI));
+                issue_docs(at(SPI), s0 + SPI);
+            }
         };
         auto issue_v = [&]() {
-            if (!SH && s0 + SPI < nst) issue(vvb, s0 + SPI, vslot(s0 + SPI));
+            if (!SH && at(SPI) < nst) issue(vvb, at(SPI), vslot(s0 + SPI));
         };
         auto issue_second = [&]() {
-            if (s0 + SPI + 1 < nst) {
-                issue(kvb, s0 + SPI + 1, kslot(s0 + SPI + 1));
-                if (!SH) issue(vvb, s0 + SPI + 1, vslot(s0 + SPI + 1));
+            if (at(SPI + 1) < nst) {
+                issue(kvb, at(SPI + 1), kslot(s0 + SPI + 1));
+                if (!SH) issue(vvb, at(SPI + 1), vslot(s0 + SPI + 1));
+                issue_docs(at(SPI + 1), s0 + SPI + 1);
             }
         };
         auto after_first_qk = [&]() {
@@ -284,18 +482,20 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         if constexpr (!SH) issue_k();
         if constexpr (!kVLate && !SH) issue_v();
         if constexpr (KH) issue_second();
-        auto stage = [&](const int s, auto after_qk) {
+        // stage s in the order computed (its ring slot), key stage st
+        auto stage = [&](const int s, const int st, const bool pure, auto after_qk) {
         const Scores cur = qk(kslot(s));
         after_qk();
         const unsigned char *vb = vslot(s);
-        const int jb = j0 + s * kStageKeys;
+        const int jb = j0 + st * kStageKeys;
 
         // Stage s's raw scores q.k; positions a boundary stage does not show to a row are
         // -inf.  A stage is fully visible to every row of the tile when its last key is at
         // or before the tile's first position, its first key is inside the window of the
         // tile's last position, and it lies inside the split.  The softmax scale (times
         // log2 e, > 0) is applied to the row maxima and inside the exponent's fma.
-        const float c2 = p.scale_log2e;
+        // (Scored: the cap and the bias first, the mask last -- a masked score may be NaN.)
+        float c2 = p.scale_log2e;
         float sv[QB][8];
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
@@ -304,8 +504,33 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sv[qb][4 * h + r] = cur.s[h][qb][r];
         const int ka_first = p.k_pos0 + jb, ka_last = ka_first + kStageKeys - 1;
-        const bool full = jb + kStageKeys <= j1 && ka_last <= qa_min &&
-                          (p.window == 0 || ka_first > qa_max - p.window);
+        const bool full = SCORED ? scored_full(jb, ka_first, ka_last, pure)
+                                 : jb + kStageKeys <= j1 && ka_last <= qa_min &&
+                                       (p.window == 0 || ka_first > qa_max - p.window);
+        if constexpr (SCORED) {
+            if (p.cap_out != 0.0f) {
+                // tanh(x) = 1 - 2 / (1 + e^2x), off by 2^-23 or so; cap_out = cap log2 e is the score's unit
+                c2 = p.cap_out;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        sv[qb][e] = __builtin_fmaf(
+                            -2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sv[qb][e] * p.cap_in)), 1.0f);
+            }
+            if (p.slopes) {
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    const int d0 = qabs[qb] - ka_first - 4 * lg;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float dist = (float) (d0 - (16 * (e / 4) + e % 4));
+                        sv[qb][e] = __builtin_fmaf(sv[qb][e], c2, -slope[qb] * __builtin_fabsf(dist));
+                    }
+                }
+                c2 = 1.0f;
+            }
+        }
         if (!full) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
@@ -317,8 +542,26 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
                     for (int r = 0; r < 4; ++r) {
                         const int j = jb + 16 * h + 4 * lg + r;
                         const int ka = p.k_pos0 + j;
-                        if (!(j < j1 && ka <= qa && ka > lo)) sv[qb][4 * h + r] = -INFINITY;
+                        if constexpr (SCORED) {
+                            if (!((j < j1) & (ka <= max(qa, p.prefix - 1)) & (ka > lo))) sv[qb][4 * h + r] = -INFINITY;
+                        } else {
+                            if (!(j < j1 && ka <= qa && ka > lo)) sv[qb][4 * h + r] = -INFINITY;
+                        }
                     }
+            }
+        }
+
+        if constexpr (SCORED) {
+            if (!pure) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const i32x4 d = *reinterpret_cast<const i32x4 *>(&dids[s & (NSL - 1)][16 * h + 4 * lg]);
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if ((d[r] != qdoc[qb]) | (d[r] < 0)) sv[qb][4 * h + r] = -INFINITY;
+                }
             }
         }
 
@@ -377,14 +620,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         // half) and 16 + 4lg .. (second half): the k order of the P^T registers.
         // The V^T tiles are read PD ahead of their MFMAs (the scheduler alone kept one in flight).
         const unsigned char *const vbh = vb + 32 * DW * hd;  // PS: this wave's dims
-        auto vtile = [&](int dt) {
-            const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4v *) (vbh + tr_off + 32 * dt));
-            const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4v *) (vbh + R::HB + tr_off + 32 * dt));
-            const short8v a8 = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-            return __builtin_bit_cast(bf16x8, a8);
-        };
+        auto vtile = [&](int dt) { return vtile_of(vbh, dt); };
         constexpr int PD = PV_DEPTH;
         bf16x8 vf[PD];
 #pragma unroll
@@ -422,13 +658,102 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         }
         };
         if constexpr (S2) {
-            stage(s0, after_first_qk);
+            stage(s0, at(0), !SCORED || cur[0].pure, after_first_qk);
             issue_second();
-            if (s0 + 1 < nst) stage(s0 + 1, [] {});
+            if (at(1) < nst) stage(s0 + 1, at(1), !SCORED || cur[SPI - 1].pure, [] {});
         } else {
-            const int s = s0 + kh;  // this wave group's stage
-            if (KH && s >= nst) continue;  // an odd stage count: the odd group's last iteration is empty
-            stage(s, after_first_qk);
+            const int s = s0 + kh, st = at(kh);  // this wave group's stage
+            if (KH && st >= nst) continue;  // an odd stage count: the odd group's last iteration is empty
+            stage(s, st, !SCORED || (kh ? cur[SPI - 1].pure : cur[0].pure), after_first_qk);
+        }
+    }
+
+    if constexpr (SCORED) {
+        // Rare: the tile again, row by row, without the keys a row does not see.  The lanes take 64
+        // keys for the scores, then the row's dims for the product.  (In the stage itself a second
+        // form of the product cost every stage: O^T no longer stayed in registers.)
+        int *const any_odd = reinterpret_cast<int *>(&dids[0][0]);
+        lds_barrier();
+        if (threadIdx.x == 0) *any_odd = 0;
+        lds_barrier();
+        if (odd && lane == 0) *any_odd = 1;
+        lds_barrier();
+        if (__builtin_expect(*any_odd != 0, 0)) {
+            constexpr int DPL = D / 64;
+            typedef uint16_t piece __attribute__((ext_vector_type(DPL)));
+            for (int r = wave; r < QT; r += NW) {
+                const long long gr = (long long) tile * QT + r;
+                if (gr >= nq) break;
+                const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
+                const uint16_t *const qr = p.q + (size_t) qh * p.q_hs + (size_t) qi * p.q_rs;
+                const int qa = p.q_pos0 + qi, lo = p.window > 0 ? qa - p.window : INT_MIN;
+                const float sl = p.slopes ? p.slopes[qh] * kLog2e : 0.0f;
+                const int doc = p.k_doc ? p.q_doc[qi] : 0;
+                float mr = -INFINITY, lr = 0.0f, o[DPL];
+#pragma unroll
+                for (int e = 0; e < DPL; ++e) o[e] = 0.0f;
+                for (int jb = j0; jb < j1; jb += 64) {
+                    const int j = jb + lane, ka = p.k_pos0 + j;
+                    bool seen = j < j1 && ka <= max(qa, p.prefix - 1) && ka > lo;
+                    if (p.k_doc && seen) seen = doc >= 0 && p.k_doc[j] == doc;
+                    unsigned long long todo = __builtin_amdgcn_ballot_w64(seen);
+                    if (todo == 0ull) continue;
+                    float x = 0.0f;
+                    if (seen) {
+                        const uint16_t *const kr = kvb + (size_t) j * D;
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 8) {
+                            const u32x4 kv = *reinterpret_cast<const u32x4 *>(kr + d);
+                            const u32x4 qv = *reinterpret_cast<const u32x4 *>(qr + d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                x = __builtin_fmaf(bf16_lo(qv[e]), bf16_lo(kv[e]), x);
+                                x = __builtin_fmaf(bf16_hi(qv[e]), bf16_hi(kv[e]), x);
+                            }
+                        }
+                        x = p.cap_out != 0.0f
+                                ? p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p.cap_in)), 1.0f)
+                                : x * p.scale_log2e;
+                        x = __builtin_fmaf(-sl, __builtin_fabsf((float) (qa - ka)), x);
+                    }
+                    float top = seen ? x : -INFINITY;
+#pragma unroll
+                    for (int i = 32; i >= 1; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+                    const float mn = fmaxf(mr, top), corr = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - mn);
+                    const float w = seen ? (float) (__bf16) __builtin_amdgcn_exp2f(x - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
+                    float sum = w;
+#pragma unroll
+                    for (int i = 32; i >= 1; i >>= 1) sum += __shfl_xor(sum, i);
+                    mr = mn;
+                    lr = lr * corr + sum;
+#pragma unroll
+                    for (int e = 0; e < DPL; ++e) o[e] *= corr;
+                    while (todo) {
+                        const int b = __builtin_ctzll(todo);
+                        todo &= todo - 1;
+                        const float wb = __shfl(w, b);
+                        const piece v = *reinterpret_cast<const piece *>(vvb + (size_t) (jb + b) * D + lane * DPL);
+#pragma unroll
+                        for (int e = 0; e < DPL; ++e)
+                            o[e] = __builtin_fmaf(wb, __builtin_bit_cast(float, (unsigned) v[e] << 16), o[e]);
+                    }
+                }
+                const long long row = (long long) qi * p.Hq + qh;
+                if (p.splits == 1) {
+                    const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+                    piece b;
+#pragma unroll
+                    for (int e = 0; e < DPL; ++e) b[e] = __builtin_bit_cast(uint16_t, (__bf16) (o[e] * inv));
+                    *reinterpret_cast<piece *>(p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + lane * DPL) = b;
+                } else {
+                    float *pa = p.part_acc + ((long long) split * nrows + row) * D + lane * DPL;
+#pragma unroll
+                    for (int e = 0; e < DPL; ++e) pa[e] = o[e];
+                    if (lane == 0)
+                        *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{mr, lr};
+                }
+            }
+            return;
         }
     }
 
@@ -493,7 +818,8 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
         const long long row = (long long) qi * p.Hq + qh;
         const int d0 = 16 * DW * hd;  // the wave's first O^T dim
         if (p.splits == 1) {
-            const float inv = 1.0f / lb[nb];
+            float inv = 1.0f / lb[nb];
+            if constexpr (SCORED) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
             uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
 #pragma unroll
             for (int dt = 0; dt < DW; ++dt) {
@@ -539,8 +865,12 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(PrefillParams p) {
 // 6.3; 16384 rows with 2 splits 17.2 against 14.4 (67 MB at 4.7 TB/s).  A wave per row of 128
 // dims, 2 a lane, had too few bytes in flight for many rows: 16,384 rows with 2 splits 6.9 us
 // against 5.4 here, 32,768 10.9 against 9.3.
-template <int D, int NS, bool GAPS = false>
-__global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
+// P = ScoredParams: a row without a live split gives 0 (and a NaN sum is live: its row is NaN).
+template <int D, int NS, bool GAPS = false, class P = PrefillParams>
+__global__ __launch_bounds__(256) void prefill_merge_kernel(P p) {
+    constexpr bool SCORED = std::is_same<P, ScoredParams>::value;
+    auto alive = [](float l) { return SCORED ? l != 0.0f : l > 0.0f; };
+    auto inverse = [](float den) { return SCORED && den == 0.0f ? 0.0f : 1.0f / den; };
     constexpr int VEC = D >= 256 || NS > 0 ? 4 : D / 64;              // dims per lane
     constexpr int LPR = D / VEC < 64 ? D / VEC : 64, RPW = 64 / LPR;  // lanes per row and wave, rows per wave
     constexpr int PARTS = D / (LPR * VEC);                            // waves per row
@@ -577,22 +907,22 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
         if (GAPS) {
 #pragma unroll
             for (int s = 0; s < NS; ++s)
-                if (mls[s][1] > 0.0f) a[s] = *reinterpret_cast<const vec *>(acc + s * ss);
+                if (alive(mls[s][1])) a[s] = *reinterpret_cast<const vec *>(acc + s * ss);
         }
         float M = -INFINITY, den = 0.0f;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) M = mls[s][1] > 0.0f ? fmaxf(M, mls[s][0]) : M;
+        for (int s = 0; s < NS; ++s) M = alive(mls[s][1]) ? fmaxf(M, mls[s][0]) : M;
         vec num = 0.0f;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             // (the operands selected, not the products: those stay fused into the sums)
-            const bool live = mls[s][1] > 0.0f;
+            const bool live = alive(mls[s][1]);
             const float w = live ? __builtin_amdgcn_exp2f(mls[s][0] - M) : 0.0f;
             den = __builtin_fmaf(live ? mls[s][1] : 0.0f, w, den);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) num[e] = __builtin_fmaf(live ? a[s][e] : 0.0f, w, num[e]);
         }
-        write(num * (1.0f / den));
+        write(num * inverse(den));
         return;
     }
     auto ml_of = [&](int s) {
@@ -600,10 +930,10 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
                             : f32x2{-INFINITY, 0.0f};
     };
     f32x2 ml = ml_of(lane);
-    float M = ml[1] > 0.0f ? ml[0] : -INFINITY;
+    float M = alive(ml[1]) ? ml[0] : -INFINITY;
     for (int s = lane + 64; s < p.splits; s += 64) {
         const f32x2 x = ml_of(s);
-        if (x[1] > 0.0f) M = fmaxf(M, x[0]);
+        if (alive(x[1])) M = fmaxf(M, x[0]);
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -611,9 +941,9 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
     vec num = 0.0f;
     for (int s0 = 0; s0 < p.splits; s0 += 64) {
         if (s0) ml = ml_of(s0 + lane);
-        const float w = ml[1] > 0.0f ? __builtin_amdgcn_exp2f(ml[0] - M) : 0.0f;
-        den += ml[1] > 0.0f ? ml[1] * w : 0.0f;
-        unsigned long long live = __builtin_amdgcn_ballot_w64(ml[1] > 0.0f);
+        const float w = alive(ml[1]) ? __builtin_amdgcn_exp2f(ml[0] - M) : 0.0f;
+        den += alive(ml[1]) ? ml[1] * w : 0.0f;
+        unsigned long long live = __builtin_amdgcn_ballot_w64(alive(ml[1]));
         while (live) {
             vec a[MB];
             float wj[MB];
@@ -634,11 +964,11 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) den += __shfl_xor(den, o);
-    write(num * (1.0f / den));
+    write(num * inverse(den));
 }
 
-template <int D>
-void launch_prefill(const PrefillParams &p, int stages, hipStream_t st) {
+template <int D, class P = PrefillParams>
+void launch_prefill(const P &p, int stages, hipStream_t st) {
     if (stages & 1) {
         // Up to 64 rows of D = 512 are one tile, and a plan, of either height; the kernel then goes by
         // the streams, which the plan does not know.  Of 499 such (chunk, split) pairs of K = V four
@@ -648,32 +978,32 @@ void launch_prefill(const PrefillParams &p, int stages, hipStream_t st) {
         const int nw = one ? (shared ? 4 : 8) : p.nw;
         const dim3 grid(p.tiles * p.Hkv * p.splits), block(64 * nw);
         if constexpr (D == 512) {
-            if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4>), grid, block, 0, st, p);
-            else if (nw == 4) hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, 4>), grid, block, 0, st, p);
-            else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true>), grid, block, 0, st, p);
-            else hipLaunchKernelGGL((prefill_kernel<512, 1>), grid, block, 0, st, p);
+            if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);
+            else if (nw == 4) hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, 4, P>), grid, block, 0, st, p);
+            else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, kWaves, P>), grid, block, 0, st, p);
+            else hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
         }
         else if constexpr (D == 128)
-            hipLaunchKernelGGL((prefill_kernel<128, 2>), grid, block, 0, st, p);
+            hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
         else if (p.qb == 2)
-            hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true>), grid, block, 0, st, p);
+            hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true, false, kWaves, P>), grid, block, 0, st, p);
         else if (p.kh)
-            hipLaunchKernelGGL((prefill_kernel<256, 1, true>), grid, block, 0, st, p);
+            hipLaunchKernelGGL((prefill_kernel<256, 1, true, false, false, false, kWaves, P>), grid, block, 0, st, p);
         else
-            hipLaunchKernelGGL((prefill_kernel<256, 1>), grid, block, 0, st, p);
+            hipLaunchKernelGGL((prefill_kernel<256, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
     }
     if ((stages & 2) && p.splits > 1) {
         const long long waves = merge_waves(p, D);
-        PrefillParams mp = p;
+        P mp = p;
         for (mp.merge_wave0 = 0; mp.merge_wave0 < waves; mp.merge_wave0 += kMergeLaunchWaves) {
             const long long n = std::min(kMergeLaunchWaves, waves - mp.merge_wave0);
             const int wpb = D == 128 && p.splits <= 8 ? 2 : 4;  // waves per block: the kernel's 4 / RPW
             const dim3 grid((unsigned) ((n + wpb - 1) / wpb)), block(64 * wpb);
-            if (p.part_gaps && p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, true>), grid, block, 0, st, mp);
-            else if (p.part_gaps && p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, true>), grid, block, 0, st, mp);
-            else if (p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4>), grid, block, 0, st, mp);
-            else if (p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8>), grid, block, 0, st, mp);
-            else hipLaunchKernelGGL((prefill_merge_kernel<D, 0>), grid, block, 0, st, mp);
+            if (p.part_gaps && p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, true, P>), grid, block, 0, st, mp);
+            else if (p.part_gaps && p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, true, P>), grid, block, 0, st, mp);
+            else if (p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, false, P>), grid, block, 0, st, mp);
+            else if (p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, false, P>), grid, block, 0, st, mp);
+            else hipLaunchKernelGGL((prefill_merge_kernel<D, 0, false, P>), grid, block, 0, st, mp);
         }
     }
 }

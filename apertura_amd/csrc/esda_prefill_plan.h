@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 #include "esda_plan.h"
 #include "esda_prefill.h"
@@ -53,6 +54,23 @@ ESDA_HD void tile_keys(const PrefillParams &p, int tile, int QT, int &j0, int &j
     if (hi < lo) hi = lo;
     j0 = (int) lo;
     j1 = (int) hi;
+}
+
+// The parameters of a call with modified scores and masks (esda_scored.h) beside a plain one's.
+struct ScoredParams : PrefillParams {
+    int prefix;               // keys before this position are visible to queries before them, too
+    float cap_in, cap_out;    // cap: score (log2 units) = cap_out tanh(cap_in raw / (2 log2 e)); cap_out 0: none
+    const float *slopes;      // distance bias of each query head, or null
+    const int *q_doc, *k_doc; // document ids of queries and keys, or null
+};
+
+// The same for a scored call: every row sees the keys of the prefix, within its window.
+ESDA_HD void tile_keys(const ScoredParams &p, int tile, int QT, int &j0, int &j1) {
+    const PrefillParams &plain = p;
+    tile_keys(plain, tile, QT, j0, j1);
+    const long long seen = (long long) p.prefix - p.k_pos0;
+    if (seen > j1) j1 = seen < p.Sk ? (int) seen : p.Sk;
+    if (j0 > j1) j0 = j1;  // rows whose window starts past the keys see none
 }
 
 // A kernel form of one head dim: 16-query blocks per wave, stage halves or not, waves, and
@@ -136,7 +154,10 @@ constexpr int kMaxRounds = 3;  // split plans of more workgroups per CU only add
 
 // Validates a description and fills the kernel parameters' shape fields and plan.  Returns
 // what is wrong with it, or null.
-inline const char *plan_prefill(const esda_prefill_desc *d, PrefillParams *p) {
+// A scored call's masks (p->prefix) are set before; its queries may see no key.
+template <class P>
+const char *plan_prefill(const esda_prefill_desc *d, P *p) {
+    constexpr bool scored = std::is_same<P, ScoredParams>::value;
     if (!d) return "esda_prefill: null description";
     const int D = d->head_dim;
     if (D != 128 && D != 256 && D != 512)
@@ -147,7 +168,7 @@ inline const char *plan_prefill(const esda_prefill_desc *d, PrefillParams *p) {
         return "esda_prefill: sizes, positions and window must be non-negative";
     if ((long long) d->q_pos0 + d->seq_q > INT_MAX || (long long) d->k_pos0 + d->seq_k > INT_MAX)
         return "esda_prefill: positions must stay below 2^31";
-    if (d->k_pos0 > d->q_pos0 || (long long) d->k_pos0 + d->seq_k < (long long) d->q_pos0 + d->seq_q)
+    if (!scored && (d->k_pos0 > d->q_pos0 || (long long) d->k_pos0 + d->seq_k < (long long) d->q_pos0 + d->seq_q))
         return "esda_prefill: the keys must hold every query's own position (k_pos0 <= q_pos0, "
                     "k_pos0 + seq_k >= q_pos0 + seq_q)";
     for (long long st : {d->q_head_stride, d->q_row_stride, d->kv_head_stride, d->out_row_stride, d->out_head_stride})
@@ -159,7 +180,7 @@ inline const char *plan_prefill(const esda_prefill_desc *d, PrefillParams *p) {
         return "esda_prefill: split_keys must be a multiple of 32";
     if (!(d->scale > 0.0f) || !std::isfinite(d->scale))
         return "esda_prefill: scale must be positive and finite";
-    *p = PrefillParams{};
+    static_cast<PrefillParams &>(*p) = PrefillParams{};
     p->Hq = d->num_q_heads;
     p->Hkv = d->num_kv_heads;
     p->G = d->num_q_heads / d->num_kv_heads;

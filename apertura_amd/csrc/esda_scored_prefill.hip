@@ -1,0 +1,98 @@
+// esda_scored_prefill.hip -- prefill attention with capped or biased scores and document and
+// prefix masks for MI355X (gfx950): prefill_kernel and prefill_merge_kernel (esda_prefill_kernel.h)
+// with ScoredParams.  The C ABI is include/esda_scored.h.
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "esda.h"
+#include "esda_internal.h"
+#include "esda_prefill_kernel.h"
+#include "esda_scored.h"
+
+namespace {
+
+int fail(int code, const std::string &msg) {
+    esda_detail::set_error(msg);
+    return code;
+}
+
+bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+// The plan of a call, or what is wrong with it.
+const char *plan(const esda_prefill_desc *d, const esda_score *s, ScoredParams *p) {
+    if (!d || !s) return "esda_scored_prefill: null description or score";
+    if (!(s->softcap >= 0.0f) || !std::isfinite(s->softcap))
+        return "esda_scored_prefill: softcap must be 0 or positive and finite";
+    if (s->prefix < 0) return "esda_scored_prefill: prefix must not be negative";
+    if ((long long) d->k_pos0 + d->seq_k > INT_MAX - 64) return "esda_scored_prefill: key positions must stay below 2^31 - 64";
+    *p = ScoredParams{};
+    p->prefix = s->prefix;
+    if (const char *why = plan_prefill(d, p)) return why;
+    if (s->softcap > 0.0f) {
+        p->cap_in = (float) (2.0 * 1.4426950408889634 * d->scale / s->softcap);
+        p->cap_out = (float) (1.4426950408889634 * s->softcap);
+        if (!std::isfinite(p->cap_in) || !std::isfinite(p->cap_out) || p->cap_in == 0.0f)
+            return "esda_scored_prefill: softcap and scale are too far apart";
+    }
+    p->slopes = s->slopes;
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+int esda_scored_prefill_workspace_size(const esda_prefill_desc *desc, const esda_score *score, size_t *bytes) {
+    if (!bytes) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill_workspace_size: null output");
+    ScoredParams p;
+    if (const char *why = plan(desc, score, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
+    *bytes = workspace_of(p, desc->head_dim);
+    return ESDA_OK;
+}
+
+int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, const esda_scored_prefill_args *a,
+                        void *stream) {
+    ScoredParams p;
+    if (const char *why = plan(desc, score, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
+    if (!a || !a->q || !a->k || !a->v || !a->out)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: null pointer");
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: tensors must be 16-byte aligned");
+    if (!a->q_doc != !a->k_doc)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: q_doc and k_doc go together");
+    if ((reinterpret_cast<uintptr_t>(a->k_doc) | reinterpret_cast<uintptr_t>(a->q_doc) |
+         reinterpret_cast<uintptr_t>(score->slopes)) & 3u)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: document ids and slopes must be 4-byte aligned");
+    const int D = desc->head_dim;
+    const size_t need = workspace_of(p, D);
+    if (need) {
+        if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+            return fail(ESDA_ERR_WORKSPACE, "esda_scored_prefill: workspace missing or smaller than "
+                                            "esda_scored_prefill_workspace_size");
+        const size_t rows = (size_t) p.Sq * p.Hq;
+        p.part_acc = static_cast<float *>(a->workspace);
+        p.part_ml = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + (size_t) p.splits * rows * D * 4);
+    }
+    const int rc = esda_detail::check_device();
+    if (rc != ESDA_OK) return rc;
+    p.q = static_cast<const uint16_t *>(a->q);
+    p.k = static_cast<const uint16_t *>(a->k);
+    p.v = static_cast<const uint16_t *>(a->v);
+    p.out = static_cast<uint16_t *>(a->out);
+    p.q_doc = a->q_doc;
+    p.k_doc = a->k_doc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (D == 512) launch_prefill<512, ScoredParams>(p, 3, st);
+    else if (D == 256) launch_prefill<256, ScoredParams>(p, 3, st);
+    else launch_prefill<128, ScoredParams>(p, 3, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(ESDA_ERR_HIP, std::string("esda_scored_prefill launch: ") + hipGetErrorString(e));
+    return ESDA_OK;
+}
+
+}  // extern "C"

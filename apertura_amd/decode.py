@@ -114,6 +114,26 @@ def _stream_ptr(stream) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _same_device(tensors: dict) -> None:
+    """Every tensor on the current device: the launch goes to its stream."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must live in GPU memory")
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name} is on {t.device}; the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _used_on(stream, *tensors) -> None:
+    """Tensors of the current stream that a launch on `stream` uses: their memory is not handed out
+    again before that launch is through."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def decode_step(step: DecodeStep, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor | None,
                 k_cache: torch.Tensor, v_cache: torch.Tensor | None, pos: torch.Tensor,
                 row_base: torch.Tensor | None = None, out: torch.Tensor | None = None,

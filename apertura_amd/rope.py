@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import RopeArgs, RopeDesc, RopeScalingDesc, check, lib
-from .decode import _stream_ptr
+from .decode import _same_device, _stream_ptr, _used_on
 
 _KINDS = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
 
@@ -41,17 +41,6 @@ def rope_frequencies(rot_dim: int, base: float, scaling: RopeScaling | None = No
     check(lib().esda_rope_frequencies(ctypes.byref(d), rot_dim, inv, ctypes.byref(factor)))
     t = torch.tensor(list(inv), dtype=torch.float32)
     return (t if device is None else t.to(device)), float(factor.value)
-
-
-def _same_device(tensors: dict) -> None:
-    """Every tensor on the current device: the launch goes to its stream."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must live in GPU memory")
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name} is on {t.device}; the current device is cuda:{torch.cuda.current_device()}")
 
 
 class RopeCall:
@@ -116,4 +105,6 @@ def rope(q, k, pos: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = Fa
          attn_factor: float = 1.0, q_out=None, k_out=None, stream=None):
     """(q_out, k_out): the rows of q [T, Hq, D] and k [T, Hk, D] (either may be None) rotated to
     positions pos [T]; see RopeCall."""
-    return RopeCall(q, k, pos, inv_freq, interleaved, inverse, attn_factor, q_out, k_out)(stream)
+    out = RopeCall(q, k, pos, inv_freq, interleaved, inverse, attn_factor, q_out, k_out)(stream)
+    _used_on(stream, *out)
+    return out
