@@ -1,5 +1,6 @@
 """ctypes binding of libesda.so (the C ABI declared in include/esda.h,
-include/esda_cache.h, include/esda_prefill.h, include/esda_rope.h and include/esda_scored.h).
+include/esda_cache.h, include/esda_prefill.h, include/esda_rope.h, include/esda_scored.h and
+include/esda_prefix.h).
 
 The library is loaded from the package directory only (built in-tree by
 ``apertura_amd/build.py``); a missing library raises instead of falling back.
@@ -41,6 +42,8 @@ EXPORTS = (
     "esda_rope", "esda_rope_frequencies",
     # include/esda_scored.h
     "esda_scored_prefill_workspace_size", "esda_scored_prefill", "esda_scored_decode",
+    # include/esda_prefix.h
+    "esda_prefix_decode_workspace_size", "esda_prefix_decode",
 )
 _VOID = ("esda_cache_destroy", "esda_cache_mark_step", "esda_cache_reset", "esda_cache_clear_rewind_mark")
 
@@ -172,6 +175,17 @@ class ScoredPrefillArgs(ctypes.Structure):
     ]
 
 
+class PrefixDesc(ctypes.Structure):
+    _fields_ = [
+        ("own", DecodeDesc), ("prefix_len", ctypes.c_int32), ("split_keys", ctypes.c_int32),
+        ("prefix_head_stride", ctypes.c_int64),
+    ]
+
+
+class PrefixArgs(ctypes.Structure):
+    _fields_ = [("own", DecodeArgs), ("prefix_k", ctypes.c_void_p), ("prefix_v", ctypes.c_void_p)]
+
+
 class Q8View(ctypes.Structure):
     """esda_q8_view: u8 rows q [kv_heads, pitch, 512], f32 scale / bias [kv_heads, pitch]."""
     _fields_ = [
@@ -258,6 +272,9 @@ def lib() -> ctypes.CDLL:
         L.esda_rope.argtypes = [ctypes.POINTER(RopeDesc), ctypes.POINTER(RopeArgs), P]
         L.esda_rope_frequencies.argtypes = [ctypes.POINTER(RopeScalingDesc), i32, ctypes.POINTER(f32),
                                             ctypes.POINTER(f32)]
+        XD = ctypes.POINTER(PrefixDesc)
+        L.esda_prefix_decode_workspace_size.argtypes = [XD, ctypes.POINTER(sz)]
+        L.esda_prefix_decode.argtypes = [XD, ctypes.POINTER(PrefixArgs), P]
         SP = ctypes.POINTER(ScoreDesc)
         L.esda_scored_prefill_workspace_size.argtypes = [PD, SP, ctypes.POINTER(sz)]
         L.esda_scored_prefill.argtypes = [PD, SP, ctypes.POINTER(ScoredPrefillArgs), P]

@@ -26,6 +26,8 @@ SOURCES = [
     "esda_rope.hip",
     "esda_scored_decode.hip",
     "esda_scored_prefill.hip",
+    "esda_prefix.hip",
+    "esda_prefix_tiles.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",
@@ -51,6 +53,7 @@ EXTRA_FLAGS = {
     "esda_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
     # the decode kernel's other forms, compiled as esda_decode.hip's
     "esda_scored_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+    "esda_prefix.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -227,28 +227,6 @@ int fail(int code, const std::string &msg) {
 
 bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
-// plan_prefill of the calling thread's last description, kept: a plan depends on the description
-// alone and takes up to 35 us of host time (half of them 0.4), and a call asks for it twice, for
-// the workspace and for the launch.
-const char *last_plan(const esda_prefill_desc *d, PrefillParams *p) {
-    static_assert(sizeof(esda_prefill_desc) == 8 * 4 + 5 * 8 + 8, "no padding: descriptions compare by their bytes");
-    struct Last {
-        esda_prefill_desc desc;
-        PrefillParams plan;
-        bool set = false;
-    };
-    thread_local Last last;
-    if (!d || !last.set || std::memcmp(d, &last.desc, sizeof(*d)) != 0) {
-        PrefillParams fresh;
-        if (const char *why = plan_prefill(d, &fresh)) return why;
-        last.desc = *d;
-        last.plan = fresh;
-        last.set = true;
-    }
-    *p = last.plan;
-    return nullptr;
-}
-
 constexpr long long kRawKvWaves = 4 * kTargetGroups;
 
 template <int D, bool Q8>
@@ -296,14 +274,14 @@ extern "C" {
 int esda_prefill_workspace_size(const esda_prefill_desc *desc, size_t *bytes) {
     if (!bytes) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefill_workspace_size: null output");
     PrefillParams p;
-    if (const char *why = last_plan(desc, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
+    if (const char *why = last_plan(desc, 0, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
     *bytes = workspace_of(p, desc->head_dim);
     return ESDA_OK;
 }
 
 int esda_prefill_stages(const esda_prefill_desc *desc, const esda_prefill_args *a, int stages, void *stream) {
     PrefillParams p;
-    if (const char *why = last_plan(desc, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
+    if (const char *why = last_plan(desc, 0, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
     if (!a || !a->q || !a->k || !a->v || !a->out) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefill: null pointer");
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefill: tensors must be 16-byte aligned");

@@ -85,6 +85,7 @@ template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool
           class P = PrefillParams>
 __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
     constexpr bool SCORED = std::is_same<P, ScoredParams>::value;
+    constexpr bool PARTS = std::is_same<P, PrefixParams>::value;  // a partial from every split, also one
     static_assert(!S2 || !KH, "two stages per iteration: all waves on both");
     static_assert(!PS || (QB == 1 && !KH), "pair split: one block per wave, every wave on every stage");
     constexpr int NQW = KH ? NW / 2 : NW;  // waves with distinct query blocks
@@ -817,7 +818,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
         const long long row = (long long) qi * p.Hq + qh;
         const int d0 = 16 * DW * hd;  // the wave's first O^T dim
-        if (p.splits == 1) {
+        if (!PARTS && p.splits == 1) {
             float inv = 1.0f / lb[nb];
             if constexpr (SCORED) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
             uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
@@ -968,30 +969,33 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(P p) {
 }
 
 template <int D, class P = PrefillParams>
-void launch_prefill(const P &p, int stages, hipStream_t st) {
-    if (stages & 1) {
-        // Up to 64 rows of D = 512 are one tile, and a plan, of either height; the kernel then goes by
-        // the streams, which the plan does not know.  Of 499 such (chunk, split) pairs of K = V four
-        // waves took 0.95 of eight's time on average (0.92 .. 0.99 from the 10th to the 90th
-        // percentile); of 117 of separate K and V 1.05 (1.03 .. 1.12).
-        const bool shared = p.k == p.v, one = D == 512 && (long long) p.Sq * p.G <= 64;
-        const int nw = one ? (shared ? 4 : 8) : p.nw;
-        const dim3 grid(p.tiles * p.Hkv * p.splits), block(64 * nw);
-        if constexpr (D == 512) {
-            if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);
-            else if (nw == 4) hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, 4, P>), grid, block, 0, st, p);
-            else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, kWaves, P>), grid, block, 0, st, p);
-            else hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
-        }
-        else if constexpr (D == 128)
-            hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
-        else if (p.qb == 2)
-            hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true, false, kWaves, P>), grid, block, 0, st, p);
-        else if (p.kh)
-            hipLaunchKernelGGL((prefill_kernel<256, 1, true, false, false, false, kWaves, P>), grid, block, 0, st, p);
-        else
-            hipLaunchKernelGGL((prefill_kernel<256, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
+void launch_tiles(const P &p, hipStream_t st) {
+    // Up to 64 rows of D = 512 are one tile, and a plan, of either height; the kernel then goes by
+    // the streams, which the plan does not know.  Of 499 such (chunk, split) pairs of K = V four
+    // waves took 0.95 of eight's time on average (0.92 .. 0.99 from the 10th to the 90th
+    // percentile); of 117 of separate K and V 1.05 (1.03 .. 1.12).
+    const bool shared = p.k == p.v, one = D == 512 && (long long) p.Sq * p.G <= 64;
+    const int nw = one ? (shared ? 4 : 8) : p.nw;
+    const dim3 grid(p.tiles * p.Hkv * p.splits), block(64 * nw);
+    if constexpr (D == 512) {
+        if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);
+        else if (nw == 4) hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, 4, P>), grid, block, 0, st, p);
+        else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, kWaves, P>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
     }
+    else if constexpr (D == 128)
+        hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
+    else if (p.qb == 2)
+        hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true, false, kWaves, P>), grid, block, 0, st, p);
+    else if (p.kh)
+        hipLaunchKernelGGL((prefill_kernel<256, 1, true, false, false, false, kWaves, P>), grid, block, 0, st, p);
+    else
+        hipLaunchKernelGGL((prefill_kernel<256, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
+}
+
+template <int D, class P = PrefillParams>
+void launch_prefill(const P &p, int stages, hipStream_t st) {
+    if (stages & 1) launch_tiles<D, P>(p, st);
     if ((stages & 2) && p.splits > 1) {
         const long long waves = merge_waves(p, D);
         P mp = p;

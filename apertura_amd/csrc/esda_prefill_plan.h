@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
+#include <cstring>
 #include <type_traits>
 
 #include "esda_plan.h"
@@ -72,6 +73,10 @@ ESDA_HD void tile_keys(const ScoredParams &p, int tile, int QT, int &j0, int &j1
     if (seen > j1) j1 = seen < p.Sk ? (int) seen : p.Sk;
     if (j0 > j1) j0 = j1;  // rows whose window starts past the keys see none
 }
+
+// A decode batch's query rows over their shared prefix (esda_prefix.h): every row (sequence, group
+// head) sees every key, and every split leaves a partial, also a single one.
+struct PrefixParams : PrefillParams {};
 
 // A kernel form of one head dim: 16-query blocks per wave, stage halves or not, waves, and
 // its cost in us: `wg` and `row` per workgroup and query row of it (Q and first-stage loads,
@@ -154,10 +159,11 @@ constexpr int kMaxRounds = 3;  // split plans of more workgroups per CU only add
 
 // Validates a description and fills the kernel parameters' shape fields and plan.  Returns
 // what is wrong with it, or null.
-// A scored call's masks (p->prefix) are set before; its queries may see no key.
+// A scored call's masks (p->prefix) are set before.  Only a plain call's keys have to hold its
+// queries' positions.
 template <class P>
 const char *plan_prefill(const esda_prefill_desc *d, P *p) {
-    constexpr bool scored = std::is_same<P, ScoredParams>::value;
+    constexpr bool plain = std::is_same<P, PrefillParams>::value;
     if (!d) return "esda_prefill: null description";
     const int D = d->head_dim;
     if (D != 128 && D != 256 && D != 512)
@@ -168,7 +174,7 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
         return "esda_prefill: sizes, positions and window must be non-negative";
     if ((long long) d->q_pos0 + d->seq_q > INT_MAX || (long long) d->k_pos0 + d->seq_k > INT_MAX)
         return "esda_prefill: positions must stay below 2^31";
-    if (!scored && (d->k_pos0 > d->q_pos0 || (long long) d->k_pos0 + d->seq_k < (long long) d->q_pos0 + d->seq_q))
+    if (plain && (d->k_pos0 > d->q_pos0 || (long long) d->k_pos0 + d->seq_k < (long long) d->q_pos0 + d->seq_q))
         return "esda_prefill: the keys must hold every query's own position (k_pos0 <= q_pos0, "
                     "k_pos0 + seq_k >= q_pos0 + seq_q)";
     for (long long st : {d->q_head_stride, d->q_row_stride, d->kv_head_stride, d->out_row_stride, d->out_head_stride})
@@ -288,6 +294,32 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
     int a, b;
     tile_keys(*p, p->tiles / 4, 16 * p->qb * (p->kh ? p->nw / 2 : p->nw), a, b);
     p->part_gaps = part_bytes > kGapBytes && b - a <= (p->splits - 1) * (long long) p->kps;
+    return nullptr;
+}
+
+// plan_prefill of the calling thread's last description (of each kind of call), kept: a plan depends
+// on the description alone and takes up to 35 us of host time (half of them 0.4), and a call asks
+// for it twice, for the workspace and for the launch.  prefix: a scored call's.
+template <class P>
+const char *last_plan(const esda_prefill_desc *d, int prefix, P *p) {
+    static_assert(sizeof(esda_prefill_desc) == 8 * 4 + 5 * 8 + 8, "no padding: descriptions compare by their bytes");
+    struct Last {
+        esda_prefill_desc desc;
+        int prefix;
+        P plan;
+        bool set = false;
+    };
+    thread_local Last last;
+    if (!d || !last.set || prefix != last.prefix || std::memcmp(d, &last.desc, sizeof(*d)) != 0) {
+        P fresh{};
+        if constexpr (std::is_same<P, ScoredParams>::value) fresh.prefix = prefix;
+        if (const char *why = plan_prefill(d, &fresh)) return why;
+        last.desc = *d;
+        last.prefix = prefix;
+        last.plan = fresh;
+        last.set = true;
+    }
+    *p = last.plan;
     return nullptr;
 }
 

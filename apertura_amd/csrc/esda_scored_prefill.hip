@@ -30,9 +30,7 @@ const char *plan(const esda_prefill_desc *d, const esda_score *s, ScoredParams *
         return "esda_scored_prefill: softcap must be 0 or positive and finite";
     if (s->prefix < 0) return "esda_scored_prefill: prefix must not be negative";
     if ((long long) d->k_pos0 + d->seq_k > INT_MAX - 64) return "esda_scored_prefill: key positions must stay below 2^31 - 64";
-    *p = ScoredParams{};
-    p->prefix = s->prefix;
-    if (const char *why = plan_prefill(d, p)) return why;
+    if (const char *why = last_plan(d, s->prefix, p)) return why;
     if (s->softcap > 0.0f) {
         p->cap_in = (float) (2.0 * 1.4426950408889634 * d->scale / s->softcap);
         p->cap_out = (float) (1.4426950408889634 * s->softcap);

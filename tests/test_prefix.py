@@ -1,0 +1,84 @@
+"""The decode step over a shared prefix on the host: its workspace and the calls esda_prefix_decode
+refuses before it touches the device."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from apertura_amd import _lib
+from apertura_amd.decode import DecodeStep, workspace_bytes
+from apertura_amd.prefix import PrefixCall, PrefixStep, prefix_workspace_bytes
+
+FAKE = 0x10000000  # never dereferenced: validation fails first
+
+
+def _step(prefix_len=100, prefix_head_stride=None, split_keys=0, **kw):
+    base = dict(batch=4, num_q_heads=8, num_kv_heads=2, head_dim=128, cap=64)
+    base.update(kw)
+    return PrefixStep(DecodeStep(**base), prefix_len, prefix_head_stride, split_keys)
+
+
+def test_workspace_holds_the_own_step_and_every_prefix_split():
+    up = lambda n: (n + 255) // 256 * 256
+    own = workspace_bytes(_step().own)
+    for keys, splits in ((32, 4), (64, 2), (128, 1)):
+        parts = splits * 4 * 8
+        assert prefix_workspace_bytes(_step(split_keys=keys)) == up(own) + up(parts * 8) + parts * 128 * 4
+
+
+@pytest.mark.parametrize("kw", [
+    dict(prefix_len=0), dict(prefix_len=-1), dict(prefix_head_stride=99 * 128), dict(prefix_head_stride=100 * 128 + 4),
+    dict(split_keys=16), dict(split_keys=-32), dict(window=16), dict(ring=True, window=64), dict(head_dim=64),
+    dict(num_q_heads=9), dict(num_q_heads=34), dict(batch=0), dict(batch=257), dict(cap=0), dict(scale=0.0),
+    dict(scale=math.nan), dict(split_rows=8),
+])
+def test_bad_descriptions_are_refused(kw):
+    with pytest.raises(_lib.EsdaError) as ei:
+        prefix_workspace_bytes(_step(**kw))
+    assert ei.value.code == 1
+
+
+def _call(step=None, prefix_k=FAKE, prefix_v=FAKE + (1 << 24), row_base=None, ws=FAKE, nbytes=None, q=FAKE,
+          k_new=FAKE, v_new=FAKE, k_cache=FAKE, v_cache=FAKE + (2 << 24), pos=FAKE, out=FAKE):
+    step = step or _step()
+    d = step.desc()
+    a = _lib.PrefixArgs(_lib.DecodeArgs(q, k_new, v_new, k_cache, v_cache, pos, row_base, out, ws,
+                                        prefix_workspace_bytes(step) if nbytes is None else nbytes), prefix_k, prefix_v)
+    return _lib.lib().esda_prefix_decode(ctypes.byref(d), ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(prefix_k=None), dict(prefix_v=None), dict(prefix_k=FAKE + 8), dict(prefix_v=FAKE), dict(row_base=FAKE),
+    dict(q=None), dict(k_new=None), dict(v_new=None), dict(k_cache=None), dict(v_cache=FAKE), dict(pos=None),
+    dict(out=FAKE + 4), dict(step=_step(kv_shared=True)), dict(step=_step(kv_shared=True), v_cache=FAKE),
+])
+def test_bad_arguments_are_refused(kw):
+    assert _call(**kw) == 1
+
+
+def test_the_workspace_is_needed():
+    assert _call(ws=None) == 4
+    assert _call(ws=FAKE + 8) == 4
+    assert _call(nbytes=prefix_workspace_bytes(_step()) - 1) == 4
+    assert _lib.lib().esda_prefix_decode(None, None, None) == 1
+    assert _lib.lib().esda_prefix_decode(ctypes.byref(_step().desc()), None, None) == 1
+
+
+def test_front_end_refuses_wrong_tensors():
+    bf = torch.bfloat16
+    pk, c = torch.zeros(2, 100, 128, dtype=bf), torch.zeros(4, 2, 64, 128, dtype=bf)
+    q, n, pos = torch.zeros(4, 8, 128, dtype=bf), torch.zeros(4, 2, 128, dtype=bf), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        PrefixStep.for_caches(pk[:, :, ::2], c, 8)
+    with pytest.raises(ValueError):
+        PrefixStep.for_caches(pk[:1], c, 8)
+    step = PrefixStep.for_caches(pk, c, 8)
+    assert step.prefix_len == 100 and step.desc().prefix_head_stride == 100 * 128
+    for args in ((q, n, n, pk, pk.clone(), c, c.clone(), pos),             # not on a GPU
+                 (q[:3], n, n, pk, pk.clone(), c, c.clone(), pos),
+                 (q, n[:, :1], n, pk, pk.clone(), c, c.clone(), pos),
+                 (q, n, n, pk[:, :99], pk.clone(), c, c.clone(), pos),
+                 (q, n, n, pk, pk.clone(), c, c.clone(), pos.long())):
+        with pytest.raises(ValueError):
+            PrefixCall(step, *args)
