@@ -74,17 +74,17 @@ struct PRing {
 // this stage's P^T.  Used by the K = V kernel at D = 512 (p512gs 436 -> 422 us on one box);
 // with separate K and V -- one stage per barrier -- it measured 1-3% slower and is not used.
 //
-// P = ScoredParams (esda_scored.h): scores s become cap_out tanh(.) and lose slope * distance, and
-// three more masks apply.  A prefix opens keys ahead of a query.  Document ids (equal, not
-// negative) close the others: each wave reads the ids of 64 stages at a time and keeps which of
-// them hold an id of the tile's range (the others are never loaded) and which hold nothing but
-// the tile's one id (those need no mask); the ids of the stages loaded come with their keys by
-// DMA.  A row that sees nothing gives 0.  In masked stages a value that is not finite reaches
-// only the rows that see its key: 0 x inf in the product would be NaN in every row of the tile.
+// P = ScoredParams (esda_scored.h): scores are capped and lose slope * distance, a prefix opens
+// keys ahead of a query, a row that sees nothing gives 0, and a value that is not finite reaches
+// only the rows that see its key.  P = DocParams: document ids (equal, not negative) close the
+// other keys, too.  The waves first read the range of ids of every 32-key stage: stages that hold
+// no id of the tile's range are never loaded, those that hold nothing but the tile's one id need
+// no mask, and the ids of the others come with their keys by DMA.
 template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves,
           class P = PrefillParams>
 __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
-    constexpr bool SCORED = std::is_same<P, ScoredParams>::value;
+    constexpr bool DOCS = std::is_same<P, DocParams>::value;
+    constexpr bool SCORED = DOCS || std::is_same<P, ScoredParams>::value;
     constexpr bool PARTS = std::is_same<P, PrefixParams>::value;  // a partial from every split, also one
     static_assert(!S2 || !KH, "two stages per iteration: all waves on both");
     static_assert(!PS || (QB == 1 && !KH), "pair split: one block per wave, every wave on every stage");
@@ -103,9 +103,20 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
     constexpr int XP = 64 * 16 + 64 * 4;
     constexpr int XPAR = NW * XP + NW * 4;
     __shared__ __attribute__((aligned(16))) unsigned char xch[PS ? 2 * XPAR + NW * 16 * 4 : 16];
-    __shared__ __attribute__((aligned(16))) int dids[SCORED ? NSL : 1][kStageKeys];  // the slots' document ids
+    __shared__ __attribute__((aligned(16))) int dids[DOCS ? NSL : 1][kStageKeys];  // the slots' document ids
+    // of each 64 stages, which to compute and which of them without a mask; those past the last
+    // of kDocWindows (131,072 keys of a split) are computed with one
+    constexpr int kDocWindows = 64;
+    __shared__ unsigned char odd_row[SCORED ? QT : 1];  // tile rows whose O^T is not finite
+    __shared__ int any_odd;
+    // the tile rows' positions, slopes (log2 units) and documents, read where a stage needs them:
+    // held in registers they cost the stages reloads of spilled ones, whose waits wait for the DMAs
+    __shared__ int row_pos[SCORED ? QT : 1], row_doc[DOCS ? QT : 1];
+    __shared__ float row_slope[SCORED ? QT : 1];
+    __shared__ unsigned long long live_of[DOCS ? kDocWindows : 1], pure_of[DOCS ? kDocWindows : 1];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // (scored: said to be scalar, which frees the registers that the score's form needs)
+    const int lane = threadIdx.x & 63, wave = SCORED ? uniform(threadIdx.x >> 6) : threadIdx.x >> 6;
     const int li = lane & 15, lg = lane >> 4;
     // Query-block wave and stage parity (both constant for the plain kernel, whose code
     // does not change: a wave-dependent parity there measured 3% slower).
@@ -165,19 +176,13 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
     // Q^T B operands: lane (li, lg) holds dims 32ks + 8lg .. +8 of its query row.
     bf16x8 qreg[QB][KS];
     int qabs[QB];  // absolute position of this lane's query in block qb
-    float slope[SCORED ? QB : 1];  // its bias per position of distance (log2 units)
-    int qdoc[SCORED ? QB : 1];     // its document
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const long long gr = qrow(qb);
         const unsigned qi = position_of(gr, p.G);
         const uint16_t *qr = p.q + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.q_hs +
                              (size_t) qi * p.q_rs + lg * 8;
-        qabs[qb] = p.q_pos0 + (int) qi;
-        if constexpr (SCORED) {
-            slope[qb] = p.slopes ? p.slopes[kvh * p.G + (int) ((unsigned) gr - qi * p.G)] * kLog2e : 0.0f;
-            qdoc[qb] = p.q_doc ? p.q_doc[qi] : 0;
-        }
+        if constexpr (!SCORED) qabs[qb] = p.q_pos0 + (int) qi;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 w = qvalid(qb) ? *reinterpret_cast<const u32x4 *>(qr + ks * 32) : u32x4{0u, 0u, 0u, 0u};
@@ -227,6 +232,18 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         }
     };
 
+    if constexpr (SCORED) {
+        for (int r = threadIdx.x; r < QT; r += 64 * NW) {
+            const long long gr = min((long long) tile * QT + r, nq - 1);
+            const unsigned qi = position_of(gr, p.G);
+            odd_row[r] = 0;
+            row_pos[r] = p.q_pos0 + (int) qi;
+            row_slope[r] = p.slopes ? p.slopes[kvh * p.G + (int) ((unsigned) gr - qi * p.G)] * kLog2e : 0.0f;
+            if constexpr (DOCS) row_doc[r] = p.q_doc[qi];
+        }
+        if (threadIdx.x == 0) any_odd = 0;
+        lds_barrier();
+    }
     const int qk_off = R::off(li) + lg * 16;                    // + 64 ks (+ HB: keys 16..31)
     const int tr_off = R::off(4 * lg + li / 4) + (li % 4) * 8;  // + 32 dt (+ HB)
     // V^T of dims 16 dt .. of a stage's slot (PS: from its half), the PV A operand
@@ -286,107 +303,85 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         return sc;
     };
 
-    // Scored: the stages to compute, in order.  cur[i] / ahead[i] are the key stages of this and of
-    // the next iteration (nst past the last), and whether their documents need no mask.  The i-th
-    // stage computed takes ring slot i % NSL.
+    // Documents: the stages to compute, in order.  cur[i] / ahead[i] are the key stages of this and
+    // of the next iteration (nst past the last), and whether they need no mask for their documents.
+    // The i-th stage computed takes ring slot i % NSL.
     struct Stage {
         int st;
         bool pure;
     };
     Stage cur[SPI], ahead[SPI];
-    int window = -1;                             // the 64 stages that live / pure describe
-    unsigned long long live = 0ull, pure = 0ull;
-    int qlo = 0, qhi = 0;                        // the tile's documents
-    bool one_doc = true;                         // all of its rows in one
-    auto load_window = [&](int w) {
-        if constexpr (SCORED) {
-            window = w;
-            live = pure = 0ull;
-#pragma unroll 1
-            for (int u = 0; u < 8; ++u) {  // 8 stages at a time, 8 lanes of 4 keys each
-                const long long j = (long long) j0 + w * 2048LL + u * 256 + 4 * lane;
-                int lo = INT_MAX, hi = -1;
+    // to[0 .. SPI-1]: the first SPI stages to compute from stage s on
+    auto next_stages = [&](int s, auto &to) {
+        if constexpr (DOCS) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {  // past the last key: its id again
+            for (int i = 0; i < SPI; ++i) {
+                to[i] = {nst, true};
+                while (s < nst) {
+                    const int w = s >> 6;
+                    const unsigned long long m = (w < kDocWindows ? live_of[w] : ~0ull) >> (s & 63);
+                    const unsigned lo = uniform((int) (unsigned) m), hi = uniform((int) (unsigned) (m >> 32));
+                    const unsigned long long um = (unsigned long long) hi << 32 | lo;
+                    if (um == 0ull) {
+                        s = (s | 63) + 1;
+                        continue;
+                    }
+                    s += __builtin_ctzll(um);
+                    if (s < nst) to[i] = {s, w < kDocWindows && uniform((int) (pure_of[w] >> (s & 63)) & 1) != 0};
+                    ++s;
+                    break;
+                }
+            }
+        }
+    };
+    if constexpr (DOCS) {
+        // lowest and highest document of the tile's positions; negative ids are nobody's
+        int qlo = INT_MAX, qhi = -1;
+        bool one_doc = true;  // all of its rows in one
+        for (int i = qa_min - p.q_pos0 + lane; i <= qa_max - p.q_pos0; i += 64) {
+            const int d = p.q_doc[i];
+            if (d < 0) one_doc = false;
+            else {
+                qlo = min(qlo, d);
+                qhi = max(qhi, d);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            qlo = min(qlo, __shfl_xor(qlo, o));
+            qhi = max(qhi, __shfl_xor(qhi, o));
+        }
+        one_doc = __builtin_amdgcn_ballot_w64(!one_doc) == 0ull && qlo == qhi;
+        // lane l of a window's wave: the ids of its stage l (past the last key: its id again)
+        for (int w = wave; w < kDocWindows && 64 * w < nst; w += NW) {
+            int lo = INT_MAX, hi = -1;
+            const long long j = (long long) j0 + 2048LL * w + 32 * lane;
+            if (64 * w + lane < nst) {
+#pragma unroll
+                for (int e = 0; e < kStageKeys; ++e) {
                     const int d = p.k_doc[min(j + e, (long long) p.Sk - 1)];
                     lo = min(lo, d);
                     hi = max(hi, d);
                 }
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) {
-                    lo = min(lo, __shfl_xor(lo, o));
-                    hi = max(hi, __shfl_xor(hi, o));
-                }
-                // bit 8i of the ballot (lane 8i: stage i of the eight) -> bit i
-                auto stages = [&](bool b) {
-                    const unsigned long long x = __builtin_amdgcn_ballot_w64(b) & 0x0101010101010101ull;
-                    return (x * 0x0102040810204080ull) >> 56 << (8 * u);
-                };
-                live |= stages(hi >= qlo && lo <= qhi);
-                pure |= stages(one_doc && lo == qlo && hi == qhi);
+            }
+            const unsigned long long a = __builtin_amdgcn_ballot_w64(hi >= qlo && lo <= qhi);
+            const unsigned long long b = __builtin_amdgcn_ballot_w64(one_doc && lo == qlo && hi == qhi);
+            if (lane == 0) {
+                live_of[w] = a;
+                pure_of[w] = b;
             }
         }
-    };
-    // to[0 .. SPI-1]: the first SPI stages to compute from stage s on
-    auto next_stages = [&](int s, auto &to) {
-        if constexpr (SCORED) {
-            if (!p.k_doc) {
-#pragma unroll
-                for (int i = 0; i < SPI; ++i) to[i] = {min(s + i, nst), true};
-                return;
-            }
-#pragma unroll
-            for (int i = 0; i < SPI; ++i) to[i] = {nst, true};
-            int n = 0;
-#pragma unroll 1
-            while (s < nst && n < SPI) {
-                if ((s >> 6) != window) load_window(s >> 6);
-                const unsigned long long m = live >> (s & 63);
-                if (m == 0ull) {
-                    s = (s | 63) + 1;
-                    continue;
-                }
-                s += __builtin_ctzll(m);
-                if (s >= nst) break;
-                to[n == 0 ? 0 : SPI - 1] = {s, ((pure >> (s & 63)) & 1) != 0};
-                ++n;
-                ++s;
-            }
-        }
-    };
-    if constexpr (SCORED) {
-        if (p.k_doc) {
-            // lowest and highest document of the tile's positions; negative ids are nobody's
-            qlo = INT_MAX;
-            qhi = -1;
-            const int i0 = qa_min - p.q_pos0, i1 = qa_max - p.q_pos0;
-            for (int i = i0 + lane; i <= i1; i += 64) {
-                const int d = p.q_doc[i];
-                if (d < 0) one_doc = false;
-                else {
-                    qlo = min(qlo, d);
-                    qhi = max(qhi, d);
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                qlo = min(qlo, __shfl_xor(qlo, o));
-                qhi = max(qhi, __shfl_xor(qhi, o));
-            }
-            qlo = __builtin_amdgcn_readfirstlane(qlo);
-            qhi = __builtin_amdgcn_readfirstlane(qhi);
-            one_doc = __builtin_amdgcn_ballot_w64(!one_doc) == 0ull && qlo == qhi;
-        }
+        lds_barrier();
         next_stages(0, cur);
     }
     auto issue_docs = [&](int st, int s) {
-        if constexpr (SCORED) {
-            if (p.k_doc && wave == 0 && lane < kStageKeys)
+        if constexpr (DOCS) {
+            if (wave == 0 && lane < kStageKeys)
                 lds_dma4(p.k_doc + min(j0 + st * kStageKeys + lane, j1 - 1), lds_addr(dids[s & (NSL - 1)]));
         }
     };
 
-    if constexpr (!SCORED) {
+    if constexpr (!DOCS) {
         issue(kvb, 0, kslot(0));  // nst >= 1 here
         if (!SH) issue(vvb, 0, vslot(0));
         if ((KH || S2) && nst > 1) {
@@ -404,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
     }
 
     auto shift = [&]() {
-        if constexpr (SCORED) {
+        if constexpr (DOCS) {
 #pragma unroll
             for (int i = 0; i < SPI; ++i) cur[i] = ahead[i];
         }
@@ -415,27 +410,10 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                    (p.window == 0 || ka_first > qa_max - p.window) && pure;
         else return false;
     };
-    // Scored: whether a masked stage holds a value that is not finite (V^T . 0 is NaN then; rare).
-    auto odd_values = [&](int s, int st, bool pure) {
-        const int jb = j0 + st * kStageKeys, ka_first = p.k_pos0 + jb, ka_last = ka_first + kStageKeys - 1;
-        if (st >= nst || scored_full(jb, ka_first, ka_last, pure)) return false;
-        const unsigned char *const vbh = vslot(s) + 32 * DW * hd;
-        f32x4 chk = {0.0f, 0.0f, 0.0f, 0.0f};
-        const bf16x8 zero = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-#pragma unroll
-        for (int dt = 0; dt < DW; ++dt) {
-            chk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vtile_of(vbh, dt), zero, chk, 0, 0, 0);
-            if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-        const float c = chk[0] + chk[1] + chk[2] + chk[3];
-        return __builtin_amdgcn_ballot_w64(c != c) != 0ull;
-    };
-
-    bool odd = false;  // a masked stage held such a value
-    for (int s0 = 0; SCORED ? cur[0].st < nst : s0 < nst; s0 += SPI, shift()) {
+    for (int s0 = 0; DOCS ? cur[0].st < nst : s0 < nst; s0 += SPI, shift()) {
         // the key stage of the i-th stage from s0 on
         auto at = [&](int i) -> int {
-            if constexpr (!SCORED) return s0 + i;
+            if constexpr (!DOCS) return s0 + i;
             else if (i < SPI) return i == 0 ? cur[0].st : cur[SPI - 1].st;
             else return i == SPI ? ahead[0].st : ahead[SPI - 1].st;
         };
@@ -443,15 +421,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         // the other waves') and every wave is done with the previous iteration
         ESDA_WAIT_VM(0);
         lds_barrier();
-        if constexpr (SCORED) {
-            next_stages(cur[SPI - 1].st + 1, ahead);
-            if constexpr (KH) {
-                odd |= odd_values(s0 + kh, kh ? cur[1].st : cur[0].st, kh ? cur[1].pure : cur[0].pure);
-            } else {
-                odd |= odd_values(s0, cur[0].st, cur[0].pure);
-                if constexpr (S2) odd |= odd_values(s0 + 1, cur[1].st, cur[1].pure);
-            }
-        }
+        if constexpr (DOCS) next_stages(cur[SPI - 1].st + 1, ahead);
         // The next iteration's DMAs, spread over this iteration so that the workgroup's loads
         // do not all queue at the barrier (each slot is free once the barrier has passed):
         //  - separate K and V (plain, S2): K of the next stage at the barrier, its V after
@@ -510,23 +480,37 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                                        (p.window == 0 || ka_first > qa_max - p.window);
         if constexpr (SCORED) {
             if (p.cap_out != 0.0f) {
-                // tanh(x) = 1 - 2 / (1 + e^2x), off by 2^-23 or so; cap_out = cap log2 e is the score's unit
-                c2 = p.cap_out;
+                // tanh(x) = 1 - 2 / (1 + e^2x), to 2^-22 or so; the softmax drops the 1, so the capped score
+                // is -1 / (1 + e^2x) in units of 2 cap log2 e
+                c2 = 2.0f * p.cap_out;
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        sv[qb][e] = __builtin_fmaf(
-                            -2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sv[qb][e] * p.cap_in)), 1.0f);
+                        sv[qb][e] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(sv[qb][e] * p.cap_in));
             }
             if (p.slopes) {
+                // Keys at or before their queries: the bias is linear, base + slope (key's place in the
+                // stage).  (Keys ahead of a query are masked unless they lie in the prefix.)
+                if (ka_last <= qa_min || p.prefix <= ka_first) {
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb) {
-                    const int d0 = qabs[qb] - ka_first - 4 * lg;
+                    for (int qb = 0; qb < QB; ++qb) {
+                        const int r = wq * 16 * QB + qb * 16 + li;
+                        const float slope = row_slope[r], base = -slope * (float) (row_pos[r] - ka_first - 4 * lg);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float dist = (float) (d0 - (16 * (e / 4) + e % 4));
-                        sv[qb][e] = __builtin_fmaf(sv[qb][e], c2, -slope[qb] * __builtin_fabsf(dist));
+                        for (int e = 0; e < 8; ++e)
+                            sv[qb][e] = __builtin_fmaf(sv[qb][e], c2, __builtin_fmaf(slope, (float) (16 * (e / 4) + e % 4), base));
+                    }
+                } else {
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) {
+                        const int r = wq * 16 * QB + qb * 16 + li, d0 = row_pos[r] - ka_first - 4 * lg;
+                        const float slope = row_slope[r];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float dist = (float) (d0 - (16 * (e / 4) + e % 4));
+                            sv[qb][e] = __builtin_fmaf(sv[qb][e], c2, -slope * __builtin_fabsf(dist));
+                        }
                     }
                 }
                 c2 = 1.0f;
@@ -535,7 +519,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         if (!full) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
-                const int qa = qabs[qb];
+                const int qa = SCORED ? row_pos[SCORED ? wq * 16 * QB + qb * 16 + li : 0] : qabs[qb];
                 const int lo = p.window > 0 ? qa - p.window : INT_MIN;  // visible: lo < ka <= qa
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -552,7 +536,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
             }
         }
 
-        if constexpr (SCORED) {
+        if constexpr (DOCS) {
             if (!pure) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -561,7 +545,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if ((d[r] != qdoc[qb]) | (d[r] < 0)) sv[qb][4 * h + r] = -INFINITY;
+                            if ((d[r] != row_doc[wq * 16 * QB + qb * 16 + li]) | (d[r] < 0)) sv[qb][4 * h + r] = -INFINITY;
                 }
             }
         }
@@ -659,44 +643,142 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         }
         };
         if constexpr (S2) {
-            stage(s0, at(0), !SCORED || cur[0].pure, after_first_qk);
+            stage(s0, at(0), !DOCS || cur[0].pure, after_first_qk);
             issue_second();
-            if (at(1) < nst) stage(s0 + 1, at(1), !SCORED || cur[SPI - 1].pure, [] {});
+            if (at(1) < nst) stage(s0 + 1, at(1), !DOCS || cur[SPI - 1].pure, [] {});
         } else {
             const int s = s0 + kh, st = at(kh);  // this wave group's stage
             if (KH && st >= nst) continue;  // an odd stage count: the odd group's last iteration is empty
-            stage(s, st, !SCORED || (kh ? cur[SPI - 1].pure : cur[0].pure), after_first_qk);
+            stage(s, st, !DOCS || (kh ? cur[SPI - 1].pure : cur[0].pure), after_first_qk);
         }
     }
 
+    if constexpr (KH) {
+        // The odd-stage wave of each query block hands its (m, l, O^T) to the even-stage
+        // wave through the ring's LDS (no DMA is outstanding and, after the barrier, no wave
+        // reads the ring): lane-major, so each store and load of a wave is one contiguous
+        // 1 KB.  A group that saw no key of a row holds m = -inf, l = 0 and adds nothing.
+        constexpr int XA = QB * DT * 64 * 16;  // O^T bytes per wave
+        constexpr int XW = XA + QB * 64 * 8;   // + (m, l)
+        static_assert(NQW * XW <= R::BYTES, "the hand-over must fit the ring");
+        unsigned char *xb = ring + wq * XW;
+        lds_barrier();
+        if (kh) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    *reinterpret_cast<f32x4 *>(xb + ((qb * DT + dt) * 64 + lane) * 16) = acc[qb][dt];
+                *reinterpret_cast<f32x2 *>(xb + XA + (qb * 64 + lane) * 8) = f32x2{m[qb], l[qb]};
+            }
+        }
+        lds_barrier();
+        if (!SCORED && kh) return;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            if (SCORED && kh) break;
+            const f32x2 mlb = *reinterpret_cast<const f32x2 *>(xb + XA + (qb * 64 + lane) * 8);
+            const float M = fmaxf(m[qb], mlb[0]);
+            const float wa = m[qb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[qb] - M);
+            const float wb = mlb[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mlb[0] - M);
+            l[qb] = l[qb] * wa + mlb[1] * wb;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                acc[qb][dt] = acc[qb][dt] * wa +
+                              *reinterpret_cast<const f32x4 *>(xb + ((qb * DT + dt) * 64 + lane) * 16) * wb;
+            m[qb] = M;
+        }
+    }
+
+    // Row totals over the four lane groups; then the output (one split) or the partial.
+    float lb[NB];  // row sums of the wave's O^T blocks
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        l[qb] += __shfl_xor(l[qb], 16);
+        l[qb] += __shfl_xor(l[qb], 32);
+        lb[qb] = l[qb];
+    }
+    if constexpr (PS) {  // the partner's row sums, through LDS past every wave's last stage
+        float *xl = reinterpret_cast<float *>(xch + 2 * XPAR);
+        if (lg == 0) xl[wave * 16 + li] = l[0];
+        lds_barrier();
+        lb[1] = xl[(wave ^ 1) * 16 + li];
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        // the block's first tile row (PS: the wave's own block, then its partner's)
+        const int br = PS ? (nb == 0 ? wave : wave ^ 1) * 16 : wq * 16 * QB + nb * 16;
+        const long long gr0 = (long long) tile * QT + br + li;
+        if (gr0 >= nq || (SCORED && KH && kh)) continue;
+        if constexpr (SCORED) {
+            float c = 0.0f;  // NaN where a value is not finite
+#pragma unroll
+            for (int dt = 0; dt < DW; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c = __builtin_fmaf(acc[nb][dt][r], 0.0f, c);
+            if (c != c) {
+                odd_row[br + li] = 1;
+                any_odd = 1;
+            }
+        }
+        const long long gr = gr0;
+        const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
+        const long long row = (long long) qi * p.Hq + qh;
+        const int d0 = 16 * DW * hd;  // the wave's first O^T dim
+        if (!PARTS && p.splits == 1) {
+            float inv = 1.0f / lb[nb];
+            if constexpr (SCORED) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
+            uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
+#pragma unroll
+            for (int dt = 0; dt < DW; ++dt) {
+                const f32x4 v4 = acc[nb][dt] * inv;
+                bf16x4 b4 = {(__bf16) v4[0], (__bf16) v4[1], (__bf16) v4[2], (__bf16) v4[3]};
+                *reinterpret_cast<bf16x4 *>(o + 16 * dt) = b4;
+            }
+        } else {
+            float *pa = p.part_acc + ((long long) split * nrows + row) * D + d0 + 4 * lg;
+            if (p.part_nt) {
+                // (the barriers keep the two branches' stores from being merged into plain ones)
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int dt = 0; dt < DW; ++dt) __builtin_nontemporal_store(acc[nb][dt], reinterpret_cast<f32x4 *>(pa + 16 * dt));
+                asm volatile("" ::: "memory");
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4 *>(pa + 16 * dt) = acc[nb][dt];
+            }
+            if (lg == 0 && nb < QB)  // (m, l) from the block's owner
+                *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{m[nb < QB ? nb : 0], l[nb < QB ? nb : 0]};
+        }
+    }
     if constexpr (SCORED) {
-        // Rare: the tile again, row by row, without the keys a row does not see.  The lanes take 64
-        // keys for the scores, then the row's dims for the product.  (In the stage itself a second
-        // form of the product cost every stage: O^T no longer stayed in registers.)
-        int *const any_odd = reinterpret_cast<int *>(&dids[0][0]);
+        // Rare: rows whose O^T is not finite.  A value that is not was seen, or met a weight of 0 (0 x inf
+        // is NaN): those rows again, over the keys they see only.  The lanes take 64 keys for the scores,
+        // then the row's dims for the product.  (Testing the values of every masked stage took 5% to 70%
+        // of a chunk's time, a second form of the product in the stage O^T's registers.)
+        ESDA_WAIT_VM(0);  // the rows as written above, before they are written again
         lds_barrier();
-        if (threadIdx.x == 0) *any_odd = 0;
-        lds_barrier();
-        if (odd && lane == 0) *any_odd = 1;
-        lds_barrier();
-        if (__builtin_expect(*any_odd != 0, 0)) {
+        if (__builtin_expect(any_odd != 0, 0)) {
             constexpr int DPL = D / 64;
             typedef uint16_t piece __attribute__((ext_vector_type(DPL)));
             for (int r = wave; r < QT; r += NW) {
+                if (!odd_row[r]) continue;
                 const long long gr = (long long) tile * QT + r;
-                if (gr >= nq) break;
                 const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
                 const uint16_t *const qr = p.q + (size_t) qh * p.q_hs + (size_t) qi * p.q_rs;
                 const int qa = p.q_pos0 + qi, lo = p.window > 0 ? qa - p.window : INT_MIN;
                 const float sl = p.slopes ? p.slopes[qh] * kLog2e : 0.0f;
-                const int doc = p.k_doc ? p.q_doc[qi] : 0;
+                int doc = 0;
+                if constexpr (DOCS) doc = p.q_doc[qi];
                 float mr = -INFINITY, lr = 0.0f, o[DPL];
 #pragma unroll
                 for (int e = 0; e < DPL; ++e) o[e] = 0.0f;
                 for (int jb = j0; jb < j1; jb += 64) {
                     const int j = jb + lane, ka = p.k_pos0 + j;
                     bool seen = j < j1 && ka <= max(qa, p.prefix - 1) && ka > lo;
-                    if (p.k_doc && seen) seen = doc >= 0 && p.k_doc[j] == doc;
+                    if constexpr (DOCS) {
+                        if (seen) seen = doc >= 0 && p.k_doc[j] == doc;
+                    }
                     unsigned long long todo = __builtin_amdgcn_ballot_w64(seen);
                     if (todo == 0ull) continue;
                     float x = 0.0f;
@@ -712,9 +794,8 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                                 x = __builtin_fmaf(bf16_hi(qv[e]), bf16_hi(kv[e]), x);
                             }
                         }
-                        x = p.cap_out != 0.0f
-                                ? p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p.cap_in)), 1.0f)
-                                : x * p.scale_log2e;
+                        x = p.cap_out != 0.0f ? 2.0f * p.cap_out * __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * p.cap_in))
+                                              : x * p.scale_log2e;
                         x = __builtin_fmaf(-sl, __builtin_fabsf((float) (qa - ka)), x);
                     }
                     float top = seen ? x : -INFINITY;
@@ -754,94 +835,6 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                         *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{mr, lr};
                 }
             }
-            return;
-        }
-    }
-
-    if constexpr (KH) {
-        // The odd-stage wave of each query block hands its (m, l, O^T) to the even-stage
-        // wave through the ring's LDS (no DMA is outstanding and, after the barrier, no wave
-        // reads the ring): lane-major, so each store and load of a wave is one contiguous
-        // 1 KB.  A group that saw no key of a row holds m = -inf, l = 0 and adds nothing.
-        constexpr int XA = QB * DT * 64 * 16;  // O^T bytes per wave
-        constexpr int XW = XA + QB * 64 * 8;   // + (m, l)
-        static_assert(NQW * XW <= R::BYTES, "the hand-over must fit the ring");
-        unsigned char *xb = ring + wq * XW;
-        lds_barrier();
-        if (kh) {
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    *reinterpret_cast<f32x4 *>(xb + ((qb * DT + dt) * 64 + lane) * 16) = acc[qb][dt];
-                *reinterpret_cast<f32x2 *>(xb + XA + (qb * 64 + lane) * 8) = f32x2{m[qb], l[qb]};
-            }
-        }
-        lds_barrier();
-        if (kh) return;
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            const f32x2 mlb = *reinterpret_cast<const f32x2 *>(xb + XA + (qb * 64 + lane) * 8);
-            const float M = fmaxf(m[qb], mlb[0]);
-            const float wa = m[qb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[qb] - M);
-            const float wb = mlb[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mlb[0] - M);
-            l[qb] = l[qb] * wa + mlb[1] * wb;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                acc[qb][dt] = acc[qb][dt] * wa +
-                              *reinterpret_cast<const f32x4 *>(xb + ((qb * DT + dt) * 64 + lane) * 16) * wb;
-            m[qb] = M;
-        }
-    }
-
-    // Row totals over the four lane groups; then the output (one split) or the partial.
-    float lb[NB];  // row sums of the wave's O^T blocks
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        l[qb] += __shfl_xor(l[qb], 16);
-        l[qb] += __shfl_xor(l[qb], 32);
-        lb[qb] = l[qb];
-    }
-    if constexpr (PS) {  // the partner's row sums, through LDS past every wave's last stage
-        float *xl = reinterpret_cast<float *>(xch + 2 * XPAR);
-        if (lg == 0) xl[wave * 16 + li] = l[0];
-        lds_barrier();
-        lb[1] = xl[(wave ^ 1) * 16 + li];
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        // the block's first tile row (PS: the wave's own block, then its partner's)
-        const int br = PS ? (nb == 0 ? wave : wave ^ 1) * 16 : wq * 16 * QB + nb * 16;
-        const long long gr0 = (long long) tile * QT + br + li;
-        if (gr0 >= nq) continue;
-        const long long gr = gr0;
-        const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
-        const long long row = (long long) qi * p.Hq + qh;
-        const int d0 = 16 * DW * hd;  // the wave's first O^T dim
-        if (!PARTS && p.splits == 1) {
-            float inv = 1.0f / lb[nb];
-            if constexpr (SCORED) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
-            uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
-#pragma unroll
-            for (int dt = 0; dt < DW; ++dt) {
-                const f32x4 v4 = acc[nb][dt] * inv;
-                bf16x4 b4 = {(__bf16) v4[0], (__bf16) v4[1], (__bf16) v4[2], (__bf16) v4[3]};
-                *reinterpret_cast<bf16x4 *>(o + 16 * dt) = b4;
-            }
-        } else {
-            float *pa = p.part_acc + ((long long) split * nrows + row) * D + d0 + 4 * lg;
-            if (p.part_nt) {
-                // (the barriers keep the two branches' stores from being merged into plain ones)
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int dt = 0; dt < DW; ++dt) __builtin_nontemporal_store(acc[nb][dt], reinterpret_cast<f32x4 *>(pa + 16 * dt));
-                asm volatile("" ::: "memory");
-            } else {
-#pragma unroll
-                for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4 *>(pa + 16 * dt) = acc[nb][dt];
-            }
-            if (lg == 0 && nb < QB)  // (m, l) from the block's owner
-                *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{m[nb < QB ? nb : 0], l[nb < QB ? nb : 0]};
         }
     }
 }
@@ -998,16 +991,17 @@ void launch_prefill(const P &p, int stages, hipStream_t st) {
     if (stages & 1) launch_tiles<D, P>(p, st);
     if ((stages & 2) && p.splits > 1) {
         const long long waves = merge_waves(p, D);
-        P mp = p;
+        using M = std::conditional_t<std::is_base_of<ScoredParams, P>::value, ScoredParams, P>;
+        M mp = p;
         for (mp.merge_wave0 = 0; mp.merge_wave0 < waves; mp.merge_wave0 += kMergeLaunchWaves) {
             const long long n = std::min(kMergeLaunchWaves, waves - mp.merge_wave0);
             const int wpb = D == 128 && p.splits <= 8 ? 2 : 4;  // waves per block: the kernel's 4 / RPW
             const dim3 grid((unsigned) ((n + wpb - 1) / wpb)), block(64 * wpb);
-            if (p.part_gaps && p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, true, P>), grid, block, 0, st, mp);
-            else if (p.part_gaps && p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, true, P>), grid, block, 0, st, mp);
-            else if (p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, false, P>), grid, block, 0, st, mp);
-            else if (p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, false, P>), grid, block, 0, st, mp);
-            else hipLaunchKernelGGL((prefill_merge_kernel<D, 0, false, P>), grid, block, 0, st, mp);
+            if (p.part_gaps && p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, true, M>), grid, block, 0, st, mp);
+            else if (p.part_gaps && p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, true, M>), grid, block, 0, st, mp);
+            else if (p.splits <= 4) hipLaunchKernelGGL((prefill_merge_kernel<D, 4, false, M>), grid, block, 0, st, mp);
+            else if (p.splits <= 8) hipLaunchKernelGGL((prefill_merge_kernel<D, 8, false, M>), grid, block, 0, st, mp);
+            else hipLaunchKernelGGL((prefill_merge_kernel<D, 0, false, M>), grid, block, 0, st, mp);
         }
     }
 }

@@ -60,9 +60,12 @@ ESDA_HD void tile_keys(const PrefillParams &p, int tile, int QT, int &j0, int &j
 // The parameters of a call with modified scores and masks (esda_scored.h) beside a plain one's.
 struct ScoredParams : PrefillParams {
     int prefix;               // keys before this position are visible to queries before them, too
-    float cap_in, cap_out;    // cap: score (log2 units) = cap_out tanh(cap_in raw / (2 log2 e)); cap_out 0: none
+    float cap_in, cap_out;    // cap log2 e tanh(x) with e^2x = 2^(cap_in q.k); cap_out = cap log2 e, 0: none
     const float *slopes;      // distance bias of each query head, or null
-    const int *q_doc, *k_doc; // document ids of queries and keys, or null
+};
+// .. and its document ids of queries and keys
+struct DocParams : ScoredParams {
+    const int *q_doc, *k_doc;
 };
 
 // The same for a scored call: every row sees the keys of the prefix, within its window.

@@ -1,6 +1,6 @@
 // esda_scored_prefill.hip -- prefill attention with capped or biased scores and document and
 // prefix masks for MI355X (gfx950): prefill_kernel and prefill_merge_kernel (esda_prefill_kernel.h)
-// with ScoredParams.  The C ABI is include/esda_scored.h.
+// with ScoredParams or, with documents, DocParams.  The C ABI is include/esda_scored.h.
 
 #include <hip/hip_runtime.h>
 
@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "esda.h"
 #include "esda_internal.h"
@@ -82,12 +83,22 @@ int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, 
     p.k = static_cast<const uint16_t *>(a->k);
     p.v = static_cast<const uint16_t *>(a->v);
     p.out = static_cast<uint16_t *>(a->out);
-    p.q_doc = a->q_doc;
-    p.k_doc = a->k_doc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (D == 512) launch_prefill<512, ScoredParams>(p, 3, st);
-    else if (D == 256) launch_prefill<256, ScoredParams>(p, 3, st);
-    else launch_prefill<128, ScoredParams>(p, 3, st);
+    auto launch = [&](const auto &x) {
+        using P = std::decay_t<decltype(x)>;
+        if (D == 512) launch_prefill<512, P>(x, 3, st);
+        else if (D == 256) launch_prefill<256, P>(x, 3, st);
+        else launch_prefill<128, P>(x, 3, st);
+    };
+    if (a->k_doc) {
+        DocParams dp{};
+        static_cast<ScoredParams &>(dp) = p;
+        dp.q_doc = a->q_doc;
+        dp.k_doc = a->k_doc;
+        launch(dp);
+    } else {
+        launch(p);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(ESDA_ERR_HIP, std::string("esda_scored_prefill launch: ") + hipGetErrorString(e));
     return ESDA_OK;
