@@ -27,7 +27,6 @@ SOURCES = [
     "esda_scored_decode.hip",
     "esda_scored_prefill.hip",
     "esda_prefix.hip",
-    "esda_prefix_tiles.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",
@@ -39,12 +38,15 @@ SOURCES = [
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # The default scheduler serialises the attend loop's LDS reads behind their uses when
-    # the loop is nested (the balanced split's segment walk); the iterative ILP strategy
-    # keeps them overlapped in every copy.
-    "-mllvm", "-amdgpu-sched-strategy=iterative-ilp",
     "-Wno-unused-command-line-argument",
 ]
+
+# The default scheduler serialises the attend loop's LDS reads behind their uses when
+# the loop is nested (the balanced split's segment walk); the iterative ILP strategy
+# keeps them overlapped in every copy.  (esda_prefix.hip: the register allocator crashes on its
+# 512-dim kernel after that strategy.)
+SCHED_FLAGS = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
+DEFAULT_SCHED = {"esda_prefix.hip"}
 
 # Per-source additions.  The raw-K ring kernel multiplies each row by diag(kw) with MFMAs whose
 # results feed VALU work; the default heuristic gives every MFMA of a kernel that uses the
@@ -53,7 +55,6 @@ EXTRA_FLAGS = {
     "esda_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
     # the decode kernel's other forms, compiled as esda_decode.hip's
     "esda_scored_decode.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
-    "esda_prefix.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
 }
 
 
@@ -69,7 +70,9 @@ def build(verbose: bool = False) -> str:
         obj = os.path.join(CSRC, os.path.basename(src) + ".o")
         # ES* C++ layer: host code only (HIP runtime API and the esda C ABI), built by
         # the host compiler so no device code is generated for it.
-        cmd = [HIPCC] + HIP_FLAGS + EXTRA_FLAGS.get(os.path.basename(src), []) + inc + ["-c", src, "-o", obj]
+        name = os.path.basename(src)
+        sched = [] if name in DEFAULT_SCHED else SCHED_FLAGS
+        cmd = [HIPCC] + HIP_FLAGS + sched + EXTRA_FLAGS.get(name, []) + inc + ["-c", src, "-o", obj]
         if src.endswith(".cpp"):
             cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__",
                    "-I", os.path.join(ROCM, "include")] + inc + ["-c", src, "-o", obj]

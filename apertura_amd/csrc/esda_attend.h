@@ -75,16 +75,6 @@ struct ScoredAttendParams : AttendParams {
     const float *slopes;
 };
 
-// A sequence's own rows behind a prefix that the batch shares (esda_prefix.h): the row of position
-// p is p - base, and every segment leaves a partial, also one that holds all of them.
-struct TailParams : AttendParams {
-    int base;
-};
-
-// Position of the first row of sequence b's linear cache.
-__device__ __forceinline__ int base_of(const AttendParams &p, int b) { return p.row_base ? p.row_base[b] : 0; }
-__device__ __forceinline__ int base_of(const TailParams &p, int) { return p.base; }
-
 // ---------------------------------------------------------------- LDS ring layout
 //
 // A workgroup streams its rows through a ring of NS stages of 16 rows in LDS.  Rows
@@ -131,8 +121,8 @@ struct Ring {
 // j1, view, slot, direct) runs each; the ring is free again when it returns (the walk puts
 // a barrier between segments).  NW: waves per workgroup; PAD: rows a pair counts beside its
 // own in a balanced plan's shares.
-template <int NW, int PAD = 0, class P, class Seg>
-__device__ __forceinline__ void walk_segments(const P &p, Seg &&segment) {
+template <int NW, int PAD = 0, class Seg>
+__device__ __forceinline__ void walk_segments(const AttendParams &p, Seg &&segment) {
     const int wg = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -140,7 +130,7 @@ __device__ __forceinline__ void walk_segments(const P &p, Seg &&segment) {
         // Fixed splits (uniform lengths: one sequence, or windowed local layers): workgroup
         // (split, kvh, b) takes rows [split * chunk, (split + 1) * chunk) of its pair.
         const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-        const SeqView sv = seq_view(p.pos[b], base_of(p, b), p.cap, p.window, p.ring);
+        const SeqView sv = seq_view(p.pos[b], p.row_base ? p.row_base[b] : 0, p.cap, p.window, p.ring);
         if (!sv.ok) {
             if (split == 0 && kvh == 0 && tid == 0) atomicAdd(p.status, 1);
             return;
@@ -165,7 +155,7 @@ __device__ __forceinline__ void walk_segments(const P &p, Seg &&segment) {
     long long rows_seq = 0;          // sum of visible rows over the batch
     if (single) {
         // one sequence: its view straight from the (wave-uniform) position word
-        w_view = seq_view(p.pos[0], base_of(p, 0), p.cap, p.window, p.ring);
+        w_view = seq_view(p.pos[0], p.row_base ? p.row_base[0] : 0, p.cap, p.window, p.ring);
         rows_seq = w_view.ok ? w_view.nvis + PAD : 0;
         if (wg == 0 && tid == 0) {
             if (!w_view.ok) atomicAdd(p.status, 1);
@@ -174,7 +164,7 @@ __device__ __forceinline__ void walk_segments(const P &p, Seg &&segment) {
     } else {
         const int t = wave_scan ? lane : tid;
         SeqView v{0, 0, 0, 0};
-        if (t < p.B) v = seq_view(p.pos[t], base_of(p, t), p.cap, p.window, p.ring);
+        if (t < p.B) v = seq_view(p.pos[t], p.row_base ? p.row_base[t] : 0, p.cap, p.window, p.ring);
         const long long nv = v.ok ? v.nvis + PAD : 0;
         long long x = nv;
 #pragma unroll
@@ -219,7 +209,7 @@ __device__ __forceinline__ void walk_segments(const P &p, Seg &&segment) {
     };
     auto view_at = [&](int b) -> SeqView {
         if (single) return w_view;
-        if (!wave_scan) return seq_view(p.pos[b], base_of(p, b), p.cap, p.window, p.ring);
+        if (!wave_scan) return seq_view(p.pos[b], p.row_base ? p.row_base[b] : 0, p.cap, p.window, p.ring);
         return SeqView{__builtin_amdgcn_readlane(w_view.nvis, b), __builtin_amdgcn_readlane(w_view.first, b),
                        __builtin_amdgcn_readlane(w_view.newrow, b), __builtin_amdgcn_readlane(w_view.ok, b)};
     };
@@ -300,7 +290,6 @@ template <int D, bool SHARED, int NW, int OCC = 1, class P = AttendParams>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * NW, 64 * NW), amdgpu_waves_per_eu(OCC * NW / 4, OCC * NW / 4)))
 void attend_kernel(P p) {
     constexpr bool SCORED = std::is_same<P, ScoredAttendParams>::value;
-    constexpr bool PARTS = std::is_same<P, TailParams>::value;  // never writes the output itself
     using R = Ring<D, SHARED, NW, 160 * 1024 / OCC>;
     // D = 512 exchanges only the live heads' partial scores (the padding columns are zero)
     constexpr bool kLiveX = D == 512;
@@ -559,7 +548,7 @@ void attend_kernel(P p) {
     // Partial of this split: every wave holds the same (m, l) and its own dim slice.
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (!PARTS && direct) {
+    if (direct) {
         // The only segment of this (sequence, kv head): normalise here, with the merge's
         // arithmetic (acc * (1 / l), then bf16); the merge skips this pair.
         if (li < p.G) {
@@ -605,7 +594,6 @@ struct MergeParams {
     int balanced, W, S, chunk;
     int pad;  // balanced: rows a pair counted beside its own (walk_segments' PAD)
 };
-__device__ __forceinline__ int base_of(const MergeParams &p, int b) { return p.row_base ? p.row_base[b] : 0; }
 
 constexpr int kMergeThreads = 256;
 constexpr int kMergeDims = 64;      // output dims per merge workgroup (16 lanes x float4)
@@ -624,8 +612,7 @@ constexpr int kMergeGroups = kMergeThreads / (kMergeDims / 4);  // split groups 
 
 // The splits that hold partials of pair (b, kvh): their count ns (0 when the sequence
 // is skipped) and the slot of the first, as the attend kernel laid them out.
-template <class P>
-__device__ __forceinline__ int pair_splits(const P &p, int b, int kvh, size_t &pbase) {
+__device__ __forceinline__ int pair_splits(const MergeParams &p, int b, int kvh, size_t &pbase) {
     int ns;
     if (p.balanced) {
         // The attend workgroups w0 .. w1 that covered pair (b, kvh) (every one of them holds
@@ -635,7 +622,7 @@ __device__ __forceinline__ int pair_splits(const P &p, int b, int kvh, size_t &p
         if (ns == 0) return 0;
         pbase = (size_t) esda_plan::share_slot((long long) b * p.Hkv + kvh, w0);
     } else {
-        const SeqView sv = seq_view(p.pos[b], base_of(p, b), p.cap, p.window, p.ring);
+        const SeqView sv = seq_view(p.pos[b], p.row_base ? p.row_base[b] : 0, p.cap, p.window, p.ring);
         if (!sv.ok) return 0;
         ns = esda_plan::grid_splits(sv.nvis, p.chunk, p.S);
         pbase = ((size_t) b * p.Hkv + kvh) * p.S;
@@ -991,8 +978,12 @@ dim3 attend_grid(const esda_decode_desc *d, const Plan &pl) {
     return pl.balanced ? dim3(pl.W) : dim3(pl.S, d->num_kv_heads / pl.pk, d->batch);
 }
 
-void fill_merge(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp, const int *pos, const int *row_base,
-                int pad, uint16_t *out, MergeParams &mp) {
+// The split merge of a step.  pad: rows a pair counted beside its own (walk_segments' PAD).
+int launch_merge(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp, const int *pos, const int *row_base,
+                 int pad, uint16_t *out, hipStream_t st) {
+    // One split per pair: the attend workgroups wrote every output themselves.
+    if (!pl.balanced && pl.S == 1) return ESDA_OK;
+    MergeParams mp;
     mp.part_acc = sp.part_acc;
     mp.part_ml = sp.part_ml;
     mp.table = sp.table;
@@ -1012,15 +1003,6 @@ void fill_merge(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp
     mp.S = pl.S;
     mp.chunk = pl.chunk;
     mp.pad = pad;
-}
-
-// The split merge of a step.  pad: rows a pair counted beside its own (walk_segments' PAD).
-int launch_merge(const esda_decode_desc *d, const Plan &pl, const DecodeSpace &sp, const int *pos, const int *row_base,
-                 int pad, uint16_t *out, hipStream_t st) {
-    // One split per pair: the attend workgroups wrote every output themselves.
-    if (!pl.balanced && pl.S == 1) return ESDA_OK;
-    MergeParams mp;
-    fill_merge(d, pl, sp, pos, row_base, pad, out, mp);
     // Partials per pair: a grid's S, or about W / pairs + 1 of the balanced shares.
     const long long pairs = (long long) d->batch * d->num_kv_heads / pl.pk;
     if (pl.balanced ? pl.W < kMergeShares * pairs : pl.S <= kMergeRowsChunk) {

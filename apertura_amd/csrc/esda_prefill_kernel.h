@@ -12,7 +12,9 @@
 #include <type_traits>
 
 #include "esda_device.h"
+#include "esda_plan.h"
 #include "esda_prefill_plan.h"
+#include "esda_stream.h"
 
 namespace {
 
@@ -48,6 +50,74 @@ constexpr int kWaves = 8;
 #define PV_DEPTH 4
 #endif
 constexpr int kPairSpin = 1 << 20;  // PS: polls of the partner's flag before a wave gives up
+
+// The sequences' own rows beside a shared prefix (esda_prefix.h), one run a workgroup of NW waves:
+// as many stages in flight as the prefill kernel's LDS holds.
+template <int D, bool SH, int NW>
+struct OwnRows {
+    static constexpr int kStage = (SH ? 1 : 2) * 2 * D * 16;  // bytes of a 16-row stage
+    static constexpr int AW = kStage * NW > 128 * 1024 ? NW / 2 : NW;
+    static constexpr int SLOTS = 2 * kStage * AW > 128 * 1024 ? 1 : 2;
+    using L = esda_stream::Layout<D, SH, AW, SLOTS>;
+
+    static __device__ __forceinline__ void store(float *acc, float *ml, size_t at, int d, const f32x4 &o, float M, float T) {
+        __builtin_nontemporal_store(o, reinterpret_cast<f32x4 *>(acc + at * D + d));
+        if (d == 0) *reinterpret_cast<f32x2 *>(ml + 2 * at) = f32x2{M, T};
+    }
+    // own workgroup w: split w % own_splits of pair w / own_splits
+    static __device__ __forceinline__ void run(const PrefixParams &p, unsigned w, unsigned char *lds) {
+        const int split = (int) (w % (unsigned) p.own_splits), pair = (int) (w / (unsigned) p.own_splits);
+        const int b = pair / p.Hkv, kvh = pair % p.Hkv;
+        const esda_plan::SeqView sv = esda_plan::seq_view(p.pos[b], p.own_base, p.own_cap, 0, 0);
+        if (!sv.ok) {
+            if (split == 0 && kvh == 0 && threadIdx.x == 0) atomicAdd(p.status, 1);
+            return;
+        }
+        esda_stream::Run x;
+        if (!esda_plan::grid_split(split, p.own_splits, p.own_chunk, sv.nvis, &x.j0, &x.j1)) return;
+        const size_t head = (size_t) b * p.own_seq_stride + (size_t) kvh * p.own_head_stride;
+        x.k = p.own_k + head;
+        x.v = p.own_v + head;
+        x.k_new = p.k_new + (size_t) pair * D;
+        x.v_new = SH ? x.k_new : p.v_new + (size_t) pair * D;
+        x.G = p.G;
+        x.nvis = sv.nvis;
+        x.first = sv.first;
+        x.cap = p.own_cap;
+        x.newrow = sv.newrow;
+        const uint16_t *const q = p.q + (size_t) b * p.q_rs + (size_t) kvh * p.G * D;
+        const size_t slot = ((size_t) pair * p.own_splits + split) * p.G;
+        esda_stream::attend_run<D, SH, NW, AW, SLOTS>(
+            lds, x, [&](int h) { return q + (size_t) h * D; }, [&](float s, int) { return s * p.scale_log2e; },
+            [&](int h, int d, const f32x4 &o, float M, float T) { store(p.own_acc, p.own_ml, slot + h, d, o, M, T); });
+    }
+    // prefix workgroup w: kv head w % Hkv, keys (w / Hkv) * run_keys on, for all B * G <= 16 query rows
+    static __device__ __forceinline__ void run_prefix(const PrefixParams &p, unsigned w, unsigned char *lds) {
+        const int kvh = (int) (w % (unsigned) p.Hkv), split = (int) (w / (unsigned) p.Hkv);
+        esda_stream::Run x{};
+        x.j0 = split * p.run_keys;
+        x.j1 = min(p.Sk, x.j0 + p.run_keys);
+        x.k = const_cast<uint16_t *>(p.k) + (size_t) kvh * p.kv_hs;
+        x.v = const_cast<uint16_t *>(p.v) + (size_t) kvh * p.kv_hs;
+        x.G = p.Sq * p.G;
+        x.nvis = p.Sk + 1;  // (no appended row)
+        x.cap = p.Sk;
+        const size_t rows = (size_t) p.Sq * p.Hq, slot = (size_t) split * rows;
+        auto row = [&](int h) { return (size_t) (h / p.G) * p.Hq + kvh * p.G + h % p.G; };
+        esda_stream::attend_run<D, SH, NW, AW, SLOTS>(
+            lds, x, [&](int h) { return p.q + row(h) * D; }, [&](float s, int) { return s * p.scale_log2e; },
+            [&](int h, int d, const f32x4 &o, float M, float T) { store(p.part_acc, p.part_ml, slot + row(h), d, o, M, T); });
+    }
+};
+
+// Prefix and own rows in runs: batches of at most 16 query rows a kv head, whose prefix no tile
+// could share further.  Four waves, two workgroups per CU.
+template <int D, bool SH>
+__global__ __launch_bounds__(256, 1) void prefix_run_kernel(PrefixParams p) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[OwnRows<D, SH, 4>::L::BYTES];
+    if (blockIdx.x < p.tile_groups) OwnRows<D, SH, 4>::run_prefix(p, blockIdx.x, lds);
+    else OwnRows<D, SH, 4>::run(p, blockIdx.x - p.tile_groups, lds);
+}
 
 template <int D, int NSL, int NT = 2>
 struct PRing {
@@ -97,7 +167,14 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
     constexpr int DT = D / 16;          // PV dim tiles
     constexpr int NB = PS ? 2 : QB;     // O^T blocks per wave
     constexpr int DW = PS ? DT / 2 : DT;  // O^T dim tiles per wave
-    __shared__ __attribute__((aligned(16))) unsigned char ring[R::BYTES];
+    constexpr int kLds = PARTS && OwnRows<D, SH, NW>::L::BYTES > R::BYTES ? OwnRows<D, SH, NW>::L::BYTES : R::BYTES;
+    __shared__ __attribute__((aligned(16))) unsigned char ring[kLds];
+    if constexpr (PARTS) {
+        if (blockIdx.x >= p.tile_groups) {
+            OwnRows<D, SH, NW>::run(p, blockIdx.x - p.tile_groups, ring);
+            return;
+        }
+    }
     // PS exchange, per stage parity: each wave's P^T (16 B per lane) and rescale factors
     // (4 B per lane), then one flag per wave; after both parities, each wave's row sums.
     constexpr int XP = 64 * 16 + 64 * 4;
@@ -303,32 +380,45 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         return sc;
     };
 
-    // Documents: the stages to compute, in order.  cur[i] / ahead[i] are the key stages of this and
-    // of the next iteration (nst past the last), and whether they need no mask for their documents.
-    // The i-th stage computed takes ring slot i % NSL.
+    // Scored: stages from the last to the first, so that a bias by distance meets its largest scores
+    // first (from the first on, steep slopes raised the maximum and rescaled O^T in every stage: 512
+    // queries over 16K keys, 32 slopes 2^-0.25 .. 2^-8, 541 us against 442).
+    // Documents: only those to compute.  cur[i] / ahead[i] are the key stages of this and of the next
+    // iteration (-1 past the last), and whether they need no mask for their documents; live and pure
+    // describe the 64 stages of `window`.  The i-th stage computed takes ring slot i % NSL.
     struct Stage {
         int st;
         bool pure;
     };
     Stage cur[SPI], ahead[SPI];
-    // to[0 .. SPI-1]: the first SPI stages to compute from stage s on
+    int window = -1;
+    unsigned long long live = 0ull, pure = 0ull;
+    // to[0 .. SPI-1]: the first SPI stages to compute from stage s down
     auto next_stages = [&](int s, auto &to) {
         if constexpr (DOCS) {
 #pragma unroll
             for (int i = 0; i < SPI; ++i) {
-                to[i] = {nst, true};
-                while (s < nst) {
-                    const int w = s >> 6;
-                    const unsigned long long m = (w < kDocWindows ? live_of[w] : ~0ull) >> (s & 63);
-                    const unsigned lo = uniform((int) (unsigned) m), hi = uniform((int) (unsigned) (m >> 32));
-                    const unsigned long long um = (unsigned long long) hi << 32 | lo;
-                    if (um == 0ull) {
-                        s = (s | 63) + 1;
+                to[i] = {-1, true};
+                while (s >= 0) {
+                    if ((s >> 6) != window) {
+                        window = s >> 6;
+                        const bool known = window < kDocWindows;
+                        auto word = [&](const unsigned long long *x) {
+                            const unsigned long long v = known ? x[window] : 0ull;
+                            return (unsigned long long) (unsigned) uniform((int) (unsigned) (v >> 32)) << 32 |
+                                   (unsigned) uniform((int) (unsigned) v);
+                        };
+                        live = known ? word(live_of) : ~0ull;
+                        pure = word(pure_of);
+                    }
+                    const unsigned long long m = live << (63 - (s & 63));
+                    if (m == 0ull) {
+                        s = (s & ~63) - 1;
                         continue;
                     }
-                    s += __builtin_ctzll(um);
-                    if (s < nst) to[i] = {s, w < kDocWindows && uniform((int) (pure_of[w] >> (s & 63)) & 1) != 0};
-                    ++s;
+                    s -= __builtin_clzll(m);
+                    to[i] = {s, ((pure >> (s & 63)) & 1) != 0};
+                    --s;
                     break;
                 }
             }
@@ -352,27 +442,35 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
             qhi = max(qhi, __shfl_xor(qhi, o));
         }
         one_doc = __builtin_amdgcn_ballot_w64(!one_doc) == 0ull && qlo == qhi;
-        // lane l of a window's wave: the ids of its stage l (past the last key: its id again)
-        for (int w = wave; w < kDocWindows && 64 * w < nst; w += NW) {
-            int lo = INT_MAX, hi = -1;
-            const long long j = (long long) j0 + 2048LL * w + 32 * lane;
-            if (64 * w + lane < nst) {
+        // Eight stages a wave and step: one load, 8 lanes of 4 keys to a stage (past the last key: its id
+        // again), lowest and highest id over those lanes, and a byte of each set.
+        typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+        for (int c = wave; c < 8 * kDocWindows && 8 * c < nst; c += NW) {
+            const long long j = (long long) j0 + 256LL * c + 4 * lane, last = p.Sk - 1;
+            i32x4 d;
+            if (j + 3 <= last) d = *reinterpret_cast<const i32x4_a4 *>(p.k_doc + j);
+            else
 #pragma unroll
-                for (int e = 0; e < kStageKeys; ++e) {
-                    const int d = p.k_doc[min(j + e, (long long) p.Sk - 1)];
-                    lo = min(lo, d);
-                    hi = max(hi, d);
-                }
-            }
-            const unsigned long long a = __builtin_amdgcn_ballot_w64(hi >= qlo && lo <= qhi);
-            const unsigned long long b = __builtin_amdgcn_ballot_w64(one_doc && lo == qlo && hi == qhi);
+                for (int e = 0; e < 4; ++e) d[e] = p.k_doc[min(j + e, last)];
+            int lo = min(min(d[0], d[1]), min(d[2], d[3])), hi = max(max(d[0], d[1]), max(d[2], d[3]));
+            // lanes ^1, ^2, then the other four of the eight
+            lo = min(lo, __builtin_amdgcn_mov_dpp(lo, 0xb1, 0xf, 0xf, true));
+            hi = max(hi, __builtin_amdgcn_mov_dpp(hi, 0xb1, 0xf, 0xf, true));
+            lo = min(lo, __builtin_amdgcn_mov_dpp(lo, 0x4e, 0xf, 0xf, true));
+            hi = max(hi, __builtin_amdgcn_mov_dpp(hi, 0x4e, 0xf, 0xf, true));
+            lo = min(lo, __builtin_amdgcn_mov_dpp(lo, 0x141, 0xf, 0xf, true));
+            hi = max(hi, __builtin_amdgcn_mov_dpp(hi, 0x141, 0xf, 0xf, true));
+            auto eight = [](bool x) {  // bit 8i of the ballot (lane 8i: stage i of the eight) -> bit i
+                return (unsigned char) (((__builtin_amdgcn_ballot_w64(x) & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+            };
+            const unsigned char a = eight(hi >= qlo && lo <= qhi), b = eight(one_doc && lo == qlo && hi == qhi);
             if (lane == 0) {
-                live_of[w] = a;
-                pure_of[w] = b;
+                reinterpret_cast<unsigned char *>(live_of)[c] = a;
+                reinterpret_cast<unsigned char *>(pure_of)[c] = b;
             }
         }
         lds_barrier();
-        next_stages(0, cur);
+        next_stages(nst - 1, cur);
     }
     auto issue_docs = [&](int st, int s) {
         if constexpr (DOCS) {
@@ -381,7 +479,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         }
     };
 
-    if constexpr (!DOCS) {
+    if constexpr (!SCORED) {
         issue(kvb, 0, kslot(0));  // nst >= 1 here
         if (!SH) issue(vvb, 0, vslot(0));
         if ((KH || S2) && nst > 1) {
@@ -390,12 +488,14 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < SPI; ++i)
-            if (cur[i].st < nst) {
-                issue(kvb, cur[i].st, kslot(i));
-                if (!SH) issue(vvb, cur[i].st, vslot(i));
-                issue_docs(cur[i].st, i);
+        for (int i = 0; i < SPI; ++i) {
+            const int st = DOCS ? cur[i].st : nst - 1 - i;
+            if (st >= 0) {
+                issue(kvb, st, kslot(i));
+                if (!SH) issue(vvb, st, vslot(i));
+                issue_docs(st, i);
             }
+        }
     }
 
     auto shift = [&]() {
@@ -410,18 +510,20 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
                    (p.window == 0 || ka_first > qa_max - p.window) && pure;
         else return false;
     };
-    for (int s0 = 0; DOCS ? cur[0].st < nst : s0 < nst; s0 += SPI, shift()) {
+    for (int s0 = 0; DOCS ? cur[0].st >= 0 : s0 < nst; s0 += SPI, shift()) {
         // the key stage of the i-th stage from s0 on
         auto at = [&](int i) -> int {
-            if constexpr (!DOCS) return s0 + i;
+            if constexpr (!SCORED) return s0 + i;
+            else if constexpr (!DOCS) return nst - 1 - (s0 + i);
             else if (i < SPI) return i == 0 ? cur[0].st : cur[SPI - 1].st;
             else return i == SPI ? ahead[0].st : ahead[SPI - 1].st;
         };
+        auto there = [&](int st) { return SCORED ? st >= 0 : st < nst; };
         // The iteration's stages s0 .. s0+SPI-1 landed (this wave's loads; the barrier covers
         // the other waves') and every wave is done with the previous iteration
         ESDA_WAIT_VM(0);
         lds_barrier();
-        if constexpr (DOCS) next_stages(cur[SPI - 1].st + 1, ahead);
+        if constexpr (DOCS) next_stages(cur[SPI - 1].st - 1, ahead);
         // The next iteration's DMAs, spread over this iteration so that the workgroup's loads
         // do not all queue at the barrier (each slot is free once the barrier has passed):
         //  - separate K and V (plain, S2): K of the next stage at the barrier, its V after
@@ -431,16 +533,16 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         //  - KH: all at the barrier (spreading measured slower there).
         constexpr bool kVLate = !SH && !KH;
         auto issue_k = [&]() {
-            if (at(SPI) < nst) {
+            if (there(at(SPI))) {
                 issue(kvb, at(SPI), kslot(s0 + SPI));
                 issue_docs(at(SPI), s0 + SPI);
             }
         };
         auto issue_v = [&]() {
-            if (!SH && at(SPI) < nst) issue(vvb, at(SPI), vslot(s0 + SPI));
+            if (!SH && there(at(SPI))) issue(vvb, at(SPI), vslot(s0 + SPI));
         };
         auto issue_second = [&]() {
-            if (at(SPI + 1) < nst) {
+            if (there(at(SPI + 1))) {
                 issue(kvb, at(SPI + 1), kslot(s0 + SPI + 1));
                 if (!SH) issue(vvb, at(SPI + 1), vslot(s0 + SPI + 1));
                 issue_docs(at(SPI + 1), s0 + SPI + 1);
@@ -645,10 +747,10 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
         if constexpr (S2) {
             stage(s0, at(0), !DOCS || cur[0].pure, after_first_qk);
             issue_second();
-            if (at(1) < nst) stage(s0 + 1, at(1), !DOCS || cur[SPI - 1].pure, [] {});
+            if (there(at(1))) stage(s0 + 1, at(1), !DOCS || cur[SPI - 1].pure, [] {});
         } else {
             const int s = s0 + kh, st = at(kh);  // this wave group's stage
-            if (KH && st >= nst) continue;  // an odd stage count: the odd group's last iteration is empty
+            if (KH && !there(st)) continue;  // an odd stage count: the odd group's last iteration is empty
             stage(s, st, !DOCS || (kh ? cur[SPI - 1].pure : cur[0].pure), after_first_qk);
         }
     }
@@ -969,7 +1071,9 @@ void launch_tiles(const P &p, hipStream_t st) {
     // percentile); of 117 of separate K and V 1.05 (1.03 .. 1.12).
     const bool shared = p.k == p.v, one = D == 512 && (long long) p.Sq * p.G <= 64;
     const int nw = one ? (shared ? 4 : 8) : p.nw;
-    const dim3 grid(p.tiles * p.Hkv * p.splits), block(64 * nw);
+    unsigned groups = p.tiles * p.Hkv * p.splits;
+    if constexpr (std::is_same<P, PrefixParams>::value) groups += p.Sq * p.Hkv * p.own_splits;
+    const dim3 grid(groups), block(64 * nw);
     if constexpr (D == 512) {
         if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);
         else if (nw == 4) hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, 4, P>), grid, block, 0, st, p);

@@ -78,8 +78,20 @@ ESDA_HD void tile_keys(const ScoredParams &p, int tile, int QT, int &j0, int &j1
 }
 
 // A decode batch's query rows over their shared prefix (esda_prefix.h): every row (sequence, group
-// head) sees every key, and every split leaves a partial, also a single one.
-struct PrefixParams : PrefillParams {};
+// head) sees every key, and every split leaves a partial, also a single one.  Behind the tiles'
+// workgroups come those of the sequences' own rows: `own_splits` of each (sequence, kv head), of
+// own_chunk rows, which leave partials too.
+struct PrefixParams : PrefillParams {
+    unsigned tile_groups;   // workgroups of the prefix
+    int run_keys;           // > 0: the prefix in runs of this many keys instead of tiles
+    uint16_t *own_k, *own_v;
+    const uint16_t *k_new, *v_new;
+    const int *pos;
+    int *status;
+    long long own_seq_stride, own_head_stride;
+    int own_cap, own_base, own_splits, own_chunk;
+    float *own_acc, *own_ml;  // [B * Hkv][own_splits][G][D] and [..][2]
+};
 
 // A kernel form of one head dim: 16-query blocks per wave, stage halves or not, waves, and
 // its cost in us: `wg` and `row` per workgroup and query row of it (Q and first-stage loads,

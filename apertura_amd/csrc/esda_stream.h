@@ -1,0 +1,178 @@
+// esda_stream.h -- decode attention over one run of cache rows by waves that do not wait for one
+// another (gfx950): wave w takes the run's 16-row stages w, w + NW, .. over the whole head dim,
+// from LDS slots of its own that it fills by DMA, and the waves' (m, l, O) meet once at the end.
+// For workgroups whose stages are short (a 16-row stage of 128-dim rows is 8 KB: a barrier and a
+// score exchange per stage, as in attend_kernel, take longer than its bytes), and for runs inside
+// another kernel's workgroup.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "esda_device.h"
+
+namespace esda_stream {
+
+// Rows [j0, j1) of a kv head's nvis visible ones, for G <= 16 query rows.
+struct Run {
+    uint16_t *k, *v;               // the cache rows of the kv head
+    const uint16_t *k_new, *v_new; // the new token's rows (the last visible row), or null
+    int G, j0, j1, nvis, first, cap, newrow;
+};
+
+// AW of the workgroup's NW waves take stages, each with SLOTS slots.
+template <int D, bool SH, int AW, int SLOTS>
+struct Layout {
+    static constexpr int BLK = 1056;                // LDS bytes per DMA block: 1 KB + 32 B pad
+    static constexpr int NI = D / 32;               // DMA blocks of a tensor's 16-row stage
+    static constexpr int HB = NI * BLK;
+    static constexpr int SLOT = (SH ? 1 : 2) * HB;
+    static constexpr int CPR = D / 8;               // 16-byte chunks per row
+    static constexpr int CH = D < 256 ? D : 256;    // dims the waves' O are summed over at a time
+    static constexpr int SUM = AW * 16 * CH * 4;
+    static constexpr int RING = AW * SLOTS * SLOT;
+    static constexpr int TOTALS = RING > SUM ? RING : SUM;
+    static constexpr int BYTES = TOTALS + (AW + 1) * 16 * 8;
+    // Row r of a stage: block r % NI, 2D bytes times r / NI into it (free of bank conflicts for both
+    // the 128-bit row reads and the transpose reads).
+    __device__ static constexpr int off(int r) { return (r % NI) * BLK + (r / NI) * 2 * D; }
+};
+
+// Attends the run; every thread of the workgroup calls it.  query(h): query row h; score(x, j): the
+// log2-domain score of raw product x and visible row j, of query row `lane & 15`; put(h, d, o, M, T):
+// called once for each query row h and four dims from d on, with O, its maximum and its sum.
+template <int D, bool SH, int NW, int AW, int SLOTS, class Query, class Score, class Put>
+__device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
+    using L = Layout<D, SH, AW, SLOTS>;
+    constexpr int KS = D / 32, DT = D / 16;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    unsigned char *const ring = lds + wave * SLOTS * L::SLOT;
+    const int all = (x.j1 - x.j0 + 15) >> 4, nst = wave < AW ? all : 0;  // this wave's range of stages
+    const bool append = x.k_new != nullptr;
+
+    const int drow = lane / L::CPR, chunk = lane % L::CPR;  // DMA: this lane's row among a block's, its chunk
+    const unsigned voff = (unsigned) ((drow * L::NI * D + chunk * 8) * 2);
+    auto dma = [&](int st, unsigned char *slot) {
+        const int jst = x.j0 + 16 * st;
+        const unsigned at = lds_addr(slot);
+        if (jst + 16 < x.j1 && x.first + jst + 16 <= x.cap) {
+            // sixteen consecutive cache rows, none clamped or new
+            const uint16_t *kb = x.k + (size_t) (x.first + jst) * D, *vb = x.v + (size_t) (x.first + jst) * D;
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) {
+                lds_dma16_s(kb + i * D, voff, at + i * L::BLK);
+                if constexpr (!SH) lds_dma16_s(vb + i * D, voff, at + L::HB + i * L::BLK);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < L::NI; ++i) {
+            const int j = min(jst + i + L::NI * drow, x.j1 - 1);  // rows past the run repeat its last, masked
+            int r = x.first + j;
+            if (r >= x.cap) r -= x.cap;
+            const bool is_new = append && j == x.nvis - 1;
+            lds_dma16((is_new ? x.k_new : x.k + (size_t) r * D) + chunk * 8, at + i * L::BLK);
+            if constexpr (!SH) lds_dma16((is_new ? x.v_new : x.v + (size_t) r * D) + chunk * 8, at + L::HB + i * L::BLK);
+        }
+    };
+
+    if (wave < nst) dma(wave, ring);
+    bf16x8 qv[KS];  // B operand: head li, dims 32 ks + 8 lg ..
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 w = li < x.G ? *reinterpret_cast<const u32x4 *>(query(li) + 32 * ks + 8 * lg) : u32x4{0u, 0u, 0u, 0u};
+        qv[ks] = __builtin_bit_cast(bf16x8, w);
+    }
+    const int qk_off = L::off(li) + lg * 16, tr_off = L::off(4 * lg + li / 4) + (li % 4) * 8;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int st = wave, it = 0; st < nst; st += AW, ++it) {
+        unsigned char *const slot = ring + (SLOTS > 1 ? (it & 1) * L::SLOT : 0);
+        ESDA_WAIT_VM(0);  // this stage landed
+        if (SLOTS > 1 && st + AW < nst) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other slot's reads are done
+            dma(st + AW, ring + ((it + 1) & 1) * L::SLOT);
+        }
+        asm volatile("" ::: "memory");
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // rows 4 lg + r of head li
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(slot + qk_off + 64 * ks), qv[ks], s, 0, 0, 0);
+        const int jt = x.j0 + 16 * st + 4 * lg;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = jt + r < x.j1 ? score(s[r], jt + r) : -INFINITY;
+        const float top = wave_max_across_groups(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+        if (__any(top > m + kRescaleSlack)) {
+            const float mn = fmaxf(m, top), corr = __builtin_amdgcn_exp2f(m - mn);
+            l *= corr;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[dt] *= corr;
+            m = mn;
+        }
+        short4v pb;  // the weights as they enter both sums: bf16
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const __bf16 w = (__bf16) __builtin_amdgcn_exp2f(s[r] - m);
+            l += (float) w;
+            pb[r] = __builtin_bit_cast(short, w);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4v *) (slot + (SH ? 0 : L::HB) + tr_off + 32 * dt));
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, pb, acc[dt], 0, 0, 0);
+        }
+        if (SLOTS == 1 && st + AW < nst) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads are done
+            dma(st + AW, ring);
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // The new row into the cache (bit-exact) by the run that ends with it; no other run reads it.
+    if (append && x.j1 == x.nvis && wave == 0)
+        for (int c = lane; c < D / 8; c += 64) {
+            *reinterpret_cast<u32x4 *>(x.k + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.k_new + 8 * c);
+            if constexpr (!SH)
+                *reinterpret_cast<u32x4 *>(x.v + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.v_new + 8 * c);
+        }
+
+    // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = -inf, l = 0.
+    f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + AW * 16;  // [AW][16], [16]
+    float *const sum = reinterpret_cast<float *>(lds);                                      // [AW][G][CH]
+    if (lg == 0 && wave < AW) ml[wave * 16 + li] = f32x2{m, l};
+    lds_barrier();  // and every wave is done with its slots
+    float M = -INFINITY, T = 0.0f;
+#pragma unroll
+    for (int w = 0; w < AW; ++w) M = fmaxf(M, ml[w * 16 + li][0]);
+    const float mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < AW; ++w) T = __builtin_fmaf(ml[w * 16 + li][1], __builtin_amdgcn_exp2f(ml[w * 16 + li][0] - mu), T);
+    if (wave == 0 && lg == 0) tot[li] = f32x2{M, T};
+    const float c = __builtin_amdgcn_exp2f(m - mu);
+    const int live = all < AW ? all : AW;  // waves that had a stage
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += L::CH) {
+        if (li < x.G && wave < live) {
+#pragma unroll
+            for (int dt = 0; dt < L::CH / 16; ++dt)
+                *reinterpret_cast<f32x4 *>(sum + (wave * x.G + li) * L::CH + 16 * dt + 4 * lg) = acc[d0 / 16 + dt] * c;
+        }
+        lds_barrier();
+        for (int t = threadIdx.x; t < x.G * (L::CH / 4); t += 64 * NW) {
+            const int h = t / (L::CH / 4), d = 4 * (t % (L::CH / 4));
+            f32x4 o = *reinterpret_cast<const f32x4 *>(sum + h * L::CH + d);
+            for (int w = 1; w < live; ++w) o += *reinterpret_cast<const f32x4 *>(sum + (w * x.G + h) * L::CH + d);
+            put(h, d0 + d, o, tot[h][0], tot[h][1]);
+        }
+        lds_barrier();  // before the next dims, or the next run's DMAs
+    }
+}
+
+}  // namespace esda_stream

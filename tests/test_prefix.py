@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from apertura_amd import _lib
-from apertura_amd.decode import DecodeStep, workspace_bytes
+from apertura_amd.decode import DecodeStep
 from apertura_amd.prefix import PrefixCall, PrefixStep, prefix_workspace_bytes
 
 FAKE = 0x10000000  # never dereferenced: validation fails first
@@ -19,12 +19,18 @@ def _step(prefix_len=100, prefix_head_stride=None, split_keys=0, **kw):
     return PrefixStep(DecodeStep(**base), prefix_len, prefix_head_stride, split_keys)
 
 
-def test_workspace_holds_the_own_step_and_every_prefix_split():
+def test_workspace_holds_every_partial():
+    """The status word, then (m, l) and O of every prefix split and own split of the 32 query rows."""
     up = lambda n: (n + 255) // 256 * 256
-    own = workspace_bytes(_step().own)
     for keys, splits in ((32, 4), (64, 2), (128, 1)):
-        parts = splits * 4 * 8
-        assert prefix_workspace_bytes(_step(split_keys=keys)) == up(own) + up(parts * 8) + parts * 128 * 4
+        for rows, own in ((16, 4), (32, 2), (0, 1)):
+            want = 256 + up(splits * 32 * 8) + up(own * 32 * 8) + (splits + own) * 32 * 128 * 4
+            assert prefix_workspace_bytes(_step(split_keys=keys, split_rows=rows)) == want
+
+
+def test_a_bound_on_own_rows_sizes_their_splits():
+    big, small = _step(cap=100000, split_rows=512), _step(cap=100000, split_rows=512, max_visible=1000)
+    assert prefix_workspace_bytes(small) < prefix_workspace_bytes(big)
 
 
 @pytest.mark.parametrize("kw", [
