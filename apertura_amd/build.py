@@ -27,6 +27,7 @@ SOURCES = [
     "esda_scored_decode.hip",
     "esda_scored_prefill.hip",
     "esda_prefix.hip",
+    "esda_prefix_tiles.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",
@@ -43,10 +44,10 @@ HIP_FLAGS = [
 
 # The default scheduler serialises the attend loop's LDS reads behind their uses when
 # the loop is nested (the balanced split's segment walk); the iterative ILP strategy
-# keeps them overlapped in every copy.  (esda_prefix.hip: the register allocator crashes on its
+# keeps them overlapped in every copy.  (esda_prefix_tiles.hip: the register allocator crashes on its
 # 512-dim kernel after that strategy.)
 SCHED_FLAGS = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
-DEFAULT_SCHED = {"esda_prefix.hip"}
+DEFAULT_SCHED = {"esda_prefix_tiles.hip"}
 
 # Per-source additions.  The raw-K ring kernel multiplies each row by diag(kw) with MFMAs whose
 # results feed VALU work; the default heuristic gives every MFMA of a kernel that uses the

@@ -87,36 +87,45 @@ struct OwnRows {
         x.newrow = sv.newrow;
         const uint16_t *const q = p.q + (size_t) b * p.q_rs + (size_t) kvh * p.G * D;
         const size_t slot = ((size_t) pair * p.own_splits + split) * p.G;
-        esda_stream::attend_run<D, SH, NW, AW, SLOTS>(
+        esda_stream::attend_run<D, SH, NW, AW, SLOTS, 1>(
             lds, x, [&](int h) { return q + (size_t) h * D; }, [&](float s, int) { return s * p.scale_log2e; },
             [&](int h, int d, const f32x4 &o, float M, float T) { store(p.own_acc, p.own_ml, slot + h, d, o, M, T); });
     }
-    // prefix workgroup w: kv head w % Hkv, keys (w / Hkv) * run_keys on, for all B * G <= 16 query rows
+    // Prefix workgroup w: 16 NG of the B * G query rows of a kv head over run_keys keys.  The row groups
+    // of the same keys are 8 workgroups apart: on one XCD, whose L2 hands the second what the first read.
+    template <int NG>
     static __device__ __forceinline__ void run_prefix(const PrefixParams &p, unsigned w, unsigned char *lds) {
-        const int kvh = (int) (w % (unsigned) p.Hkv), split = (int) (w / (unsigned) p.Hkv);
+        const unsigned i = w >> 3, pair = i / (unsigned) p.row_groups * 8 + (w & 7);
+        const int r0 = (int) (i % (unsigned) p.row_groups) * 16 * NG;
+        const int kvh = (int) (pair % (unsigned) p.Hkv), split = (int) (pair / (unsigned) p.Hkv);
+        if (split >= p.splits) return;
         esda_stream::Run x{};
         x.j0 = split * p.run_keys;
         x.j1 = min(p.Sk, x.j0 + p.run_keys);
         x.k = const_cast<uint16_t *>(p.k) + (size_t) kvh * p.kv_hs;
         x.v = const_cast<uint16_t *>(p.v) + (size_t) kvh * p.kv_hs;
-        x.G = p.Sq * p.G;
+        x.G = min(p.Sq * p.G - r0, 16 * NG);
         x.nvis = p.Sk + 1;  // (no appended row)
         x.cap = p.Sk;
         const size_t rows = (size_t) p.Sq * p.Hq, slot = (size_t) split * rows;
-        auto row = [&](int h) { return (size_t) (h / p.G) * p.Hq + kvh * p.G + h % p.G; };
-        esda_stream::attend_run<D, SH, NW, AW, SLOTS>(
+        auto row = [&](int h) { return (size_t) ((r0 + h) / p.G) * p.Hq + kvh * p.G + (r0 + h) % p.G; };
+        esda_stream::attend_run<D, SH, NW, AW, SLOTS, NG>(
             lds, x, [&](int h) { return p.q + row(h) * D; }, [&](float s, int) { return s * p.scale_log2e; },
             [&](int h, int d, const f32x4 &o, float M, float T) { store(p.part_acc, p.part_ml, slot + row(h), d, o, M, T); });
     }
 };
 
-// Prefix and own rows in runs: batches of at most 16 query rows a kv head, whose prefix no tile
-// could share further.  Four waves, two workgroups per CU.
-template <int D, bool SH>
+// Prefix and own rows in runs, for batches of few query rows a kv head: every wave holds 16 NG of
+// them and its own keys, so that a K or V value is read from LDS once for those, where the tiles'
+// waves each hold 16 rows and read every key.  The registers bound NG (O^T and Q^T take 6 D NG / 16
+// of 512 a lane: NG D = 1024 spills); more rows are row_groups workgroups of the same keys.
+template <int D, bool SH, int NG>
 __global__ __launch_bounds__(256, 1) void prefix_run_kernel(PrefixParams p) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[OwnRows<D, SH, 4>::L::BYTES];
-    if (blockIdx.x < p.tile_groups) OwnRows<D, SH, 4>::run_prefix(p, blockIdx.x, lds);
-    else OwnRows<D, SH, 4>::run(p, blockIdx.x - p.tile_groups, lds);
+    using O = OwnRows<D, SH, 4>;
+    using L = esda_stream::Layout<D, SH, O::AW, O::SLOTS, NG>;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
+    if (blockIdx.x >= p.own_groups) O::template run_prefix<NG>(p, blockIdx.x - p.own_groups, lds);
+    else O::run(p, blockIdx.x, lds);
 }
 
 template <int D, int NSL, int NT = 2>
@@ -1072,7 +1081,7 @@ void launch_tiles(const P &p, hipStream_t st) {
     const bool shared = p.k == p.v, one = D == 512 && (long long) p.Sq * p.G <= 64;
     const int nw = one ? (shared ? 4 : 8) : p.nw;
     unsigned groups = p.tiles * p.Hkv * p.splits;
-    if constexpr (std::is_same<P, PrefixParams>::value) groups += p.Sq * p.Hkv * p.own_splits;
+    if constexpr (std::is_same<P, PrefixParams>::value) groups += p.own_groups;
     const dim3 grid(groups), block(64 * nw);
     if constexpr (D == 512) {
         if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);

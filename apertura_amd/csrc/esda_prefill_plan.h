@@ -78,12 +78,13 @@ ESDA_HD void tile_keys(const ScoredParams &p, int tile, int QT, int &j0, int &j1
 }
 
 // A decode batch's query rows over their shared prefix (esda_prefix.h): every row (sequence, group
-// head) sees every key, and every split leaves a partial, also a single one.  Behind the tiles'
-// workgroups come those of the sequences' own rows: `own_splits` of each (sequence, kv head), of
-// own_chunk rows, which leave partials too.
+// head) sees every key, and every split leaves a partial, also a single one.  The same grid holds
+// the workgroups of the sequences' own rows: `own_splits` of each (sequence, kv head), of own_chunk
+// rows, which leave partials too (behind the tiles', which are longer; before the runs').
 struct PrefixParams : PrefillParams {
-    unsigned tile_groups;   // workgroups of the prefix
-    int run_keys;           // > 0: the prefix in runs of this many keys instead of tiles
+    unsigned tile_groups, own_groups;  // workgroups of the prefix and of the own rows
+    int run_keys;           // > 0: the prefix in runs of this many keys instead of tiles ..
+    int row_groups;         // .. each in this many groups of query rows
     uint16_t *own_k, *own_v;
     const uint16_t *k_new, *v_new;
     const int *pos;

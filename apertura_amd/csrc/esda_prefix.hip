@@ -11,13 +11,16 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "esda.h"
 #include "esda_attend.h"
 #include "esda_internal.h"
 #include "esda_prefill_kernel.h"
 #include "esda_prefix.h"
+#include "esda_prefix_tiles.h"
 
 namespace {
 
@@ -153,9 +156,52 @@ struct PrefixPlan {
     size_t off_pre_ml, off_own_ml, off_pre_acc, off_own_acc, bytes;
 };
 
-constexpr int kRunRows = 128;  // fewest rows of a run: two stages a wave of four
+constexpr int kRunRows = 64;  // fewest rows of a run: a stage for each of four waves
 
-int make_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
+// How the prefix's query rows can be laid out: as tiles (nw > 0: a prefill form), or in runs of 16 NG
+// rows.  us of a workgroup: `start`, and per KB of K and V `per_kb`; slots: workgroups the GPU holds at
+// once.  Fitted to graph-replayed steps of forced splits (the keys in the Infinity Cache), us, runs /
+// tiles at the best split: D = 512 over one K = V buffer, 16 rows x 4096 keys 17.4 / 15.2, x 32768
+// 31.7 / 41.8, 32 rows 18.8 / 18.5 and 42.3 / 45.0, 64 rows x 16384 41.0 / 35.7; D = 128, 8 rows x 8192
+// keys 11.3 / 19.8, 16 x 32768 25.1 / 45.2, 32 x 16384 19.3 / 29.0, 64 28.2 / 30.6, 128 38.4 / 34.8;
+// D = 256, 8 rows x 8192 27.5 / 27.8, 32 37.5 / 30.1: always tiles.
+struct Form {
+    int qb, kh, nw, ng;
+    float start, per_kb;
+    int slots;
+    int rows() const { return ng ? 16 * ng : 16 * qb * (kh ? nw / 2 : nw); }
+};
+
+// The forms a step may take; returns their number.
+int forms_of(int D, int rows, bool shared, Form *f) {
+    int n = 0;
+    const Tiling *t = D == 512 ? kTilings512 : D == 256 ? kTilings256 : kTilings128;
+    const int nt = D == 512 ? 2 : D == 256 ? 3 : 1;
+    const float stage_kb = 32.0f * 2 * D * (shared ? 1 : 2) / 1024;
+    for (int i = 0; i < nt; ++i)
+        if (!(D == 512 && rows <= 64 && t[i].nw == (shared ? 8 : 4)))  // (launch_tiles' choice for one tile)
+            f[n++] = {t[i].qb, t[i].kh, t[i].nw, 0, t[i].wg + t[i].row * std::min(rows, t[i].rows()), t[i].stage / stage_kb, 256};
+    if (D == 512 && rows <= 32) f[n++] = {0, 0, 0, 1, 13.0f, 1 / 60.0f, 256};
+    if (D == 128 && rows <= 64) f[n++] = rows <= 16 ? Form{0, 0, 0, 1, 8.0f, 1 / 58.0f, 512}
+                                         : rows <= 32 ? Form{0, 0, 0, 2, 8.0f, 1 / 43.0f, 512} : Form{0, 0, 0, 4, 10.0f, 1 / 27.0f, 256};
+    return n;
+}
+
+// us of na workgroups of `a` us, then nb of `b` us, on `slots`.
+float makespan(long long na, float a, long long nb, float b, int slots) {
+    const long long rem = na % slots, idle = slots - rem;  // slots of the first kind's last round, and without it
+    const float early = (float) (na / slots) * a, late = early + (rem ? a : 0.0f);
+    if (nb <= idle) return std::max(late, early + (nb ? b : 0.0f));
+    // whole rounds that both sorts of slots take (the first sort starts late - early behind), then the rest
+    const long long rounds = std::max(0LL, nb / slots - 2);
+    nb -= rounds * slots;
+    for (int i = 1;; ++i) {
+        const long long by_idle = i * idle, by_rem = (long long) (std::max(0.0f, early + i * b - late) / b) * rem;
+        if (by_idle + by_rem >= nb) return std::max(late, early + (rounds + i) * b);
+    }
+}
+
+int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     if (!d) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: null description");
     Plan own;
     const int rc = make_plan(&d->own, &own);  // its checks, and the bound on own rows
@@ -168,44 +214,84 @@ int make_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     if (d->prefix_head_stride < (int64_t) d->prefix_len * d->own.head_dim || d->prefix_head_stride % 8)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: prefix_head_stride must be >= prefix_len * head_dim "
                                                "and a multiple of 8");
+    if (d->split_keys < 0 || d->split_keys % kStageKeys)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: split_keys must be a multiple of 32");
+    if (!(d->own.scale > 0.0f) || !std::isfinite(d->own.scale))
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: scale must be positive and finite");
     const int D = d->own.head_dim, B = d->own.batch, Hkv = d->own.num_kv_heads, P = d->prefix_len;
+    const bool shared = d->own.kv_shared != 0;
     const size_t rows = (size_t) B * d->own.num_q_heads;
-    esda_prefill_desc t{};
-    t.num_q_heads = d->own.num_q_heads;
-    t.num_kv_heads = Hkv;
-    t.head_dim = D;
-    t.seq_q = B;
-    t.seq_k = P;
-    t.q_pos0 = P - 1;  // every row at or past the last key
-    t.q_head_stride = D;
-    t.q_row_stride = (int64_t) t.num_q_heads * D;
-    t.kv_head_stride = d->prefix_head_stride;
-    t.split_keys = d->split_keys;
-    t.scale = d->own.scale;
     PrefixParams &p = pl->p;
-    if (const char *why = last_plan(&t, 0, &p)) return fail(ESDA_ERR_INVALID_ARGUMENT, why);
-    if (B * p.G <= 16) {
-        // runs: a workgroup per CU (two at 8 KB a stage), no fewer than kRunRows keys each
-        const int per_head = std::max(1, (2 * D * (d->own.kv_shared ? 1 : 2) <= 512 ? 512 : 256) / Hkv);
-        int keys = d->split_keys;
-        if (keys == 0) {
-            keys = std::max(kRunRows, ((P + per_head - 1) / per_head + 15) / 16 * 16);
-            keys = std::min(keys, (P + 15) / 16 * 16);
-        }
-        p.run_keys = keys;
-        p.splits = (P + keys - 1) / keys;
-        p.tile_groups = (unsigned) (p.splits * Hkv);
-    } else {
-        p.run_keys = 0;
-        p.tile_groups = (unsigned) (p.tiles * Hkv * p.splits);
-    }
-    // Own rows: runs of 128 KB, so that a workgroup of the grid takes about as long as a tile's.
-    const int row_bytes = 2 * D * (d->own.kv_shared ? 1 : 2);
-    int chunk = d->own.split_rows > 0 ? d->own.split_rows : std::max(kRunRows, 128 * 1024 / row_bytes);
+    p = PrefixParams{};
+    p.Hq = d->own.num_q_heads;
+    p.Hkv = Hkv;
+    p.G = own.G;
+    p.Sq = B;
+    p.Sk = P;
+    p.q_pos0 = P - 1;  // every row at or past the last key
+    p.q_hs = D;
+    p.q_rs = (long long) p.Hq * D;
+    p.kv_hs = d->prefix_head_stride;
+    p.scale_log2e = d->own.scale * kLog2e;
+    // Own rows: about two workgroups a CU, no fewer than kRunRows rows each.
+    const long long own_rows = (long long) own.maxvis * B * Hkv;
+    int chunk = d->own.split_rows;
+    if (chunk == 0) chunk = (int) std::max<long long>(kRunRows, (own_rows / 512 + 15) / 16 * 16);
     if ((own.maxvis + chunk - 1) / chunk > 64) chunk = ((own.maxvis + 63) / 64 + 15) / 16 * 16;
     p.own_chunk = chunk;
     p.own_splits = (own.maxvis + chunk - 1) / chunk;
-    if ((long long) p.tile_groups + (long long) B * Hkv * p.own_splits > INT_MAX / 512)
+    // Form and key splits of the prefix: the cheapest by the workgroups of both kinds on the GPU, the
+    // bytes at what HBM gives, and the merge of the partials.
+    const float row_kb = 2.0f * D * (shared ? 1 : 2) / 1024;
+    const int group_rows = B * p.G;
+    const float own_us = 6.0f + std::min(chunk, own.maxvis) * row_kb / 40.0f;
+    const long long own_groups = (long long) B * Hkv * p.own_splits;
+    const float floor_us = 6.0f + ((float) P * Hkv + own_rows) * row_kb / 5600.0f;
+    Form f[4];
+    const int nf = forms_of(D, group_rows, shared, f);
+    float best = INFINITY;
+    for (int i = 0; i < nf; ++i) {
+        const int least = f[i].ng ? kRunRows : kStageKeys, unit = f[i].ng ? 16 : kStageKeys;
+        const int tiles = (group_rows + f[i].rows() - 1) / f[i].rows();
+        auto consider = [&](int keys) {
+            const int splits = (P + keys - 1) / keys;
+            const long long groups = (long long) tiles * Hkv * splits;
+            const float us = f[i].start + std::min(keys, P) * row_kb * f[i].per_kb;
+            const float span = f[i].ng ? makespan(own_groups, own_us, groups, us, f[i].slots)
+                                       : makespan(groups, us, own_groups, own_us, f[i].slots);
+            const int n = splits + p.own_splits;
+            // (plans that the bytes bound alike: the shorter workgroups keep more loads in flight)
+            const float cost = std::max(span, floor_us) + 0.3f * std::min(span, floor_us) + (n <= 8 ? 3.5f : 4.0f) +
+                               2.2e-7f * 4 * D * rows * n;
+            if (cost >= best) return;
+            best = cost;
+            p.qb = f[i].qb;
+            p.kh = f[i].kh;
+            p.nw = f[i].nw;
+            p.tiles = tiles;
+            p.splits = splits;
+            p.kps = keys;
+            p.run_keys = f[i].ng ? keys : 0;
+            p.row_groups = f[i].ng ? tiles : 0;
+        };
+        if (d->split_keys > 0) {
+            consider(d->split_keys);
+            continue;
+        }
+        int last = 0;
+        for (int s = 1; s <= 512; s += s < 64 ? 1 : 8) {
+            const int keys = std::max(least, ((P + s - 1) / s + unit - 1) / unit * unit);
+            if (keys != last) consider(keys);
+            if (keys == least) break;
+            last = keys;
+        }
+    }
+    p.part_nt = 4.0f * D * rows * p.splits <= kPartNtBytes;
+    if (p.splits > 65535 || (long long) p.tiles * Hkv * p.splits > INT_MAX / 1024)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: too many key splits");
+    p.tile_groups = (unsigned) (p.run_keys ? (p.splits * Hkv + 7) / 8 * 8 * p.row_groups : p.tiles * Hkv * p.splits);
+    p.own_groups = (unsigned) (B * Hkv * p.own_splits);
+    if ((long long) p.tile_groups + p.own_groups > INT_MAX / 512)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: too many splits");
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t pre = rows * p.splits, mine = rows * p.own_splits;
@@ -217,14 +303,45 @@ int make_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     return ESDA_OK;
 }
 
+// The plan of the calling thread's last description, kept: it depends on that alone, and a step asks
+// for it at every call.  (Descriptions compare by their bytes; other padding only plans anew.)
+int make_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
+    struct Last {
+        esda_prefix_desc desc;
+        PrefixPlan plan;
+        bool set = false;
+    };
+    thread_local Last last;
+    if (!d || !last.set || std::memcmp(d, &last.desc, sizeof(*d)) != 0) {
+        const int rc = fresh_prefix_plan(d, pl);
+        if (rc) return rc;
+        std::memcpy(&last.desc, d, sizeof(*d));
+        last.plan = *pl;
+        last.set = true;
+        return ESDA_OK;
+    }
+    *pl = last.plan;
+    return ESDA_OK;
+}
+
 template <int D>
 hipError_t launch_step(const PrefixParams &p, const PrefixMergeParams &m, bool shared, hipStream_t st) {
     if (p.run_keys > 0) {
-        const dim3 grid(p.tile_groups + (unsigned) (p.Sq * p.Hkv * p.own_splits)), block(256);
-        if (shared) hipLaunchKernelGGL((prefix_run_kernel<D, true>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((prefix_run_kernel<D, false>), grid, block, 0, st, p);
+        const dim3 grid(p.tile_groups + p.own_groups), block(256);
+        auto run = [&](auto ng) {
+            constexpr int NG = decltype(ng)::value;
+            if (shared) hipLaunchKernelGGL((prefix_run_kernel<D, true, NG>), grid, block, 0, st, p);
+            else hipLaunchKernelGGL((prefix_run_kernel<D, false, NG>), grid, block, 0, st, p);
+        };
+        // (forms_of: 16 rows a workgroup at D = 512, up to 64 at D = 128)
+        if constexpr (D == 512) run(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            if (p.Sq * p.G <= 16) run(std::integral_constant<int, 1>{});
+            else if (p.Sq * p.G <= 32) run(std::integral_constant<int, 2>{});
+            else run(std::integral_constant<int, 4>{});
+        }
     } else {
-        launch_tiles<D>(p, st);
+        esda_detail::prefix_tiles(p, D, st);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -14,37 +14,42 @@
 
 namespace esda_stream {
 
-// Rows [j0, j1) of a kv head's nvis visible ones, for G <= 16 query rows.
+// Rows [j0, j1) of a kv head's nvis visible ones, for G query rows.
 struct Run {
     uint16_t *k, *v;               // the cache rows of the kv head
     const uint16_t *k_new, *v_new; // the new token's rows (the last visible row), or null
     int G, j0, j1, nvis, first, cap, newrow;
 };
 
-// AW of the workgroup's NW waves take stages, each with SLOTS slots.
-template <int D, bool SH, int AW, int SLOTS>
+// AW of the workgroup's NW waves take stages, each with SLOTS slots; up to 16 NG query rows.
+template <int D, bool SH, int AW, int SLOTS, int NG = 1>
 struct Layout {
     static constexpr int BLK = 1056;                // LDS bytes per DMA block: 1 KB + 32 B pad
     static constexpr int NI = D / 32;               // DMA blocks of a tensor's 16-row stage
     static constexpr int HB = NI * BLK;
     static constexpr int SLOT = (SH ? 1 : 2) * HB;
     static constexpr int CPR = D / 8;               // 16-byte chunks per row
-    static constexpr int CH = D < 256 ? D : 256;    // dims the waves' O are summed over at a time
-    static constexpr int SUM = AW * 16 * CH * 4;
+    static constexpr int ROWS = 16 * NG;
+    static constexpr int CH = D < 32768 / (AW * ROWS) ? D : 32768 / (AW * ROWS);  // dims the waves' O are summed over at a time
+    static constexpr int PITCH = CH + 4;            // floats between the rows of that sum: 16 rows a multiple of
+                                                    // 128 bytes apart made each of its writes 16 (512 dims: 7 us)
+    static constexpr int SUM = AW * ROWS * PITCH * 4;
+    static_assert(CH % 16 == 0 && D % CH == 0, "whole tiles of dims at a time");
     static constexpr int RING = AW * SLOTS * SLOT;
     static constexpr int TOTALS = RING > SUM ? RING : SUM;
-    static constexpr int BYTES = TOTALS + (AW + 1) * 16 * 8;
+    static constexpr int BYTES = TOTALS + (AW + 1) * ROWS * 8;
     // Row r of a stage: block r % NI, 2D bytes times r / NI into it (free of bank conflicts for both
     // the 128-bit row reads and the transpose reads).
     __device__ static constexpr int off(int r) { return (r % NI) * BLK + (r / NI) * 2 * D; }
 };
 
 // Attends the run; every thread of the workgroup calls it.  query(h): query row h; score(x, j): the
-// log2-domain score of raw product x and visible row j, of query row `lane & 15`; put(h, d, o, M, T):
-// called once for each query row h and four dims from d on, with O, its maximum and its sum.
-template <int D, bool SH, int NW, int AW, int SLOTS, class Query, class Score, class Put>
+// log2-domain score of raw product x and visible row j, of query row `lane & 15` (of each 16);
+// put(h, d, o, M, T): called once for each query row h and four dims from d on, with O, its maximum
+// and its sum.  Each K and V read from LDS serves NG products of 16 query rows.
+template <int D, bool SH, int NW, int AW, int SLOTS, int NG, class Query, class Score, class Put>
 __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
-    using L = Layout<D, SH, AW, SLOTS>;
+    using L = Layout<D, SH, AW, SLOTS, NG>;
     constexpr int KS = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
@@ -79,17 +84,27 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
     };
 
     if (wave < nst) dma(wave, ring);
-    bf16x8 qv[KS];  // B operand: head li, dims 32 ks + 8 lg ..
+    bf16x8 qv[NG][KS];  // B operands: query row 16 g + li, dims 32 ks + 8 lg ..
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 w = li < x.G ? *reinterpret_cast<const u32x4 *>(query(li) + 32 * ks + 8 * lg) : u32x4{0u, 0u, 0u, 0u};
-        qv[ks] = __builtin_bit_cast(bf16x8, w);
+    for (int g = 0; g < NG; ++g) {
+        const bool there = 16 * g + li < x.G;
+        const uint16_t *const qr = query(there ? 16 * g + li : 0) + 8 * lg;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(qr + 32 * ks);
+            qv[g][ks] = __builtin_bit_cast(bf16x8, there ? w : u32x4{0u, 0u, 0u, 0u});
+        }
     }
     const int qk_off = L::off(li) + lg * 16, tr_off = L::off(4 * lg + li / 4) + (li % 4) * 8;
-    float m = -INFINITY, l = 0.0f;
-    f32x4 acc[DT];
+    float m[NG], l[NG];
+    f32x4 acc[NG][DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < NG; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[g][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     for (int st = wave, it = 0; st < nst; st += AW, ++it) {
         unsigned char *const slot = ring + (SLOTS > 1 ? (it & 1) * L::SLOT : 0);
@@ -99,41 +114,77 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
             dma(st + AW, ring + ((it + 1) & 1) * L::SLOT);
         }
         asm volatile("" ::: "memory");
-        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // rows 4 lg + r of head li
+        // Every K read of the stage, then the products, then every V read, which lands during the
+        // softmax.  The scores of few rows go through several sums (a chain of D / 32 products waits for
+        // each of them).
+        constexpr int CHAINS = NG >= 4 ? 1 : 4 / NG;
+        bf16x8 k8[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(slot + qk_off + 64 * ks), qv[ks], s, 0, 0, 0);
-        const int jt = x.j0 + 16 * st + 4 * lg;
+        for (int ks = 0; ks < KS; ++ks) k8[ks] = *reinterpret_cast<const bf16x8 *>(slot + qk_off + 64 * ks);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 s[NG];  // rows 4 lg + r of query row 16 g + li
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = jt + r < x.j1 ? score(s[r], jt + r) : -INFINITY;
-        const float top = wave_max_across_groups(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-        if (__any(top > m + kRescaleSlack)) {
-            const float mn = fmaxf(m, top), corr = __builtin_amdgcn_exp2f(m - mn);
-            l *= corr;
+        for (int g = 0; g < NG; ++g) {
+            f32x4 part[CHAINS];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[dt] *= corr;
-            m = mn;
+            for (int c = 0; c < CHAINS; ++c) part[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                part[ks % CHAINS] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8[ks], qv[g][ks], part[ks % CHAINS], 0, 0, 0);
+            s[g] = part[0];
+#pragma unroll
+            for (int c = 1; c < CHAINS; ++c) s[g] += part[c];
         }
-        short4v pb;  // the weights as they enter both sums: bf16
+        short4v va[DT];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const __bf16 w = (__bf16) __builtin_amdgcn_exp2f(s[r] - m);
-            l += (float) w;
-            pb[r] = __builtin_bit_cast(short, w);
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        for (int dt = 0; dt < DT; ++dt)
+            va[dt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) short4v *) (slot + (SH ? 0 : L::HB) + tr_off + 32 * dt));
-            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, pb, acc[dt], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        const int jt = x.j0 + 16 * st + 4 * lg;
+        float top[NG];
+        bool raise = false;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[g][r] = jt + r < x.j1 ? score(s[g][r], jt + r) : -INFINITY;
+            top[g] = wave_max_across_groups(fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])));
+            raise = raise || top[g] > m[g] + kRescaleSlack;
         }
+        if (__any(raise)) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float mn = top[g] > m[g] + kRescaleSlack ? top[g] : m[g];
+                const float corr = mn == m[g] ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mn);
+                l[g] *= corr;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[g][dt] *= corr;
+                m[g] = mn;
+            }
+        }
+        short4v pb[NG];  // the weights as they enter both sums: bf16
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const __bf16 w = (__bf16) __builtin_amdgcn_exp2f(s[g][r] - m[g]);
+                l[g] += (float) w;
+                pb[g][r] = __builtin_bit_cast(short, w);
+            }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(va[dt], pb[g], acc[g][dt], 0, 0, 0);
         if (SLOTS == 1 && st + AW < nst) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads are done
             dma(st + AW, ring);
         }
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        l[g] += __shfl_xor(l[g], 16);
+        l[g] += __shfl_xor(l[g], 32);
+    }
 
     // The new row into the cache (bit-exact) by the run that ends with it; no other run reads it.
     if (append && x.j1 == x.nvis && wave == 0)
@@ -144,31 +195,41 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         }
 
     // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = -inf, l = 0.
-    f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + AW * 16;  // [AW][16], [16]
-    float *const sum = reinterpret_cast<float *>(lds);                                      // [AW][G][CH]
-    if (lg == 0 && wave < AW) ml[wave * 16 + li] = f32x2{m, l};
+    f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + AW * L::ROWS;  // [AW][ROWS], [ROWS]
+    float *const sum = reinterpret_cast<float *>(lds);                                           // [AW][G][PITCH]
+    if (lg == 0 && wave < AW)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) ml[wave * L::ROWS + 16 * g + li] = f32x2{m[g], l[g]};
     lds_barrier();  // and every wave is done with its slots
-    float M = -INFINITY, T = 0.0f;
+    float c[NG];
 #pragma unroll
-    for (int w = 0; w < AW; ++w) M = fmaxf(M, ml[w * 16 + li][0]);
-    const float mu = M == -INFINITY ? 0.0f : M;
+    for (int g = 0; g < NG; ++g) {
+        const f32x2 *const of = ml + 16 * g + li;
+        float M = -INFINITY, T = 0.0f;
 #pragma unroll
-    for (int w = 0; w < AW; ++w) T = __builtin_fmaf(ml[w * 16 + li][1], __builtin_amdgcn_exp2f(ml[w * 16 + li][0] - mu), T);
-    if (wave == 0 && lg == 0) tot[li] = f32x2{M, T};
-    const float c = __builtin_amdgcn_exp2f(m - mu);
+        for (int w = 0; w < AW; ++w) M = fmaxf(M, of[w * L::ROWS][0]);
+        const float mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < AW; ++w) T = __builtin_fmaf(of[w * L::ROWS][1], __builtin_amdgcn_exp2f(of[w * L::ROWS][0] - mu), T);
+        if (wave == 0 && lg == 0) tot[16 * g + li] = f32x2{M, T};
+        c[g] = __builtin_amdgcn_exp2f(m[g] - mu);
+    }
     const int live = all < AW ? all : AW;  // waves that had a stage
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += L::CH) {
-        if (li < x.G && wave < live) {
+        if (wave < live)
 #pragma unroll
-            for (int dt = 0; dt < L::CH / 16; ++dt)
-                *reinterpret_cast<f32x4 *>(sum + (wave * x.G + li) * L::CH + 16 * dt + 4 * lg) = acc[d0 / 16 + dt] * c;
-        }
+            for (int g = 0; g < NG; ++g)
+                if (16 * g + li < x.G) {
+#pragma unroll
+                    for (int dt = 0; dt < L::CH / 16; ++dt)
+                        *reinterpret_cast<f32x4 *>(sum + (wave * x.G + 16 * g + li) * L::PITCH + 16 * dt + 4 * lg) = acc[g][d0 / 16 + dt] * c[g];
+                }
         lds_barrier();
         for (int t = threadIdx.x; t < x.G * (L::CH / 4); t += 64 * NW) {
             const int h = t / (L::CH / 4), d = 4 * (t % (L::CH / 4));
-            f32x4 o = *reinterpret_cast<const f32x4 *>(sum + h * L::CH + d);
-            for (int w = 1; w < live; ++w) o += *reinterpret_cast<const f32x4 *>(sum + (w * x.G + h) * L::CH + d);
+            f32x4 o = *reinterpret_cast<const f32x4 *>(sum + h * L::PITCH + d);
+            for (int w = 1; w < live; ++w) o += *reinterpret_cast<const f32x4 *>(sum + (w * x.G + h) * L::PITCH + d);
             put(h, d0 + d, o, tot[h][0], tot[h][1]);
         }
         lds_barrier();  // before the next dims, or the next run's DMAs
