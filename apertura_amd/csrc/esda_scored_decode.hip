@@ -1,6 +1,6 @@
 // esda_scored_decode.hip -- the decode step with capped or biased scores for MI355X (gfx950):
-// attend_kernel (esda_attend.h) with ScoredAttendParams, and the plain step's split merge.  The C
-// ABI is include/esda_scored.h.
+// attend_kernel (esda_attend.h) with ScoredAttendParams, at head_dim 128 stream_kernel below, and
+// the plain step's plan and split merge.  The C ABI is include/esda_scored.h.
 
 #include <hip/hip_runtime.h>
 
@@ -11,11 +11,62 @@
 #include "esda_attend.h"
 #include "esda_internal.h"
 #include "esda_scored.h"
+#include "esda_stream.h"
+
+namespace {
+
+// head_dim 128: a 16-row stage is 4 or 8 KB, too little for a barrier and a score exchange between
+// the waves.  Here each of eight waves streams stages of its own: a step of 16 sequences of 2K .. 16K
+// rows, 8 kv heads, 599 MB 101 us (5.9 TB/s; attend_kernel 144), one of 131,072 rows 82 us (6.5 TB/s;
+// 115), of 16,384 16.3 (22.3), of 300 8.1 (9.0); K = V, 16 of 512 .. 4096 23.4 (39.4).
+constexpr int kStreamWaves = 8;
+
+template <bool SH>
+__global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(ScoredAttendParams p) {
+    constexpr int D = 128, SLOTS = 2;
+    using L = esda_stream::Layout<D, SH, kStreamWaves, SLOTS>;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
+    const int li = threadIdx.x & 15;
+    auto segment = [&](const int b, const int kvh, const int j0, const int j1, const SeqView sv, const size_t slot,
+                       const bool direct) __attribute__((always_inline)) {
+        const size_t head = (size_t) b * p.seq_stride + (size_t) kvh * p.head_stride, at = ((size_t) b * p.Hkv + kvh) * D;
+        const esda_stream::Run x{p.k_cache + head, p.v_cache + head, p.k_new + at, SH ? p.k_new + at : p.v_new + at,
+                                 p.G, j0, j1, sv.nvis, sv.first, p.cap, sv.newrow};
+        const uint16_t *const q = p.q + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;
+        uint16_t *const out = p.out + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;
+        const float slope = p.slopes && li < p.G ? p.slopes[kvh * p.G + li] * kLog2e : 0.0f;
+        esda_stream::attend_run<D, SH, kStreamWaves, kStreamWaves, SLOTS, 1>(
+            lds, x, [&](int h) { return q + (size_t) h * D; },
+            [&](float s, int j) {
+                float y = s * p.scale_log2e;
+                if (p.cap_out != 0.0f)  // tanh(y) = 1 - 2 / (1 + e^2y)
+                    y = p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.cap_in)), 1.0f);
+                return __builtin_fmaf(-slope, (float) (sv.nvis - 1 - j), y);
+            },
+            [&](int h, int d, const f32x4 &o, float M, float T) {
+                if (direct) {
+                    const float inv = 1.0f / T;
+                    bf16x4 r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] = (__bf16) (o[e] * inv);
+                    *reinterpret_cast<bf16x4 *>(out + (size_t) h * D + d) = r;
+                } else {
+                    const size_t at = slot * p.G + h;
+                    *reinterpret_cast<f32x4 *>(p.part_acc + at * D + d) = o;
+                    if (d == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * at) = f32x2{M, T};
+                }
+            });
+    };
+    walk_segments<kStreamWaves>(p, segment);
+}
+
+}  // namespace
 
 extern "C" int esda_scored_decode(const esda_decode_desc *d, const esda_score *s, const esda_decode_args *a, void *stream) {
     Plan pl;
     int rc = make_plan(d, &pl);
     if (rc) return rc;
+    if (d->head_dim == 128) pl.pk = 1;  // stream_kernel takes one kv head a workgroup (the same partials)
     if (!s) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: null score");
     if (!(s->softcap >= 0.0f) || !std::isfinite(s->softcap))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: softcap must be 0 or positive and finite");
@@ -43,7 +94,14 @@ extern "C" int esda_scored_decode(const esda_decode_desc *d, const esda_score *s
     uint16_t *out = static_cast<uint16_t *>(a->out);
     fill_attend(d, pl, sp, static_cast<int *>(a->workspace), out, ap);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = dispatch_attend(d->head_dim, d->kv_shared != 0, ap, attend_grid(d, pl), st);
+    hipError_t e;
+    if (d->head_dim == 128) {
+        if (d->kv_shared) hipLaunchKernelGGL(stream_kernel<true>, attend_grid(d, pl), dim3(64 * kStreamWaves), 0, st, ap);
+        else hipLaunchKernelGGL(stream_kernel<false>, attend_grid(d, pl), dim3(64 * kStreamWaves), 0, st, ap);
+        e = hipGetLastError();
+    } else {
+        e = dispatch_attend(d->head_dim, d->kv_shared != 0, ap, attend_grid(d, pl), st);
+    }
     if (e != hipSuccess) return hip_fail(e, "attend_kernel launch");
     return launch_merge(d, pl, sp, a->pos, a->row_base, 0, out, st);
 }
