@@ -161,7 +161,8 @@ struct PRing {
 // no mask, and the ids of the others come with their keys by DMA.
 template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves,
           class P = PrefillParams>
-__global__ __launch_bounds__(64 * NW, 1) void prefill_kernel(P p) {
+// (D == 128 on four waves: two workgroups per CU)
+__global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_kernel(P p) {
     constexpr bool DOCS = std::is_same<P, DocParams>::value;
     constexpr bool SCORED = DOCS || std::is_same<P, ScoredParams>::value;
     constexpr bool PARTS = std::is_same<P, PrefixParams>::value;  // a partial from every split, also one
@@ -1089,6 +1090,8 @@ void launch_tiles(const P &p, hipStream_t st) {
         else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, kWaves, P>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
     }
+    else if constexpr (D == 128 && std::is_base_of<ScoredParams, P>::value)
+        hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, 4, P>), grid, block, 0, st, p);
     else if constexpr (D == 128)
         hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
     else if (p.qb == 2)

@@ -104,6 +104,7 @@ struct PrefixParams : PrefillParams {
 struct Tiling {
     int qb, kh, nw;
     float wg, row, stage;
+    int occ = 1;  // workgroups per CU
     int rows() const { return 16 * qb * (kh ? nw / 2 : nw); }
 };
 
@@ -117,6 +118,11 @@ constexpr Tiling kTilings512[] = {{1, 0, 8, 5.7f, 0.076f, 1.54f}, {1, 0, 4, 6.2f
 constexpr Tiling kTilings256[] = {{2, 0, 8, 5.47f, 0.033f, 1.7f}, {1, 0, 8, 4.94f, 0.036f, 1.014f},
                                   {1, 1, 8, 5.93f, 0.05f, 0.62f}};
 constexpr Tiling kTilings128[] = {{2, 0, 8, 5.16f, 0.017f, 1.055f}};
+// Scored calls at D = 128 are bound by the scores' instructions and, with documents, by tiles of
+// unlike length: two workgroups of four waves per CU overlap one's start, masks and softmax with the
+// other's products.  4096 queries of 32 heads over 8 182 -> 164 us, 1500 64 -> 52, packed documents of
+// 16 .. 1000 tokens 93 -> 80 and 46 -> 38.
+constexpr Tiling kTilings128Scored[] = {{2, 0, 4, 5.2f, 0.017f, 1.16f, 2}};
 
 constexpr int kXcds = 8, kEngines = 4, kEngineCus = kTargetGroups / (kXcds * kEngines);
 constexpr float kEmptyUs = 1.0f;  // a workgroup whose split holds no key of its tile
@@ -130,7 +136,8 @@ constexpr float kEmptyUs = 1.0f;  // a workgroup whose split holds no key of its
 // of the GPU, or of the XCD, to the next workgroup: 52 and 73 us estimated for those two.)
 // nst: stages of each tile, latest first; last_rows: query rows of the latest tile.
 inline float makespan(const Tiling &t, const int *nst, int tiles, int last_rows, int Hkv, int splits, int per) {
-    float ends[kXcds][kEngines][kEngineCus] = {}, front[kXcds] = {};
+    float ends[kXcds][kEngines][2 * kEngineCus] = {}, front[kXcds] = {};
+    const unsigned cus = kEngineCus * t.occ;  // workgroups an engine holds
     float most = 0.0f;
     unsigned wg = 0;
     for (int i = 0; i < tiles; ++i)
@@ -141,9 +148,9 @@ inline float makespan(const Tiling &t, const int *nst, int tiles, int last_rows,
                 const unsigned xcd = wg % kXcds;
                 float *e = ends[xcd][wg / kXcds % kEngines];
                 unsigned cu = wg / (kXcds * kEngines);
-                if (cu >= kEngineCus) {
+                if (cu >= cus) {
                     cu = 0;
-                    for (int c = 1; c < kEngineCus; ++c) cu = e[c] < e[cu] ? c : cu;
+                    for (unsigned c = 1; c < cus; ++c) cu = e[c] < e[cu] ? c : cu;
                     front[xcd] = std::max(front[xcd], e[cu]);
                 }
                 e[cu] = front[xcd] + us;
@@ -221,7 +228,8 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
     // rounds of 256 CUs: 333 queries over 5933 keys (K = V, 21 tiles of 4 heads) take 126 us as 252
     // workgroups and 190 as 336, whose second round is mostly idle.
     const long long rows = (long long) d->seq_q * p->G;
-    const Tiling *forms = D == 512 ? kTilings512 : D == 256 ? kTilings256 : kTilings128;
+    const Tiling *forms = D == 512 ? kTilings512 : D == 256 ? kTilings256
+                          : std::is_same<P, ScoredParams>::value ? kTilings128Scored : kTilings128;
     const int nforms = D == 512 ? 2 : D == 256 ? 3 : 1;
     float best = INFINITY;
     int kps = 0, most_stages = 0;  // of the best plan
@@ -247,7 +255,8 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
             if (i || last_rows == QT) most_full = std::max(most_full, n);
             total += t.wg + t.row * (i ? QT : last_rows) + n * t.stage;
         }
-        const float even = (float) (total * d->num_kv_heads / kTargetGroups);
+        const int slots = kTargetGroups * t.occ;
+        const float even = (float) (total * d->num_kv_heads / slots);
         auto consider = [&](int per) {  // per: stages per split
             const int splits = (most + per - 1) / per;
             float us = splits > 1 ? split_cost(4.0f * D * (float) rows * d->num_kv_heads * splits, splits) : 0.0f;
@@ -255,7 +264,7 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
                                            most_full ? t.wg + t.row * QT + std::min(per, most_full) * t.stage : 0.0f);
             // no plan is faster than its longest workgroup, nor than its work spread evenly
             if (us + std::max(longest, even) >= best) return;
-            if (groups * splits <= kTargetGroups) {
+            if (groups * splits <= slots) {
                 us += longest;  // one round
             } else if (few && groups * splits <= 2LL * kMaxRounds * kTargetGroups) {
                 // nor than its pieces' work spread evenly, nor the rounds that its whole pieces take
@@ -264,8 +273,8 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
                     whole += nst[i] / per;
                     pieces += (nst[i] + per - 1) / per;
                 }
-                const int rounds = (whole * d->num_kv_heads + kTargetGroups - 1) / kTargetGroups;
-                const float spread = even + (float) (pieces - tiles) * d->num_kv_heads * t.wg / kTargetGroups;
+                const int rounds = (whole * d->num_kv_heads + slots - 1) / slots;
+                const float spread = even + (float) (pieces - tiles) * d->num_kv_heads * t.wg / slots;
                 if (us + std::max(spread, rounds * (t.wg + per * t.stage)) >= best) return;
                 us += makespan(t, nst, (int) tiles, last_rows, d->num_kv_heads, splits, per);
             } else {
@@ -273,7 +282,7 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
                 // the CUs stay busy but for the end of the last round.  (70 chunks of forced splits that
                 // took shorter tiles without the pieces' starts: 14% less time on average; 3028 queries
                 // over 3787 keys in 4 splits, D = 256, 16 heads, 344 us in 128-row tiles, 229 in 256-row.)
-                const double more = (double) tiles * (splits - 1) * d->num_kv_heads / kTargetGroups;
+                const double more = (double) tiles * (splits - 1) * d->num_kv_heads / slots;
                 us += even + (float) more * (t.wg + t.row * QT) + 0.5f * (t.wg + t.row * QT + std::min(per, most) * t.stage);
             }
             if (us < best) {
