@@ -208,7 +208,8 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     if (rc) return rc;
     if (d->own.ring || d->own.window)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: own caches are linear and without a window");
-    if (d->prefix_len <= 0) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: prefix_len must be positive");
+    if (d->prefix_len <= 0 || d->prefix_len > 1 << 30)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: prefix_len must be 1 .. 2^30");
     if ((long long) d->prefix_len + d->own.batch > INT_MAX || (long long) d->prefix_len + d->own.cap > INT_MAX)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: positions must stay below 2^31");
     if (d->prefix_head_stride < (int64_t) d->prefix_len * d->own.head_dim || d->prefix_head_stride % 8)
@@ -236,10 +237,11 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     // Own rows: about two workgroups a CU, no fewer than kRunRows rows each.
     const long long own_rows = (long long) own.maxvis * B * Hkv;
     int chunk = d->own.split_rows;
-    if (chunk == 0) chunk = (int) std::max<long long>(kRunRows, (own_rows / 512 + 15) / 16 * 16);
-    if ((own.maxvis + chunk - 1) / chunk > 64) chunk = ((own.maxvis + 63) / 64 + 15) / 16 * 16;
+    if (chunk == 0) chunk = (int) std::max<long long>(kRunRows, (std::min<long long>(own_rows / 512, own.maxvis) + 15) / 16 * 16);
+    auto own_splits = [&] { return (int) (((long long) own.maxvis + chunk - 1) / chunk); };
+    if (own_splits() > 64) chunk = (own.maxvis / 64 + 16) / 16 * 16;
     p.own_chunk = chunk;
-    p.own_splits = (own.maxvis + chunk - 1) / chunk;
+    p.own_splits = own_splits();
     // Form and key splits of the prefix: the cheapest by the workgroups of both kinds on the GPU, the
     // bytes at what HBM gives, and the merge of the partials.
     const float row_kb = 2.0f * D * (shared ? 1 : 2) / 1024;

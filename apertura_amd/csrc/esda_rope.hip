@@ -197,8 +197,8 @@ int esda_rope(const esda_rope_desc *d, const esda_rope_args *a, void *stream) {
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: head_dim must be 128, 256 or 512");
     if (d->rot_dim < 2 || d->rot_dim > D || d->rot_dim % 2)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: rot_dim must be even, 2 .. head_dim");
-    if (T < 0 || Hq < 0 || Hk < 0 || Hq > 65536 || Hk > 65536 || Hq + Hk == 0)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: tokens and head counts must not be negative, and some head given");
+    if (T < 0 || T > 1 << 30 || Hq < 0 || Hk < 0 || Hq > 65536 || Hk > 65536 || Hq + Hk == 0)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: 0 .. 2^30 tokens, 0 .. 65536 heads of each kind, and some head given");
     if ((d->interleaved & ~1) || (d->inverse & ~1))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: interleaved and inverse are 0 or 1");
     if (!std::isfinite(d->attn_factor))

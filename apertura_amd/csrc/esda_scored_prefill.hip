@@ -62,6 +62,8 @@ int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, 
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: null pointer");
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: tensors must be 16-byte aligned");
+    if (a->out == a->q || a->out == a->k || a->out == a->v)
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: out must not be an input");
     if (!a->q_doc != !a->k_doc)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: q_doc and k_doc go together");
     if ((reinterpret_cast<uintptr_t>(a->k_doc) | reinterpret_cast<uintptr_t>(a->q_doc) |

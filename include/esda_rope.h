@@ -31,9 +31,9 @@ extern "C" {
  * the first n frequencies (the reference's global layers).
  * An output may be its input with the same strides; otherwise they must not overlap. */
 typedef struct esda_rope_desc {
-    int32_t tokens;       /* >= 0                                             */
-    int32_t num_q_heads;  /* >= 0; 0: no q                                    */
-    int32_t num_k_heads;  /* >= 0; 0: no k                                    */
+    int32_t tokens;       /* 0 .. 2^30                                        */
+    int32_t num_q_heads;  /* 0 .. 65536; 0: no q                              */
+    int32_t num_k_heads;  /* 0 .. 65536; 0: no k                              */
     int32_t head_dim;     /* 128, 256 or 512                                  */
     int32_t rot_dim;      /* even, 2 .. head_dim                              */
     int32_t interleaved;  /* 0: pairs (i, i + rot_dim/2); 1: pairs (2i, 2i+1) */

@@ -41,7 +41,8 @@ typedef struct esda_score {
 /* ------------------------------------------------------------------------- prefill
  * esda_prefill with these scores and masks.  The keys need not hold the queries' own positions
  * (key positions stay below 2^31 - 64).  A value of k or v that is not finite reaches only the
- * queries that see its key. */
+ * queries that see its key.  out must not overlap q, k or v (unlike the plain call's, q's rows may
+ * be read after rows of out are written). */
 typedef struct esda_scored_prefill_args {
     const void *q, *k, *v; /* as esda_prefill_args; k == v allowed            */
     void *out;

@@ -34,7 +34,7 @@ def test_a_bound_on_own_rows_sizes_their_splits():
 
 
 @pytest.mark.parametrize("kw", [
-    dict(prefix_len=0), dict(prefix_len=-1), dict(prefix_head_stride=99 * 128), dict(prefix_head_stride=100 * 128 + 4),
+    dict(prefix_len=0), dict(prefix_len=-1), dict(prefix_len=2 ** 30 + 1), dict(prefix_head_stride=99 * 128), dict(prefix_head_stride=100 * 128 + 4),
     dict(split_keys=16), dict(split_keys=-32), dict(window=16), dict(ring=True, window=64), dict(head_dim=64),
     dict(num_q_heads=9), dict(num_q_heads=34), dict(batch=0), dict(batch=257), dict(cap=0), dict(scale=0.0),
     dict(scale=math.nan), dict(split_rows=8),

@@ -90,7 +90,7 @@ def _call(q=FAKE, k=FAKE + (1 << 24), q_out=FAKE + (2 << 24), k_out=FAKE + (3 <<
 
 
 @pytest.mark.parametrize("kw", [
-    dict(head_dim=64), dict(head_dim=96), dict(rot_dim=0), dict(rot_dim=3), dict(rot_dim=130), dict(tokens=-1),
+    dict(head_dim=64), dict(head_dim=96), dict(rot_dim=0), dict(rot_dim=3), dict(rot_dim=130), dict(tokens=-1), dict(tokens=2 ** 30 + 1), dict(num_k_heads=65537),
     dict(num_q_heads=-1), dict(num_q_heads=0, num_k_heads=0), dict(interleaved=2), dict(inverse=-1),
     dict(attn_factor=math.nan), dict(attn_factor=math.inf), dict(q=None), dict(k=None), dict(q_out=None),
     dict(k_out=None), dict(pos=None), dict(inv=None), dict(q=FAKE + 1), dict(pos=FAKE + 2), dict(q_row_stride=-8),

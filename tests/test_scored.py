@@ -57,14 +57,14 @@ def test_bad_chunks_are_refused(kw):
     assert ei.value.code == 1
 
 
-def _prefill(q=FAKE, k=FAKE, v=FAKE, out=FAKE, ws=None, nbytes=0, q_doc=None, k_doc=None, slopes=None, step=None):
+def _prefill(q=FAKE, k=FAKE, v=FAKE, out=FAKE + (1 << 24), ws=None, nbytes=0, q_doc=None, k_doc=None, slopes=None, step=None):
     d = (step or _step()).desc()
     s = _lib.ScoreDesc(0.0, 0, slopes)
     a = _lib.ScoredPrefillArgs(q, k, v, out, ws, nbytes, q_doc, k_doc)
     return _lib.lib().esda_scored_prefill(ctypes.byref(d), ctypes.byref(s), ctypes.byref(a), None)
 
 
-@pytest.mark.parametrize("kw", [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=FAKE + 8),
+@pytest.mark.parametrize("kw", [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=FAKE + 8), dict(out=FAKE),
                                 dict(out=FAKE + 2), dict(q_doc=FAKE), dict(k_doc=FAKE), dict(q_doc=FAKE, k_doc=FAKE + 1),
                                 dict(q_doc=FAKE + 2, k_doc=FAKE), dict(slopes=FAKE + 2)])
 def test_bad_prefill_arguments_are_refused(kw):

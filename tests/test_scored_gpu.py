@@ -166,6 +166,14 @@ def test_documents_far_behind(D, split):
     _run(D, 40, 6100 - 40, docs=(q_doc, k_doc), split=split, biased=True)
 
 
+def test_documents_over_more_keys_than_are_summed_up():
+    """140,000 keys in one split: the stages past the first 131,072 keys are computed with their mask."""
+    n = 140000
+    k_doc = (torch.arange(n, device=DEV) // 5000).to(torch.int32)
+    q_doc = torch.tensor([0, 26, 27, 27, -1, 13], dtype=torch.int32, device=DEV)
+    _run(128, 6, n - 6, docs=(q_doc, k_doc), split=1 << 20, biased=True, heads=(2, 1, False))
+
+
 @pytest.mark.parametrize("D", [128, 256, 512])
 def test_documents_with_prefix_and_window(D):
     ids = _ids("runs", 200, _gen(3))
