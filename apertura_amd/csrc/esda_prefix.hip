@@ -156,15 +156,15 @@ struct PrefixPlan {
     size_t off_pre_ml, off_own_ml, off_pre_acc, off_own_acc, bytes;
 };
 
-constexpr int kRunRows = 64;  // fewest rows of a run: a stage for each of four waves
+constexpr int kRunRows = 64;    // fewest rows of a run: a stage for each of four waves
+constexpr int kOwnSplits = 64;  // most own splits
 
 // How the prefix's query rows can be laid out: as tiles (nw > 0: a prefill form), or in runs of 16 NG
 // rows.  us of a workgroup: `start`, and per KB of K and V `per_kb`; slots: workgroups the GPU holds at
-// once.  Fitted to graph-replayed steps of forced splits (the keys in the Infinity Cache), us, runs /
-// tiles at the best split: D = 512 over one K = V buffer, 16 rows x 4096 keys 17.4 / 15.2, x 32768
-// 31.7 / 41.8, 32 rows 18.8 / 18.5 and 42.3 / 45.0, 64 rows x 16384 41.0 / 35.7; D = 128, 8 rows x 8192
-// keys 11.3 / 19.8, 16 x 32768 25.1 / 45.2, 32 x 16384 19.3 / 29.0, 64 28.2 / 30.6, 128 38.4 / 34.8;
-// D = 256, 8 rows x 8192 27.5 / 27.8, 32 37.5 / 30.1: always tiles.
+// once.  Runs / tiles at the best split, us: D = 512 over one K = V buffer, 16 rows x 4096 keys 17.4 /
+// 15.2, x 32768 31.7 / 41.8, 32 rows 18.8 / 18.5 and 42.3 / 45.0, 64 rows x 16384 41.0 / 35.7; D = 128,
+// 8 rows x 8192 keys 11.3 / 19.8, 16 x 32768 25.1 / 45.2, 32 x 16384 19.3 / 29.0, 64 28.2 / 30.6, 128
+// 38.4 / 34.8; D = 256, 8 rows x 8192 27.5 / 27.8, 32 37.5 / 30.1: always tiles.
 struct Form {
     int qb, kh, nw, ng;
     float start, per_kb;
@@ -172,18 +172,37 @@ struct Form {
     int rows() const { return ng ? 16 * ng : 16 * qb * (kh ? nw / 2 : nw); }
 };
 
+// What else a step's time goes by: us of an own workgroup and its KB per us; us and KB per us of the
+// bytes of both kinds; the share by which the two bounds add up; us of a merge of at most 8 partials a
+// row and of more; us per byte of partials.
+// These and the forms' costs are fitted, per head dim, to 330 steps (1 .. 64 sequences, prefixes of
+// 64 .. 40,000 keys, own caches of 64 .. 2048 rows, full, at random and nearly empty), each in every
+// form, in up to 7 own chunks and 9 prefix splits, graph-replayed (the keys in the Infinity Cache).
+struct StepCosts {
+    float own_start, own_rate, start, rate, add, few, many, part;
+};
+constexpr StepCosts kCosts512 = {8.0f, 40.0f, 8.7f, 7900.0f, 0.11f, 4.3f, 4.0f, 1.8e-7f};
+constexpr StepCosts kCosts256 = {4.6f, 77.0f, 3.5f, 5360.0f, 0.54f, 4.3f, 3.8f, 1.5e-7f};
+constexpr StepCosts kCosts128 = {4.4f, 43.0f, 5.3f, 7900.0f, 0.25f, 5.8f, 2.9f, 2.9e-7f};
+
 // The forms a step may take; returns their number.
 int forms_of(int D, int rows, bool shared, Form *f) {
     int n = 0;
     const Tiling *t = D == 512 ? kTilings512 : D == 256 ? kTilings256 : kTilings128;
     const int nt = D == 512 ? 2 : D == 256 ? 3 : 1;
+    // (a prefill workgroup's costs, and what a step's add to its start and to its stages)
+    constexpr float kMore512[][2] = {{5.1f, 0.96f}, {0.0f, 1.0f}};
+    constexpr float kMore256[][2] = {{6.9f, 1.15f}, {-2.4f, 1.15f}, {0.0f, 1.0f}};
+    constexpr float kMore128[][2] = {{0.0f, 1.6f}};
+    const float(*more)[2] = D == 512 ? kMore512 : D == 256 ? kMore256 : kMore128;
     const float stage_kb = 32.0f * 2 * D * (shared ? 1 : 2) / 1024;
     for (int i = 0; i < nt; ++i)
         if (!(D == 512 && rows <= 64 && t[i].nw == (shared ? 8 : 4)))  // (launch_tiles' choice for one tile)
-            f[n++] = {t[i].qb, t[i].kh, t[i].nw, 0, t[i].wg + t[i].row * std::min(rows, t[i].rows()), t[i].stage / stage_kb, 256};
-    if (D == 512 && rows <= 32) f[n++] = {0, 0, 0, 1, 13.0f, 1 / 60.0f, 256};
-    if (D == 128 && rows <= 64) f[n++] = rows <= 16 ? Form{0, 0, 0, 1, 8.0f, 1 / 58.0f, 512}
-                                         : rows <= 32 ? Form{0, 0, 0, 2, 8.0f, 1 / 43.0f, 512} : Form{0, 0, 0, 4, 10.0f, 1 / 27.0f, 256};
+            f[n++] = {t[i].qb, t[i].kh, t[i].nw, 0, t[i].wg + t[i].row * std::min(rows, t[i].rows()) + more[i][0],
+                      t[i].stage / stage_kb * more[i][1], 256};
+    if (D == 512 && rows <= 32) f[n++] = {0, 0, 0, 1, 11.6f, 1 / 60.0f, 256};
+    if (D == 128 && rows <= 64) f[n++] = rows <= 16 ? Form{0, 0, 0, 1, 5.8f, 1 / 65.0f, 512}
+                                         : rows <= 32 ? Form{0, 0, 0, 2, 13.2f, 1 / 56.0f, 512} : Form{0, 0, 0, 4, 13.1f, 1 / 32.0f, 256};
     return n;
 }
 
@@ -234,58 +253,65 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     p.q_rs = (long long) p.Hq * D;
     p.kv_hs = d->prefix_head_stride;
     p.scale_log2e = d->own.scale * kLog2e;
-    // Own rows: about two workgroups a CU, no fewer than kRunRows rows each.
-    const long long own_rows = (long long) own.maxvis * B * Hkv;
-    int chunk = d->own.split_rows;
-    if (chunk == 0) chunk = (int) std::max<long long>(kRunRows, (std::min<long long>(own_rows / 512, own.maxvis) + 15) / 16 * 16);
-    auto own_splits = [&] { return (int) (((long long) own.maxvis + chunk - 1) / chunk); };
-    if (own_splits() > 64) chunk = (own.maxvis / 64 + 16) / 16 * 16;
-    p.own_chunk = chunk;
-    p.own_splits = own_splits();
-    // Form and key splits of the prefix: the cheapest by the workgroups of both kinds on the GPU, the
-    // bytes at what HBM gives, and the merge of the partials.
+    // Own chunk, form and key splits of the prefix: the cheapest by the workgroups of both kinds on the
+    // GPU, the bytes, and the merge of the partials.  (With the own rows in about two workgroups a CU
+    // whatever the prefix takes, drawn steps were 17% longer on average, up to three times as long.)
+    const StepCosts &c = D == 512 ? kCosts512 : D == 256 ? kCosts256 : kCosts128;
     const float row_kb = 2.0f * D * (shared ? 1 : 2) / 1024;
     const int group_rows = B * p.G;
-    const float own_us = 6.0f + std::min(chunk, own.maxvis) * row_kb / 40.0f;
-    const long long own_groups = (long long) B * Hkv * p.own_splits;
-    const float floor_us = 6.0f + ((float) P * Hkv + own_rows) * row_kb / 5600.0f;
+    const float floor_us = c.start + ((float) P * Hkv + (float) own.maxvis * B * Hkv) * row_kb / c.rate;
     Form f[4];
     const int nf = forms_of(D, group_rows, shared, f);
     float best = INFINITY;
-    for (int i = 0; i < nf; ++i) {
-        const int least = f[i].ng ? kRunRows : kStageKeys, unit = f[i].ng ? 16 : kStageKeys;
-        const int tiles = (group_rows + f[i].rows() - 1) / f[i].rows();
-        auto consider = [&](int keys) {
-            const int splits = (P + keys - 1) / keys;
-            const long long groups = (long long) tiles * Hkv * splits;
-            const float us = f[i].start + std::min(keys, P) * row_kb * f[i].per_kb;
-            const float span = f[i].ng ? makespan(own_groups, own_us, groups, us, f[i].slots)
-                                       : makespan(groups, us, own_groups, own_us, f[i].slots);
-            const int n = splits + p.own_splits;
-            // (plans that the bytes bound alike: the shorter workgroups keep more loads in flight)
-            const float cost = std::max(span, floor_us) + 0.3f * std::min(span, floor_us) + (n <= 8 ? 3.5f : 4.0f) +
-                               2.2e-7f * 4 * D * rows * n;
-            if (cost >= best) return;
-            best = cost;
-            p.qb = f[i].qb;
-            p.kh = f[i].kh;
-            p.nw = f[i].nw;
-            p.tiles = tiles;
-            p.splits = splits;
-            p.kps = keys;
-            p.run_keys = f[i].ng ? keys : 0;
-            p.row_groups = f[i].ng ? tiles : 0;
-        };
-        if (d->split_keys > 0) {
-            consider(d->split_keys);
-            continue;
+    auto consider = [&](const Form &form, int chunk, int keys) {
+        const int splits = (P + keys - 1) / keys, tiles = (group_rows + form.rows() - 1) / form.rows();
+        const int own_splits = (int) ((own.maxvis + chunk - 1LL) / chunk), n = splits + own_splits;
+        const long long groups = (long long) tiles * Hkv * splits, own_groups = (long long) B * Hkv * own_splits;
+        const float us = form.start + std::min(keys, P) * row_kb * form.per_kb;
+        const float own_us = c.own_start + std::min(chunk, own.maxvis) * row_kb / c.own_rate;
+        const float span = form.ng ? makespan(own_groups, own_us, groups, us, form.slots)
+                                   : makespan(groups, us, own_groups, own_us, form.slots);
+        const float cost = std::max(span, floor_us) + c.add * std::min(span, floor_us) + (n <= 8 ? c.few : c.many) +
+                           c.part * 4 * D * rows * n;
+        if (cost >= best) return;
+        best = cost;
+        p.qb = form.qb;
+        p.kh = form.kh;
+        p.nw = form.nw;
+        p.tiles = tiles;
+        p.splits = splits;
+        p.kps = keys;
+        p.run_keys = form.ng ? keys : 0;
+        p.row_groups = form.ng ? tiles : 0;
+        p.own_chunk = chunk;
+        p.own_splits = own_splits;
+    };
+    auto with_chunk = [&](int chunk) {
+        for (int i = 0; i < nf; ++i) {
+            if (d->split_keys > 0) {
+                consider(f[i], chunk, d->split_keys);
+                continue;
+            }
+            const int least = f[i].ng ? kRunRows : kStageKeys, unit = f[i].ng ? 16 : kStageKeys;
+            int last = 0;
+            for (int s = 1; s <= 512; s += std::max(1, s / 8)) {
+                const int keys = std::max(least, ((P + s - 1) / s + unit - 1) / unit * unit);
+                if (keys != last) consider(f[i], chunk, keys);
+                if (keys == least) break;
+                last = keys;
+            }
         }
+    };
+    const int least_chunk = (own.maxvis / kOwnSplits + 16) / 16 * 16;  // (at most kOwnSplits of them)
+    if (d->own.split_rows > 0) {
+        with_chunk((own.maxvis + d->own.split_rows - 1LL) / d->own.split_rows > kOwnSplits ? least_chunk : d->own.split_rows);
+    } else {
         int last = 0;
-        for (int s = 1; s <= 512; s += s < 64 ? 1 : 8) {
-            const int keys = std::max(least, ((P + s - 1) / s + unit - 1) / unit * unit);
-            if (keys != last) consider(keys);
-            if (keys == least) break;
-            last = keys;
+        for (int s = 1; s <= kOwnSplits; s += std::max(1, s / 2)) {
+            const int chunk = (int) std::max<long long>(kRunRows, std::min((own.maxvis + s - 1LL) / s + 15, (long long) INT_MAX) / 16 * 16);
+            if (chunk != last) with_chunk(chunk);
+            if (chunk == kRunRows) break;
+            last = chunk;
         }
     }
     p.part_nt = 4.0f * D * rows * p.splits <= kPartNtBytes;
