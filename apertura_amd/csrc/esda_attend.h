@@ -505,6 +505,15 @@ void attend_kernel(P p) {
             }
             sc[r] = hmatch && (jt + r) < j1 ? x : -INFINITY;
         }
+        if constexpr (SCORED) {
+            // rows past the end repeat the last one: with a weight of 0, but 0 x inf is NaN
+            if (st + 1 == nst) {
+#pragma unroll
+                for (int dt = 0; dt < DTW; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) va[dt][r] = jt + r < j1 ? va[dt][r] : (short) 0;
+            }
+        }
         const float tmax = wave_max_across_groups(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
         if (__any(tmax > m + kRescaleSlack)) {
             const float mnew = fmaxf(m, tmax);

@@ -533,6 +533,17 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         // the other waves') and every wave is done with the previous iteration
         ESDA_WAIT_VM(0);
         lds_barrier();
+        if constexpr (PARTS) {
+            // rows past the prefix repeat its last key: with a weight of 0, but 0 x inf is NaN
+            const int past = j1 - (j0 + s0 * kStageKeys);  // keys from this iteration's first on
+            if (s0 + SPI >= nst && past % kStageKeys != 0) {
+                for (int r = past % kStageKeys + wave; r < kStageKeys; r += NW) {
+                    unsigned char *const row = vslot(nst - 1) + (r >> 4) * R::HB + R::off(r & 15);
+                    for (int c = lane; c < D / 8; c += 64) *reinterpret_cast<u32x4 *>(row + 16 * c) = u32x4{0u, 0u, 0u, 0u};
+                }
+                lds_barrier();
+            }
+        }
         if constexpr (DOCS) next_stages(cur[SPI - 1].st - 1, ahead);
         // The next iteration's DMAs, spread over this iteration so that the workgroup's loads
         // do not all queue at the barrier (each slot is free once the barrier has passed):

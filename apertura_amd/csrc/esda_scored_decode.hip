@@ -66,7 +66,8 @@ extern "C" int esda_scored_decode(const esda_decode_desc *d, const esda_score *s
     Plan pl;
     int rc = make_plan(d, &pl);
     if (rc) return rc;
-    if (d->head_dim == 128) pl.pk = 1;  // stream_kernel takes one kv head a workgroup (the same partials)
+    // One kv head a workgroup (the same partials): a value that is not finite stays with its head's queries.
+    pl.pk = 1;
     if (!s) return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: null score");
     if (!(s->softcap >= 0.0f) || !std::isfinite(s->softcap))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: softcap must be 0 or positive and finite");

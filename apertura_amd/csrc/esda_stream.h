@@ -114,6 +114,10 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
             dma(st + AW, ring + ((it + 1) & 1) * L::SLOT);
         }
         asm volatile("" ::: "memory");
+        // Rows past the run repeat its last one, with a weight of 0; but 0 x inf is NaN.
+        for (int r = x.j1 - (x.j0 + 16 * st); r < 16; ++r)
+            if (lane < D / 8) *reinterpret_cast<u32x4 *>(slot + (SH ? 0 : L::HB) + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        asm volatile("" ::: "memory");
         // Every K read of the stage, then the products, then every V read, which lands during the
         // softmax.  The scores of few rows go through several sums (a chain of D / 32 products waits for
         // each of them).

@@ -11,7 +11,8 @@
  * Sequence b's keys are the prefix rows, positions 0 .. prefix_len - 1, then the rows of its own
  * cache, positions prefix_len .. pos[b] (the row of position p is p - prefix_len):
  *   out = softmax(scale q.k over both) v
- * the values of esda_decode over one cache that holds prefix and own rows, to its rounding. */
+ * the values of esda_decode over one cache that holds prefix and own rows, to its rounding.  A value
+ * that is not finite reaches only the queries that see its row. */
 #ifndef APERTURA_ESDA_PREFIX_H
 #define APERTURA_ESDA_PREFIX_H
 

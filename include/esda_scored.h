@@ -59,7 +59,8 @@ int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, 
 /* ------------------------------------------------------------------------- decode
  * esda_decode with these scores: append, attend, merge (esda_decode_args; every cache mode of
  * esda_decode_desc).  Workspace: esda_decode_workspace_size; skipped sequences:
- * esda_decode_status. */
+ * esda_decode_status.  A value of k or v that is not finite reaches only the queries of its
+ * sequence and kv head. */
 int esda_scored_decode(const esda_decode_desc *desc, const esda_score *score, const esda_decode_args *args,
                        void *stream);
 

@@ -255,3 +255,21 @@ def test_two_samples_of_one_prompt():
         err = (a.float() - b.float()).abs()
         assert float(err.max()) <= 2e-2 and float(err.mean()) <= 2e-3
     assert torch.equal(kc[:, :, :3], full_k[:, :, P:P + 3]) and torch.equal(vc[:, :, :3], full_v[:, :, P:P + 3])
+
+
+@pytest.mark.parametrize("split", [0, 64])
+@pytest.mark.parametrize("B,hq,hkv,D,P", [(3, 8, 2, 128, 45), (3, 8, 2, 128, 161), (30, 16, 2, 128, 161), (70, 8, 2, 128, 90),
+                                          (5, 8, 4, 256, 45), (40, 8, 4, 256, 200), (90, 8, 2, 256, 173),
+                                          (3, 8, 2, 512, 45), (3, 8, 2, 512, 201), (40, 8, 2, 512, 173)])
+def test_value_that_is_infinite_reaches_its_queries_only(B, hq, hkv, D, P, split):
+    """In the prefix's last row and in a sequence's last own row: infinite in its dim for the queries
+    that see it (0 x inf from the rows that fill a stage would be NaN), the rest bit for bit."""
+    G, own = hq // hkv, [(7 * i + 3) % 50 for i in range(B)]
+    c = Case(B, hq, hkv, D, P, 50, own, split_keys=split, seed=20)
+    a = c.run()
+    c.pv[1, P - 1, 5], c.pv[0, 2, 6], c.vn[2, 0, 9] = float("inf"), float("inf"), -float("inf")
+    b = prefix_decode(c.step, *c.args())
+    assert bool((b[:, G:2 * G, 5] == float("inf")).all()) and bool((b[:, :G, 6] == float("inf")).all())
+    assert bool((b[2, :G, 9] == -float("inf")).all())
+    b[:, G:2 * G, 5], b[:, :G, 6], b[2, :G, 9] = a[:, G:2 * G, 5], a[:, :G, 6], a[2, :G, 9]
+    assert torch.equal(a, b)

@@ -493,3 +493,25 @@ def test_rope_prefill_and_decode_of_a_capped_layer():
         k0, v0 = kc.clone(), vc.clone()
         got = scored_decode(dstep, score, qt, kt, x_v[t:t + 1], kc, vc, p)
         _check_decode(dstep, score, qt, k0, v0, kt, x_v[t:t + 1], [t], got)
+
+
+@pytest.mark.parametrize("B,hq,hkv,D,cap,ring", [(3, 8, 2, 128, 150, False), (3, 8, 4, 256, 150, False),
+                                                 (3, 4, 2, 512, 150, False), (1, 4, 2, 256, 700, False),
+                                                 (2, 4, 2, 512, 64, True), (64, 32, 16, 256, 24, True)])
+def test_decode_value_that_is_infinite_reaches_its_queries_only(B, hq, hkv, D, cap, ring):
+    """An infinite value in the last visible row (a stage's rows past it must not add 0 x inf) and one
+    before: infinite in its dim for the queries of its kv head, every other element bit for bit."""
+    g, G = _gen(30), hq // hkv
+    q, kc, vc = _rows((B, hq, D), g), _rows((B, hkv, cap, D), g), _rows((B, hkv, cap, D), g)
+    kn, vn = _rows((B, hkv, D), g), _rows((B, hkv, D), g)
+    pos = [(i * 37 + 20) % (5 * cap if ring else cap) for i in range(B)]
+    step = DecodeStep(B, hq, hkv, D, cap, window=cap if ring else 0, ring=ring, scale=D ** -0.5)
+    posd = torch.tensor(pos, dtype=torch.int32, device=DEV)
+    score = Score(20.0, _slopes(hq) * 2.0 ** -6)
+    a = scored_decode(step, score, q, kn, vn, kc, vc, posd)
+    vn[0, 0, 7], vc[0, hkv - 1, 3, 11] = float("inf"), -float("inf")
+    b = scored_decode(step, score, q, kn, vn, kc, vc, posd)
+    assert bool(a.isfinite().all())
+    assert bool((b[0, :G, 7] == float("inf")).all()) and bool((b[0, hq - G:, 11] == -float("inf")).all())
+    b[0, :G, 7], b[0, hq - G:, 11] = a[0, :G, 7], a[0, hq - G:, 11]
+    assert torch.equal(a, b)
