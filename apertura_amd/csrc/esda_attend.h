@@ -1,6 +1,7 @@
 // esda_attend.h -- the decode attention kernel over a bf16 cache, the split merges and the host
 // side that plans and launches them (gfx950), for the sources that build entry points on them:
-// esda_decode.hip.  What the kernels do is described at the head of esda_decode.hip.
+// esda_decode.hip, and esda_scored_decode.hip (ScoredAttendParams); esda_prefix.hip takes its plan
+// and checks.  What the kernels do is described at the head of esda_decode.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -20,6 +20,7 @@
 //   raw_attend_kernel  the same over a raw-K or q8 raw-K stream, K and V rebuilt per row.
 //   merge_kernel   reduces the partials of all splits per (sequence, query head).
 //   append_kernel  multi-row append (slice_update) for prefill-style callers.
+// attend_kernel, the merges and their launch are in esda_attend.h, which other entry points use too.
 // The C ABI (include/esda.h) is at the end of the file.
 
 #include <hip/hip_runtime.h>

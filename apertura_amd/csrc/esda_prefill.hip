@@ -34,7 +34,8 @@
 //   prefill_merge_kernel  reduces split partials (m, l, acc) per (query row, head).
 //   raw_prefill_kv_kernel rebuilds K and V of a raw-K (or q8 raw-K) stream by the
 //                       reference's op-level rounding points.
-// The C ABI (include/esda_prefill.h) is at the end of the file.
+// prefill_kernel, its merge and their launch are in esda_prefill_kernel.h, which other entry points
+// use too.  The C ABI (include/esda_prefill.h) is at the end of the file.
 
 #include <hip/hip_runtime.h>
 

@@ -1,6 +1,8 @@
 // esda_prefill_kernel.h -- the prefill attention kernel, its split merge and their launch
-// (gfx950), for the sources that build entry points on them: esda_prefill.hip (causal and
-// sliding masks).  What the kernel does is described at the head of esda_prefill.hip.
+// (gfx950), for the sources that build entry points on them: esda_prefill.hip (causal and sliding
+// masks), esda_scored_prefill.hip (capped and biased scores, document and prefix masks) and
+// esda_prefix_tiles.hip (the rows of a decode batch over its shared prefix).  What the kernel does
+// is described at the head of esda_prefill.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -115,7 +117,9 @@ struct OwnRows {
     }
 };
 
-// Prefix and own rows in runs, for batches of few query rows a kv head: every wave holds 16 NG of
+// Prefix and own rows in runs, for batches of few query rows a kv head (esda_prefix.hip's forms):
+// memory-bound where the prefix is long (2 sequences behind 32,768 tokens, 8 query rows over 4 heads
+// of one 512-dim stream, 135 MB in 32 us), else by the latency of a stage.  Every wave holds 16 NG of
 // them and its own keys, so that a K or V value is read from LDS once for those, where the tiles'
 // waves each hold 16 rows and read every key.  The registers bound NG (O^T and Q^T take 6 D NG / 16
 // of 512 a lane: NG D = 1024 spills); more rows are row_groups workgroups of the same keys.
@@ -155,10 +159,13 @@ struct PRing {
 //
 // P = ScoredParams (esda_scored.h): scores are capped and lose slope * distance, a prefix opens
 // keys ahead of a query, a row that sees nothing gives 0, and a value that is not finite reaches
-// only the rows that see its key.  P = DocParams: document ids (equal, not negative) close the
-// other keys, too.  The waves first read the range of ids of every 32-key stage: stages that hold
-// no id of the tile's range are never loaded, those that hold nothing but the tile's one id need
-// no mask, and the ids of the others come with their keys by DMA.
+// only the rows that see its key.  Bound as the plain form, by the MFMAs and the softmax in turn: a
+// cap adds 6 .. 9% at D = 256 and 512 (2048 queries 92 -> 100 us, 143 -> 151) and 25% at D = 128,
+// whose stages have half or a quarter of the products to a score (4096 queries 150 -> 187).
+// P = DocParams: document ids (equal, not negative) close the other keys, too.  The waves first
+// read the range of ids of every 32-key stage: stages that hold no id of the tile's range are never
+// loaded, those that hold nothing but the tile's one id need no mask, and the ids of the others
+// come with their keys by DMA.
 template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves,
           class P = PrefillParams>
 // (D == 128 on four waves: two workgroups per CU)

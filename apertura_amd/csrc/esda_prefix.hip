@@ -2,9 +2,13 @@
 //
 // Two launches.  The first leaves partials (m, l, O) of the prefix and of the sequences' own rows,
 // whose workgroups stand side by side in one grid: the prefix as query tiles, each key read once
-// for the B * G query rows of its kv head (prefill_kernel with PrefixParams), or, for at most 16 of
-// them, in runs (prefix_run_kernel); the own rows in runs, with the fused append.  The second
-// merges them.  The C ABI is include/esda_prefix.h.
+// for the B * G query rows of its kv head (prefill_kernel with PrefixParams), or, for few of them,
+// in runs (prefix_run_kernel); the own rows in runs, with the fused append.  The second merges them.
+// A step of few rows is bound by the latency of the two (2 sequences behind 2049 tokens: 15 us), a
+// long one by reading prefix and own rows once (4 behind 32,768, 138 MB: 40 us), one of many sequences
+// by both kinds of workgroups sharing the CUs (64 behind 16,384, 200 MB and 18 GFLOP: 64 us).  With
+// prefix, own rows and their merges in launches one after the other these took 48, 99 and 123 us.
+// The C ABI is include/esda_prefix.h.
 
 #include <hip/hip_runtime.h>
 
@@ -178,6 +182,8 @@ struct Form {
 // These and the forms' costs are fitted, per head dim, to 330 steps (1 .. 64 sequences, prefixes of
 // 64 .. 40,000 keys, own caches of 64 .. 2048 rows, full, at random and nearly empty), each in every
 // form, in up to 7 own chunks and 9 prefix splits, graph-replayed (the keys in the Infinity Cache).
+// The plan then takes 1.05 of the best forced one's time on average; for 396 other steps, whose keys
+// came from HBM (4 .. 24 copies in turn), 1.03 (1.01 at D = 512; 95th percentile 1.2).
 struct StepCosts {
     float own_start, own_rate, start, rate, add, few, many, part;
 };

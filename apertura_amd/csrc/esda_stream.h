@@ -2,8 +2,8 @@
 // another (gfx950): wave w takes the run's 16-row stages w, w + NW, .. over the whole head dim,
 // from LDS slots of its own that it fills by DMA, and the waves' (m, l, O) meet once at the end.
 // For workgroups whose stages are short (a 16-row stage of 128-dim rows is 8 KB: a barrier and a
-// score exchange per stage, as in attend_kernel, take longer than its bytes), and for runs inside
-// another kernel's workgroup.
+// score exchange per stage, as in attend_kernel, take longer than its bytes: 571 MB 144 us, here 98),
+// and for runs inside another kernel's workgroup.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,8 +31,8 @@ struct Layout {
     static constexpr int CPR = D / 8;               // 16-byte chunks per row
     static constexpr int ROWS = 16 * NG;
     static constexpr int CH = D < 32768 / (AW * ROWS) ? D : 32768 / (AW * ROWS);  // dims the waves' O are summed over at a time
-    static constexpr int PITCH = CH + 4;            // floats between the rows of that sum: 16 rows a multiple of
-                                                    // 128 bytes apart made each of its writes 16 (512 dims: 7 us)
+    static constexpr int PITCH = CH + 4;            // floats between the rows of that sum (16 rows a multiple of 128
+                                                    // bytes apart: each write 16; a 512-dim run of one stage 9.6 us, 12.6)
     static constexpr int SUM = AW * ROWS * PITCH * 4;
     static_assert(CH % 16 == 0 && D % CH == 0, "whole tiles of dims at a time");
     static constexpr int RING = AW * SLOTS * SLOT;
