@@ -118,8 +118,8 @@ struct OwnRows {
 };
 
 // Prefix and own rows in runs, for batches of few query rows a kv head (esda_prefix.hip's forms):
-// memory-bound where the prefix is long (2 sequences behind 32,768 tokens, 8 query rows over 4 heads
-// of one 512-dim stream, 135 MB in 32 us), else by the latency of a stage.  Every wave holds 16 NG of
+// bound by memory where the prefix is long (2 sequences behind 32,768 tokens, 4 kv heads of one
+// 512-dim stream, 135 MB in 32 us), else by the latency of a few stages.  Every wave holds 16 NG of
 // them and its own keys, so that a K or V value is read from LDS once for those, where the tiles'
 // waves each hold 16 rows and read every key.  The registers bound NG (O^T and Q^T take 6 D NG / 16
 // of 512 a lane: NG D = 1024 spills); more rows are row_groups workgroups of the same keys.
