@@ -247,6 +247,8 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     const int D = d->own.head_dim, B = d->own.batch, Hkv = d->own.num_kv_heads, P = d->prefix_len;
     const bool shared = d->own.kv_shared != 0;
     const size_t rows = (size_t) B * d->own.num_q_heads;
+    if (rows * (D / 64) >= 1u << 24)  // a launch holds fewer than 2^32 threads, the merge 256 for 64 dims
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_prefix_decode: too many query rows");
     PrefixParams &p = pl->p;
     p = PrefixParams{};
     p.Hq = d->own.num_q_heads;

@@ -29,7 +29,7 @@ typedef struct esda_prefix_desc {
     esda_decode_desc own;       /* batch, heads, head_dim, scale, and the sequences' own caches: linear
                                    rows (ring 0), no window; cap, max_visible and split_rows count own
                                    rows.  kv_shared: V aliases K in the prefix and in the own caches */
-    int32_t prefix_len;         /* 1 .. 2^30                                                 */
+    int32_t prefix_len;         /* 1 .. 2^30; prefix_len + own.cap below 2^31                */
     int32_t split_keys;         /* prefix keys per split (0 = automatic; multiple of 32)     */
     int64_t prefix_head_stride; /* elements; >= prefix_len * head_dim, multiple of 8: element
                                    (kvh, j, d) at prefix[kvh*prefix_head_stride + j*head_dim + d] */

@@ -2,6 +2,7 @@
 refuses before it touches the device."""
 import ctypes
 import math
+import time
 
 import pytest
 import torch
@@ -37,7 +38,8 @@ def test_a_bound_on_own_rows_sizes_their_splits():
     dict(prefix_len=0), dict(prefix_len=-1), dict(prefix_len=2 ** 30 + 1), dict(prefix_head_stride=99 * 128), dict(prefix_head_stride=100 * 128 + 4),
     dict(split_keys=16), dict(split_keys=-32), dict(window=16), dict(ring=True, window=64), dict(head_dim=64),
     dict(num_q_heads=9), dict(num_q_heads=34), dict(batch=0), dict(batch=257), dict(cap=0), dict(scale=0.0),
-    dict(scale=math.nan), dict(split_rows=8),
+    dict(scale=math.nan), dict(split_rows=8), dict(batch=128, num_q_heads=16 * 16384, num_kv_heads=16384),
+    dict(prefix_len=2 ** 30, cap=2 ** 30),
 ])
 def test_bad_descriptions_are_refused(kw):
     with pytest.raises(_lib.EsdaError) as ei:
@@ -88,3 +90,21 @@ def test_front_end_refuses_wrong_tensors():
                  (q, n, n, pk, pk.clone(), c, c.clone(), pos.long())):
         with pytest.raises(ValueError):
             PrefixCall(step, *args)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(prefix_len=2 ** 30, batch=256, cap=2 ** 22), dict(prefix_len=2 ** 30, batch=1, cap=1), dict(prefix_len=1, cap=2 ** 30),
+    dict(prefix_len=2 ** 29, cap=2 ** 30, batch=7, head_dim=512, num_q_heads=32), dict(prefix_len=1, batch=1, cap=1, head_dim=256),
+    dict(prefix_len=2 ** 30, batch=200, cap=16, num_q_heads=1024, num_kv_heads=64), dict(prefix_len=2 ** 30, cap=2 ** 30 - 1, split_rows=16),
+    dict(prefix_len=3, batch=256, cap=2 ** 20, num_q_heads=16, num_kv_heads=1, head_dim=512, kv_shared=True),
+])
+def test_extreme_descriptions_plan_quickly(kw):
+    """Every size of the documented range has a plan, found in milliseconds, of at most 64 own splits and
+    at most 512 prefix splits and a workspace for them."""
+    step = _step(**kw)
+    t = time.perf_counter()
+    n = prefix_workspace_bytes(step)
+    assert time.perf_counter() - t < 0.25
+    o = step.own
+    row = o.batch * o.num_q_heads * (4 * o.head_dim + 8)
+    assert 2 * row <= n <= (512 + 64) * row + 4096

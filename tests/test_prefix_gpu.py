@@ -273,3 +273,34 @@ def test_value_that_is_infinite_reaches_its_queries_only(B, hq, hkv, D, P, split
     assert bool((b[2, :G, 9] == -float("inf")).all())
     b[:, G:2 * G, 5], b[:, :G, 6], b[2, :G, 9] = a[:, G:2 * G, 5], a[:, :G, 6], a[2, :G, 9]
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,hq", [(128, 8), (256, 4), (512, 8)])
+def test_own_caches_past_32_bits(D, hq):
+    """The second sequence's own cache 2^31 + 4096 elements behind the first's."""
+    hkv, cap, gap, g = 2, 70, 2 ** 31 + 4096, _gen(21)
+    buf = torch.empty(gap + hkv * cap * D, dtype=BF, device=DEV)
+    kc = torch.as_strided(buf, (2, hkv, cap, D), (gap, cap * D, D, 1))
+    c = Case(2, hq, hkv, D, 100, cap, [33, 69], shared=True, seed=22)
+    kc.copy_(c.kc)
+    c.kc = c.vc = kc
+    c.step = PrefixStep.for_caches(c.pk, kc, hq, kv_shared=True, scale=D ** -0.5)
+    c.run()
+
+
+@pytest.mark.parametrize("B,D", [(2, 128), (40, 128), (3, 256), (2, 512), (12, 512)])
+def test_two_steps_at_once(B, D):
+    """Two layers' steps over one prefix on two streams, each in a workspace of its own, ten times: as one
+    after the other."""
+    cases = [Case(B, 8, 2, D, 500, 130, [(11 * i + 7 * s) % 130 for i in range(B)], shared=D == 512, seed=23 + s)
+             for s in (0, 1)]
+    cases[1].pk, cases[1].pv = cases[0].pk, cases[0].pv
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = [[prefix_decode(c.step, *c.args(), stream=s) for c, s in zip(cases, streams)] for _ in range(10)]
+    torch.cuda.synchronize()
+    for got in outs:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

@@ -515,3 +515,40 @@ def test_decode_value_that_is_infinite_reaches_its_queries_only(B, hq, hkv, D, c
     assert bool((b[0, :G, 7] == float("inf")).all()) and bool((b[0, hq - G:, 11] == -float("inf")).all())
     b[0, :G, 7], b[0, hq - G:, 11] = a[0, :G, 7], a[0, hq - G:, 11]
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_decode_cache_past_32_bits(D):
+    """The second sequence's cache 2^31 + 4096 elements behind the first's."""
+    B, hq, hkv, cap, gap, g = 2, 8, 2, 300, 2 ** 31 + 4096, _gen(31)
+    buf = torch.empty(gap + hkv * cap * D, dtype=BF, device=DEV)
+    kc = torch.as_strided(buf, (B, hkv, cap, D), (gap, cap * D, D, 1))
+    kc.copy_(_rows((B, hkv, cap, D), g))
+    q, kn, pos = _rows((B, hq, D), g, 2.5), _rows((B, hkv, D), g), [260, 299]
+    step = DecodeStep.for_cache(kc, hq, kv_shared=True, scale=D ** -0.5)
+    score, k0 = Score(9.0, _slopes(hq)), kc.clone()
+    out = scored_decode(step, score, q, kn, None, kc, kc, torch.tensor(pos, dtype=torch.int32, device=DEV))
+    _check_decode(step, score, q, k0, k0, kn, kn, pos, out)
+    k0[0, :, 260], k0[1, :, 299] = kn[0], kn[1]
+    assert torch.equal(kc, k0)
+
+
+def test_calls_at_once_on_two_streams():
+    """A prefill chunk in splits and a decode step, each on a stream and in a workspace of its own, over
+    one cache's rows: ten rounds of both at once give what they give one after the other."""
+    hq, hkv, D, n, g = 8, 2, 256, 600, _gen(32)
+    q, k, v = _rows((hq, 40, D), g, 2.5), _rows((hkv, n, D), g), _rows((hkv, n, D), g)
+    step, score = PrefillStep(hq, hkv, D, 40, n, n - 40, 0, 0, D ** -0.5, 128), Score(20.0, _slopes(hq))
+    kc, vc, qd, kn, vn = (_rows(s, g) for s in ((3, hkv, 500, D), (3, hkv, 500, D), (3, hq, D), (3, hkv, D), (3, hkv, D)))
+    dstep = DecodeStep(3, hq, hkv, D, 500, scale=D ** -0.5)
+    pos = torch.tensor([499, 120, 3], dtype=torch.int32, device=DEV)
+    want = scored_prefill(step, score, q, k, v)
+    dwant = scored_decode(dstep, score, qd, kn, vn, kc, vc, pos)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (a, b):
+        s.wait_stream(torch.cuda.current_stream())
+    outs = [(scored_prefill(step, score, q, k, v, stream=a), scored_decode(dstep, score, qd, kn, vn, kc, vc, pos, stream=b))
+            for _ in range(10)]
+    torch.cuda.synchronize()
+    for x, y in outs:
+        assert torch.equal(x, want) and torch.equal(y, dwant)
