@@ -53,14 +53,32 @@ constexpr int kWaves = 8;
 #endif
 constexpr int kPairSpin = 1 << 20;  // PS: polls of the partner's flag before a wave gives up
 
-// The sequences' own rows beside a shared prefix (esda_prefix.h), one run a workgroup of NW waves:
-// as many stages in flight as the prefill kernel's LDS holds.
-template <int D, bool SH, int NW>
+// A run of the prefix step (esda_prefix.h) on a workgroup of NW waves, for up to 16 NG query rows: by
+// waves that stream stages of their own, as many in flight as the prefill kernel's LDS holds; short
+// runs of 512 dims, whose waves' O^T would take longer to sum than the run, in groups of stages.  A
+// step of 128 such runs over one K = V buffer, streamed / in groups, us: 64 rows 15.5 / 12.4, 128 16.5 /
+// 13.7, 256 19.8 / 18.5, 384 22.5 / 22.3, 512 25.4 / 26.6, 1024 35.1 / 41.5.  (256 dims: 64 rows 9.1 /
+// 9.0, 256 14.4 / 15.0, 1024 30.7 / 35.3.)
+template <int D, bool SH, int NW, int NG = 1>
 struct OwnRows {
     static constexpr int kStage = (SH ? 1 : 2) * 2 * D * 16;  // bytes of a 16-row stage
-    static constexpr int AW = kStage * NW > 128 * 1024 ? NW / 2 : NW;
-    static constexpr int SLOTS = 2 * kStage * AW > 128 * 1024 ? 1 : 2;
-    using L = esda_stream::Layout<D, SH, AW, SLOTS>;
+    static constexpr int SLOTS = 2 * kStage * NW > 128 * 1024 ? 1 : 2;
+    static constexpr bool GROUPS = D == 512, ONLY = GROUPS && NW > 4;  // (eight waves' registers do not hold the streaming form)
+    static constexpr int kGroupRows = 384;  // longest run in groups
+    static constexpr int kGroupBytes = esda_stream::GroupLayout<D, SH>::BYTES;
+    static constexpr int kStreamBytes = esda_stream::Layout<D, SH, NW, SLOTS, NG>::BYTES;
+    static constexpr int BYTES = ONLY || (GROUPS && kGroupBytes > kStreamBytes) ? kGroupBytes : kStreamBytes;
+    template <class Query, class Score, class Put>
+    static __device__ __forceinline__ void attend(unsigned char *lds, const esda_stream::Run &x, Query &&query, Score &&score, Put &&put) {
+        if constexpr (GROUPS) {
+            static_assert(NG == 1, "16 query rows a group");
+            if (ONLY || x.j1 - x.j0 <= kGroupRows) {
+                esda_stream::attend_groups<D, SH, NW>(lds, x, query, score, put);
+                return;
+            }
+        }
+        if constexpr (!ONLY) esda_stream::attend_run<D, SH, NW, SLOTS, NG>(lds, x, query, score, put);
+    }
 
     static __device__ __forceinline__ void store(float *acc, float *ml, size_t at, int d, const f32x4 &o, float M, float T) {
         __builtin_nontemporal_store(o, reinterpret_cast<f32x4 *>(acc + at * D + d));
@@ -89,13 +107,12 @@ struct OwnRows {
         x.newrow = sv.newrow;
         const uint16_t *const q = p.q + (size_t) b * p.q_rs + (size_t) kvh * p.G * D;
         const size_t slot = ((size_t) pair * p.own_splits + split) * p.G;
-        esda_stream::attend_run<D, SH, NW, AW, SLOTS, 1>(
+        attend(
             lds, x, [&](int h) { return q + (size_t) h * D; }, [&](float s, int) { return s * p.scale_log2e; },
             [&](int h, int d, const f32x4 &o, float M, float T) { store(p.own_acc, p.own_ml, slot + h, d, o, M, T); });
     }
     // Prefix workgroup w: 16 NG of the B * G query rows of a kv head over run_keys keys.  The row groups
     // of the same keys are 8 workgroups apart: on one XCD, whose L2 hands the second what the first read.
-    template <int NG>
     static __device__ __forceinline__ void run_prefix(const PrefixParams &p, unsigned w, unsigned char *lds) {
         const unsigned i = w >> 3, pair = i / (unsigned) p.row_groups * 8 + (w & 7);
         const int r0 = (int) (i % (unsigned) p.row_groups) * 16 * NG;
@@ -111,7 +128,7 @@ struct OwnRows {
         x.cap = p.Sk;
         const size_t rows = (size_t) p.Sq * p.Hq, slot = (size_t) split * rows;
         auto row = [&](int h) { return (size_t) ((r0 + h) / p.G) * p.Hq + kvh * p.G + (r0 + h) % p.G; };
-        esda_stream::attend_run<D, SH, NW, AW, SLOTS, NG>(
+        attend(
             lds, x, [&](int h) { return p.q + row(h) * D; }, [&](float s, int) { return s * p.scale_log2e; },
             [&](int h, int d, const f32x4 &o, float M, float T) { store(p.part_acc, p.part_ml, slot + row(h), d, o, M, T); });
     }
@@ -119,17 +136,16 @@ struct OwnRows {
 
 // Prefix and own rows in runs, for batches of few query rows a kv head (esda_prefix.hip's forms):
 // bound by memory where the prefix is long (2 sequences behind 32,768 tokens, 4 kv heads of one
-// 512-dim stream, 135 MB in 32 us), else by the latency of a few stages.  Every wave holds 16 NG of
-// them and its own keys, so that a K or V value is read from LDS once for those, where the tiles'
+// 512-dim stream, 135 MB in 32 us), else by the latency of a few stages.  Every wave holds 16 NG query
+// rows and its own keys, so that a K or V value is read from LDS once for those, where the tiles'
 // waves each hold 16 rows and read every key.  The registers bound NG (O^T and Q^T take 6 D NG / 16
-// of 512 a lane: NG D = 1024 spills); more rows are row_groups workgroups of the same keys.
+// of 512 a lane: NG D = 1024 spills, and 32 rows of 512 dims in groups of stages took 42 us where two
+// workgroups of 16 take 40); more rows are row_groups workgroups of the same keys.
 template <int D, bool SH, int NG>
 __global__ __launch_bounds__(256, 1) void prefix_run_kernel(PrefixParams p) {
-    using O = OwnRows<D, SH, 4>;
-    using L = esda_stream::Layout<D, SH, O::AW, O::SLOTS, NG>;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
-    if (blockIdx.x >= p.own_groups) O::template run_prefix<NG>(p, blockIdx.x - p.own_groups, lds);
-    else O::run(p, blockIdx.x, lds);
+    __shared__ __attribute__((aligned(16))) unsigned char lds[OwnRows<D, SH, 4, NG>::BYTES];
+    if (blockIdx.x >= p.own_groups) OwnRows<D, SH, 4, NG>::run_prefix(p, blockIdx.x - p.own_groups, lds);
+    else OwnRows<D, SH, 4>::run(p, blockIdx.x, lds);
 }
 
 template <int D, int NSL, int NT = 2>
@@ -184,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     constexpr int DT = D / 16;          // PV dim tiles
     constexpr int NB = PS ? 2 : QB;     // O^T blocks per wave
     constexpr int DW = PS ? DT / 2 : DT;  // O^T dim tiles per wave
-    constexpr int kLds = PARTS && OwnRows<D, SH, NW>::L::BYTES > R::BYTES ? OwnRows<D, SH, NW>::L::BYTES : R::BYTES;
+    constexpr int kLds = PARTS && OwnRows<D, SH, NW>::BYTES > R::BYTES ? OwnRows<D, SH, NW>::BYTES : R::BYTES;
     __shared__ __attribute__((aligned(16))) unsigned char ring[kLds];
     if constexpr (PARTS) {
         if (blockIdx.x >= p.tile_groups) {

@@ -165,10 +165,9 @@ constexpr int kOwnSplits = 64;  // most own splits
 
 // How the prefix's query rows can be laid out: as tiles (nw > 0: a prefill form), or in runs of 16 NG
 // rows.  us of a workgroup: `start`, and per KB of K and V `per_kb`; slots: workgroups the GPU holds at
-// once.  Runs / tiles at the best split, us: D = 512 over one K = V buffer, 16 rows x 4096 keys 17.4 /
-// 15.2, x 32768 31.7 / 41.8, 32 rows 18.8 / 18.5 and 42.3 / 45.0, 64 rows x 16384 41.0 / 35.7; D = 128,
-// 8 rows x 8192 keys 11.3 / 19.8, 16 x 32768 25.1 / 45.2, 32 x 16384 19.3 / 29.0, 64 28.2 / 30.6, 128
-// 38.4 / 34.8; D = 256, 8 rows x 8192 27.5 / 27.8, 32 37.5 / 30.1: always tiles.
+// once.  Runs against tiles at the best splits and own chunks of random steps (StepCosts), time of the
+// one over that of the other: D = 128, up to 16 rows 0.76, 32 0.84, 64 1.08 (0.83 .. 1.35); D = 256, 16
+// rows 0.93, 32 1.10 (not offered); D = 512, 16 rows 0.90 (0.58 .. 1.33), 32 0.93.
 struct Form {
     int qb, kh, nw, ng;
     float start, per_kb;
@@ -179,16 +178,16 @@ struct Form {
 // What else a step's time goes by: us of an own workgroup and its KB per us; us and KB per us of the
 // bytes of both kinds; the share by which the two bounds add up; us of a merge of at most 8 partials a
 // row and of more; us per byte of partials.
-// These and the forms' costs are fitted, per head dim, to 330 steps (1 .. 64 sequences, prefixes of
-// 64 .. 40,000 keys, own caches of 64 .. 2048 rows, full, at random and nearly empty), each in every
-// form, in up to 7 own chunks and 9 prefix splits, graph-replayed (the keys in the Infinity Cache).
-// The plan then takes 1.05 of the best forced one's time on average; for 396 other steps, whose keys
-// came from HBM (4 .. 24 copies in turn), 1.03 (1.01 at D = 512; 95th percentile 1.2).
+// These and the forms' costs are fitted, per head dim, to 230 .. 500 random steps (1 .. 64 sequences,
+// prefixes of 64 .. 40,000 keys, own caches of 64 .. 2048 rows, full, at random and nearly empty), each in
+// every form, up to 7 own chunks and 9 prefix splits, graph-replayed, at D = 256 and 512 over 4 .. 24
+// copies of the caches in turn (from HBM).  The cheapest by them takes 1.03 of the best forced plan's
+// time on average, 1.15 at the 95th percentile.
 struct StepCosts {
     float own_start, own_rate, start, rate, add, few, many, part;
 };
-constexpr StepCosts kCosts512 = {8.0f, 40.0f, 8.7f, 7900.0f, 0.11f, 4.3f, 4.0f, 1.8e-7f};
-constexpr StepCosts kCosts256 = {4.6f, 77.0f, 3.5f, 5360.0f, 0.54f, 4.3f, 3.8f, 1.5e-7f};
+constexpr StepCosts kCosts512 = {6.3f, 40.0f, 3.8f, 5600.0f, 0.13f, 4.3f, 3.5f, 2.6e-7f};
+constexpr StepCosts kCosts256 = {5.4f, 79.0f, 11.4f, 16500.0f, 0.09f, 4.5f, 4.0f, 3.3e-7f};
 constexpr StepCosts kCosts128 = {4.4f, 43.0f, 5.3f, 7900.0f, 0.25f, 5.8f, 2.9f, 2.9e-7f};
 
 // The forms a step may take; returns their number.
@@ -197,8 +196,8 @@ int forms_of(int D, int rows, bool shared, Form *f) {
     const Tiling *t = D == 512 ? kTilings512 : D == 256 ? kTilings256 : kTilings128;
     const int nt = D == 512 ? 2 : D == 256 ? 3 : 1;
     // (a prefill workgroup's costs, and what a step's add to its start and to its stages)
-    constexpr float kMore512[][2] = {{5.1f, 0.96f}, {0.0f, 1.0f}};
-    constexpr float kMore256[][2] = {{6.9f, 1.15f}, {-2.4f, 1.15f}, {0.0f, 1.0f}};
+    constexpr float kMore512[][2] = {{1.8f, 1.02f}, {0.0f, 0.96f}};
+    constexpr float kMore256[][2] = {{4.6f, 1.37f}, {-0.7f, 1.47f}, {-1.0f, 1.63f}};
     constexpr float kMore128[][2] = {{0.0f, 1.6f}};
     const float(*more)[2] = D == 512 ? kMore512 : D == 256 ? kMore256 : kMore128;
     const float stage_kb = 32.0f * 2 * D * (shared ? 1 : 2) / 1024;
@@ -206,7 +205,8 @@ int forms_of(int D, int rows, bool shared, Form *f) {
         if (!(D == 512 && rows <= 64 && t[i].nw == (shared ? 8 : 4)))  // (launch_tiles' choice for one tile)
             f[n++] = {t[i].qb, t[i].kh, t[i].nw, 0, t[i].wg + t[i].row * std::min(rows, t[i].rows()) + more[i][0],
                       t[i].stage / stage_kb * more[i][1], 256};
-    if (D == 512 && rows <= 32) f[n++] = {0, 0, 0, 1, 11.6f, 1 / 60.0f, 256};
+    if (D == 512 && rows <= 32) f[n++] = {0, 0, 0, 1, 8.0f, rows <= 16 ? 1 / 54.0f : 1 / 49.0f, 256};
+    if (D == 256 && rows <= 16) f[n++] = {0, 0, 0, 1, 4.6f, 1 / 65.0f, 256};
     if (D == 128 && rows <= 64) f[n++] = rows <= 16 ? Form{0, 0, 0, 1, 5.8f, 1 / 65.0f, 512}
                                          : rows <= 32 ? Form{0, 0, 0, 2, 13.2f, 1 / 56.0f, 512} : Form{0, 0, 0, 4, 13.1f, 1 / 32.0f, 256};
     return n;
@@ -369,8 +369,8 @@ hipError_t launch_step(const PrefixParams &p, const PrefixMergeParams &m, bool s
             if (shared) hipLaunchKernelGGL((prefix_run_kernel<D, true, NG>), grid, block, 0, st, p);
             else hipLaunchKernelGGL((prefix_run_kernel<D, false, NG>), grid, block, 0, st, p);
         };
-        // (forms_of: 16 rows a workgroup at D = 512, up to 64 at D = 128)
-        if constexpr (D == 512) run(std::integral_constant<int, 1>{});
+        // (forms_of: 16 rows a workgroup at D = 256 and 512, up to 64 at D = 128)
+        if constexpr (D >= 256) run(std::integral_constant<int, 1>{});
         if constexpr (D == 128) {
             if (p.Sq * p.G <= 16) run(std::integral_constant<int, 1>{});
             else if (p.Sq * p.G <= 32) run(std::integral_constant<int, 2>{});

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(ScoredAtte
         const uint16_t *const q = p.q + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;
         uint16_t *const out = p.out + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;
         const float slope = p.slopes && li < p.G ? p.slopes[kvh * p.G + li] * kLog2e : 0.0f;
-        esda_stream::attend_run<D, SH, kStreamWaves, kStreamWaves, SLOTS, 1>(
+        esda_stream::attend_run<D, SH, kStreamWaves, SLOTS, 1>(
             lds, x, [&](int h) { return q + (size_t) h * D; },
             [&](float s, int j) {
                 float y = s * p.scale_log2e;

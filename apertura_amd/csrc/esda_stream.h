@@ -21,8 +21,8 @@ struct Run {
     int G, j0, j1, nvis, first, cap, newrow;
 };
 
-// AW of the workgroup's NW waves take stages, each with SLOTS slots; up to 16 NG query rows.
-template <int D, bool SH, int AW, int SLOTS, int NG = 1>
+// NW waves with SLOTS slots each; up to 16 NG query rows.
+template <int D, bool SH, int NW, int SLOTS, int NG = 1>
 struct Layout {
     static constexpr int BLK = 1056;                // LDS bytes per DMA block: 1 KB + 32 B pad
     static constexpr int NI = D / 32;               // DMA blocks of a tensor's 16-row stage
@@ -30,14 +30,14 @@ struct Layout {
     static constexpr int SLOT = (SH ? 1 : 2) * HB;
     static constexpr int CPR = D / 8;               // 16-byte chunks per row
     static constexpr int ROWS = 16 * NG;
-    static constexpr int CH = D < 32768 / (AW * ROWS) ? D : 32768 / (AW * ROWS);  // dims the waves' O are summed over at a time
+    static constexpr int CH = D < 32768 / (NW * ROWS) ? D : 32768 / (NW * ROWS);  // dims the waves' O are summed over at a time
     static constexpr int PITCH = CH + 4;            // floats between the rows of that sum (16 rows a multiple of 128
                                                     // bytes apart: each write 16; a 512-dim run of one stage 9.6 us, 12.6)
-    static constexpr int SUM = AW * ROWS * PITCH * 4;
+    static constexpr int SUM = NW * ROWS * PITCH * 4;
     static_assert(CH % 16 == 0 && D % CH == 0, "whole tiles of dims at a time");
-    static constexpr int RING = AW * SLOTS * SLOT;
+    static constexpr int RING = NW * SLOTS * SLOT;
     static constexpr int TOTALS = RING > SUM ? RING : SUM;
-    static constexpr int BYTES = TOTALS + (AW + 1) * ROWS * 8;
+    static constexpr int BYTES = TOTALS + (NW + 1) * ROWS * 8;
     // Row r of a stage: block r % NI, 2D bytes times r / NI into it (free of bank conflicts for both
     // the 128-bit row reads and the transpose reads).
     __device__ static constexpr int off(int r) { return (r % NI) * BLK + (r / NI) * 2 * D; }
@@ -47,14 +47,14 @@ struct Layout {
 // log2-domain score of raw product x and visible row j, of query row `lane & 15` (of each 16);
 // put(h, d, o, M, T): called once for each query row h and four dims from d on, with O, its maximum
 // and its sum.  Each K and V read from LDS serves NG products of 16 query rows.
-template <int D, bool SH, int NW, int AW, int SLOTS, int NG, class Query, class Score, class Put>
+template <int D, bool SH, int NW, int SLOTS, int NG, class Query, class Score, class Put>
 __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
-    using L = Layout<D, SH, AW, SLOTS, NG>;
+    using L = Layout<D, SH, NW, SLOTS, NG>;
     constexpr int KS = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
     unsigned char *const ring = lds + wave * SLOTS * L::SLOT;
-    const int all = (x.j1 - x.j0 + 15) >> 4, nst = wave < AW ? all : 0;  // this wave's range of stages
+    const int nst = (x.j1 - x.j0 + 15) >> 4;
     const bool append = x.k_new != nullptr;
 
     const int drow = lane / L::CPR, chunk = lane % L::CPR;  // DMA: this lane's row among a block's, its chunk
@@ -106,12 +106,12 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         for (int dt = 0; dt < DT; ++dt) acc[g][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    for (int st = wave, it = 0; st < nst; st += AW, ++it) {
+    for (int st = wave, it = 0; st < nst; st += NW, ++it) {
         unsigned char *const slot = ring + (SLOTS > 1 ? (it & 1) * L::SLOT : 0);
         ESDA_WAIT_VM(0);  // this stage landed
-        if (SLOTS > 1 && st + AW < nst) {
+        if (SLOTS > 1 && st + NW < nst) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other slot's reads are done
-            dma(st + AW, ring + ((it + 1) & 1) * L::SLOT);
+            dma(st + NW, ring + ((it + 1) & 1) * L::SLOT);
         }
         asm volatile("" ::: "memory");
         // Rows past the run repeat its last one, with a weight of 0; but 0 x inf is NaN.
@@ -179,9 +179,9 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int g = 0; g < NG; ++g) acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(va[dt], pb[g], acc[g][dt], 0, 0, 0);
-        if (SLOTS == 1 && st + AW < nst) {
+        if (SLOTS == 1 && st + NW < nst) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads are done
-            dma(st + AW, ring);
+            dma(st + NW, ring);
         }
     }
 #pragma unroll
@@ -199,9 +199,9 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         }
 
     // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = -inf, l = 0.
-    f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + AW * L::ROWS;  // [AW][ROWS], [ROWS]
-    float *const sum = reinterpret_cast<float *>(lds);                                           // [AW][G][PITCH]
-    if (lg == 0 && wave < AW)
+    f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + NW * L::ROWS;  // [NW][ROWS], [ROWS]
+    float *const sum = reinterpret_cast<float *>(lds);                                           // [NW][G][PITCH]
+    if (lg == 0)
 #pragma unroll
         for (int g = 0; g < NG; ++g) ml[wave * L::ROWS + 16 * g + li] = f32x2{m[g], l[g]};
     lds_barrier();  // and every wave is done with its slots
@@ -211,14 +211,14 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         const f32x2 *const of = ml + 16 * g + li;
         float M = -INFINITY, T = 0.0f;
 #pragma unroll
-        for (int w = 0; w < AW; ++w) M = fmaxf(M, of[w * L::ROWS][0]);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, of[w * L::ROWS][0]);
         const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-        for (int w = 0; w < AW; ++w) T = __builtin_fmaf(of[w * L::ROWS][1], __builtin_amdgcn_exp2f(of[w * L::ROWS][0] - mu), T);
+        for (int w = 0; w < NW; ++w) T = __builtin_fmaf(of[w * L::ROWS][1], __builtin_amdgcn_exp2f(of[w * L::ROWS][0] - mu), T);
         if (wave == 0 && lg == 0) tot[16 * g + li] = f32x2{M, T};
         c[g] = __builtin_amdgcn_exp2f(m[g] - mu);
     }
-    const int live = all < AW ? all : AW;  // waves that had a stage
+    const int live = nst < NW ? nst : NW;  // waves that had a stage
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += L::CH) {
         if (wave < live)
@@ -238,6 +238,162 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         }
         lds_barrier();  // before the next dims, or the next run's DMAs
     }
+}
+
+// The same run by waves that work together, for up to 16 query rows whose O^T over the whole head dim
+// takes long to sum (512 dims): groups of SUB 16-row stages in two slots; wave w < SUB scores stage w
+// over the whole head dim, every wave reads all scores and holds O^T of D / NW dims.  Two barriers a
+// group (64 rows of 1 KB in 1.9 us; attend_run's waves take them in 1.1), and nothing to sum at the end
+// (3 us there).
+template <int D, bool SH>
+struct GroupLayout {
+    static constexpr int BLK = 1056, NI = D / 32, HB = NI * BLK;  // (as in Layout)
+    static constexpr int CPR = D / 8;
+    static constexpr int SUB = (SH ? 1 : 2) * D > 512 ? 2 : 4;
+    static constexpr int ROWS = 16 * SUB;
+    static constexpr int SLOT = (SH ? 1 : 2) * SUB * HB;
+    static constexpr int BYTES = 2 * SLOT + SUB * 1024;  // two slots, then the scores
+    __device__ static constexpr int off(int r) { return (r % NI) * BLK + (r / NI) * 2 * D; }
+};
+
+// Arguments as attend_run's; put's four dims come from one lane, the rows of 16 side by side.
+template <int D, bool SH, int NW, class Query, class Score, class Put>
+__device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
+    using L = GroupLayout<D, SH>;
+    constexpr int KS = D / 32, DT = D / 16 / NW, SUB = L::SUB;  // k-steps; O^T dim tiles a wave
+    constexpr int LOADS = (SH ? 1 : 2) * L::NI;                 // DMAs of a stage
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const bool scores = wave < SUB, append = x.k_new != nullptr;
+    const int groups = (x.j1 - x.j0 + L::ROWS - 1) / L::ROWS;
+    f32x4 *const xch = reinterpret_cast<f32x4 *>(lds + 2 * L::SLOT);  // [SUB][64 lanes]
+
+    const int drow = lane / L::CPR, chunk = lane % L::CPR;
+    const unsigned voff = (unsigned) ((drow * L::NI * D + chunk * 8) * 2);
+    // This wave's stage of group i; false where it has none or holds no row.
+    auto dma = [&](int i) {
+        const int jst = x.j0 + L::ROWS * i + 16 * wave;
+        if (!scores || jst >= x.j1) return false;
+        const unsigned at = lds_addr(lds) + (i & 1) * L::SLOT + wave * L::HB;
+        if (jst + 16 < x.j1 && x.first + jst + 16 <= x.cap) {
+            const uint16_t *kb = x.k + (size_t) (x.first + jst) * D, *vb = x.v + (size_t) (x.first + jst) * D;
+#pragma unroll
+            for (int t = 0; t < L::NI; ++t) {
+                lds_dma16_s(kb + t * D, voff, at + t * L::BLK);
+                if constexpr (!SH) lds_dma16_s(vb + t * D, voff, at + SUB * L::HB + t * L::BLK);
+            }
+            return true;
+        }
+#pragma unroll
+        for (int t = 0; t < L::NI; ++t) {
+            const int j = min(jst + t + L::NI * drow, x.j1 - 1);  // rows past the run repeat its last, masked
+            int r = x.first + j;
+            if (r >= x.cap) r -= x.cap;
+            const bool is_new = append && j == x.nvis - 1;
+            lds_dma16((is_new ? x.k_new : x.k + (size_t) r * D) + chunk * 8, at + t * L::BLK);
+            if constexpr (!SH) lds_dma16((is_new ? x.v_new : x.v + (size_t) r * D) + chunk * 8, at + SUB * L::HB + t * L::BLK);
+        }
+        return true;
+    };
+
+    dma(0);
+    u32x4 qv[KS];  // B operands: query row li, dims 32 ks + 8 lg ..
+    const bool there = scores && li < x.G;
+    const uint16_t *const qr = query(there ? li : 0) + 8 * lg;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(qr + 32 * ks);
+        qv[ks] = there ? w : u32x4{0u, 0u, 0u, 0u};
+    }
+    // q in registers before the second group's DMAs (its loads would be waited for with them)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qv[ks]));
+    ESDA_WAIT_VM(0);
+    bool ahead = groups > 1 && dma(1);  // the next group's stage is under way
+    const int qk_off = L::off(li) + lg * 16, tr_off = L::off(4 * lg + li / 4) + (li % 4) * 8;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int i = 0; i < groups; ++i) {
+        unsigned char *const slot = lds + (i & 1) * L::SLOT;
+        if (ahead) ESDA_WAIT_VM(LOADS);
+        else ESDA_WAIT_VM(0);
+        if (scores) {
+            unsigned char *const kb = slot + wave * L::HB, *const vb = SH ? kb : kb + SUB * L::HB;
+            const int jst = x.j0 + L::ROWS * i + 16 * wave;
+            // Rows past the run repeat its last one or hold anything, with a weight of 0; but 0 x inf is NaN.
+            for (int r = max(0, x.j1 - jst); r < 16; ++r)
+                if (lane < D / 8) *reinterpret_cast<u32x4 *>(vb + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+            asm volatile("" ::: "memory");
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // (in four sums, as attend_run's, the step took as long)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const bf16x8 k8 = *reinterpret_cast<const bf16x8 *>(kb + qk_off + 64 * ks);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, __builtin_bit_cast(bf16x8, qv[ks]), s, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] = jst + 4 * lg + r < x.j1 ? score(s[r], jst + 4 * lg + r) : -INFINITY;
+            xch[wave * 64 + lane] = s;
+        }
+        lds_barrier();  // every score written, every stage landed
+        const unsigned char *const vt = slot + (SH ? 0 : SUB * L::HB) + tr_off + 32 * DT * wave;
+        short4v va[DT][SUB];  // V^T, in flight during the softmax
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+                va[dt][u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4v *) (vt + u * L::HB + 32 * dt));
+        f32x4 s[SUB];
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            s[u] = xch[u * 64 + lane];
+            top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+        }
+        top = wave_max_across_groups(top);
+        if (__any(top > m + kRescaleSlack)) {
+            const float mn = top > m + kRescaleSlack ? top : m;
+            const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= corr;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[dt] *= corr;
+            m = mn;
+        }
+        bf16x8 pb[SUB / 2];  // the weights as they enter both sums: bf16
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const __bf16 w = (__bf16) __builtin_amdgcn_exp2f(s[u][r] - m);
+                l += (float) w;
+                pb[u / 2][4 * (u % 2) + r] = w;
+            }
+#pragma unroll
+        for (int u = 0; u < SUB; u += 2)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const short4v a0 = va[dt][u], a1 = va[dt][u + 1];
+                const short8v a8 = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+                acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a8), pb[u / 2], acc[dt], 0, 0, 0);
+            }
+        lds_barrier();  // every wave is done with the slot and the scores
+        ahead = i + 2 < groups && dma(i + 2);
+    }
+
+    if (append && x.j1 == x.nvis && wave == 0)  // the new row into the cache, as in attend_run
+        for (int c = lane; c < D / 8; c += 64) {
+            *reinterpret_cast<u32x4 *>(x.k + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.k_new + 8 * c);
+            if constexpr (!SH)
+                *reinterpret_cast<u32x4 *>(x.v + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.v_new + 8 * c);
+        }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (li < x.G)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) put(li, 16 * (DT * wave + dt) + 4 * lg, acc[dt], m, l);
 }
 
 }  // namespace esda_stream
