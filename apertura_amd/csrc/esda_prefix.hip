@@ -381,10 +381,19 @@ hipError_t launch_step(const PrefixParams &p, const PrefixMergeParams &m, bool s
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    // The threads of the first form hold a row's partials side by side: up to 8 of them always, up to 40
+    // where there are threads to cover the loads.  64 rows (2,048 .. 8,192 threads) in 21 partials, first
+    // form / second: 10.5 / 8.9, 19.0 / 17.5, 15.4 / 14.1 us a step (D = 128, 256, 512); 32,768 threads, 11
+    // 15.3 / 16.3 and 20.9 / 21.8, 21 20.7 / 20.5 and 22.2 / 22.3; 65,536 20.1 / 23.7 and 24.7 / 28.4, 31
+    // 33.6 / 35.5 and 41.3 / 43.6; 262,144 in 11 37.6 / 48.5, in 31 77.4 / 79.6.
     const int rows = m.B * m.Hq, n = m.splits + m.own_splits;
-    const unsigned few = (unsigned) (((long long) rows * (D / 4) + 255) / 256);
+    const long long threads = (long long) rows * (D / 4);
+    const unsigned few = (unsigned) ((threads + 255) / 256);
     if (n <= 4) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 4>), dim3(few), dim3(256), 0, st, m);
     else if (n <= 8) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 8>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 16 && threads >= 1 << 15) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 16>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 24 && threads >= 1 << 15) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 24>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 40 && threads >= 1 << 16) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 40>), dim3(few), dim3(256), 0, st, m);
     else hipLaunchKernelGGL(prefix_merge_many_kernel<D>, dim3(rows * (D / 64)), dim3(256), 0, st, m);
     return hipGetLastError();
 }
