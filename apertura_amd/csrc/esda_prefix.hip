@@ -4,9 +4,9 @@
 // whose workgroups stand side by side in one grid: the prefix as query tiles, each key read once
 // for the B * G query rows of its kv head (prefill_kernel with PrefixParams), or, for few of them,
 // in runs (prefix_run_kernel); the own rows in runs, with the fused append.  The second merges them.
-// A step of few rows is bound by the latency of the two (2 sequences behind 2049 tokens: 15 us), a
+// A step of few rows is bound by the latency of the two (2 sequences behind 2049 tokens: 13.5 us), a
 // long one by reading prefix and own rows once (4 behind 32,768, 138 MB: 40 us), one of many sequences
-// by both kinds of workgroups sharing the CUs (64 behind 16,384, 200 MB and 18 GFLOP: 64 us).  With
+// by both kinds of workgroups sharing the CUs (64 behind 16,384, 200 MB and 18 GFLOP: 61 us).  With
 // prefix, own rows and their merges in launches one after the other these took 48, 99 and 123 us.
 // The C ABI is include/esda_prefix.h.
 
