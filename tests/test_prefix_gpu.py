@@ -304,3 +304,20 @@ def test_two_steps_at_once(B, D):
     for got in outs:
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("split_rows,split_keys", [(0, 0), (64, 384), (384, 416), (400, 352), (896, 1024), (16, 64)])
+@pytest.mark.parametrize("shared,B", [(True, 2), (True, 14), (False, 3), (False, 20)])
+def test_runs_of_every_length_at_head_dim_512(shared, B, split_rows, split_keys):
+    """Own rows and prefix on both sides of the length up to which runs go in groups of stages, beside
+    runs (few query rows), four-wave tiles and eight-wave ones."""
+    own = [0, 899, 1, 15, 16, 17, 63, 64, 65, 127, 383, 384, 385, 400, 447, 448, 600, 31, 32, 33][:B]
+    Case(B, 8, 1, 512, 1300, 900, own, shared, split_keys, split_rows, seed=25).run()
+
+
+@pytest.mark.parametrize("D,hq,hkv,P,split_keys", [(128, 32, 8, 700, 64), (256, 32, 16, 500, 32), (512, 32, 4, 640, 64),
+                                                   (128, 32, 8, 1200, 32)])
+def test_merges_of_many_partials(D, hq, hkv, P, split_keys):
+    """10 .. 41 partials a row, of few rows (groups in turn) and of many (a thread each)."""
+    for B in (1, 64):
+        Case(B, hq, hkv, D, P, 100, _own(B, 100, B), D == 512, split_keys, 48, seed=26 + B).run()
