@@ -76,8 +76,8 @@ ESDA_HD bool grid_split(int s, int S, int chunk, int nvis, int *j0, int *j1) {
 
 // Splits of a grid pair that wrote partials (the merge reads these).
 ESDA_HD int grid_splits(int nvis, int chunk, int S) {
-    const int n = (nvis + chunk - 1) / chunk;
-    return n < S ? n : S;
+    const unsigned n = ((unsigned) nvis + (unsigned) chunk - 1u) / (unsigned) chunk;  // (the sum may pass 2^31)
+    return n < (unsigned) S ? (int) n : S;
 }
 
 // Workgroups that hold rows: every share must hold at least one, and fewer rows may be

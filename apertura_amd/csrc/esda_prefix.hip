@@ -272,8 +272,8 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     const int nf = forms_of(D, group_rows, shared, f);
     float best = INFINITY;
     auto consider = [&](const Form &form, int chunk, int keys) {
-        const int splits = (P + keys - 1) / keys, tiles = (group_rows + form.rows() - 1) / form.rows();
-        const int own_splits = (int) ((own.maxvis + chunk - 1LL) / chunk), n = splits + own_splits;
+        const int splits = (int) (((long long) P + keys - 1) / keys), tiles = (group_rows + form.rows() - 1) / form.rows();
+        const int own_splits = (int) (((long long) own.maxvis + chunk - 1) / chunk), n = splits + own_splits;
         const long long groups = (long long) tiles * Hkv * splits, own_groups = (long long) B * Hkv * own_splits;
         const float us = form.start + std::min(keys, P) * row_kb * form.per_kb;
         const float own_us = c.own_start + std::min(chunk, own.maxvis) * row_kb / c.own_rate;
@@ -294,10 +294,13 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
         p.own_chunk = chunk;
         p.own_splits = own_splits;
     };
+    // Forced splits longer than the rows are cut to them, in whole units (the kernels add one to a row).
+    auto whole = [](long long n, int unit) { return (n + unit - 1) / unit * unit; };
+    const int forced_keys = (int) std::min<long long>(d->split_keys, whole(P, kStageKeys));
     auto with_chunk = [&](int chunk) {
         for (int i = 0; i < nf; ++i) {
-            if (d->split_keys > 0) {
-                consider(f[i], chunk, d->split_keys);
+            if (forced_keys > 0) {
+                consider(f[i], chunk, forced_keys);
                 continue;
             }
             const int least = f[i].ng ? kRunRows : kStageKeys, unit = f[i].ng ? 16 : kStageKeys;
@@ -312,11 +315,12 @@ int fresh_prefix_plan(const esda_prefix_desc *d, PrefixPlan *pl) {
     };
     const int least_chunk = (own.maxvis / kOwnSplits + 16) / 16 * 16;  // (at most kOwnSplits of them)
     if (d->own.split_rows > 0) {
-        with_chunk((own.maxvis + d->own.split_rows - 1LL) / d->own.split_rows > kOwnSplits ? least_chunk : d->own.split_rows);
+        const int forced = (int) std::min<long long>(d->own.split_rows, whole(d->own.cap, kTile));
+        with_chunk(((long long) own.maxvis + forced - 1) / forced > kOwnSplits ? least_chunk : forced);
     } else {
         int last = 0;
         for (int s = 1; s <= kOwnSplits; s += std::max(1, s / 2)) {
-            const int chunk = (int) std::max<long long>(kRunRows, std::min((own.maxvis + s - 1LL) / s + 15, (long long) INT_MAX) / 16 * 16);
+            const int chunk = (int) std::max<long long>(kRunRows, std::min(((long long) own.maxvis + s - 1) / s + 15, (long long) INT_MAX) / 16 * 16);
             if (chunk != last) with_chunk(chunk);
             if (chunk == kRunRows) break;
             last = chunk;

@@ -199,3 +199,27 @@ def test_balanced_merges_the_edge_cases_rely_on(name, merge, longest):
     assert (kernel, most) == (merge, longest)
     if "loop" in name:
         assert most > (64 if kernel == "merge_kernel<4>" else 256)
+
+
+def test_grid_splits_of_chunks_to_the_end_of_int32(tmp_path):
+    """The merge's count of the splits that hold rows, beside the same in 64 bits."""
+    src = tmp_path / "grid.cpp"
+    src.write_text("""
+#include "esda_plan.h"
+#include <cstdio>
+int main() {
+    const int splits[] = {1, 2, 64, 16384};
+    const int edge[] = {1, 2, 15, 16, 17, 100, 1 << 20, (1 << 30) - 1, 1 << 30, (1 << 30) + 1, 2147483600, 2147483632, 2147483647};
+    for (int nvis : edge)
+        for (int chunk : edge)
+            for (int S : splits) {
+                const long long n = ((long long) nvis + chunk - 1) / chunk;
+                const int got = esda_plan::grid_splits(nvis, chunk, S);
+                if (got != (n < S ? n : S)) return std::printf("nvis %d chunk %d S %d: %d\\n", nvis, chunk, S, got), 1;
+            }
+    return esda_plan::grid_splits(0, 16, 4) != 0;
+}
+""")
+    exe = _build(tmp_path, src=str(src))
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout

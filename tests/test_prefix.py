@@ -108,3 +108,18 @@ def test_extreme_descriptions_plan_quickly(kw):
     o = step.own
     row = o.batch * o.num_q_heads * (4 * o.head_dim + 8)
     assert 2 * row <= n <= (512 + 64) * row + 4096
+
+
+def test_splits_longer_than_the_rows_are_one_split():
+    """Forced splits up to the end of int32, alone and together, plan as one split of the prefix and
+    one of the own rows; so does every length in between."""
+    one = prefix_workspace_bytes(_step(split_keys=128, split_rows=64))
+    top_keys, top_rows = 2 ** 31 - 32, 2 ** 31 - 16
+    for keys, rows in ((top_keys, 64), (128, top_rows), (top_keys, top_rows), (2 ** 30, 2 ** 30), (2 ** 31 - 96, 2 ** 31 - 64)):
+        assert prefix_workspace_bytes(_step(split_keys=keys, split_rows=rows)) == one
+    for kw in (dict(cap=2 ** 30, max_visible=40), dict(cap=2 ** 30), dict(prefix_len=2 ** 30), dict(cap=2 ** 31 - 102)):
+        n = prefix_workspace_bytes(_step(split_keys=top_keys, split_rows=top_rows, **kw))
+        assert n == one
+    # own rows take at most 64 splits, 100 keys of a prefix at most four
+    assert prefix_workspace_bytes(_step(cap=2 ** 31 - 102, split_rows=16)) <= 68 * 32 * (4 * 128 + 8) + 4096
+    assert prefix_workspace_bytes(_step(cap=2 ** 31 - 102)) <= 68 * 32 * (4 * 128 + 8) + 4096

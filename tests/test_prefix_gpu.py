@@ -321,3 +321,12 @@ def test_merges_of_many_partials(D, hq, hkv, P, split_keys):
     """10 .. 41 partials a row, of few rows (groups in turn) and of many (a thread each)."""
     for B in (1, 64):
         Case(B, hq, hkv, D, P, 100, _own(B, 100, B), D == 512, split_keys, 48, seed=26 + B).run()
+
+
+@pytest.mark.parametrize("D,hq,hkv,shared", [(128, 8, 2, False), (256, 4, 2, False), (512, 8, 1, True)])
+def test_forced_splits_longer_than_any_row(D, hq, hkv, shared):
+    """split_keys and split_rows up to the end of int32: one split of each, also where more own rows
+    are visible than the estimate says."""
+    for keys, rows in ((2 ** 31 - 32, 0), (0, 2 ** 31 - 16), (2 ** 31 - 32, 2 ** 31 - 16)):
+        Case(4, hq, hkv, D, 100, 64, [63, 0, 17, 40], shared, keys, rows, seed=40).run()
+        Case(2, hq, hkv, D, 300, 200, [199, 60], shared, keys, rows, max_visible=32, seed=41).run()
