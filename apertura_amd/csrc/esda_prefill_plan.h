@@ -308,7 +308,8 @@ const char *plan_prefill(const esda_prefill_desc *d, P *p) {
         }
         if (!few) break;  // many rounds of the tallest tiles: nothing for shorter ones to fill
     }
-    if (d->split_keys > 0) kps = d->split_keys;
+    // (A forced split is cut to the longest tile's stages: the kernel adds it to a tile's first key.)
+    if (d->split_keys > 0) kps = (int) std::min<long long>(d->split_keys, (long long) most_stages * kStageKeys);
     const long long splits = ((long long) most_stages * kStageKeys + kps - 1) / kps;
     if (splits > 65535 || (long long) p->tiles * d->num_kv_heads * splits > INT_MAX)
         return "esda_prefill: too many key splits";

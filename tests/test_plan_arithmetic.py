@@ -223,3 +223,18 @@ int main() {
     exe = _build(tmp_path, src=str(src))
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout
+
+
+def test_forced_splits_longer_than_a_tile_s_keys(tmp_path):
+    """A forced split up to the end of int32 is one split of at most the keys' stages: the kernel adds it
+    to a tile's first key, which a window moves past 0."""
+    exe = _build(tmp_path, src=os.path.join(ROOT, "tests", "prefill_plan_check.cpp"))
+    chunks = [(8, 2, 128, 600, 1600, 1000, 0, 64), (4, 2, 256, 300, 363, 5000, 4937, 64), (8, 1, 512, 100, 700, 600, 0, 32),
+              (4, 2, 128, 50, 50, 0, 0, 0)]
+    for split in (2 ** 31 - 32, 2 ** 31 - 64, 2 ** 30):
+        lines = "".join(" ".join(map(str, c)) + f" {split}\n" for c in chunks)
+        r = subprocess.run([str(exe)], input=lines, capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0
+        for c, line in zip(chunks, r.stdout.splitlines(), strict=True):
+            _, _, _, splits, kps, _, nbytes = map(int, line.split())
+            assert (splits, nbytes) == (1, 0) and 0 < kps <= c[4] + 32 and kps % 32 == 0

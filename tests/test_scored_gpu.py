@@ -552,3 +552,18 @@ def test_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for x, y in outs:
         assert torch.equal(x, want) and torch.equal(y, dwant)
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_a_forced_split_longer_than_any_tile_s_keys(D):
+    """split_keys at the end of int32 under a window, whose later tiles begin past key 0: every row as
+    unsplit."""
+    hq, hkv, shared = HEADS[D]
+    _run(D, 400, 300, softcap=20.0, biased=True, window=64, split=2 ** 31 - 32)
+    _run(D, 200, 0, window=33, prefix=70, split=2 ** 31 - 64)
+    g = _gen(33)
+    q, k = _rows((hq, 400, D), g, 2.5), _rows((hkv, 700, D), g)
+    v = k if shared else _rows((hkv, 700, D), g)
+    step = PrefillStep(hq, hkv, D, 400, 700, 300, 0, 64, D ** -0.5, 2 ** 31 - 32)
+    out = torch.full((400, hq, D), 9.0, dtype=BF, device=DEV)
+    _check_prefill(step, Score(), q, k, v, prefill(step, q, k, v, out=out))
