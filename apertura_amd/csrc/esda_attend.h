@@ -17,6 +17,7 @@
 #include "esda_device.h"
 #include "esda_internal.h"
 #include "esda_plan.h"
+#include "esda_softcap.h"
 
 namespace {
 
@@ -69,10 +70,10 @@ struct AttendParams {
 
 
 
-// A step with modified scores (esda_scored.h): score (log2 units) = cap_out tanh(cap_in raw /
-// (2 log2 e)) where cap_out is not 0, less slopes[head] log2 e per position of distance.
+// A step with modified scores (esda_scored.h): capped by `soft`, less slopes[head] log2 e per position
+// of distance.
 struct ScoredAttendParams : AttendParams {
-    float cap_in, cap_out;
+    SoftCap soft;
     const float *slopes;
 };
 
@@ -499,9 +500,8 @@ void attend_kernel(P p) {
         for (int r = 0; r < 4; ++r) {
             float x = sc[r] * p.scale_log2e;
             if constexpr (SCORED) {
-                // tanh(y) = 1 - 2 / (1 + e^2y)
-                if (p.cap_out != 0.0f)
-                    x = p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[r] * p.cap_in)), 1.0f);
+                if (p.soft.wide) x = capped_wide(sc[r], x, p.soft);
+                else if (p.soft.out != 0.0f) x = capped_narrow(sc[r], p.soft);
                 x = __builtin_fmaf(-slope, (float) (sv.nvis - 1 - jt - r), x);
             }
             sc[r] = hmatch && (jt + r) < j1 ? x : -INFINITY;

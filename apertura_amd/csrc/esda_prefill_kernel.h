@@ -177,7 +177,9 @@ struct PRing {
 // keys ahead of a query, a row that sees nothing gives 0, and a value that is not finite reaches
 // only the rows that see its key.  Bound as the plain form, by the MFMAs and the softmax in turn: a
 // cap adds 6 .. 9% at D = 256 and 512 (2048 queries 92 -> 100 us, 143 -> 151) and 25% at D = 128,
-// whose stages have half or a quarter of the products to a score (4096 queries 150 -> 187).
+// whose stages have half or a quarter of the products to a score (4096 queries 150 -> 187).  Wide caps
+// have kernels of their own (P = WideScoredParams, WideDocParams): as a branch in these, their form cost
+// the others up to 8% (4096 local queries at D = 256, 153 -> 166, no cap).
 // P = DocParams: document ids (equal, not negative) close the other keys, too.  The waves first
 // read the range of ids of every 32-key stage: stages that hold no id of the tile's range are never
 // loaded, those that hold nothing but the tile's one id need no mask, and the ids of the others
@@ -186,8 +188,9 @@ template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool
           class P = PrefillParams>
 // (D == 128 on four waves: two workgroups per CU)
 __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_kernel(P p) {
-    constexpr bool DOCS = std::is_same<P, DocParams>::value;
-    constexpr bool SCORED = DOCS || std::is_same<P, ScoredParams>::value;
+    constexpr bool DOCS = std::is_base_of<DocParams, P>::value;
+    constexpr bool SCORED = std::is_base_of<ScoredParams, P>::value;
+    constexpr bool WIDE = std::is_same<P, WideScoredParams>::value || std::is_same<P, WideDocParams>::value;
     constexpr bool PARTS = std::is_same<P, PrefixParams>::value;  // a partial from every split, also one
     static_assert(!S2 || !KH, "two stages per iteration: all waves on both");
     static_assert(!PS || (QB == 1 && !KH), "pair split: one block per wave, every wave on every stage");
@@ -625,15 +628,20 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                                  : jb + kStageKeys <= j1 && ka_last <= qa_min &&
                                        (p.window == 0 || ka_first > qa_max - p.window);
         if constexpr (SCORED) {
-            if (p.cap_out != 0.0f) {
-                // tanh(x) = 1 - 2 / (1 + e^2x), to 2^-22 or so; the softmax drops the 1, so the capped score
-                // is -1 / (1 + e^2x) in units of 2 cap log2 e
-                c2 = 2.0f * p.cap_out;
+            if constexpr (WIDE) {
+                c2 = 1.0f;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sv[qb][e] = capped_wide(sv[qb][e], sv[qb][e] * p.scale_log2e, p.soft);
+            } else if (p.soft.out != 0.0f) {
+                // the softmax drops the 1 of 1 - 2 / (1 + e^2x): -1 / (1 + e^2x) in units of 2 cap log2 e
+                c2 = 2.0f * p.soft.out;
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        sv[qb][e] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(sv[qb][e] * p.cap_in));
+                        sv[qb][e] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(sv[qb][e] * p.soft.in));
             }
             if (p.slopes) {
                 // Keys at or before their queries: the bias is linear, base + slope (key's place in the
@@ -940,8 +948,11 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                                 x = __builtin_fmaf(bf16_hi(qv[e]), bf16_hi(kv[e]), x);
                             }
                         }
-                        x = p.cap_out != 0.0f ? 2.0f * p.cap_out * __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * p.cap_in))
-                                              : x * p.scale_log2e;
+                        const float raw = x;
+                        x *= p.scale_log2e;
+                        if constexpr (WIDE) x = capped_wide(raw, x, p.soft);
+                        else if (p.soft.out != 0.0f)
+                            x = 2.0f * p.soft.out * __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(raw * p.soft.in));
                         x = __builtin_fmaf(-sl, __builtin_fabsf((float) (qa - ka)), x);
                     }
                     float top = seen ? x : -INFINITY;

@@ -14,6 +14,7 @@
 
 #include "esda_plan.h"
 #include "esda_prefill.h"
+#include "esda_softcap.h"
 
 namespace esda_prefill_plan {
 
@@ -60,13 +61,16 @@ ESDA_HD void tile_keys(const PrefillParams &p, int tile, int QT, int &j0, int &j
 // The parameters of a call with modified scores and masks (esda_scored.h) beside a plain one's.
 struct ScoredParams : PrefillParams {
     int prefix;               // keys before this position are visible to queries before them, too
-    float cap_in, cap_out;    // cap log2 e tanh(x) with e^2x = 2^(cap_in q.k); cap_out = cap log2 e, 0: none
+    SoftCap soft;
     const float *slopes;      // distance bias of each query head, or null
 };
 // .. and its document ids of queries and keys
 struct DocParams : ScoredParams {
     const int *q_doc, *k_doc;
 };
+// .. and both with a wide cap (esda_softcap.h), in kernels of their own
+struct WideScoredParams : ScoredParams {};
+struct WideDocParams : DocParams {};
 
 // The same for a scored call: every row sees the keys of the prefix, within its window.
 ESDA_HD void tile_keys(const ScoredParams &p, int tile, int QT, int &j0, int &j1) {

@@ -39,8 +39,8 @@ __global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(ScoredAtte
             lds, x, [&](int h) { return q + (size_t) h * D; },
             [&](float s, int j) {
                 float y = s * p.scale_log2e;
-                if (p.cap_out != 0.0f)  // tanh(y) = 1 - 2 / (1 + e^2y)
-                    y = p.cap_out * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.cap_in)), 1.0f);
+                if (p.soft.wide) y = capped_wide(s, y, p.soft);
+                else if (p.soft.out != 0.0f) y = capped_narrow(s, p.soft);
                 return __builtin_fmaf(-slope, (float) (sv.nvis - 1 - j), y);
             },
             [&](int h, int d, const f32x4 &o, float M, float T) {
@@ -82,12 +82,8 @@ extern "C" int esda_scored_decode(const esda_decode_desc *d, const esda_score *s
         return fail(ESDA_ERR_WORKSPACE, "esda_scored_decode: workspace missing or smaller than esda_decode_workspace_size");
     ScoredAttendParams ap{};
     static_cast<AttendParams &>(ap) = decode_params(d, a);
-    if (s->softcap > 0.0f) {
-        ap.cap_in = (float) (2.0 * 1.4426950408889634 * d->scale / s->softcap);
-        ap.cap_out = (float) (1.4426950408889634 * s->softcap);
-        if (!std::isfinite(ap.cap_in) || !std::isfinite(ap.cap_out) || ap.cap_in == 0.0f)
-            return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: softcap and scale are too far apart");
-    }
+    if (!set_softcap(s->softcap, d->scale, &ap.soft))
+        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_decode: softcap and scale are too far apart");
     ap.slopes = s->slopes;
     rc = esda_detail::check_device();
     if (rc) return rc;

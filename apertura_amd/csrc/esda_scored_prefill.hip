@@ -32,12 +32,7 @@ const char *plan(const esda_prefill_desc *d, const esda_score *s, ScoredParams *
     if (s->prefix < 0) return "esda_scored_prefill: prefix must not be negative";
     if ((long long) d->k_pos0 + d->seq_k > INT_MAX - 64) return "esda_scored_prefill: key positions must stay below 2^31 - 64";
     if (const char *why = last_plan(d, s->prefix, p)) return why;
-    if (s->softcap > 0.0f) {
-        p->cap_in = (float) (2.0 * 1.4426950408889634 * d->scale / s->softcap);
-        p->cap_out = (float) (1.4426950408889634 * s->softcap);
-        if (!std::isfinite(p->cap_in) || !std::isfinite(p->cap_out) || p->cap_in == 0.0f)
-            return "esda_scored_prefill: softcap and scale are too far apart";
-    }
+    if (!set_softcap(s->softcap, d->scale, &p->soft)) return "esda_scored_prefill: softcap and scale are too far apart";
     p->slopes = s->slopes;
     return nullptr;
 }
@@ -92,12 +87,19 @@ int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, 
         else if (D == 256) launch_prefill<256, P>(x, 3, st);
         else launch_prefill<128, P>(x, 3, st);
     };
-    if (a->k_doc) {
-        DocParams dp{};
+    auto with_documents = [&](auto dp) {
         static_cast<ScoredParams &>(dp) = p;
         dp.q_doc = a->q_doc;
         dp.k_doc = a->k_doc;
         launch(dp);
+    };
+    if (a->k_doc) {
+        if (p.soft.wide) with_documents(WideDocParams{});
+        else with_documents(DocParams{});
+    } else if (p.soft.wide) {
+        WideScoredParams wp{};
+        static_cast<ScoredParams &>(wp) = p;
+        launch(wp);
     } else {
         launch(p);
     }

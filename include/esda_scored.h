@@ -10,7 +10,8 @@
  * (ESGemma4TextModel.mm:68-83).
  *
  * With x = scale q.k of query position qAbs (query head h) and key position kAbs:
- *   s = softcap tanh(x / softcap)      (softcap 0: s = x)
+ *   s = softcap tanh(x / softcap)      (softcap 0: s = x; within 2^-21 softcap of it up to a softcap
+ *                                       of 256, within 2^-21 of itself past that)
  *   s = s - slopes[h] |qAbs - kAbs|    (slopes NULL: no bias)
  * and key j visible to query i iff
  *   (kAbs <= qAbs or kAbs < prefix) and (window == 0 or kAbs > qAbs - window)
@@ -31,7 +32,8 @@ extern "C" {
 #endif
 
 typedef struct esda_score {
-    float softcap;       /* > 0: the cap; 0: none                                          */
+    float softcap;       /* > 0: the cap; 0: none.  One whose quotient with the scale fp32
+                            cannot hold, or near fp32's largest number, is refused         */
     int32_t prefix;      /* prefill: keys at positions below it are visible to earlier queries,
                             too (>= 0).  In a decode step every visible key is at or before the
                             token, so it changes nothing                                   */

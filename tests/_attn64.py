@@ -12,9 +12,10 @@ times the largest sum |q k| scale, plus 2^-20 times the largest score that a cap
 import torch
 
 
-def attend64(q, k, v, seen, scale, softcap=0.0, bias=None):
+def attend64(q, k, v, seen, scale, softcap=0.0, bias=None, score_err=0.0):
     """q [n, D], k / v [m, D], seen [n, m] bool, bias [n, m] (taken off) -> (o [n, D], bound [n, D]),
-    float64.  A row that sees nothing is 0.  Masked keys and values may be anything."""
+    float64.  A row that sees nothing is 0.  Masked keys and values may be anything.  score_err: what a
+    score may be off by beside the above."""
     q, k, v = q.double(), k.double(), v.double()
     used = seen.any(0)
     kz = torch.where(used[:, None], k, 0.0)  # keys that no row sees: never read
@@ -30,7 +31,7 @@ def attend64(q, k, v, seen, scale, softcap=0.0, bias=None):
     p = torch.exp(s - torch.where(top.isinf(), 0.0, top))
     total = p.sum(1, keepdim=True)
     p = p / torch.where(total == 0, 1.0, total)
-    ds = torch.where(seen, (q.shape[1] + 8) * 2.0 ** -24 * size + 2.0 ** -20 * extra, 0.0).amax(1, keepdim=True)
+    ds = torch.where(seen, (q.shape[1] + 8) * 2.0 ** -24 * size + 2.0 ** -20 * extra, 0.0).amax(1, keepdim=True) + score_err
     vz = torch.where(used[:, None], v, 0.0)
     o = p @ vz
     e = 2.0 ** -8 + torch.expm1(2 * ds)  # a weight's score against the largest one's: both off

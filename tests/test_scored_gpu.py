@@ -567,3 +567,75 @@ def test_a_forced_split_longer_than_any_tile_s_keys(D):
     step = PrefillStep(hq, hkv, D, 400, 700, 300, 0, 64, D ** -0.5, 2 ** 31 - 32)
     out = torch.full((400, hq, D), 9.0, dtype=BF, device=DEV)
     _check_prefill(step, Score(), q, k, v, prefill(step, q, k, v, out=out))
+
+
+# Caps far above the scores, and around them.  Up to 256 the capped score may be off by 2^-21 of the cap
+# (an exponential and a reciprocal of half a step or one each, 2^-22 of a tanh), past it by 2^-21 of
+# itself (the bound's 2^-20 holds that).
+CAPS = [60.0, 256.0, 256.5, 1e3, 1e4, 1e5, 1e6, 1e8, 1e20, 1e30]
+
+
+def _score_err(cap):
+    return 2.0 ** -21 * cap if cap <= 256 else 0.0
+
+
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("gain", [2.5, 400.0])
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_caps_of_any_size(D, gain, cap):
+    hq, hkv, shared = HEADS[D]
+    for Sq, past, split, biased in ((70, 0, 0, False), (33, 300, 64, True)):
+        g = _gen(50)
+        q, k = _rows((hq, Sq, D), g, gain), _rows((hkv, past + Sq, D), g)
+        v = k if shared else _rows((hkv, past + Sq, D), g)
+        score = Score(cap, _slopes(hq) if biased else None)
+        step = PrefillStep(hq, hkv, D, Sq, past + Sq, past, 0, 0, D ** -0.5, split)
+        out = scored_prefill(step, score, q, k, v)
+        seen, dist = _seen(step, score)
+        for h in range(hq):
+            bias = score.slopes[h].double() * dist if biased else None
+            o, b = attend64(q[h], k[h // (hq // hkv)], v[h // (hq // hkv)], seen, step.scale, cap, bias, _score_err(cap))
+            check(out[:, h], o, b, f"cap {cap} head {h}")
+
+
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("gain", [2.5, 400.0])
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_decode_caps_of_any_size(D, gain, cap):
+    hq, hkv, shared = SHAPES[D]
+    g, n = _gen(51), 333
+    for biased in (False, True):
+        q, kc, kn = _rows((1, hq, D), g, gain), _rows((1, hkv, n, D), g), _rows((1, hkv, D), g)
+        vc, vn = (kc, kn) if shared else (_rows((1, hkv, n, D), g), _rows((1, hkv, D), g))
+        step = DecodeStep(1, hq, hkv, D, n, kv_shared=shared, scale=D ** -0.5)
+        score = Score(cap, _slopes(hq) if biased else None)
+        out = scored_decode(step, score, q, kn, None if shared else vn, kc, vc,
+                            torch.tensor([n - 1], dtype=torch.int32, device=DEV))
+        dist = torch.arange(n - 1, -1, -1, device=DEV).double()[None]  # (the new row is in the cache now)
+        for h in range(hq):
+            bias = score.slopes[h].double() * dist if biased else None
+            seen = torch.ones((1, n), dtype=torch.bool, device=DEV)
+            o, b = attend64(q[0, h][None], kc[0, h // (hq // hkv)], vc[0, h // (hq // hkv)], seen, step.scale, cap, bias,
+                            _score_err(cap))
+            check(out[0, h][None], o, b, f"cap {cap} head {h}")
+
+
+@pytest.mark.parametrize("split", [0, 64])
+@pytest.mark.parametrize("cap", [0.0, 20.0, 1e7])
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_rows_that_see_an_infinite_value_keep_their_other_dims(D, cap, split):
+    """An infinite value of one dim: that dim infinite from its key on, the others of those rows as
+    without it."""
+    hq, hkv, n, g = 4, 2, 150, _gen(52)
+    q, k, v = _rows((hq, n, D), g, 2.5), _rows((hkv, n, D), g), _rows((hkv, n, D), g)
+    v[:, 60, 5] = float("inf")
+    score = Score(cap, _slopes(hq))
+    step = PrefillStep(hq, hkv, D, n, n, scale=D ** -0.5, split_keys=split)
+    out = scored_prefill(step, score, q, k, v)
+    assert bool((out[60:, :, 5] == float("inf")).all()) and bool(out[:60].isfinite().all())
+    seen, dist = _seen(step, score)
+    v[:, 60, 5] = 0.0
+    for h in range(hq):
+        o, b = attend64(q[h], k[h // 2], v[h // 2], seen, step.scale, cap, score.slopes[h].double() * dist, _score_err(cap))
+        rest = torch.arange(D, device=DEV) != 5
+        check(out[:, h][:, rest], o[:, rest], b[:, rest], f"head {h}")
