@@ -76,6 +76,8 @@ struct ScoredAttendParams : AttendParams {
     SoftCap soft;
     const float *slopes;
 };
+// .. with a wide cap (esda_softcap.h), in kernels of their own
+struct WideScoredAttendParams : ScoredAttendParams {};
 
 // ---------------------------------------------------------------- LDS ring layout
 //
@@ -283,7 +285,8 @@ __device__ __forceinline__ void walk_segments(const AttendParams &p, Seg &&segme
 // k_new/v_new and no other workgroup reads it, so the copy needs no ordering.
 //
 // P = ScoredAttendParams: the four scores a lane holds of a stage are capped and biased before
-// the softmax; row j of the visible ones lies nvis - 1 - j positions behind the token.
+// the softmax; row j of the visible ones lies nvis - 1 - j positions behind the token.  (Wide caps
+// as a branch here: 16 sequences of 1024 .. 8192 rows of 512 dims 64 us -> 68, capped 72.)
 template <int D, bool SHARED, int NW, int OCC = 1, class P = AttendParams>
 // The LDS ring allows OCC workgroups per CU, i.e. OCC * NW/4 waves per SIMD: telling the
 // compiler so lifts the register limit it would otherwise keep for higher occupancy,
@@ -291,7 +294,8 @@ template <int D, bool SHARED, int NW, int OCC = 1, class P = AttendParams>
 // workgroup per CU on a kernel built with OCC = 2: its shallower ring is what they want.)
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * NW, 64 * NW), amdgpu_waves_per_eu(OCC * NW / 4, OCC * NW / 4)))
 void attend_kernel(P p) {
-    constexpr bool SCORED = std::is_same<P, ScoredAttendParams>::value;
+    constexpr bool SCORED = std::is_base_of<ScoredAttendParams, P>::value;
+    constexpr bool WIDE = std::is_same<P, WideScoredAttendParams>::value;
     using R = Ring<D, SHARED, NW, 160 * 1024 / OCC>;
     // D = 512 exchanges only the live heads' partial scores (the padding columns are zero)
     constexpr bool kLiveX = D == 512;
@@ -500,7 +504,7 @@ void attend_kernel(P p) {
         for (int r = 0; r < 4; ++r) {
             float x = sc[r] * p.scale_log2e;
             if constexpr (SCORED) {
-                if (p.soft.wide) x = capped_wide(sc[r], x, p.soft);
+                if constexpr (WIDE) x = capped_wide(sc[r], x, p.soft);
                 else if (p.soft.out != 0.0f) x = capped_narrow(sc[r], p.soft);
                 x = __builtin_fmaf(-slope, (float) (sv.nvis - 1 - jt - r), x);
             }

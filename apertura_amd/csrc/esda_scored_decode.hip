@@ -6,6 +6,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "esda.h"
 #include "esda_attend.h"
@@ -21,8 +22,8 @@ namespace {
 // 115), of 16,384 16.3 (22.3), of 300 8.1 (9.0); K = V, 16 of 512 .. 4096 23.4 (39.4).
 constexpr int kStreamWaves = 8;
 
-template <bool SH>
-__global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(ScoredAttendParams p) {
+template <bool SH, class P>
+__global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(P p) {
     constexpr int D = 128, SLOTS = 2;
     using L = esda_stream::Layout<D, SH, kStreamWaves, SLOTS>;
     __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(ScoredAtte
             lds, x, [&](int h) { return q + (size_t) h * D; },
             [&](float s, int j) {
                 float y = s * p.scale_log2e;
-                if (p.soft.wide) y = capped_wide(s, y, p.soft);
+                if constexpr (std::is_same<P, WideScoredAttendParams>::value) y = capped_wide(s, y, p.soft);
                 else if (p.soft.out != 0.0f) y = capped_narrow(s, p.soft);
                 return __builtin_fmaf(-slope, (float) (sv.nvis - 1 - j), y);
             },
@@ -91,13 +92,21 @@ extern "C" int esda_scored_decode(const esda_decode_desc *d, const esda_score *s
     uint16_t *out = static_cast<uint16_t *>(a->out);
     fill_attend(d, pl, sp, static_cast<int *>(a->workspace), out, ap);
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    auto launch = [&](const auto &x) {
+        using P = std::decay_t<decltype(x)>;
+        const dim3 grid = attend_grid(d, pl), block(64 * kStreamWaves);
+        if (d->head_dim != 128) return dispatch_attend(d->head_dim, d->kv_shared != 0, x, grid, st);
+        if (d->kv_shared) hipLaunchKernelGGL((stream_kernel<true, P>), grid, block, 0, st, x);
+        else hipLaunchKernelGGL((stream_kernel<false, P>), grid, block, 0, st, x);
+        return hipGetLastError();
+    };
     hipError_t e;
-    if (d->head_dim == 128) {
-        if (d->kv_shared) hipLaunchKernelGGL(stream_kernel<true>, attend_grid(d, pl), dim3(64 * kStreamWaves), 0, st, ap);
-        else hipLaunchKernelGGL(stream_kernel<false>, attend_grid(d, pl), dim3(64 * kStreamWaves), 0, st, ap);
-        e = hipGetLastError();
+    if (ap.soft.wide) {
+        WideScoredAttendParams wp{};
+        static_cast<ScoredAttendParams &>(wp) = ap;
+        e = launch(wp);
     } else {
-        e = dispatch_attend(d->head_dim, d->kv_shared != 0, ap, attend_grid(d, pl), st);
+        e = launch(ap);
     }
     if (e != hipSuccess) return hip_fail(e, "attend_kernel launch");
     return launch_merge(d, pl, sp, a->pos, a->row_base, 0, out, st);
