@@ -427,7 +427,7 @@ void attend_kernel(P p) {
     const int tr_off = R::off(4 * lg + li / 4, wave, 0) + (li % 4) * 8;  // + 32*dt
     constexpr int VOFF = SHARED ? 0 : R::TB;
 
-    float m = -INFINITY, l = 0.0f;
+    float m = kNoScore, l = 0.0f;
     f32x4 acc[DTW];
 #pragma unroll
     for (int dt = 0; dt < DTW; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

@@ -66,6 +66,10 @@ __device__ __forceinline__ unsigned wave_sum_across_groups(unsigned x) {
 // far from fp32 / bf16 limits, and the final division by l is unchanged.
 constexpr float kRescaleSlack = 8.0f;
 
+// The running max before any score, in the decode kernels: the lowest finite number, which every score
+// but -inf (an infinite key) reaches, and against which the weight of -inf is 0.  (-inf - -inf is NaN.)
+constexpr float kNoScore = -3.402823466e38f;
+
 // x *= c for a value that lives in an accumulation register (AGPR): read, multiply and
 // write back in place.  With a plain multiply of the PV accumulators the compiler keeps
 // VGPR copies of all of them, refreshed at every stage, for a rescale that is rare.

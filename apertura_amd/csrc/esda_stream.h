@@ -100,7 +100,7 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
     f32x4 acc[NG][DT];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        m[g] = -INFINITY;
+        m[g] = kNoScore;
         l[g] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[g][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -198,7 +198,7 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
                 *reinterpret_cast<u32x4 *>(x.v + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.v_new + 8 * c);
         }
 
-    // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = -inf, l = 0.
+    // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = kNoScore, l = 0.
     f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + NW * L::ROWS;  // [NW][ROWS], [ROWS]
     float *const sum = reinterpret_cast<float *>(lds);                                           // [NW][G][PITCH]
     if (lg == 0)
@@ -212,11 +212,10 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         float M = -INFINITY, T = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) M = fmaxf(M, of[w * L::ROWS][0]);
-        const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) T = __builtin_fmaf(of[w * L::ROWS][1], __builtin_amdgcn_exp2f(of[w * L::ROWS][0] - mu), T);
+        for (int w = 0; w < NW; ++w) T = __builtin_fmaf(of[w * L::ROWS][1], __builtin_amdgcn_exp2f(of[w * L::ROWS][0] - M), T);
         if (wave == 0 && lg == 0) tot[16 * g + li] = f32x2{M, T};
-        c[g] = __builtin_amdgcn_exp2f(m[g] - mu);
+        c[g] = __builtin_amdgcn_exp2f(m[g] - M);
     }
     const int live = nst < NW ? nst : NW;  // waves that had a stage
 #pragma unroll
@@ -311,7 +310,7 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, 
     ESDA_WAIT_VM(0);
     bool ahead = groups > 1 && dma(1);  // the next group's stage is under way
     const int qk_off = L::off(li) + lg * 16, tr_off = L::off(4 * lg + li / 4) + (li % 4) * 8;
-    float m = -INFINITY, l = 0.0f;
+    float m = kNoScore, l = 0.0f;
     f32x4 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

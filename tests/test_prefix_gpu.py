@@ -330,3 +330,29 @@ def test_forced_splits_longer_than_any_row(D, hq, hkv, shared):
     for keys, rows in ((2 ** 31 - 32, 0), (0, 2 ** 31 - 16), (2 ** 31 - 32, 2 ** 31 - 16)):
         Case(4, hq, hkv, D, 100, 64, [63, 0, 17, 40], shared, keys, rows, seed=40).run()
         Case(2, hq, hkv, D, 300, 200, [199, 60], shared, keys, rows, max_visible=32, seed=41).run()
+
+
+@pytest.mark.parametrize("keys", [[32], list(range(32)), list(range(64)), list(range(16, 33)), []])
+@pytest.mark.parametrize("B", [1, 3, 9, 33])
+@pytest.mark.parametrize("D,hq,hkv,shared", HEADS)
+def test_keys_of_minus_infinity(D, hq, hkv, shared, B, keys):
+    """Prefix keys whose scores are -inf, alone in a stage or a whole split of them, and a new token that
+    is its sequence's one own row: weights of 0, whichever kind of workgroup meets them."""
+    P = 33 if keys == [32] else 100
+    for split in (0, 32, 64):
+        c = Case(B, hq, hkv, D, P, 40, _own(B, 40, 5), shared, split_keys=split, seed=60)
+        c.q[..., 3] = c.q[..., 3].abs() + 0.5
+        c.pk[:, keys, 3] = -float("inf")
+        c.kn[..., 3] = -float("inf")
+        k0, v0 = c.kc.clone(), c.vc.clone()
+        out = prefix_decode(c.step, *c.args())
+        G, vn = hq // hkv, c.kn if shared else c.vn
+        dims = torch.arange(D, device=DEV) != 3 if shared else torch.ones(D, dtype=torch.bool, device=DEV)
+        for b, m in enumerate(c.own):
+            seen = torch.ones((G, P + m + 1), dtype=torch.bool, device=DEV)
+            seen[:, keys + [P + m]] = False
+            for h in range(hkv):
+                k = torch.cat([c.pk[h], k0[b, h, :m], c.kn[b, h][None]])
+                v = torch.cat([c.pv[h], v0[b, h, :m], vn[b, h][None]])
+                o, bound = attend64(c.q[b, h * G:(h + 1) * G], k, v, seen, D ** -0.5)
+                check(out[b, h * G:(h + 1) * G][:, dims], o[:, dims], bound[:, dims], f"sequence {b} kv head {h}")

@@ -639,3 +639,38 @@ def test_rows_that_see_an_infinite_value_keep_their_other_dims(D, cap, split):
         o, b = attend64(q[h], k[h // 2], v[h // 2], seen, step.scale, cap, score.slopes[h].double() * dist, _score_err(cap))
         rest = torch.arange(D, device=DEV) != 5
         check(out[:, h][:, rest], o[:, rest], b[:, rest], f"head {h}")
+
+
+# ------------------------------------------------------------ keys whose score is -inf: a weight of 0
+
+@pytest.mark.parametrize("rows,split", [([20], 16), ([16], 16), (list(range(16)), 0), (list(range(32)), 0), (list(range(4, 40)), 16),
+                                        (list(range(150)), 16)])
+@pytest.mark.parametrize("D,heads", [(128, (8, 2, False)), (256, (4, 2, False)), (512, (8, 1, True)), (512, (4, 2, False))])
+@pytest.mark.parametrize("scored", [True, False])
+def test_decode_keys_of_minus_infinity(D, heads, rows, split, scored):
+    """Whole stages and splits of them, first, last or alone: the row over the other keys (one K = V
+    buffer: 0 x inf in the infinite dim alone)."""
+    hq, hkv, shared = heads
+    g = _gen(60)
+    for n in ((21, 160) if rows == [20] else (17, 160) if rows == [16] else (160,)):
+        q, kc, kn = _rows((2, hq, D), g, 2.5), _rows((2, hkv, n, D), g), _rows((2, hkv, D), g)
+        vc, vn = (kc, None) if shared else (_rows((2, hkv, n, D), g), _rows((2, hkv, D), g))
+        q[..., 3] = q[..., 3].abs() + 0.5
+        for r in rows:
+            if r < n - 1:
+                kc[:, :, r, 3] = -float("inf")
+            else:
+                kn[..., 3] = -float("inf")
+        step = DecodeStep(2, hq, hkv, D, n, kv_shared=shared, scale=D ** -0.5, split_rows=split)
+        pos = torch.tensor([n - 1, n - 1], dtype=torch.int32, device=DEV)
+        if scored:
+            out = scored_decode(step, Score(), q, kn, vn, kc, vc, pos)
+        else:
+            out = decode_step(step, q, kn, vn, kc, vc, pos)
+        seen = torch.ones((1, n), dtype=torch.bool, device=DEV)
+        seen[:, [r for r in rows if r < n]] = False
+        dims = torch.arange(D, device=DEV) != 3 if shared else torch.ones(D, dtype=torch.bool, device=DEV)
+        for b in range(2):
+            for h in range(hq):
+                o, bound = attend64(q[b, h][None], kc[b, h // (hq // hkv)], vc[b, h // (hq // hkv)], seen, step.scale)
+                check(out[b, h][None][:, dims], o[:, dims], bound[:, dims], f"n {n} sequence {b} head {h}")
