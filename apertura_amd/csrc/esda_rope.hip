@@ -9,12 +9,12 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
-#include <utility>
 
 #include "esda.h"
 #include "esda_device.h"
 #include "esda_internal.h"
 #include "esda_rope.h"
+#include "esda_views.h"
 
 namespace {
 
@@ -150,43 +150,6 @@ int fail(int code, const std::string &msg) {
     return code;
 }
 
-// Elements from the first to the last of a tensor's rows, or -1 past what an address holds.
-long long extent(int tokens, long long rs, int heads, long long hs, int D) {
-    const __int128 n = (__int128) (tokens - 1) * rs + (__int128) (heads - 1) * hs + D;
-    return n > (__int128) 1 << 60 ? -1 : (long long) n;
-}
-
-// One tensor's rows: T rows of `width` elements (its heads), rs apart.
-struct View {
-    const char *name;
-    const void *ptr;
-    long long rs, hs;
-    int heads;
-    long long width, n;  // elements of one token's heads, and from the first element to the last
-};
-
-// Whether two views share no element: apart in memory, or rows of one buffer side by side (the
-// q and the k part of a packed row).
-bool disjoint(const View &a, const View &b) {
-    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.ptr), pb = reinterpret_cast<uintptr_t>(b.ptr);
-    if (pa >= pb + 2 * (uintptr_t) b.n || pb >= pa + 2 * (uintptr_t) a.n) return true;
-    if (a.rs != b.rs || a.rs <= 0) return false;
-    long long delta = (long long) (((intptr_t) pb - (intptr_t) pa) / 2) % a.rs;
-    if (delta < 0) delta += a.rs;
-    return delta >= a.width && delta + b.width <= a.rs;
-}
-
-// Rows or heads of an output that overlap one another would race.
-bool overlaps_itself(int tokens, long long rs, int heads, long long hs, int D) {
-    long long n[2] = {tokens, heads}, st[2] = {rs, hs};
-    if (st[0] > st[1]) {
-        std::swap(n[0], n[1]);
-        std::swap(st[0], st[1]);
-    }
-    if (n[0] > 1 && st[0] < D) return true;
-    return n[1] > 1 && (__int128) st[1] < (__int128) (n[0] - 1) * st[0] + D;
-}
-
 constexpr long long kThreads = 256 * 512;  // aimed at: 8 waves a CU
 constexpr unsigned kMaxBlocks = 1u << 20;
 
@@ -212,25 +175,28 @@ int esda_rope(const esda_rope_desc *d, const esda_rope_args *a, void *stream) {
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: null device pointer");
     if ((reinterpret_cast<uintptr_t>(a->pos) & 3u) || (reinterpret_cast<uintptr_t>(a->inv_freq) & 3u))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_rope: pos and inv_freq must be 4-byte aligned");
-    View v[4] = {{"q", a->q, d->q_row_stride, d->q_head_stride, Hq, 0, 0},
-                 {"q_out", a->q_out, d->q_out_row_stride, d->q_out_head_stride, Hq, 0, 0},
-                 {"k", a->k, d->k_row_stride, d->k_head_stride, Hk, 0, 0},
-                 {"k_out", a->k_out, d->k_out_row_stride, d->k_out_head_stride, Hk, 0, 0}};
+    const char *const names[4] = {"q", "q_out", "k", "k_out"};
+    auto view = [&](const void *ptr, int heads, long long rs, long long hs) {
+        return esda_views::View{reinterpret_cast<uintptr_t>(ptr), {T, heads}, {rs, hs}, D};
+    };
+    const esda_views::View v[4] = {view(a->q, Hq, d->q_row_stride, d->q_head_stride),
+                                   view(a->q_out, Hq, d->q_out_row_stride, d->q_out_head_stride),
+                                   view(a->k, Hk, d->k_row_stride, d->k_head_stride),
+                                   view(a->k_out, Hk, d->k_out_row_stride, d->k_out_head_stride)};
     int vec = 8;
     bool copy = false;
     for (int i = 0; i < 4; ++i) {
-        if (!v[i].heads) continue;
-        const std::string name = std::string("esda_rope: ") + v[i].name;
-        if (v[i].rs < 0 || v[i].hs < 0) return fail(ESDA_ERR_INVALID_ARGUMENT, name + " strides must not be negative");
-        v[i].n = extent(T, v[i].rs, v[i].heads, v[i].hs, D);
-        v[i].width = extent(1, 0, v[i].heads, v[i].hs, D);
-        if (v[i].n < 0) return fail(ESDA_ERR_INVALID_ARGUMENT, name + " strides are too large");
-        const uintptr_t at = reinterpret_cast<uintptr_t>(v[i].ptr);
+        const long long heads = v[i].n[1], rs = v[i].st[0], hs = v[i].st[1];
+        if (!heads) continue;
+        const std::string name = std::string("esda_rope: ") + names[i];
+        if (rs < 0 || hs < 0) return fail(ESDA_ERR_INVALID_ARGUMENT, name + " strides must not be negative");
+        if (v[i].extent() > (__int128) 1 << 60) return fail(ESDA_ERR_INVALID_ARGUMENT, name + " strides are too large");
+        const uintptr_t at = v[i].ptr;
         if (at & 1u) return fail(ESDA_ERR_INVALID_ARGUMENT, name + " must be 2-byte aligned");
         // runs of VEC elements need every row to start on one
-        while (vec > 1 && (at % (2 * vec) || (T > 1 && v[i].rs % vec) || (v[i].heads > 1 && v[i].hs % vec))) vec /= 2;
+        while (vec > 1 && (at % (2 * vec) || (T > 1 && rs % vec) || (heads > 1 && hs % vec))) vec /= 2;
         if (i & 1) {
-            if (overlaps_itself(T, v[i].rs, v[i].heads, v[i].hs, D))
+            if (esda_views::overlaps_itself(v[i]))
                 return fail(ESDA_ERR_INVALID_ARGUMENT, name + " strides make rows overlap");
             if (v[i - 1].ptr != v[i].ptr) copy = true;
         }
@@ -238,11 +204,11 @@ int esda_rope(const esda_rope_desc *d, const esda_rope_args *a, void *stream) {
     // An output may be its own input; otherwise no output shares an element with another tensor.
     for (int o = 1; o < 4; o += 2)
         for (int i = 0; i < 4; ++i) {
-            if (i == o || !v[o].heads || !v[i].heads) continue;
-            const bool same = i == o - 1 && v[i].ptr == v[o].ptr && (T == 1 || v[i].rs == v[o].rs) &&
-                              (v[i].heads == 1 || v[i].hs == v[o].hs);
-            if (!same && !disjoint(v[i], v[o]))
-                return fail(ESDA_ERR_INVALID_ARGUMENT, std::string("esda_rope: ") + v[o].name + " overlaps " + v[i].name +
+            if (i == o || !v[o].n[1] || !v[i].n[1]) continue;
+            const bool same = i == o - 1 && v[i].ptr == v[o].ptr && (T == 1 || v[i].st[0] == v[o].st[0]) &&
+                              (v[i].n[1] == 1 || v[i].st[1] == v[o].st[1]);
+            if (!same && !esda_views::disjoint(v[i], v[o]))
+                return fail(ESDA_ERR_INVALID_ARGUMENT, std::string("esda_rope: ") + names[o] + " overlaps " + names[i] +
                                                            (i == o - 1 ? " without being the same view" : ""));
         }
     while (vec > 1 && (d->rot_dim / 2 % vec || (D - d->rot_dim) % (2 * vec))) vec /= 2;

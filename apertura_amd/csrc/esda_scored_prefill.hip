@@ -7,6 +7,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -14,6 +15,7 @@
 #include "esda_internal.h"
 #include "esda_prefill_kernel.h"
 #include "esda_scored.h"
+#include "esda_views.h"
 
 namespace {
 
@@ -57,14 +59,25 @@ int esda_scored_prefill(const esda_prefill_desc *desc, const esda_score *score, 
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: null pointer");
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: tensors must be 16-byte aligned");
-    if (a->out == a->q || a->out == a->k || a->out == a->v)
-        return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: out must not be an input");
+    const int D = desc->head_dim;
+    // (a row of q is read again after rows of out are written, where a value is not finite)
+    auto view = [](const void *ptr, long long rows, long long rs, long long heads, long long hs, long long width) {
+        return esda_views::View{reinterpret_cast<uintptr_t>(ptr), {rows, heads}, {rs, hs}, width};
+    };
+    const long long keys = (long long) p.Sk * D;
+    const esda_views::View out = view(a->out, p.Sq, p.o_rs, p.Hq, p.o_hs, D);
+    for (const auto &in : {view(a->q, p.Sq, p.q_rs, p.Hq, p.q_hs, D), view(a->k, 1, 0, p.Hkv, p.kv_hs, keys),
+                           view(a->v, 1, 0, p.Hkv, p.kv_hs, keys)}) {
+        if (in.extent() > (__int128) 1 << 60 || out.extent() > (__int128) 1 << 60)
+            return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: strides are too large");
+        if (!esda_views::disjoint(in, out))
+            return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: out must not overlap q, k or v");
+    }
     if (!a->q_doc != !a->k_doc)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: q_doc and k_doc go together");
     if ((reinterpret_cast<uintptr_t>(a->k_doc) | reinterpret_cast<uintptr_t>(a->q_doc) |
          reinterpret_cast<uintptr_t>(score->slopes)) & 3u)
         return fail(ESDA_ERR_INVALID_ARGUMENT, "esda_scored_prefill: document ids and slopes must be 4-byte aligned");
-    const int D = desc->head_dim;
     const size_t need = workspace_of(p, D);
     if (need) {
         if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))

@@ -238,3 +238,10 @@ def test_forced_splits_longer_than_a_tile_s_keys(tmp_path):
         for c, line in zip(chunks, r.stdout.splitlines(), strict=True):
             _, _, _, splits, kps, _, nbytes = map(int, line.split())
             assert (splits, nbytes) == (1, 0) and 0 < kps <= c[4] + 32 and kps % 32 == 0
+
+
+def test_views_that_share_memory_are_told_from_those_that_do_not(tmp_path):
+    """esda_views.h beside the views' elements."""
+    exe = _build(tmp_path, src=os.path.join(ROOT, "tests", "views_check.cpp"))
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout

@@ -134,3 +134,17 @@ def test_front_end_refuses_wrong_tensors():
         ScoredDecodeCall(step, Score(), torch.zeros(2, 8, 128, dtype=bf), torch.zeros(2, 2, 128, dtype=bf), None,
                          torch.zeros(2, 2, 64, 128, dtype=bf), torch.zeros(2, 2, 64, 128, dtype=bf),
                          torch.zeros(2, dtype=torch.int32))
+
+
+def test_an_output_that_overlaps_an_input_is_refused():
+    """By any element: a view further into q, k or v, one that ends inside them, heads or rows between
+    theirs.  (Calls that pass would be launched: those have real memory, in the GPU tests.)"""
+    q_bytes, kv_bytes = 8 * 64 * 128 * 2, 2 * 64 * 128 * 2
+    k, v = FAKE + (1 << 20), FAKE + (2 << 20)
+    for out in (FAKE, FAKE + 16, FAKE + q_bytes - 16, FAKE - q_bytes + 16, k + 256, k + kv_bytes - 16, v - 16, v + kv_bytes - 16):
+        assert _prefill(k=k, v=v, out=out) == 1, hex(out - FAKE)
+    assert "overlap" in _lib.lib().esda_last_error().decode()
+    # rows of one buffer whose out columns reach into k's, and heads that reach into the next
+    rows = _step(q_row_stride=12 * 128, q_head_stride=128, out_row_stride=12 * 128, out_head_stride=128)
+    assert _prefill(step=rows, k=k, v=v, out=FAKE + 2 * 128 * 7) == 1
+    assert _prefill(step=_step(out_row_stride=2 ** 60, out_head_stride=128), k=k, v=v) == 1

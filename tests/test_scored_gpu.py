@@ -674,3 +674,25 @@ def test_decode_keys_of_minus_infinity(D, heads, rows, split, scored):
             for h in range(hq):
                 o, bound = attend64(q[b, h][None], kc[b, h // (hq // hkv)], vc[b, h // (hq // hkv)], seen, step.scale)
                 check(out[b, h][None][:, dims], o[:, dims], bound[:, dims], f"n {n} sequence {b} head {h}")
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_out_beside_its_inputs_in_one_buffer(D):
+    """Packed rows that hold q and out side by side, and an out between the kv heads of one arena: memory
+    shared, elements not."""
+    hq, hkv, n, g = 4, 2, 50, _gen(70)
+    rows = torch.zeros((n, 2 * hq, D), dtype=BF, device=DEV)
+    rows[:, :hq] = _rows((n, hq, D), g, 2.5)
+    k, v = _rows((hkv, n, D), g), _rows((hkv, n, D), g)
+    q, out, score = rows[:, :hq].transpose(0, 1), rows[:, hq:], Score(20.0, _slopes(hq))
+    step = PrefillStep.for_tensors(q, k, out, scale=D ** -0.5)
+    scored_prefill(step, score, q, k, v, out=out)
+    _check_prefill(step, score, q, k, v, out)
+    arena = torch.zeros(3 * n * D + n * hq * D, dtype=BF, device=DEV)
+    ka = torch.as_strided(arena, (hkv, n, D), ((1 + hq) * n * D, D, 1))
+    ka.copy_(k)
+    out = arena[n * D:n * D + n * hq * D].view(n, hq, D)
+    step = PrefillStep.for_tensors(q, ka, out, scale=D ** -0.5)
+    scored_prefill(step, score, q, ka, ka, out=out)
+    _check_prefill(step, score, q, ka, ka, out)
+    assert torch.equal(ka, k)
