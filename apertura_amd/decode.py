@@ -6,6 +6,7 @@ CUDA (HIP) tensors; torch is only the allocator and stream provider here.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -125,6 +126,12 @@ def _same_device(tensors: dict) -> None:
             raise ValueError(f"{name} is on {t.device}; the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _on(stream):
+    """Work of this block on the launch's stream: a workspace that is cleared on another one could be
+    cleared after the launch has written to it."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
 def _used_on(stream, *tensors) -> None:
     """Tensors of the current stream that a launch on `stream` uses: their memory is not handed out
     again before that launch is through."""
@@ -156,7 +163,8 @@ def decode_step(step: DecodeStep, q: torch.Tensor, k_new: torch.Tensor, v_new: t
     if out is None:
         out = torch.empty_like(q)
     if workspace is None:
-        workspace = new_workspace(step, q.device)
+        with _on(stream):
+            workspace = new_workspace(step, q.device)
     args = DecodeArgs(_dev_ptr(q, bf), _dev_ptr(k_new, bf),
                       _dev_ptr(v_new, bf) if (v_new is not None and not step.kv_shared) else None,
                       _dev_ptr(k_cache, bf), _dev_ptr(vc, bf), _dev_ptr(pos),
@@ -164,6 +172,7 @@ def decode_step(step: DecodeStep, q: torch.Tensor, k_new: torch.Tensor, v_new: t
                       workspace.numel() * workspace.element_size())
     d = step.desc()
     check(lib().esda_decode_stages(ctypes.byref(d), ctypes.byref(args), stages, _stream_ptr(stream)))
+    _used_on(stream, out, workspace)
     return out
 
 
@@ -225,7 +234,8 @@ class DecodeCall:
     """A decode step with its C-ABI arguments marshalled once (the host-side cost of a
     launch is then one ctypes call).  Tensors are referenced, not copied: refill q,
     k_new, v_new and pos in place between calls.  Also usable under HIP graph capture
-    (the library issues only kernel launches on the given stream)."""
+    (the library issues only kernel launches on the given stream).  A workspace that is not
+    given is cleared here, on the current stream: calls on another one go behind that."""
 
     def __init__(self, step: DecodeStep, q, k_new, v_new, k_cache, v_cache, pos, row_base=None,
                  out=None, workspace=None, stages: int = STAGE_ATTEND | STAGE_MERGE):
@@ -343,12 +353,14 @@ def decode_raw(step: RawStep, q: torch.Tensor, k_new: torch.Tensor | None, raw_c
     if out is None:
         out = torch.empty_like(q)
     if workspace is None:
-        workspace = new_raw_workspace(step, q.device)
+        with _on(stream):
+            workspace = new_raw_workspace(step, q.device)
     args = RawArgs(_dev_ptr(q, bf), _dev_ptr(k_new, bf), _dev_ptr(raw_cache, bf), _dev_ptr(pos),
                    _dev_ptr(kw, bf), _dev_ptr(inv_freq), _dev_ptr(out, bf), _dev_ptr(workspace),
                    workspace.numel() * workspace.element_size(), *_table(rope_table))
     d = step.desc()
     check(lib().esda_decode_raw_stages(ctypes.byref(d), ctypes.byref(args), stages, _stream_ptr(stream)))
+    _used_on(stream, out, workspace)
     return out
 
 
@@ -437,10 +449,12 @@ def decode_raw_q8(step: RawStep, q: torch.Tensor, k_new: torch.Tensor | None, q8
     if out is None:
         out = torch.empty_like(q)
     if workspace is None:
-        workspace = new_raw_workspace(step, q.device)
+        with _on(stream):
+            workspace = new_raw_workspace(step, q.device)
     args = _q8_args(step, q, k_new, q8, scale, bias, pos, kw, inv_freq, out, workspace, rope_table)
     d = step.desc()
     check(lib().esda_decode_raw_q8_stages(ctypes.byref(d), ctypes.byref(args), stages, _stream_ptr(stream)))
+    _used_on(stream, out, workspace)
     return out
 
 

@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import PrefillArgs, PrefillDesc, check, lib
-from .decode import _dev_ptr, _stream_ptr
+from .decode import _dev_ptr, _stream_ptr, _used_on
 
 
 @dataclass
@@ -108,6 +108,7 @@ def prefill(step: PrefillStep, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     a = PrefillArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                     _dev_ptr(workspace) if nbytes else None, nbytes)
     check(lib().esda_prefill_stages(ctypes.byref(d), ctypes.byref(a), int(stages), _stream_ptr(stream)))
+    _used_on(stream, out, workspace)
     return out
 
 

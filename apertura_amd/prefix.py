@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import DecodeArgs, PrefixArgs, PrefixDesc, check, lib
-from .decode import DecodeStep, _check_cache, _dev_ptr, _same_device, _stream_ptr, _used_on
+from .decode import DecodeStep, _check_cache, _dev_ptr, _on, _same_device, _stream_ptr, _used_on
 
 
 @dataclass
@@ -55,7 +55,8 @@ def new_prefix_workspace(step: PrefixStep, device) -> torch.Tensor:
 class PrefixCall:
     """A decode step over a shared prefix with its C-ABI arguments marshalled once (as
     DecodeCall): refill q, k_new, v_new and pos in place between calls.  Usable under HIP graph
-    capture.  pos [B] int32: absolute positions, prefix_len or more."""
+    capture.  pos [B] int32: absolute positions, prefix_len or more.  A workspace that is not given is
+    cleared here, on the current stream."""
 
     def __init__(self, step: PrefixStep, q, k_new, v_new, prefix_k, prefix_v, k_cache, v_cache, pos, out=None,
                  workspace=None):
@@ -118,6 +119,9 @@ def prefix_decode(step: PrefixStep, q: torch.Tensor, k_new: torch.Tensor, v_new:
                   workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Append the new rows to the sequences' own caches and attend the shared prefix and them; out
     [B, Hq, D] bf16."""
+    if workspace is None:
+        with _on(stream):
+            workspace = new_prefix_workspace(step, q.device)
     call = PrefixCall(step, q, k_new, v_new, prefix_k, prefix_v, k_cache, v_cache, pos, out, workspace)
     out = call(stream)
     _used_on(stream, out, call.workspace)

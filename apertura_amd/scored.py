@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import DecodeArgs, ScoreDesc, ScoredPrefillArgs, check, lib
-from .decode import (DecodeStep, _check_cache, _check_row_base, _dev_ptr, _same_device, _stream_ptr,
+from .decode import (DecodeStep, _check_cache, _check_row_base, _dev_ptr, _on, _same_device, _stream_ptr,
                      _used_on, new_workspace)
 from .prefill import PrefillStep
 
@@ -82,7 +82,8 @@ def scored_prefill(step: PrefillStep, score: Score, q: torch.Tensor, k: torch.Te
 
 class ScoredDecodeCall:
     """A decode step with modified scores, its C-ABI arguments marshalled once (as DecodeCall):
-    refill q, k_new, v_new and pos in place between calls.  Usable under HIP graph capture."""
+    refill q, k_new, v_new and pos in place between calls.  Usable under HIP graph capture.  A
+    workspace that is not given is cleared here, on the current stream."""
 
     def __init__(self, step: DecodeStep, score: Score, q, k_new, v_new, k_cache, v_cache, pos, row_base=None, out=None,
                  workspace=None):
@@ -130,6 +131,9 @@ def scored_decode(step: DecodeStep, score: Score, q: torch.Tensor, k_new: torch.
                   row_base: torch.Tensor | None = None, out: torch.Tensor | None = None,
                   workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """decode_step with ``score``'s scores: append the new rows and attend; out [B, Hq, D] bf16."""
+    if workspace is None:
+        with _on(stream):
+            workspace = new_workspace(step, q.device)
     call = ScoredDecodeCall(step, score, q, k_new, v_new, k_cache, v_cache, pos, row_base, out, workspace)
     out = call(stream)
     _used_on(stream, out, call.workspace)
