@@ -334,8 +334,8 @@ void attend_kernel(P p) {
 
     // Packed kv heads: a stage holds RPP = 16 / pk rows of each of the pk kv heads (stage
     // row r belongs to kv head r / RPP, row r % RPP of the stage's row range).  pk is 1, 2
-    // or 4 and the same in every lane.
-    const int pk = uniform(p.pk);
+    // or 4 and the same in every lane (scored steps: 1).
+    const int pk = SCORED ? 1 : uniform(p.pk);
     const int lrpp = 4 - __builtin_ctz(pk), RPP = 1 << lrpp;
     // Query head li belongs to kv head li / gk of the group (padding heads li >= G take
     // the last); the C rows 4lg .. 4lg+3 of this lane come from one kv head (RPP >= 4).
@@ -944,7 +944,10 @@ template <class P>
 hipError_t dispatch_attend(int D, bool shared, const P &ap, dim3 grid, hipStream_t st) {
     constexpr int O256 = kOcc256, O512 = kOcc512Shared;
     switch (D) {
-        case 128: return shared ? launch_attend<128, true, 1>(ap, grid, st) : launch_attend<128, false, 1>(ap, grid, st);
+        case 128:
+            // (scored steps of 128 dims run stream_kernel)
+            if constexpr (std::is_base_of<ScoredAttendParams, P>::value) return hipErrorInvalidValue;
+            else return shared ? launch_attend<128, true, 1>(ap, grid, st) : launch_attend<128, false, 1>(ap, grid, st);
         case 256:
             return shared ? launch_attend<256, true, O256>(ap, grid, st)
                           : launch_attend<256, false, O256>(ap, grid, st);

@@ -198,3 +198,14 @@ def test_prefill_descriptions_are_validated_without_device():
         with pytest.raises(EsdaError) as ei:
             prefill_workspace_bytes(PrefillStep(**{**good, **bad}))
         assert ei.value.code == 1, bad
+
+
+def test_no_scored_kernel_is_built_that_nothing_launches():
+    """Scored decode steps of 128 dims run stream_kernel: attend_kernel's forms of them stay unbuilt."""
+    import shutil
+    import subprocess
+    if not shutil.which("nm"):
+        pytest.skip("nm not found")
+    names = subprocess.run(["nm", "-C", os.path.join(ROOT, "apertura_amd", "libesda.so")], capture_output=True, text=True, check=True).stdout
+    assert "stream_kernel<" in names and "attend_kernel<256, false" in names
+    assert not [n for n in names.splitlines() if "attend_kernel<128" in n and "Scored" in n]
