@@ -58,6 +58,13 @@ class EsdaError(RuntimeError):
         self.code = code
 
 
+def check_int32(**values: int) -> None:
+    """ctypes wraps what a 32-bit field cannot hold; such values are refused."""
+    for name, x in values.items():
+        if not -2 ** 31 <= x < 2 ** 31:
+            raise ValueError(f"{name} = {x} does not fit in 32 bits")
+
+
 class DecodeDesc(ctypes.Structure):
     _fields_ = [
         ("batch", ctypes.c_int32), ("num_q_heads", ctypes.c_int32),

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import DecodeArgs, DecodeDesc, RawArgs, RawDesc, RawQ8Args, check, lib
+from ._lib import DecodeArgs, DecodeDesc, RawArgs, RawDesc, RawQ8Args, check, check_int32, lib
 
 STAGE_ATTEND = 1
 STAGE_MERGE = 2
@@ -43,6 +43,7 @@ class DecodeStep:
     def desc(self) -> DecodeDesc:
         hs = self.head_stride if self.head_stride is not None else self.cap * self.head_dim
         ss = self.seq_stride if self.seq_stride is not None else self.num_kv_heads * hs
+        check_int32(window=self.window, max_visible=self.max_visible, split_rows=self.split_rows)
         return DecodeDesc(self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim,
                           self.cap, self.window, 1 if self.ring else 0, 1 if self.kv_shared else 0,
                           ss, hs, self.max_visible, self.split_rows, self.scale)

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import PrefillArgs, PrefillDesc, check, lib
+from ._lib import PrefillArgs, PrefillDesc, check, check_int32, lib
 from .decode import _dev_ptr, _stream_ptr, _used_on
 
 
@@ -47,6 +47,7 @@ class PrefillStep:
         kvhs = self.kv_head_stride if self.kv_head_stride is not None else self.seq_k * D
         ors = self.out_row_stride if self.out_row_stride is not None else self.num_q_heads * D
         ohs = self.out_head_stride if self.out_head_stride is not None else D
+        check_int32(q_pos0=self.q_pos0, k_pos0=self.k_pos0, window=self.window, split_keys=self.split_keys)
         return PrefillDesc(self.num_q_heads, self.num_kv_heads, D, self.seq_q, self.seq_k, self.q_pos0,
                            self.k_pos0, self.window, qhs, qrs, kvhs, ors, ohs, self.split_keys, self.scale)
 

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import DecodeArgs, PrefixArgs, PrefixDesc, check, lib
+from ._lib import DecodeArgs, PrefixArgs, PrefixDesc, check, check_int32, lib
 from .decode import DecodeStep, _check_cache, _dev_ptr, _on, _same_device, _stream_ptr, _used_on
 
 
@@ -28,6 +28,7 @@ class PrefixStep:
 
     def desc(self) -> PrefixDesc:
         hs = self.prefix_head_stride if self.prefix_head_stride is not None else self.prefix_len * self.own.head_dim
+        check_int32(prefix_len=self.prefix_len, split_keys=self.split_keys)
         return PrefixDesc(self.own.desc(), self.prefix_len, self.split_keys, hs)
 
     @classmethod

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import RopeArgs, RopeDesc, RopeScalingDesc, check, lib
+from ._lib import RopeArgs, RopeDesc, RopeScalingDesc, check, check_int32, lib
 from .decode import _same_device, _stream_ptr, _used_on
 
 _KINDS = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
@@ -36,6 +36,7 @@ def rope_frequencies(rot_dim: int, base: float, scaling: RopeScaling | None = No
     s = scaling or RopeScaling()
     if s.kind not in _KINDS:
         raise ValueError(f"unknown rotary scaling {s.kind!r}")
+    check_int32(rot_dim=rot_dim, trained_len=s.trained_len)
     d = RopeScalingDesc(_KINDS[s.kind], s.trained_len, base, s.factor, s.low, s.high)
     inv, factor = (ctypes.c_float * max(1, rot_dim // 2))(), ctypes.c_float(0.0)
     check(lib().esda_rope_frequencies(ctypes.byref(d), rot_dim, inv, ctypes.byref(factor)))
@@ -85,6 +86,7 @@ class RopeCall:
         def ptr(t):
             return t.data_ptr() if t is not None else None
 
+        check_int32(tokens=T, rot_dim=2 * inv_freq.numel())
         self._keep = (q, k, pos, inv_freq)
         self.q_out, self.k_out = q_out, k_out
         self._desc = RopeDesc(T, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0, D,

@@ -11,7 +11,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import DecodeArgs, ScoreDesc, ScoredPrefillArgs, check, lib
+from ._lib import DecodeArgs, ScoreDesc, ScoredPrefillArgs, check, check_int32, lib
 from .decode import (DecodeStep, _check_cache, _check_row_base, _dev_ptr, _on, _same_device, _stream_ptr,
                      _used_on, new_workspace)
 from .prefill import PrefillStep
@@ -33,6 +33,9 @@ class Score:
         s = self.slopes
         if s is not None and (s.dtype != torch.float32 or s.shape != (num_q_heads,) or not s.is_contiguous()):
             raise ValueError("slopes must be contiguous float32 [Hq]")
+        check_int32(prefix=self.prefix)
+        if self.softcap > 0 and ctypes.c_float(self.softcap).value == 0:
+            raise ValueError(f"softcap = {self.softcap} is 0 in float32, which is no cap")
         return ScoreDesc(self.softcap, self.prefix, None if s is None else s.data_ptr())
 
 

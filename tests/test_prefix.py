@@ -123,3 +123,9 @@ def test_splits_longer_than_the_rows_are_one_split():
     # own rows take at most 64 splits, 100 keys of a prefix at most four
     assert prefix_workspace_bytes(_step(cap=2 ** 31 - 102, split_rows=16)) <= 68 * 32 * (4 * 128 + 8) + 4096
     assert prefix_workspace_bytes(_step(cap=2 ** 31 - 102)) <= 68 * 32 * (4 * 128 + 8) + 4096
+
+
+@pytest.mark.parametrize("kw", [dict(prefix_len=2 ** 32 + 100), dict(split_keys=2 ** 32 + 32), dict(split_rows=2 ** 32 + 16)])
+def test_values_that_a_description_would_wrap_are_refused(kw):
+    with pytest.raises(ValueError):
+        _step(**kw).desc()

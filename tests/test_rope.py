@@ -142,3 +142,10 @@ def test_front_end_refuses_wrong_tensors():
                  (q[0], None, pos, inv)):
         with pytest.raises(ValueError):
             RopeCall(*args)
+
+
+def test_values_that_a_description_would_wrap_are_refused():
+    with pytest.raises(ValueError):
+        rope_frequencies(2 ** 32 + 64, 10000.0)
+    with pytest.raises(ValueError):
+        rope_frequencies(64, 10000.0, RopeScaling("yarn", 8.0, 2 ** 32 + 8192, 1.0, 32.0))

@@ -148,3 +148,17 @@ def test_an_output_that_overlaps_an_input_is_refused():
     rows = _step(q_row_stride=12 * 128, q_head_stride=128, out_row_stride=12 * 128, out_head_stride=128)
     assert _prefill(step=rows, k=k, v=v, out=FAKE + 2 * 128 * 7) == 1
     assert _prefill(step=_step(out_row_stride=2 ** 60, out_head_stride=128), k=k, v=v) == 1
+
+
+@pytest.mark.parametrize("make", [
+    lambda: Score(prefix=2 ** 32).desc(8), lambda: Score(prefix=2 ** 31).desc(8), lambda: Score(softcap=1e-46).desc(8),
+    lambda: _step(q_pos0=2 ** 32 + 5).desc(), lambda: _step(k_pos0=-2 ** 32).desc(), lambda: _step(window=2 ** 32 + 8).desc(),
+    lambda: _step(split_keys=2 ** 32 + 32).desc(),
+    lambda: DecodeStep(batch=2, num_q_heads=8, num_kv_heads=2, head_dim=128, cap=64, window=2 ** 32 + 8).desc(),
+    lambda: DecodeStep(batch=2, num_q_heads=8, num_kv_heads=2, head_dim=128, cap=64, max_visible=2 ** 32 + 8).desc(),
+])
+def test_values_that_a_description_would_change_are_refused(make):
+    """A 32-bit field wraps what it cannot hold (a prefix of 2^32 would be none), and a cap below
+    float32's smallest number is 0, which is no cap."""
+    with pytest.raises(ValueError):
+        make()
