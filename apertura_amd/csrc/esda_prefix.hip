@@ -5,9 +5,12 @@
 // for the B * G query rows of its kv head (prefill_kernel with PrefixParams), or, for few of them,
 // in runs (prefix_run_kernel); the own rows in runs, with the fused append.  The second merges them.
 // A step of few rows is bound by the latency of the two (2 sequences behind 2049 tokens: 13.5 us), a
-// long one by reading prefix and own rows once (4 behind 32,768, 138 MB: 40 us), one of many sequences
-// by both kinds of workgroups sharing the CUs (64 behind 16,384, 200 MB and 18 GFLOP: 61 us).  With
-// prefix, own rows and their merges in launches one after the other these took 48, 99 and 123 us.
+// long one by the runs' starts and the reads that a key's two row groups do not share (4 behind 32,768:
+// 169 MB read for 140, the first launch 34.7 us, 4.9 TB/s, where a step of plain decode reads such rows at
+// 7; 40 us in all), one of many sequences by both kinds of workgroups sharing the CUs (64 behind 16,384,
+// 200 MB and 18 GFLOP: 61 us).  At 512 dims a batch is bound by its tiles' starts and partials: 32 behind
+// 8191 write 46 MB of them and read them back for 70 MB of keys, 50 us.  With prefix, own rows and their
+// merges in launches one after the other the first three took 48, 99 and 123 us.
 // The C ABI is include/esda_prefix.h.
 
 #include <hip/hip_runtime.h>

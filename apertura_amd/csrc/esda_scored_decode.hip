@@ -18,8 +18,10 @@ namespace {
 
 // head_dim 128: a 16-row stage is 4 or 8 KB, too little for a barrier and a score exchange between
 // the waves.  Here each of eight waves streams stages of its own: a step of 16 sequences of 2K .. 16K
-// rows, 8 kv heads, 599 MB 101 us (5.9 TB/s; attend_kernel 144), one of 131,072 rows 82 us (6.5 TB/s;
-// 115), of 16,384 16.3 (22.3), of 300 8.1 (9.0); K = V, 16 of 512 .. 4096 23.4 (39.4).
+// rows, 8 kv heads, 599 MB 101 us (5.9 TB/s; attend_kernel 144), one of 131,072 rows 83 us (6.5 TB/s;
+// 115), of 16,384 16.1 (22.3), of 300 8.2 (9.0); K = V, 16 of 512 .. 4096 24.2 (40).  At 256 and 512 dims
+// attend_kernel: 16 of 1024 .. 8192 rows of 512 dims, K = V, 318 MB 74 us from HBM (4.2 TB/s), one of
+// 131,072 90 (6.0).
 constexpr int kStreamWaves = 8;
 
 template <bool SH, class P>

@@ -166,7 +166,8 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
                 m[g] = mn;
             }
         }
-        short4v pb[NG];  // the weights as they enter both sums: bf16
+        // The weights as they enter both sums: bf16, the product's operands (see prefill_kernel).
+        short4v pb[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -361,7 +362,7 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, 
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= corr;
             m = mn;
         }
-        bf16x8 pb[SUB / 2];  // the weights as they enter both sums: bf16
+        bf16x8 pb[SUB / 2];  // the weights as they enter both sums: bf16, the product's operands
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll

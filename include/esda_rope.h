@@ -25,8 +25,8 @@ extern "C" {
  * likewise (bf16).  Pair i < rot_dim / 2 of a row is (x0, x1) = dims (i, i + rot_dim/2), or
  * (2i, 2i + 1) when interleaved; with a = pos[t] * inv_freq[i]:
  *   y0 = f (x0 cos a - x1 sin a),  y1 = f (x1 cos a + x0 sin a),  f = attn_factor
- * and with -a for a when inverse (the rotation's gradient; un-rotating cached rows).  Dims
- * rot_dim .. head_dim - 1 are copied.  An inverse frequency of 0 leaves its pair unturned, so a
+ * and with -a for a when inverse (the rotation's gradient; un-rotating cached rows, with 1 / f where they
+ * were turned with f).  Dims rot_dim .. head_dim - 1 are copied.  An inverse frequency of 0 leaves its pair unturned, so a
  * rotation of pairs (d, d + head_dim/2), d < n, alone is rot_dim = head_dim with zeros behind
  * the first n frequencies (the reference's global layers).
  * An output may be its input with the same strides; otherwise they must not overlap. */
