@@ -322,7 +322,9 @@ def _plain_fork(st: dict):
     fresh = _free_pages(refs)[(part.long().cumsum(0) - 1).clamp(min=0)]
     last = table[src].gather(1, full.clamp(max=table.shape[1] - 1).unsqueeze(1)).squeeze(1).long()
     last = torch.where(part, last, table[0, 0].long())
-    pool[:, torch.where(part, fresh, last)] = pool[:, last]
+    fresh = torch.where(part, fresh, last)
+    used = (torch.arange(R, device=DEV) < (rows % R).unsqueeze(1)).view(-1, 1, R, 1)  # the rest of a page stays
+    pool[:, fresh] = torch.where(used, pool[:, last], pool[:, fresh])
     _hold(refs, fresh, part, 1)
     new = torch.where((k == full.unsqueeze(1)) & part.unsqueeze(1), fresh.int().unsqueeze(1), new)
     table[dst] = new
@@ -512,7 +514,7 @@ def _exact_fork(s: dict, case: dict) -> list:
             refs[table[src][k]] += 1
         if rows % R:
             page = next(lowest)
-            pool[:, page] = s["pool"][:, table[src][rows // R]]
+            pool[:, page, :, :rows % R] = s["pool"][:, table[src][rows // R], :, :rows % R]
             table[dst][rows // R], refs[page] = page, 1
         length[dst] = rows
     for _, dst, rows, then in jobs:
