@@ -1,6 +1,6 @@
 """ctypes binding of libesda.so (the C ABI declared in include/esda.h,
-include/esda_cache.h, include/esda_prefill.h, include/esda_rope.h, include/esda_scored.h and
-include/esda_prefix.h).
+include/esda_cache.h, include/esda_prefill.h, include/esda_rope.h, include/esda_scored.h,
+include/esda_prefix.h, include/esda_pages.h and include/esda_tree.h).
 
 The library is loaded from the package directory only (built in-tree by
 ``apertura_amd/build.py``); a missing library raises instead of falling back.
@@ -44,7 +44,13 @@ EXPORTS = (
     "esda_scored_prefill_workspace_size", "esda_scored_prefill", "esda_scored_decode",
     # include/esda_prefix.h
     "esda_prefix_decode_workspace_size", "esda_prefix_decode",
+    # include/esda_pages.h
+    "esda_pages_workspace_size", "esda_pages_reserve", "esda_pages_free", "esda_pages_fork", "esda_pages_compact",
+    "esda_pages_status", "esda_pages_write", "esda_pages_read",
+    # include/esda_tree.h
+    "esda_tree_workspace_size", "esda_tree_decode", "esda_tree_commit",
 )
+MAX_POOLS, MAX_ENTRIES = 8, 1024  # ESDA_MAX_POOLS, ESDA_MAX_ENTRIES
 _VOID = ("esda_cache_destroy", "esda_cache_mark_step", "esda_cache_reset", "esda_cache_clear_rewind_mark")
 
 # const char *(*)(int32_t pos, void *user): the caller's prefix fingerprint at a marker
@@ -193,6 +199,57 @@ class PrefixArgs(ctypes.Structure):
     _fields_ = [("own", DecodeArgs), ("prefix_k", ctypes.c_void_p), ("prefix_v", ctypes.c_void_p)]
 
 
+class Pool(ctypes.Structure):
+    """esda_pool"""
+    _fields_ = [
+        ("data", ctypes.c_void_p), ("planes", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("pad", ctypes.c_int32),
+        ("plane_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+    ]
+
+
+class Pages(ctypes.Structure):
+    """esda_pages"""
+    _fields_ = [
+        ("num_pages", ctypes.c_int32), ("page_rows", ctypes.c_int32), ("slots", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p), ("refs", ctypes.c_void_p), ("length", ctypes.c_void_p),
+        ("num_pools", ctypes.c_int32), ("pad", ctypes.c_int32), ("pools", Pool * MAX_POOLS),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PageRowsDesc(ctypes.Structure):
+    """esda_page_rows_desc"""
+    _fields_ = [
+        ("pool", Pool), ("num_pages", ctypes.c_int32), ("page_rows", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("rows", ctypes.c_int32), ("pad", ctypes.c_int32),
+        ("linear_plane_stride", ctypes.c_int64), ("linear_seq_stride", ctypes.c_int64),
+        ("linear_head_stride", ctypes.c_int64),
+    ]
+
+
+class TreeDesc(ctypes.Structure):
+    """esda_tree_desc"""
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("nodes", ctypes.c_int32), ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("kv_shared", ctypes.c_int32),
+        ("window", ctypes.c_int32), ("num_pages", ctypes.c_int32), ("page_rows", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64), ("max_visible", ctypes.c_int32), ("split_rows", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("pad", ctypes.c_int32),
+    ]
+
+
+class TreeArgs(ctypes.Structure):
+    """esda_tree_args"""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p), ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("length", ctypes.c_void_p), ("parent", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class Q8View(ctypes.Structure):
     """esda_q8_view: u8 rows q [kv_heads, pitch, 512], f32 scale / bias [kv_heads, pitch]."""
     _fields_ = [
@@ -286,6 +343,20 @@ def lib() -> ctypes.CDLL:
         L.esda_scored_prefill_workspace_size.argtypes = [PD, SP, ctypes.POINTER(sz)]
         L.esda_scored_prefill.argtypes = [PD, SP, ctypes.POINTER(ScoredPrefillArgs), P]
         L.esda_scored_decode.argtypes = [ctypes.POINTER(DecodeDesc), SP, ctypes.POINTER(DecodeArgs), P]
+        CP = ctypes.POINTER(Pages)
+        L.esda_pages_workspace_size.argtypes = [CP, ctypes.POINTER(sz)]
+        L.esda_pages_reserve.argtypes = [CP, P, P, i32, P]
+        L.esda_pages_free.argtypes = [CP, P, i32, P]
+        L.esda_pages_fork.argtypes = [CP, P, P, P, i32, P]
+        L.esda_pages_compact.argtypes = [CP, P]
+        L.esda_pages_status.argtypes = [P, pi32, P]
+        RD = ctypes.POINTER(PageRowsDesc)
+        L.esda_pages_write.argtypes = [RD, P, P, P, P]
+        L.esda_pages_read.argtypes = [RD, P, P, P, P]
+        TD = ctypes.POINTER(TreeDesc)
+        L.esda_tree_workspace_size.argtypes = [TD, ctypes.POINTER(sz)]
+        L.esda_tree_decode.argtypes = [TD, ctypes.POINTER(TreeArgs), P]
+        L.esda_tree_commit.argtypes = [CP, P, i64, i32, P, P]
         for name in EXPORTS:
             if name in _VOID:
                 getattr(L, name).restype = None

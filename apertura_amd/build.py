@@ -28,6 +28,8 @@ SOURCES = [
     "esda_scored_prefill.hip",
     "esda_prefix.hip",
     "esda_prefix_tiles.hip",
+    "esda_pages.hip",
+    "esda_tree.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",

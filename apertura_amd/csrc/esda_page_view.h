@@ -1,0 +1,58 @@
+// esda_page_view.h -- where the rows of a cache in pages lie, and what a description of one must
+// satisfy: for esda_pages.hip, esda_tree.hip and their kernels.  The checks are host code.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+#include "esda_pages.h"
+
+namespace esda_page_view {
+
+constexpr int kMaxPages = 1 << 22, kMaxPageRows = 4096, kMaxSlots = 1 << 20, kMaxTable = 1 << 20;
+constexpr int kMaxPlanes = 4096;
+
+// Blocks of `block` elements at i st[0] + j st[1] + k st[2], i < n[0] .., that do not overlap, and end
+// below 2^60.  (Ordered by stride, each step is at least as wide as what lies within it.)
+inline bool blocks_apart(const long long (&count)[3], const long long (&stride)[3], long long block) {
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return stride[a] < stride[b]; });
+    __int128 width = block;
+    for (int i : order) {
+        if (count[i] <= 1) continue;
+        if (stride[i] < width) return false;
+        width += (__int128) (count[i] - 1) * stride[i];
+    }
+    return width < (__int128) 1 << 60;
+}
+
+inline bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
+inline bool whole16(long long a) { return a >= 0 && a % 8 == 0; }
+
+// What is wrong with a pool of pages of page_rows rows, or null.
+inline const char *check_pool(const esda_pool &p, int num_pages, int page_rows) {
+    if (!p.data || (reinterpret_cast<uintptr_t>(p.data) & 15u)) return "a pool must be 16-byte aligned device memory";
+    if (p.planes <= 0 || p.planes > kMaxPlanes || p.num_kv_heads <= 0 || p.num_kv_heads > kMaxPlanes)
+        return "a pool has 1 .. 4096 planes and kv heads";
+    if (p.head_dim != 128 && p.head_dim != 256 && p.head_dim != 512) return "head_dim must be 128, 256 or 512";
+    if (!whole16(p.plane_stride) || !whole16(p.page_stride) || !whole16(p.head_stride))
+        return "strides must be non-negative multiples of 8";
+    if (!blocks_apart({p.planes, num_pages, p.num_kv_heads}, {p.plane_stride, p.page_stride, p.head_stride},
+                      (long long) page_rows * p.head_dim))
+        return "the pages of a pool overlap";
+    return nullptr;
+}
+
+// What is wrong with the pages of a table, or null.
+inline const char *check_table(int num_pages, int page_rows, int slots, int max_pages, long long table_stride) {
+    if (num_pages <= 0 || num_pages > kMaxPages) return "num_pages must be 1 .. 2^22";
+    if (!power_of_two(page_rows) || page_rows < 16 || page_rows > kMaxPageRows)
+        return "page_rows must be a power of two, 16 .. 4096";
+    if (slots <= 0 || slots > kMaxSlots) return "slots must be 1 .. 2^20";
+    if (max_pages <= 0 || max_pages > kMaxTable || (long long) max_pages * page_rows >= 1LL << 31)
+        return "max_pages must be 1 .. 2^20 and hold fewer than 2^31 rows";
+    if (table_stride < max_pages || table_stride > 1LL << 40) return "table_stride must be at least max_pages";
+    return nullptr;
+}
+
+}  // namespace esda_page_view

@@ -1,0 +1,816 @@
+// esda_pages.hip -- the upkeep of caches in pages for MI355X (gfx950): pages taken and given up,
+// sequences forked and cut, the pages in use moved together, rows copied in and out, and the accepted
+// rows of a step of drafted tokens moved behind the committed ones.  The C ABI is include/esda_pages.h
+// and, for the last, include/esda_tree.h.
+//
+// What to do is decided on the device, from the table and the references, so that a serving loop never
+// waits for it on the host: small kernels of a workgroup per list entry, or of one workgroup where
+// entries compete for free pages, write a list of moves, and a grid of waves carries it out.  The copies
+// are bound by memory; calls of few bytes by their launches.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "esda.h"
+#include "esda_device.h"
+#include "esda_internal.h"
+#include "esda_page_view.h"
+#include "esda_pages.h"
+#include "esda_tree.h"
+
+namespace {
+
+using namespace esda_page_view;
+
+constexpr int kPieceBytes = 16384;  // what a wave copies at a time
+constexpr int kCopyGroups = 2048;   // most workgroups of a copy: 8 a CU
+constexpr int kOneGroup = 1024;     // threads of the kernels that are one workgroup
+
+struct Pool {
+    uint16_t *data;
+    int planes, heads, D, pieces;  // pieces of at most kPieceBytes in a page of one head
+    long long plane_stride, page_stride, head_stride;
+    __host__ __device__ int rows_per_piece() const { return kPieceBytes / 2 / D; }
+};
+
+// (src page, dst page, rows, 0)
+typedef int Move __attribute__((ext_vector_type(4)));
+
+enum EntryState { kLeftOut = 0, kShared = 1, kNeedsPage = 2, kFailed = 3 };
+
+struct Entry {
+    int state, dst, rows;
+    int tail;  // the page to copy from; ~page where it was the entry's own
+};
+
+struct Header {
+    int left_out, ticket, moves, live;
+};
+
+struct Params {
+    int N, R, shift, S, P;
+    long long table_stride;
+    int *table, *refs, *length;
+    int num_pools;
+    unsigned pieces;  // of one move, over all pools
+    Header *head;
+    Entry *entries;
+    Move *moves;
+    int *ids;   // [N]: free pages in order, or where each page goes
+    int *rows;  // [min(S, ESDA_MAX_ENTRIES)][P]: the new rows of a fork's table
+    Pool pools[ESDA_MAX_POOLS];
+};
+
+__device__ __forceinline__ bool is_page(int id, int N) { return (unsigned) id < (unsigned) N; }
+
+__device__ __forceinline__ void add(int *at, int by) { __hip_atomic_fetch_add(at, by, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether list[i] stands in list before i; every thread of the workgroup calls it.
+__device__ __forceinline__ bool named_before(const int *list, int i) {
+    const int x = list[i];
+    bool found = false;
+    for (int j = threadIdx.x; j < i; j += blockDim.x) found = found || list[j] == x;
+    return __syncthreads_or(found);
+}
+
+// `chunks` 16-byte pieces by the lanes of a wave, eight loads in flight each.
+__device__ __forceinline__ void wave_copy(uint16_t *dst, const uint16_t *src, int chunks, int lane) {
+    constexpr int U = 8;
+    const u32x4 *s = reinterpret_cast<const u32x4 *>(src);
+    u32x4 *d = reinterpret_cast<u32x4 *>(dst);
+    for (int c = lane; c < chunks; c += 64 * U) {
+        u32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c + 64 * u < chunks) v[u] = s[c + 64 * u];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c + 64 * u < chunks) d[c + 64 * u] = v[u];
+    }
+}
+
+// Piece i of a move's: its pool, its place in a page of the pool and its first row.
+struct Piece {
+    const Pool *pool;
+    long long at;  // elements from the page's start
+    int row;
+};
+__device__ __forceinline__ Piece piece_of(const Params &p, unsigned i) {
+    int k = 0;
+    for (; k + 1 < p.num_pools; ++k) {
+        const unsigned n = (unsigned) p.pools[k].planes * p.pools[k].heads * p.pools[k].pieces;
+        if (i < n) break;
+        i -= n;
+    }
+    const Pool &o = p.pools[k];
+    const unsigned part = i % (unsigned) o.pieces, block = i / (unsigned) o.pieces;
+    const int row = (int) part * o.rows_per_piece();
+    return {&o, (long long) (block / (unsigned) o.heads) * o.plane_stride + (long long) (block % (unsigned) o.heads) * o.head_stride +
+                    (long long) row * o.D, row};
+}
+
+// The listed moves, a wave to a piece.
+__device__ void carry_out(const Params &p) {
+    if (p.num_pools == 0) return;
+    const int lane = threadIdx.x & 63;
+    const unsigned waves = gridDim.x * (blockDim.x / 64);
+    const unsigned long long all = (unsigned long long) (unsigned) p.head->moves * p.pieces;
+    for (unsigned long long u = blockIdx.x * (blockDim.x / 64) + (unsigned) uniform(threadIdx.x >> 6); u < all; u += waves) {
+        const unsigned m = (unsigned) (u / p.pieces);
+        const Piece x = piece_of(p, (unsigned) (u - (unsigned long long) m * p.pieces));
+        const Move mv = p.moves[m];
+        const int rows = min(mv[2] - x.row, min(p.R, x.pool->rows_per_piece()));
+        if (rows <= 0) continue;
+        uint16_t *const base = x.pool->data + x.at;
+        wave_copy(base + (long long) mv[1] * x.pool->page_stride, base + (long long) mv[0] * x.pool->page_stride, rows * x.pool->D / 8, lane);
+    }
+}
+
+// Exclusive sum over the threads of a workgroup of kOneGroup, and the total.
+struct Scan {
+    int before, total;
+};
+__device__ __forceinline__ Scan scan(int x) {
+    __shared__ int of[kOneGroup / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int in = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(in, o);
+        if (lane >= o) in += y;
+    }
+    __syncthreads();  // (the last call's sums are read)
+    if (lane == 63) of[wave] = in;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kOneGroup / 64; ++w) {
+        before += w < wave ? of[w] : 0;
+        total += of[w];
+    }
+    return {before + in - x, total};
+}
+
+// The lowest `need` free pages in order, put(rank, page) for each; how many there are (at most need).
+template <class Put>
+__device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put) {
+    int got = 0;
+    for (int base = 0; base < p.N && got < need; base += 4 * kOneGroup) {
+        bool free[4];
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int id = base + 4 * (int) threadIdx.x + e;
+            free[e] = id < p.N && p.refs[id] == 0;
+            n += free[e];
+        }
+        const Scan s = scan(n);
+        int rank = got + s.before;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (free[e]) {
+                if (rank < need) put(rank, base + 4 * (int) threadIdx.x + e);
+                ++rank;
+            }
+        got += s.total;
+    }
+    return min(got, need);
+}
+
+// ------------------------------------------------------------------------ kernels
+
+// A workgroup per entry.
+__global__ __launch_bounds__(256) void free_kernel(Params p, const int *slots) {
+    const int i = blockIdx.x, s = slots[i];
+    const bool twice = named_before(slots, i);
+    if (twice || (unsigned) s >= (unsigned) p.S) {
+        if (threadIdx.x == 0) add(&p.head->left_out, 1);
+        return;
+    }
+    int *const row = p.table + (long long) s * p.table_stride;
+    for (int k = threadIdx.x; k < p.P; k += 256) {
+        const int id = row[k];
+        if (is_page(id, p.N)) add(p.refs + id, -1);
+        row[k] = -1;
+    }
+    if (threadIdx.x == 0) p.length[s] = 0;
+}
+
+// One workgroup: what each entry lacks, which pages are free, who gets them.
+__global__ __launch_bounds__(kOneGroup) void reserve_kernel(Params p, const int *slots, const int *rows, int n) {
+    __shared__ int slot[ESDA_MAX_ENTRIES], first[ESDA_MAX_ENTRIES], last[ESDA_MAX_ENTRIES], lack[ESDA_MAX_ENTRIES], from[ESDA_MAX_ENTRIES];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if (t < n) slot[t] = slots[t];
+    __syncthreads();
+    if (t < n) {
+        const int s = slot[t], r = rows[t];
+        bool ok = (unsigned) s < (unsigned) p.S && r >= 0 && r <= (long long) p.P * p.R;
+        for (int j = 0; j < t; ++j) ok = ok && slot[j] != s;
+        int len = 0;
+        if (ok) {
+            len = p.length[s];
+            ok = len >= 0;
+        }
+        if (!ok) add(&p.head->left_out, 1);
+        first[t] = ok ? len >> p.shift : 0;
+        last[t] = ok ? (int) (((long long) r + p.R - 1) >> p.shift) : 0;
+    }
+    __syncthreads();
+    for (int i = wave; i < n; i += kOneGroup / 64) {
+        const int *const row = p.table + (long long) slot[i] * p.table_stride;
+        int sum = 0;
+        for (int k = first[i]; k < last[i]; k += 64)
+            sum += __popcll(__builtin_amdgcn_ballot_w64(k + lane < last[i] && !is_page(row[k + lane], p.N)));
+        if (lane == 0) lack[i] = sum;
+    }
+    __syncthreads();
+    const Scan s = scan(t < n ? lack[t] : 0);  // (1024 entries of at most 2^20)
+    if (t < n) from[t] = s.before;
+    const int got = lowest_free(p, min(s.total, p.N), [&](int rank, int id) { p.ids[rank] = id; });
+    __syncthreads();
+    for (int i = wave; i < n; i += kOneGroup / 64) {
+        int at = from[i];
+        if (lack[i] == 0) continue;
+        if (at > got - lack[i]) {
+            if (lane == 0) add(&p.head->left_out, 1);
+            continue;
+        }
+        int *const row = p.table + (long long) slot[i] * p.table_stride;
+        for (int k = first[i]; k < last[i]; k += 64) {
+            const bool needs = k + lane < last[i] && !is_page(row[k + lane], p.N);
+            const unsigned long long who = __builtin_amdgcn_ballot_w64(needs);
+            if (needs) {
+                const int id = p.ids[at + __popcll(who & ((1ull << lane) - 1))];
+                row[k + lane] = id;
+                p.refs[id] = 1;
+            }
+            at += __popcll(who);
+        }
+    }
+}
+
+// A fork, first launch: a workgroup per entry.  References of what it shares and gives up, the new row
+// of its table (dst's may be another's source), and what is left to copy.  The page to copy from holds a
+// reference more until the free pages are given out, so that it is none of them.
+__global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, const int *dst, const int *rows) {
+    const int i = blockIdx.x, s = src[i], d = dst[i];
+    Entry &entry = p.entries[i];
+    const bool twice = named_before(dst, i);
+    bool ok = !twice && (unsigned) s < (unsigned) p.S && (unsigned) d < (unsigned) p.S;
+    int len = 0, r = 0;
+    if (ok) {
+        len = p.length[s];
+        r = rows ? min(rows[i], len) : len;
+        ok = r >= 0 && len <= (long long) p.P * p.R;
+    }
+    const int full = r >> p.shift, part = r & (p.R - 1);
+    const int *const from = p.table + (long long) (ok ? s : 0) * p.table_stride;
+    bool there = true;
+    if (ok)
+        for (int k = threadIdx.x; k < full + (part > 0); k += 256) there = there && is_page(from[k], p.N);
+    if (__syncthreads_or(!there) || !ok) {
+        if (threadIdx.x == 0) {
+            add(&p.head->left_out, 1);
+            entry = Entry{kLeftOut, 0, 0, 0};
+        }
+        return;
+    }
+    // a cut within the page of the sequence's own last rows keeps that page
+    const bool keep = s == d && part > 0 && full == len >> p.shift;
+    const int *const old = p.table + (long long) d * p.table_stride;
+    int *const row = p.rows + (long long) i * p.P;
+    for (int k = threadIdx.x; k < p.P; k += 256) {
+        const int was = old[k];
+        int is = -1;
+        if (k < full || (keep && k == full)) {
+            is = from[k];
+            if (s != d) add(p.refs + is, 1);
+        }
+        if (is_page(was, p.N) && !(s == d && is >= 0)) add(p.refs + was, -1);
+        row[k] = is;
+    }
+    if (threadIdx.x == 0) {
+        const bool copies = part > 0 && !keep;
+        entry = Entry{copies ? kNeedsPage : kShared, d, r, copies ? (s == d ? ~from[full] : from[full]) : 0};
+        if (copies) add(p.refs + from[full], 1);
+    }
+}
+
+// .. second launch, one workgroup: a free page for every entry that copies.
+__global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) {
+    __shared__ int ids[ESDA_MAX_ENTRIES];
+    const int t = threadIdx.x;
+    const Entry e = t < n ? p.entries[t] : Entry{kLeftOut, 0, 0, 0};
+    const int tail = e.tail < 0 ? ~e.tail : e.tail, full = e.rows >> p.shift;
+    int *const row = p.rows + (long long) t * p.P;
+    bool needs = e.state == kNeedsPage;
+    if (needs && e.tail < 0 && p.refs[tail] == 1) {  // a sequence cut within a page that nobody else holds or copies
+        row[full] = tail;
+        needs = false;
+    }
+    const Scan s = scan(needs);
+    const int got = lowest_free(p, s.total, [&](int rank, int id) { ids[rank] = id; });
+    __syncthreads();
+    if (needs) {
+        add(p.refs + tail, -1);
+        if (s.before < got) {
+            const int id = ids[s.before];
+            row[full] = id;
+            p.refs[id] = 1;
+            p.moves[s.before] = Move{tail, id, e.rows & (p.R - 1), 0};
+        } else {  // rare: no page left
+            add(&p.head->left_out, 1);
+            for (int k = 0; k < full; ++k) {
+                add(p.refs + row[k], -1);
+                row[k] = -1;
+            }
+            p.entries[t].state = kFailed;
+        }
+    }
+    if (t == 0) p.head->moves = got;
+}
+
+// .. third: the tables, and the rows of the last pages.
+__global__ __launch_bounds__(256) void fork_copy_kernel(Params p, int n) {
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const Entry e = p.entries[i];
+        if (e.state == kLeftOut) continue;
+        int *const to = p.table + (long long) e.dst * p.table_stride;
+        const int *const row = p.rows + (long long) i * p.P;
+        for (int k = threadIdx.x; k < p.P; k += 256) to[k] = row[k];
+        if (threadIdx.x == 0) p.length[e.dst] = e.state == kFailed ? 0 : e.rows;
+    }
+    carry_out(p);
+}
+
+// Compaction, first launch, one workgroup: the pages in use at or above their number, and the free ones
+// below it, both in order; references and the way of each page that moves.
+__global__ __launch_bounds__(kOneGroup) void compact_kernel(Params p) {
+    const int t = threadIdx.x;
+    int n = 0;
+    for (int id = t; id < p.N; id += kOneGroup) n += p.refs[id] != 0;
+    const int live = scan(n).total;
+    int moves = 0, holes = 0;
+    for (int base = 0; base < p.N; base += 4 * kOneGroup) {
+        bool mover[4], hole[4];
+        int m = 0, h = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int id = base + 4 * t + e;
+            const bool used = id < p.N && p.refs[id] != 0;
+            mover[e] = used && id >= live;
+            hole[e] = !used && id < live;
+            m += mover[e];
+            h += hole[e];
+        }
+        const Scan s = scan(m << 16 | h);  // (4096 of them at most)
+        int mr = moves + (s.before >> 16), hr = holes + (s.before & 0xffff);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int id = base + 4 * t + e;
+            if (mover[e]) reinterpret_cast<int *>(p.moves + mr++)[0] = id;
+            else if (id >= live && id < p.N) p.ids[id] = id;  // (nobody's)
+            if (hole[e]) reinterpret_cast<int *>(p.moves + hr++)[1] = id;
+        }
+        moves += s.total >> 16;
+        holes += s.total & 0xffff;
+    }
+    __syncthreads();
+    for (int i = t; i < moves; i += kOneGroup) {
+        const int from = p.moves[i][0], to = p.moves[i][1];
+        reinterpret_cast<int *>(p.moves + i)[2] = p.R;
+        p.ids[from] = to;
+        p.refs[to] = p.refs[from];
+        p.refs[from] = 0;
+    }
+    if (t == 0) {
+        p.head->moves = moves;
+        p.head->live = live;
+    }
+}
+
+__global__ __launch_bounds__(256) void compact_copy_kernel(Params p) {
+    const int live = p.head->live;
+    if (p.head->moves == 0) return;
+    for (long long x = blockIdx.x * 256LL + threadIdx.x; x < (long long) p.S * p.P; x += 256LL * gridDim.x) {
+        int *const at = p.table + x / p.P * p.table_stride + x % p.P;
+        const int id = *at;
+        if (id >= live && id < p.N) *at = p.ids[id];
+    }
+    carry_out(p);
+}
+
+// ---- rows in and out
+
+struct RowsParams {
+    Pool pool;
+    int N, R, shift, P, batch, rows;
+    unsigned pieces;  // of a sequence's rows, more than they can touch
+    long long table_stride, plane_stride, seq_stride, head_stride;  // of the table, of the linear rows
+    const int *table, *row0;
+    uint16_t *linear;
+};
+
+// A wave to a piece: rows of one page, one head, one plane.
+template <bool WRITE>
+__global__ __launch_bounds__(256) void rows_kernel(RowsParams p) {
+    const int lane = threadIdx.x & 63;
+    const int per = min(p.R, p.pool.rows_per_piece());
+    const unsigned waves = gridDim.x * 4u;
+    const unsigned long long all = (unsigned long long) p.pool.planes * p.pool.heads * p.batch * p.pieces;
+    for (unsigned long long u = blockIdx.x * 4u + (unsigned) uniform(threadIdx.x >> 6); u < all; u += waves) {
+        const unsigned long long of = u / p.pieces;
+        const int piece = (int) (u - of * p.pieces);
+        const int b = (int) (of % (unsigned) p.batch);
+        const unsigned block = (unsigned) (of / (unsigned) p.batch);
+        const int head = (int) (block % (unsigned) p.pool.heads), plane = (int) (block / (unsigned) p.pool.heads);
+        const long long first = p.row0[b], start = (first & -(long long) per) + (long long) piece * per;
+        const long long i = max(first, start), j = min(first + p.rows, start + per);
+        if (i >= j) continue;
+        const long long k = start >> p.shift;  // (a piece lies in one page, or before row 0)
+        const int id = k >= 0 && k < p.P ? p.table[b * p.table_stride + k] : -1;
+        if (!is_page(id, p.N)) {
+            if constexpr (!WRITE) {
+                u32x4 *const to = reinterpret_cast<u32x4 *>(p.linear + plane * p.plane_stride + b * p.seq_stride +
+                                                            head * p.head_stride + (i - first) * p.pool.D);
+                for (int c = lane; c < (int) (j - i) * p.pool.D / 8; c += 64) to[c] = u32x4{0u, 0u, 0u, 0u};
+            }
+            continue;
+        }
+        uint16_t *const page = p.pool.data + plane * p.pool.plane_stride + (long long) id * p.pool.page_stride +
+                               head * p.pool.head_stride + (i & (p.R - 1)) * p.pool.D;
+        uint16_t *const rows = p.linear + plane * p.plane_stride + b * p.seq_stride + head * p.head_stride + (i - first) * p.pool.D;
+        wave_copy(WRITE ? page : rows, WRITE ? rows : page, (int) (j - i) * p.pool.D / 8, lane);
+    }
+}
+
+// ---- accepted rows
+
+struct CommitParams {
+    int N, shift, S, P, cap, linear;  // linear: slot s in page s, rows below cap
+    long long table_stride, accept_stride;
+    const int *table, *accept, *count;
+    int *length;
+    int max_accept, num_pools;
+    unsigned groups;  // workgroups of a slot, over all pools
+    Header *head;
+    Pool pools[ESDA_MAX_POOLS];
+};
+
+// Slot s's list, as a wave: lane i has the place of the row to take (page, row) and of the one it becomes.
+// False where the slot is left as it was.
+__device__ __forceinline__ bool accepted(const CommitParams &p, int s, int lane, int &n, int &take, int &c, int2 &from, int2 &to) {
+    n = p.length[s];
+    c = p.count[s];
+    bool ok = n >= 0 && c >= 0 && c <= p.max_accept;
+    take = ok && lane < c ? p.accept[s * p.accept_stride + lane] : -1;
+    const int before = __shfl_up(take, 1);
+    if (ok && lane < c) ok = take >= 0 && take < 64 && (lane == 0 || take > before);
+    if (ok && lane < c) {
+        auto place = [&](long long row, int2 &at) {
+            const long long k = row >> p.shift;
+            if (p.linear) {
+                at = int2{s, (int) row};
+                return row < p.cap;
+            }
+            if (k >= p.P) return false;
+            at = int2{p.table[s * p.table_stride + k], (int) (row & ((1 << p.shift) - 1))};
+            return is_page(at.x, p.N);
+        };
+        const bool a = place((long long) n + take, from), b = place((long long) n + lane, to);
+        ok = a && b;
+    }
+    return __builtin_amdgcn_ballot_w64(!ok) == 0ull;
+}
+
+// Groups of D / 8 lanes, each a (plane, kv head) of one slot: they take the moved rows in order, eight
+// at a time.  The rows rise, so that a row is written after it was read: row i becomes accept[i] >= i,
+// and what is read later lies above accept[i].  The workgroup that is the last to have read its slot's
+// list moves the lengths on.  Bound by the latency of the list, its pages and the rows.
+__global__ __launch_bounds__(256) void commit_kernel(CommitParams p) {
+    __shared__ int2 from[64], to[64];
+    __shared__ int moved, last;
+    const int s = (int) (blockIdx.x / p.groups), lane = threadIdx.x & 63;
+    if (threadIdx.x < 64) {
+        int n, take, c;
+        int2 a{0, 0}, b{0, 0};
+        const bool ok = accepted(p, s, lane, n, take, c, a, b);
+        const bool moves = ok && lane < c && take != lane;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(moves);
+        if (moves) {
+            const int at = __popcll(who & ((1ull << lane) - 1));
+            from[at] = a;
+            to[at] = b;
+        }
+        if (lane == 0) moved = __popcll(who);
+    }
+    __syncthreads();  // the list was read
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(&p.head->ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int) gridDim.x - 1;
+    unsigned g = blockIdx.x % p.groups;
+    int k = 0;
+    for (; k + 1 < p.num_pools; ++k) {
+        const unsigned of = (unsigned) (p.pools[k].planes * p.pools[k].heads * (p.pools[k].D / 8) + 255) / 256;
+        if (g < of) break;
+        g -= of;
+    }
+    const Pool &o = p.pools[k];
+    const unsigned lanes = (unsigned) o.D / 8, block = (g * 256 + threadIdx.x) / lanes;
+    if (block < (unsigned) (o.planes * o.heads)) {
+        constexpr int U = 8;
+        uint16_t *const base = o.data + (long long) (block / (unsigned) o.heads) * o.plane_stride +
+                               (long long) (block % (unsigned) o.heads) * o.head_stride + 8 * (threadIdx.x % lanes);
+        auto at = [&](const int2 &x) { return reinterpret_cast<u32x4 *>(base + x.x * o.page_stride + (long long) x.y * o.D); };
+        for (int i = 0; i < moved; i += U) {
+            u32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u < moved) v[u] = *at(from[i + u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u < moved) *at(to[i + u]) = v[u];
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int x = threadIdx.x >> 6; x < p.S; x += 4) {
+        int n, take, c;
+        int2 a, b;
+        const bool ok = accepted(p, x, lane, n, take, c, a, b);
+        if (lane == 0) {
+            if (ok) p.length[x] = n + c;
+            else add(&p.head->left_out, 1);
+        }
+    }
+    if (threadIdx.x == 0) p.head->ticket = 0;
+}
+
+// ------------------------------------------------------------------------ host side
+
+int fail(int code, const std::string &msg) {
+    esda_detail::set_error(msg);
+    return code;
+}
+
+int refuse(const char *call, const char *why) { return fail(ESDA_ERR_INVALID_ARGUMENT, std::string(call) + ": " + why); }
+
+int launched(const char *call) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? ESDA_OK : fail(ESDA_ERR_HIP, std::string(call) + " launch: " + hipGetErrorString(e));
+}
+
+bool aligned(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+struct Layout {
+    size_t entries, moves, ids, rows, bytes;
+};
+
+Layout layout(int num_pages, int slots, int max_pages) {
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Layout l;
+    l.entries = 256;
+    l.moves = l.entries + sizeof(Entry) * ESDA_MAX_ENTRIES;
+    l.ids = l.moves + sizeof(Move) * std::max<size_t>(ESDA_MAX_ENTRIES, num_pages / 2 + 1);
+    l.rows = l.ids + up(sizeof(int) * (size_t) num_pages);
+    l.bytes = l.rows + sizeof(int) * (size_t) std::min(slots, ESDA_MAX_ENTRIES) * max_pages;
+    return l;
+}
+
+Pool pool_params(const esda_pool &x, int page_rows) {
+    Pool o{static_cast<uint16_t *>(x.data), x.planes, x.num_kv_heads, x.head_dim, 0, x.plane_stride, x.page_stride, x.head_stride};
+    o.pieces = (page_rows + o.rows_per_piece() - 1) / o.rows_per_piece();
+    return o;
+}
+
+const char *check_pools(const esda_pages *c, int page_rows) {
+    if (c->num_pools < 0 || c->num_pools > ESDA_MAX_POOLS) return "at most 8 pools";
+    for (int i = 0; i < c->num_pools; ++i) {
+        if (const char *why = check_pool(c->pools[i], c->num_pages, page_rows)) return why;
+        for (int j = 0; j < i; ++j)
+            if (c->pools[i].data == c->pools[j].data) return "two pools are the same memory";
+    }
+    return nullptr;
+}
+
+// Fills the kernels' parameters; an error code where the cache is none.
+int page_params(const char *call, const esda_pages *c, Params *p) {
+    if (!c) return refuse(call, "null cache");
+    if (const char *why = check_table(c->num_pages, c->page_rows, c->slots, c->max_pages, c->table_stride)) return refuse(call, why);
+    if (!c->table || !c->refs || !c->length || !aligned(c->table, 4) || !aligned(c->refs, 4) || !aligned(c->length, 4))
+        return refuse(call, "table, refs and length must be 4-byte aligned device memory");
+    if (const char *why = check_pools(c, c->page_rows)) return refuse(call, why);
+    const Layout l = layout(c->num_pages, c->slots, c->max_pages);
+    if (!c->workspace || c->workspace_bytes < l.bytes || !aligned(c->workspace, 16))
+        return fail(ESDA_ERR_WORKSPACE, std::string(call) + ": workspace missing or smaller than esda_pages_workspace_size");
+    char *const ws = static_cast<char *>(c->workspace);
+    *p = Params{};
+    p->N = c->num_pages;
+    p->R = c->page_rows;
+    p->shift = __builtin_ctz((unsigned) c->page_rows);
+    p->S = c->slots;
+    p->P = c->max_pages;
+    p->table_stride = c->table_stride;
+    p->table = c->table;
+    p->refs = c->refs;
+    p->length = c->length;
+    p->num_pools = c->num_pools;
+    p->head = reinterpret_cast<Header *>(ws);
+    p->entries = reinterpret_cast<Entry *>(ws + l.entries);
+    p->moves = reinterpret_cast<Move *>(ws + l.moves);
+    p->ids = reinterpret_cast<int *>(ws + l.ids);
+    p->rows = reinterpret_cast<int *>(ws + l.rows);
+    long long pieces = 0;
+    for (int i = 0; i < c->num_pools; ++i) {
+        p->pools[i] = pool_params(c->pools[i], c->page_rows);
+        pieces += (long long) p->pools[i].planes * p->pools[i].heads * p->pools[i].pieces;
+    }
+    if (pieces >= 1LL << 31) return refuse(call, "too many planes and heads");
+    p->pieces = (unsigned) std::max(1LL, pieces);
+    return ESDA_OK;
+}
+
+const char *check_list(const void *list, int n) {
+    if (n < 0 || n > ESDA_MAX_ENTRIES) return "a call names at most 1024 slots";
+    if (n > 0 && (!list || !aligned(list, 4))) return "lists must be 4-byte aligned device memory";
+    return nullptr;
+}
+
+// Workgroups of four waves for at most `moves` moves.
+unsigned copy_groups(const Params &p, long long moves) {
+    return (unsigned) std::max(1LL, std::min<long long>(kCopyGroups, (moves * p.pieces + 3) / 4));
+}
+
+int rows_call(const char *call, bool write, const esda_page_rows_desc *d, const int32_t *table, const int32_t *row0, void *linear,
+              hipStream_t st) {
+    if (!d) return refuse(call, "null description");
+    if (const char *why = check_table(d->num_pages, d->page_rows, d->batch, d->max_pages, d->table_stride)) return refuse(call, why);
+    if (const char *why = check_pool(d->pool, d->num_pages, d->page_rows)) return refuse(call, why);
+    if (d->rows < 0 || d->rows > 1 << 30) return refuse(call, "rows must be 0 .. 2^30");
+    if (!whole16(d->linear_plane_stride) || !whole16(d->linear_seq_stride) || !whole16(d->linear_head_stride))
+        return refuse(call, "strides must be non-negative multiples of 8");
+    if (!table || !row0 || !aligned(table, 4) || !aligned(row0, 4)) return refuse(call, "table and row0 must be 4-byte aligned device memory");
+    if (!linear || !aligned(linear, 16)) return refuse(call, "linear rows must be 16-byte aligned device memory");
+    if (!write && !blocks_apart({d->pool.planes, d->batch, d->pool.num_kv_heads},
+                                {d->linear_plane_stride, d->linear_seq_stride, d->linear_head_stride}, (long long) d->rows * d->pool.head_dim))
+        return refuse(call, "the linear rows overlap");
+    const int rc = esda_detail::check_device();
+    if (rc || d->rows == 0) return rc;
+    RowsParams p{};
+    p.pool = pool_params(d->pool, d->page_rows);
+    p.N = d->num_pages;
+    p.R = d->page_rows;
+    p.shift = __builtin_ctz((unsigned) d->page_rows);
+    p.P = d->max_pages;
+    p.batch = d->batch;
+    p.rows = d->rows;
+    p.table_stride = d->table_stride;
+    p.plane_stride = d->linear_plane_stride;
+    p.seq_stride = d->linear_seq_stride;
+    p.head_stride = d->linear_head_stride;
+    p.table = table;
+    p.row0 = row0;
+    p.linear = static_cast<uint16_t *>(linear);
+    const int per = std::min(p.R, p.pool.rows_per_piece());
+    p.pieces = (unsigned) (d->rows / per + 2);
+    const __int128 waves = (__int128) p.pool.planes * p.pool.heads * p.batch * p.pieces;
+    if (waves > (__int128) 1 << 60) return refuse(call, "too many rows");
+    const unsigned groups = (unsigned) std::min<__int128>(kCopyGroups, (waves + 3) / 4);
+    if (write) hipLaunchKernelGGL(rows_kernel<true>, dim3(groups), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(rows_kernel<false>, dim3(groups), dim3(256), 0, st, p);
+    return launched(call);
+}
+
+}  // namespace
+
+extern "C" {
+
+int esda_pages_workspace_size(const esda_pages *c, size_t *bytes) {
+    const char *call = "esda_pages_workspace_size";
+    if (!c || !bytes) return refuse(call, "null argument");
+    if (const char *why = check_table(c->num_pages, 16, c->slots, 1, 1)) return refuse(call, why);
+    if (c->max_pages <= 0 || c->max_pages > kMaxTable) return refuse(call, "max_pages must be 1 .. 2^20");
+    *bytes = layout(c->num_pages, c->slots, c->max_pages).bytes;
+    return ESDA_OK;
+}
+
+int esda_pages_reserve(const esda_pages *c, const int32_t *slots, const int32_t *rows, int32_t n, void *stream) {
+    const char *call = "esda_pages_reserve";
+    Params p;
+    if (const int rc = page_params(call, c, &p)) return rc;
+    for (const int32_t *list : {slots, rows})
+        if (const char *why = check_list(list, n)) return refuse(call, why);
+    if (const int rc = esda_detail::check_device()) return rc;
+    if (n == 0) return ESDA_OK;
+    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kOneGroup), 0, static_cast<hipStream_t>(stream), p, slots, rows, n);
+    return launched(call);
+}
+
+int esda_pages_free(const esda_pages *c, const int32_t *slots, int32_t n, void *stream) {
+    const char *call = "esda_pages_free";
+    Params p;
+    if (const int rc = page_params(call, c, &p)) return rc;
+    if (const char *why = check_list(slots, n)) return refuse(call, why);
+    if (const int rc = esda_detail::check_device()) return rc;
+    if (n == 0) return ESDA_OK;
+    hipLaunchKernelGGL(free_kernel, dim3(n), dim3(256), 0, static_cast<hipStream_t>(stream), p, slots);
+    return launched(call);
+}
+
+int esda_pages_fork(const esda_pages *c, const int32_t *src, const int32_t *dst, const int32_t *rows, int32_t n, void *stream) {
+    const char *call = "esda_pages_fork";
+    Params p;
+    if (const int rc = page_params(call, c, &p)) return rc;
+    for (const int32_t *list : {src, dst, rows ? rows : dst})
+        if (const char *why = check_list(list, n)) return refuse(call, why);
+    if (n > c->slots) return refuse(call, "more entries than slots");
+    if (const int rc = esda_detail::check_device()) return rc;
+    if (n == 0) return ESDA_OK;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(fork_kernel, dim3(n), dim3(256), 0, st, p, src, dst, rows);
+    hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kOneGroup), 0, st, p, n);
+    hipLaunchKernelGGL(fork_copy_kernel, dim3(std::max<unsigned>(n, copy_groups(p, n))), dim3(256), 0, st, p, n);
+    return launched(call);
+}
+
+int esda_pages_compact(const esda_pages *c, void *stream) {
+    const char *call = "esda_pages_compact";
+    Params p;
+    if (const int rc = page_params(call, c, &p)) return rc;
+    if (const int rc = esda_detail::check_device()) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const long long moves = p.num_pools ? p.N / 2 : 0;
+    hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kOneGroup), 0, st, p);
+    hipLaunchKernelGGL(compact_copy_kernel, dim3(std::max(copy_groups(p, moves), (unsigned) std::min(256LL, ((long long) p.S * p.P + 255) / 256))),
+                       dim3(256), 0, st, p);
+    return launched(call);
+}
+
+int esda_pages_status(void *workspace, int32_t *left_out, void *stream) {
+    const char *call = "esda_pages_status";
+    if (!workspace || !aligned(workspace, 16) || !left_out) return refuse(call, "null or unaligned argument");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    hipError_t e = hipMemcpyAsync(left_out, workspace, sizeof(int32_t), hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipMemsetAsync(workspace, 0, sizeof(int32_t), st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    return e == hipSuccess ? ESDA_OK : fail(ESDA_ERR_HIP, std::string(call) + ": " + hipGetErrorString(e));
+}
+
+int esda_pages_write(const esda_page_rows_desc *d, const int32_t *table, const int32_t *row0, const void *linear, void *stream) {
+    return rows_call("esda_pages_write", true, d, table, row0, const_cast<void *>(linear), static_cast<hipStream_t>(stream));
+}
+
+int esda_pages_read(const esda_page_rows_desc *d, const int32_t *table, const int32_t *row0, void *linear, void *stream) {
+    return rows_call("esda_pages_read", false, d, table, row0, linear, static_cast<hipStream_t>(stream));
+}
+
+int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_stride, int32_t max_accept, const int32_t *count,
+                     void *stream) {
+    const char *call = "esda_tree_commit";
+    if (!c) return refuse(call, "null cache");
+    const bool linear = !c->table;
+    if (const char *why = check_table(c->num_pages, linear ? 16 : c->page_rows, c->slots, linear ? 1 : c->max_pages, linear ? 1 : c->table_stride))
+        return refuse(call, why);
+    if (linear && (c->max_pages != 1 || c->num_pages != c->slots || c->page_rows <= 0 || c->page_rows > 1 << 30))
+        return refuse(call, "without a table: slots pages, one a slot, of 1 .. 2^30 rows");
+    if (!c->length || !aligned(c->length, 4) || !aligned(c->table, 4)) return refuse(call, "table and length must be 4-byte aligned device memory");
+    if (const char *why = check_pools(c, c->page_rows)) return refuse(call, why);
+    if (max_accept < 1 || max_accept > 64 || accept_stride < max_accept || accept_stride > 1LL << 40)
+        return refuse(call, "max_accept must be 1 .. 64, accept_stride at least that");
+    if (!accept || !count || !aligned(accept, 4) || !aligned(count, 4))
+        return refuse(call, "accept and count must be 4-byte aligned device memory");
+    if (!c->workspace || c->workspace_bytes < 256 || !aligned(c->workspace, 16))
+        return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: a workspace of 256 bytes or more is needed");
+    CommitParams p{};
+    p.N = c->num_pages;
+    p.linear = linear;
+    p.shift = linear ? 30 : __builtin_ctz((unsigned) c->page_rows);
+    p.S = c->slots;
+    p.P = c->max_pages;
+    p.cap = c->page_rows;
+    p.table_stride = c->table_stride;
+    p.accept_stride = accept_stride;
+    p.table = c->table;
+    p.accept = accept;
+    p.count = count;
+    p.length = c->length;
+    p.max_accept = max_accept;
+    p.num_pools = c->num_pools;
+    p.head = static_cast<Header *>(c->workspace);
+    long long groups = 0;
+    for (int i = 0; i < c->num_pools; ++i) {
+        p.pools[i] = pool_params(c->pools[i], c->page_rows);
+        groups += ((long long) p.pools[i].planes * p.pools[i].heads * (p.pools[i].D / 8) + 255) / 256;
+    }
+    groups = std::max(1LL, groups);
+    if (groups * c->slots > 1LL << 23) return refuse(call, "too many slots, planes and heads");
+    p.groups = (unsigned) groups;
+    const int rc = esda_detail::check_device();
+    if (rc) return rc;
+    hipLaunchKernelGGL(commit_kernel, dim3((unsigned) (groups * c->slots)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    return launched(call);
+}
+
+}  // extern "C"

@@ -68,8 +68,9 @@ struct OwnRows {
     static constexpr int kGroupBytes = esda_stream::GroupLayout<D, SH>::BYTES;
     static constexpr int kStreamBytes = esda_stream::Layout<D, SH, NW, SLOTS, NG>::BYTES;
     static constexpr int BYTES = ONLY || (GROUPS && kGroupBytes > kStreamBytes) ? kGroupBytes : kStreamBytes;
-    template <class Query, class Score, class Put>
-    static __device__ __forceinline__ void attend(unsigned char *lds, const esda_stream::Run &x, Query &&query, Score &&score, Put &&put) {
+    using Run = esda_stream::RunOf<D, SH>;
+    template <class Rows, class Query, class Score, class Put>
+    static __device__ __forceinline__ void attend(unsigned char *lds, Rows &x, Query &&query, Score &&score, Put &&put) {
         if constexpr (GROUPS) {
             static_assert(NG == 1, "16 query rows a group");
             if (ONLY || x.j1 - x.j0 <= kGroupRows) {
@@ -93,7 +94,7 @@ struct OwnRows {
             if (split == 0 && kvh == 0 && threadIdx.x == 0) atomicAdd(p.status, 1);
             return;
         }
-        esda_stream::Run x;
+        Run x;
         if (!esda_plan::grid_split(split, p.own_splits, p.own_chunk, sv.nvis, &x.j0, &x.j1)) return;
         const size_t head = (size_t) b * p.own_seq_stride + (size_t) kvh * p.own_head_stride;
         x.k = p.own_k + head;
@@ -118,7 +119,7 @@ struct OwnRows {
         const int r0 = (int) (i % (unsigned) p.row_groups) * 16 * NG;
         const int kvh = (int) (pair % (unsigned) p.Hkv), split = (int) (pair / (unsigned) p.Hkv);
         if (split >= p.splits) return;
-        esda_stream::Run x{};
+        Run x{};
         x.j0 = split * p.run_keys;
         x.j1 = min(p.Sk, x.j0 + p.run_keys);
         x.k = const_cast<uint16_t *>(p.k) + (size_t) kvh * p.kv_hs;

@@ -98,6 +98,23 @@ struct PrefixParams : PrefillParams {
     float *own_acc, *own_ml;  // [B * Hkv][own_splits][G][D] and [..][2]
 };
 
+// A step of drafted tokens (esda_tree.h): Sq nodes of each of B sequences, whose keys are the rows of a
+// cache in pages (kv_hs: between the heads of a page) or linear, and the nodes' own.  Keys are counted
+// from the first one that any node sees; `kps` of them a split, and every (sequence, kv head) has
+// `splits`, of which those hold keys that its length reaches.
+struct TreeParams : PrefillParams {
+    int B;
+    int run_rows;     // > 0: in runs (esda_tree.hip), 16 * this many query rows a workgroup
+    int row_groups;   // .. workgroups of the same keys
+    int N, P, shift;  // pages, entries of a sequence's table, log2 of a page's rows
+    int linear, cap;  // linear: sequence b in page b, rows below cap
+    long long page_stride, table_stride;
+    const int *table, *length, *parent;
+    const uint16_t *k_new, *v_new;
+    int *status;
+    int *views;       // [B]: keys of a sequence, -1 where it is skipped, for the merge
+};
+
 // A kernel form of one head dim: 16-query blocks per wave, stage halves or not, waves, and
 // its cost in us: `wg` and `row` per workgroup and query row of it (Q and first-stage loads,
 // the pipeline's fill, epilogue) and `stage` per 32-key stage.  Fitted, with the split's costs

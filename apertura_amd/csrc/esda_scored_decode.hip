@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 1) void stream_kernel(P p) {
     auto segment = [&](const int b, const int kvh, const int j0, const int j1, const SeqView sv, const size_t slot,
                        const bool direct) __attribute__((always_inline)) {
         const size_t head = (size_t) b * p.seq_stride + (size_t) kvh * p.head_stride, at = ((size_t) b * p.Hkv + kvh) * D;
-        const esda_stream::Run x{p.k_cache + head, p.v_cache + head, p.k_new + at, SH ? p.k_new + at : p.v_new + at,
+        esda_stream::RunOf<D, SH> x{p.k_cache + head, p.v_cache + head, p.k_new + at, SH ? p.k_new + at : p.v_new + at,
                                  p.G, j0, j1, sv.nvis, sv.first, p.cap, sv.newrow};
         const uint16_t *const q = p.q + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;
         uint16_t *const out = p.out + ((size_t) b * p.Hq + (size_t) kvh * p.G) * D;

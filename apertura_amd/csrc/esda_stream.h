@@ -9,17 +9,64 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "esda_device.h"
 
 namespace esda_stream {
 
-// Rows [j0, j1) of a kv head's nvis visible ones, for G query rows.
-struct Run {
+// What a run is given by: G query rows, rows [j0, j1) (in 16-row stages from j0 on), and
+//   dense(jst, stage)    whether rows jst .. jst + 15 of the run lie one behind another: stage.k, stage.v;
+//                        every wave calls it for its stages in order, before their loads
+//   row(j, k, v)         where row j lies, for stages that are not dense
+//   Stage::end           rows of the stage from it on have no weight
+//   appended(wave, lane) called once by every wave after its last stage
+// A run of linear or ring rows, the last one maybe new: rows [j0, j1) of a kv head's nvis visible ones.
+template <int D, bool SH>
+struct RunOf {
     uint16_t *k, *v;               // the cache rows of the kv head
     const uint16_t *k_new, *v_new; // the new token's rows (the last visible row), or null
     int G, j0, j1, nvis, first, cap, newrow;
+
+    struct Stage {
+        const uint16_t *k, *v;
+        int end;
+    };
+    __device__ __forceinline__ bool dense(int jst, Stage &st) const {
+        st.end = j1;
+        st.k = k + (size_t) (first + jst) * D;
+        st.v = v + (size_t) (first + jst) * D;
+        return jst + 16 < j1 && first + jst + 16 <= cap;  // sixteen consecutive cache rows, none clamped or new
+    }
+    __device__ __forceinline__ void row(int j, const uint16_t *&kr, const uint16_t *&vr) const {
+        int r = first + j;
+        if (r >= cap) r -= cap;
+        const bool is_new = k_new != nullptr && j == nvis - 1;
+        kr = is_new ? k_new : k + (size_t) r * D;
+        if constexpr (!SH) vr = is_new ? v_new : v + (size_t) r * D;
+    }
+    // The new row into the cache (bit-exact) by the run that ends with it; no other run reads it.
+    __device__ __forceinline__ void appended(int wave, int lane) const {
+        if (k_new != nullptr && j1 == nvis && wave == 0)
+            for (int c = lane; c < D / 8; c += 64) {
+                *reinterpret_cast<u32x4 *>(k + (size_t) newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(k_new + 8 * c);
+                if constexpr (!SH)
+                    *reinterpret_cast<u32x4 *>(v + (size_t) newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(v_new + 8 * c);
+            }
+    }
 };
+
+// The log2-domain scores of a stage's raw products s (rows jst + 4 lg .. of query row 16 g + li), -inf for
+// rows without weight: by score(x, j) one at a time, or by score(s, jst, end, g) together.
+template <class Score>
+__device__ __forceinline__ void stage_scores(const Score &score, f32x4 &s, int jst, int end, int lg, int g) {
+    if constexpr (std::is_invocable<const Score &, f32x4 &, int, int, int>::value) {
+        score(s, jst, end, g);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = jst + 4 * lg + r < end ? score(s[r], jst + 4 * lg + r) : -INFINITY;
+    }
+}
 
 // NW waves with SLOTS slots each; up to 16 NG query rows.
 template <int D, bool SH, int NW, int SLOTS, int NG = 1>
@@ -43,47 +90,45 @@ struct Layout {
     __device__ static constexpr int off(int r) { return (r % NI) * BLK + (r / NI) * 2 * D; }
 };
 
-// Attends the run; every thread of the workgroup calls it.  query(h): query row h; score(x, j): the
-// log2-domain score of raw product x and visible row j, of query row `lane & 15` (of each 16);
-// put(h, d, o, M, T): called once for each query row h and four dims from d on, with O, its maximum
+// Attends the run; every thread of the workgroup calls it.  query(h): query row h; score: as
+// stage_scores has it, of query row `lane & 15` (of each 16); put(h, d, o, M, T): called once for each query row h and four dims from d on, with O, its maximum
 // and its sum.  Each K and V read from LDS serves NG products of 16 query rows.
-template <int D, bool SH, int NW, int SLOTS, int NG, class Query, class Score, class Put>
-__device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
+template <int D, bool SH, int NW, int SLOTS, int NG, class Run, class Query, class Score, class Put>
+__device__ __forceinline__ void attend_run(unsigned char *lds, Run &x, Query &&query, Score &&score, Put &&put) {
     using L = Layout<D, SH, NW, SLOTS, NG>;
     constexpr int KS = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
     unsigned char *const ring = lds + wave * SLOTS * L::SLOT;
     const int nst = (x.j1 - x.j0 + 15) >> 4;
-    const bool append = x.k_new != nullptr;
 
     const int drow = lane / L::CPR, chunk = lane % L::CPR;  // DMA: this lane's row among a block's, its chunk
     const unsigned voff = (unsigned) ((drow * L::NI * D + chunk * 8) * 2);
-    auto dma = [&](int st, unsigned char *slot) {
+    auto dma = [&](int st, unsigned char *slot) -> int {  // the stage's end
         const int jst = x.j0 + 16 * st;
         const unsigned at = lds_addr(slot);
-        if (jst + 16 < x.j1 && x.first + jst + 16 <= x.cap) {
-            // sixteen consecutive cache rows, none clamped or new
-            const uint16_t *kb = x.k + (size_t) (x.first + jst) * D, *vb = x.v + (size_t) (x.first + jst) * D;
+        typename Run::Stage rows;
+        if (x.dense(jst, rows)) {
 #pragma unroll
             for (int i = 0; i < L::NI; ++i) {
-                lds_dma16_s(kb + i * D, voff, at + i * L::BLK);
-                if constexpr (!SH) lds_dma16_s(vb + i * D, voff, at + L::HB + i * L::BLK);
+                lds_dma16_s(rows.k + i * D, voff, at + i * L::BLK);
+                if constexpr (!SH) lds_dma16_s(rows.v + i * D, voff, at + L::HB + i * L::BLK);
             }
-            return;
+            return rows.end;
         }
 #pragma unroll
         for (int i = 0; i < L::NI; ++i) {
             const int j = min(jst + i + L::NI * drow, x.j1 - 1);  // rows past the run repeat its last, masked
-            int r = x.first + j;
-            if (r >= x.cap) r -= x.cap;
-            const bool is_new = append && j == x.nvis - 1;
-            lds_dma16((is_new ? x.k_new : x.k + (size_t) r * D) + chunk * 8, at + i * L::BLK);
-            if constexpr (!SH) lds_dma16((is_new ? x.v_new : x.v + (size_t) r * D) + chunk * 8, at + L::HB + i * L::BLK);
+            const uint16_t *kr, *vr;
+            x.row(j, kr, vr);
+            lds_dma16(kr + chunk * 8, at + i * L::BLK);
+            if constexpr (!SH) lds_dma16(vr + chunk * 8, at + L::HB + i * L::BLK);
         }
+        return rows.end;
     };
 
-    if (wave < nst) dma(wave, ring);
+    int end = 0, next_end = 0;  // of this stage and the next
+    if (wave < nst) end = dma(wave, ring);
     bf16x8 qv[NG][KS];  // B operands: query row 16 g + li, dims 32 ks + 8 lg ..
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -111,11 +156,11 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         ESDA_WAIT_VM(0);  // this stage landed
         if (SLOTS > 1 && st + NW < nst) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other slot's reads are done
-            dma(st + NW, ring + ((it + 1) & 1) * L::SLOT);
+            next_end = dma(st + NW, ring + ((it + 1) & 1) * L::SLOT);
         }
         asm volatile("" ::: "memory");
         // Rows past the run repeat its last one, with a weight of 0; but 0 x inf is NaN.
-        for (int r = x.j1 - (x.j0 + 16 * st); r < 16; ++r)
+        for (int r = max(0, end - (x.j0 + 16 * st)); r < 16; ++r)
             if (lane < D / 8) *reinterpret_cast<u32x4 *>(slot + (SH ? 0 : L::HB) + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
         asm volatile("" ::: "memory");
         // Every K read of the stage, then the products, then every V read, which lands during the
@@ -145,13 +190,11 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
             va[dt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) short4v *) (slot + (SH ? 0 : L::HB) + tr_off + 32 * dt));
         __builtin_amdgcn_sched_barrier(0);
-        const int jt = x.j0 + 16 * st + 4 * lg;
         float top[NG];
         bool raise = false;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[g][r] = jt + r < x.j1 ? score(s[g][r], jt + r) : -INFINITY;
+            stage_scores(score, s[g], x.j0 + 16 * st, end, lg, g);
             top[g] = wave_max_across_groups(fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])));
             raise = raise || top[g] > m[g] + kRescaleSlack;
         }
@@ -182,8 +225,9 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
             for (int g = 0; g < NG; ++g) acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(va[dt], pb[g], acc[g][dt], 0, 0, 0);
         if (SLOTS == 1 && st + NW < nst) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads are done
-            dma(st + NW, ring);
+            next_end = dma(st + NW, ring);
         }
+        end = next_end;
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -191,13 +235,7 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, const Run &x, Que
         l[g] += __shfl_xor(l[g], 32);
     }
 
-    // The new row into the cache (bit-exact) by the run that ends with it; no other run reads it.
-    if (append && x.j1 == x.nvis && wave == 0)
-        for (int c = lane; c < D / 8; c += 64) {
-            *reinterpret_cast<u32x4 *>(x.k + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.k_new + 8 * c);
-            if constexpr (!SH)
-                *reinterpret_cast<u32x4 *>(x.v + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.v_new + 8 * c);
-        }
+    x.appended(wave, lane);
 
     // The waves' totals, then their O over CH dims at a time.  A wave without a stage has m = kNoScore, l = 0.
     f32x2 *const ml = reinterpret_cast<f32x2 *>(lds + L::TOTALS), *const tot = ml + NW * L::ROWS;  // [NW][ROWS], [ROWS]
@@ -257,46 +295,49 @@ struct GroupLayout {
 };
 
 // Arguments as attend_run's; put's four dims come from one lane, the rows of 16 side by side.
-template <int D, bool SH, int NW, class Query, class Score, class Put>
-__device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, Query &&query, Score &&score, Put &&put) {
+template <int D, bool SH, int NW, class Run, class Query, class Score, class Put>
+__device__ __forceinline__ void attend_groups(unsigned char *lds, Run &x, Query &&query, Score &&score, Put &&put) {
     using L = GroupLayout<D, SH>;
     constexpr int KS = D / 32, DT = D / 16 / NW, SUB = L::SUB;  // k-steps; O^T dim tiles a wave
     constexpr int LOADS = (SH ? 1 : 2) * L::NI;                 // DMAs of a stage
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
-    const bool scores = wave < SUB, append = x.k_new != nullptr;
+    const bool scores = wave < SUB;
     const int groups = (x.j1 - x.j0 + L::ROWS - 1) / L::ROWS;
     f32x4 *const xch = reinterpret_cast<f32x4 *>(lds + 2 * L::SLOT);  // [SUB][64 lanes]
 
     const int drow = lane / L::CPR, chunk = lane % L::CPR;
     const unsigned voff = (unsigned) ((drow * L::NI * D + chunk * 8) * 2);
     // This wave's stage of group i; false where it has none or holds no row.
+    int end = x.j1, next_end = x.j1;  // of this wave's stage in this group and the next
     auto dma = [&](int i) {
         const int jst = x.j0 + L::ROWS * i + 16 * wave;
         if (!scores || jst >= x.j1) return false;
         const unsigned at = lds_addr(lds) + (i & 1) * L::SLOT + wave * L::HB;
-        if (jst + 16 < x.j1 && x.first + jst + 16 <= x.cap) {
-            const uint16_t *kb = x.k + (size_t) (x.first + jst) * D, *vb = x.v + (size_t) (x.first + jst) * D;
+        typename Run::Stage rows;
+        const bool dense = x.dense(jst, rows);
+        next_end = rows.end;
+        if (dense) {
 #pragma unroll
             for (int t = 0; t < L::NI; ++t) {
-                lds_dma16_s(kb + t * D, voff, at + t * L::BLK);
-                if constexpr (!SH) lds_dma16_s(vb + t * D, voff, at + SUB * L::HB + t * L::BLK);
+                lds_dma16_s(rows.k + t * D, voff, at + t * L::BLK);
+                if constexpr (!SH) lds_dma16_s(rows.v + t * D, voff, at + SUB * L::HB + t * L::BLK);
             }
             return true;
         }
 #pragma unroll
         for (int t = 0; t < L::NI; ++t) {
             const int j = min(jst + t + L::NI * drow, x.j1 - 1);  // rows past the run repeat its last, masked
-            int r = x.first + j;
-            if (r >= x.cap) r -= x.cap;
-            const bool is_new = append && j == x.nvis - 1;
-            lds_dma16((is_new ? x.k_new : x.k + (size_t) r * D) + chunk * 8, at + t * L::BLK);
-            if constexpr (!SH) lds_dma16((is_new ? x.v_new : x.v + (size_t) r * D) + chunk * 8, at + SUB * L::HB + t * L::BLK);
+            const uint16_t *kr, *vr;
+            x.row(j, kr, vr);
+            lds_dma16(kr + chunk * 8, at + t * L::BLK);
+            if constexpr (!SH) lds_dma16(vr + chunk * 8, at + SUB * L::HB + t * L::BLK);
         }
         return true;
     };
 
     dma(0);
+    end = next_end;
     u32x4 qv[KS];  // B operands: query row li, dims 32 ks + 8 lg ..
     const bool there = scores && li < x.G;
     const uint16_t *const qr = query(there ? li : 0) + 8 * lg;
@@ -324,7 +365,7 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, 
             unsigned char *const kb = slot + wave * L::HB, *const vb = SH ? kb : kb + SUB * L::HB;
             const int jst = x.j0 + L::ROWS * i + 16 * wave;
             // Rows past the run repeat its last one or hold anything, with a weight of 0; but 0 x inf is NaN.
-            for (int r = max(0, x.j1 - jst); r < 16; ++r)
+            for (int r = max(0, end - jst); r < 16; ++r)
                 if (lane < D / 8) *reinterpret_cast<u32x4 *>(vb + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
             asm volatile("" ::: "memory");
             f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // (in four sums, as attend_run's, the step took as long)
@@ -333,8 +374,7 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, 
                 const bf16x8 k8 = *reinterpret_cast<const bf16x8 *>(kb + qk_off + 64 * ks);
                 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, __builtin_bit_cast(bf16x8, qv[ks]), s, 0, 0, 0);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] = jst + 4 * lg + r < x.j1 ? score(s[r], jst + 4 * lg + r) : -INFINITY;
+            stage_scores(score, s, jst, end, lg, 0);
             xch[wave * 64 + lane] = s;
         }
         lds_barrier();  // every score written, every stage landed
@@ -380,15 +420,11 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, const Run &x, 
                 acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a8), pb[u / 2], acc[dt], 0, 0, 0);
             }
         lds_barrier();  // every wave is done with the slot and the scores
+        end = next_end;
         ahead = i + 2 < groups && dma(i + 2);
     }
 
-    if (append && x.j1 == x.nvis && wave == 0)  // the new row into the cache, as in attend_run
-        for (int c = lane; c < D / 8; c += 64) {
-            *reinterpret_cast<u32x4 *>(x.k + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.k_new + 8 * c);
-            if constexpr (!SH)
-                *reinterpret_cast<u32x4 *>(x.v + (size_t) x.newrow * D + 8 * c) = *reinterpret_cast<const u32x4 *>(x.v_new + 8 * c);
-        }
+    x.appended(wave, lane);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (li < x.G)

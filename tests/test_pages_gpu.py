@@ -1,0 +1,361 @@
+"""GPU tests of the calls of esda_pages.h and esda_tree_commit against their model on lists
+(_pages_model.py): tables, references, lengths, what was left out, and every byte of the pools."""
+import random
+
+import pytest
+import torch
+
+from _pages_model import Model
+from apertura_amd.pages import PagedCache, pages_read, pages_write
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+DEV = "cuda"
+# (planes, kv heads, head_dim) of the pools of one cache
+POOLS = [[(1, 1, 128)], [(2, 3, 256)], [(3, 1, 512), (1, 5, 128)], [(2, 2, 128), (2, 1, 256), (1, 1, 512)]]
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _make(pools, N, R, order=(0, 1, 2)):
+    """Pools whose element values name their row, head and plane: bytes 0 .. 65535 as bf16 patterns, every row
+    another.  order: of planes, pages and heads in memory."""
+    made = []
+    for planes, heads, D in pools:
+        size = (planes, N, heads)
+        t = torch.randint(0, 2 ** 15, [size[i] for i in order] + [R, D], dtype=torch.int16, device=DEV)
+        back = [order.index(i) for i in range(3)] + [3, 4]
+        made.append(t.permute(back).view(BF) if order == (0, 1, 2) else t.view(BF).permute(back))
+    return made
+
+
+class Both:
+    """A cache and its model."""
+
+    def __init__(self, pools, N, R, S, most, order=(0, 1, 2), spread=0.0, seed=0):
+        self.rng = random.Random(seed)
+        torch.manual_seed(seed)
+        self.pools = _make(pools, N, R, order)
+        self.first = [p.clone() for p in self.pools]
+        self.R, self.N = R, N
+        self.table = torch.full((S, most + 2), -1, dtype=torch.int32, device=DEV)[:, :most]
+        self.cache = PagedCache(self.pools, self.table, torch.zeros(S, dtype=torch.int32, device=DEV))
+        rows = {(p, r): (p, r) for p in range(N) for r in range(R)}
+        self.model = Model(self.table.tolist(), [0] * N, [0] * S, R, rows)
+
+    def set_length(self, lengths):
+        self.cache.length.copy_(_ints(lengths))
+        self.model.length = list(lengths)
+
+    def call(self, name, *lists):
+        getattr(self.cache, name)(*[None if x is None else _ints(x) for x in lists])
+        getattr(self.model, name)(*lists)
+
+    def check(self):
+        torch.cuda.synchronize()
+        m = self.model
+        assert self.cache.table.tolist() == m.table
+        assert self.cache.refs.tolist() == m.refs
+        assert self.cache.length.tolist() == m.length
+        assert self.cache.left_out() == m.left_out
+        m.left_out = 0
+        at = torch.tensor([m.rows[p, r] for p in range(self.N) for r in range(self.R)], device=DEV)
+        for pool, first in zip(self.pools, self.first):
+            want = first[:, at[:, 0], :, at[:, 1]].view(self.N, self.R, *pool.shape[0:1], *pool.shape[2:3], pool.shape[4])
+            assert torch.equal(pool.contiguous().view(torch.int16), want.permute(2, 0, 3, 1, 4).contiguous().view(torch.int16))
+
+
+def _filled(pools, N, R, S, most, lengths, **kw):
+    b = Both(pools, N, R, S, most, **kw)
+    b.call("reserve", list(range(len(lengths))), lengths)
+    b.set_length(lengths + [0] * (S - len(lengths)))
+    b.check()
+    return b
+
+
+@pytest.mark.parametrize("pools", POOLS)
+@pytest.mark.parametrize("R", [16, 64])
+def test_reserve_and_free(pools, R):
+    b = Both(pools, 40, R, 6, 12)
+    b.call("reserve", [0, 2, 5], [1, 3 * R, R + 1])
+    b.check()
+    b.set_length([1, 0, 2 * R, 0, 0, R])
+    b.call("reserve", [2, 0, 5, 3], [3 * R + 1, R, 0, 12 * R])
+    b.check()
+    b.call("free", [2, 4, 0])
+    b.check()
+    b.call("reserve", [4, 0], [5 * R, 2])  # the lowest free pages again
+    b.check()
+
+
+def test_reserve_leaves_out_what_it_cannot_do():
+    b = Both(POOLS[0], 10, 16, 5, 8)
+    b.call("reserve", [0, 7, -1, 0, 1], [40, 16, 16, 96, 8 * 16 + 1])  # outside, outside, twice, too many rows
+    b.check()
+    b.set_length([10, 0, 0, -5, 0])
+    b.call("reserve", [3, 2, 1, 4, 0], [16, 16 * 5, 16 * 3, 16, 30])  # a bad length; 5 pages, then 3 of 2 left; none for 4; 0 has its
+    b.check()
+    b.call("reserve", [], [])
+    b.check()
+
+
+@pytest.mark.parametrize("pools", POOLS)
+def test_free_twice_and_outside(pools):
+    b = _filled(pools, 12, 16, 4, 6, [33, 0, 17, 5])
+    b.call("free", [2, 2, 9, -3, 0])
+    b.check()
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (1, 0, 2), (1, 2, 0), (2, 1, 0)])
+@pytest.mark.parametrize("pools", POOLS)
+@pytest.mark.parametrize("R", [16, 128])
+def test_fork(pools, R, order):
+    b = _filled(pools, 40, R, 9, 8, [3 * R + 5, 2 * R, 0, R - 1], order=order)
+    b.call("fork", [0, 1, 2, 3, 0], [4, 5, 6, 7, 8], None)
+    b.check()
+    b.call("fork", [0, 0, 1], [4, 5, 6], [2 * R + 1, R, 2 ** 31 - 1])  # over forks; rows of a full page, no row of the last
+    b.check()
+    b.call("fork", [4, 0], [0, 4], None)  # a swap: both as they were before
+    b.check()
+    b.call("fork", [3, 3, 3], [3, 1, 2], None)  # a sequence that goes on, and its copies
+    b.check()
+    b.call("free", [0, 3])
+    b.call("reserve", [1, 2, 5], [R + 1, R, 2 * R + 1])
+    b.check()
+
+
+@pytest.mark.parametrize("R", [16, 32])
+def test_cuts(R):
+    b = _filled(POOLS[1], 20, R, 5, 6, [4 * R + 3, 3 * R])
+    b.call("reserve", [0], [6 * R])
+    b.check()
+    b.call("fork", [0], [0], [4 * R + 1])  # within its own last page, which stays; the pages behind it go
+    b.check()
+    b.call("fork", [0], [2], [3 * R])
+    b.call("fork", [0], [0], [2 * R + 3])  # within a page that it shares: a page of its own
+    b.check()
+    b.call("fork", [1], [1], [R + 1])      # within a page that nobody else holds, which stays
+    b.check()
+    b.call("fork", [1, 1], [1, 3], [1, 1])  # the same, copied by another
+    b.check()
+    b.call("fork", [0, 2], [0, 2], [0, R])
+    b.check()
+
+
+def test_fork_leaves_out_what_it_cannot_do():
+    R = 16
+    b = _filled(POOLS[0], 6, R, 6, 5, [2 * R + 1, R])  # 4 of 6 pages
+    b.call("fork", [0, 9, -1, 0, 1, 1], [2, 3, 3, 2, 6, -1], None)  # dst twice, slots outside
+    b.check()
+    b.call("fork", [0, 0], [3, 4], None)  # one page left for two: the second is empty
+    b.check()
+    b.set_length(b.model.length[:5] + [3])  # rows that lie in no page
+    b.call("fork", [5, 0], [1, 3], [2, -1])
+    b.check()
+    b.set_length([-1] + b.model.length[1:])
+    b.call("fork", [0], [1], None)
+    b.check()
+
+
+@pytest.mark.parametrize("pools", POOLS)
+@pytest.mark.parametrize("N,S", [(60, 7), (5000, 40)])
+def test_compact(pools, N, S):
+    rng = random.Random(N)
+    lengths = [rng.randrange(0, 7 * 16) for _ in range(S)]
+    b = Both(pools, N, 16, S, 8, seed=1)
+    ids = rng.sample(range(N), N)
+    for s, n in enumerate(lengths):
+        for k in range((n + 15) // 16):
+            p = ids.pop()
+            b.table[s, k] = p
+            b.model.table[s][k] = p
+            b.model.refs[p] = 1
+    b.cache.refs.copy_(_ints(b.model.refs))
+    b.set_length(lengths)
+    b.call("fork", [0, 1], [2, 3], None)
+    b.check()
+    b.call("compact")
+    b.check()
+    b.call("compact")  # nothing left to move
+    b.check()
+    b.call("free", list(range(0, S, 2)))
+    b.call("compact")
+    b.check()
+
+
+def test_compact_of_none_and_all():
+    b = Both(POOLS[0], 8, 16, 4, 4)
+    b.call("compact")
+    b.check()
+    b.call("reserve", [0, 1], [64, 64])
+    b.call("compact")
+    b.check()
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (1, 2, 0)])
+@pytest.mark.parametrize("pools", POOLS)
+@pytest.mark.parametrize("R", [16, 64])
+def test_commit(pools, R, order):
+    S = 7
+    b = _filled(pools, 60, R, S, 8, [R - 3, 0, 5, 2 * R, 1, 9, 40], order=order)
+    b.call("reserve", list(range(S)), [n + 64 for n in b.model.length])
+    b.check()
+    accept = [[0, 1, 2, 3, 4], [0, 3, 4, 9, 63], [1, 2, 3, 4, 5], [5, 6, 7, 8, 9], [0, 1, 7, 8, 50], [2, 1, 0, 0, 0], [7, 8, 9, 99, -1]]
+    b.call("commit", accept, [5, 5, 4, 0, 3, 1, 3])
+    b.check()
+    b.call("commit", accept, [1, 2, 5, 1, 5, 0, 0])
+    b.check()
+
+
+def test_commit_leaves_out_what_it_cannot_do():
+    b = _filled(POOLS[1], 30, 16, 6, 4, [10, 10, 10, 10, 10, 10])
+    b.call("reserve", [0, 1, 2, 3, 4], [64] * 5)
+    # falling, twice the same, too many, negative count, negative node, no page
+    b.call("commit", [[3, 2], [2, 2], [0, 1], [0, 1], [-1, 3], [2, 9]], [2, 2, 3, -1, 2, 2])
+    b.check()
+    b.set_length([63, 64, 62, -1, 0, 0])
+    b.call("commit", [[0, 1], [0, 1], [0, 1], [0, 1], [64, 65], [0, 1]], [2, 1, 2, 1, 1, 0])
+    b.check()
+
+
+def test_commit_over_linear_caches():
+    from apertura_amd import _lib
+    import ctypes
+
+    B, cap = 3, 50
+    pool = torch.randint(0, 2 ** 15, (2, B, 3, cap, 128), dtype=torch.int16, device=DEV)
+    first = pool.clone()
+    length, ws = _ints([10, 44, 47]), torch.zeros(256, dtype=torch.uint8, device=DEV)
+    c = _lib.Pages(num_pages=B, page_rows=cap, slots=B, max_pages=1, length=length.data_ptr(), num_pools=1,
+                   workspace=ws.data_ptr(), workspace_bytes=256)
+    c.pools[0] = _lib.Pool(pool.data_ptr(), 2, 3, 128, 0, *pool.stride()[:3])
+    accept, count = _ints([[1, 4, 8], [0, 3, 5], [0, 1, 3]]), _ints([3, 3, 3])
+    _lib.check(_lib.lib().esda_tree_commit(ctypes.byref(c), accept.data_ptr(), 3, 3, count.data_ptr(), None))
+    torch.cuda.synchronize()
+    for b, n, path in ((0, 10, [1, 4, 8]), (1, 44, [0, 3, 5])):
+        for i, a in enumerate(path):
+            pool_want = first[:, b, :, n + a]
+            assert torch.equal(pool[:, b, :, n + i], pool_want)
+    assert torch.equal(pool[:, 2], first[:, 2])
+    assert length.tolist() == [13, 47, 47] and ws[:4].view(torch.int32).item() == 1
+
+
+@pytest.mark.parametrize("planes,hkv,D", [(1, 1, 128), (2, 3, 256), (1, 2, 512)])
+@pytest.mark.parametrize("R", [16, 64, 256])
+@pytest.mark.parametrize("n", [1, 15, 17, 300])
+def test_rows_in_and_out(planes, hkv, D, R, n):
+    B, most = 3, n // R + 4
+    pool = _make([(planes, hkv, D)], B * most, R, (1, 0, 2))[0]
+    table = torch.randperm(B * most, device=DEV).to(torch.int32).view(B, most)
+    starts = [0, R - 1, 2 * R - 16]
+    table[2, 0] = -1
+    table[1, (starts[1] + n - 1) // R] = B * most  # the last rows lie in no page
+    row0 = _ints(starts)
+    big = torch.randint(0, 2 ** 15, (planes, B, hkv, n + 3, D), dtype=torch.int16, device=DEV).view(BF)
+    rows = big[:, :, :, :n]
+    want = pool.clone()
+    back = torch.zeros_like(rows)
+    for b in range(B):
+        for i in range(n):
+            k = (starts[b] + i) // R
+            p = int(table[b, k])
+            if 0 <= p < B * most:
+                want[:, p, :, (starts[b] + i) % R] = rows[:, b, :, i]
+                back[:, b, :, i] = rows[:, b, :, i]
+    pages_write(pool, table, row0, rows)
+    assert torch.equal(pool.contiguous().view(torch.int16), want.contiguous().view(torch.int16))
+    out = torch.full_like(big, 3.0)
+    pages_read(pool, table, row0, n, out[:, :, :, :n])
+    assert torch.equal(out[:, :, :, :n].contiguous().view(torch.int16), back.contiguous().view(torch.int16))
+    assert bool((out[:, :, :, n:] == 3.0).all())
+
+
+def test_rows_before_the_first_and_behind_the_last_page():
+    pool = _make([(1, 2, 128)], 4, 16)[0]
+    table, row0 = _ints([[0, 1], [2, 3]]), _ints([-5, 20])
+    first = pool.clone()
+    rows = torch.randn((1, 2, 2, 20, 128), device=DEV).to(BF)
+    pages_write(pool, table, row0, rows)
+    first[0, 0, :, :15] = rows[0, 0, :, 5:]
+    first[0, 3, :, 4:] = rows[0, 1, :, :12]
+    assert torch.equal(pool.view(torch.int16), first.view(torch.int16))
+    out = pages_read(pool, table, row0, 20)
+    assert torch.equal(out[0, 0, :, 5:], rows[0, 0, :, 5:]) and torch.equal(out[0, 1, :, :12], rows[0, 1, :, :12])
+    assert not bool(out[0, 0, :, :5].any()) and not bool(out[0, 1, :, 12:].any())
+    assert pages_read(pool, table, row0, 0).shape == (1, 2, 2, 0, 128)
+
+
+def test_random_lives():
+    """Sequences come, grow, fork, are cut and end, with now and then a compaction."""
+    R, S, most, N = 16, 12, 6, 45
+    for seed in range(4):
+        b = Both(POOLS[seed % len(POOLS)], N, R, S, most, seed=seed)
+        rng = b.rng
+        for _ in range(25):
+            what = rng.choice(["grow", "grow", "fork", "cut", "free", "commit", "compact"])
+            slots = rng.sample(range(S), rng.randrange(1, 5))
+            m = b.model
+            if what == "grow":
+                rows = [min(most * R, m.length[s] + rng.randrange(1, 40)) for s in slots]
+                b.call("reserve", slots, rows)
+                grown = list(m.length)
+                for s, r in zip(slots, rows):
+                    if all(m.page(s, k) is not None for k in range((r + R - 1) // R)):
+                        grown[s] = max(grown[s], r)
+                b.set_length(grown)
+            elif what == "fork":
+                b.call("fork", [rng.randrange(S) for _ in slots], slots, rng.choice([None, [rng.randrange(0, 60) for _ in slots]]))
+            elif what == "cut":
+                b.call("fork", slots, slots, [rng.randrange(0, 90) for _ in slots])
+            elif what == "commit":
+                # (rows of pages that a slot does not own alone are not written: pages behind its rows are its own)
+                b.call("commit", [sorted(rng.sample(range(20), 4)) for _ in range(S)], [rng.choice([0, 0, 2, 4]) for _ in range(S)])
+            elif what == "free":
+                b.call("free", slots)
+            else:
+                b.call("compact")
+            b.check()
+            held = [0] * N
+            for s in range(S):
+                for p in b.model.held(s):
+                    held[p] += 1
+            assert held == b.model.refs
+
+
+def test_graph_replays():
+    R = 16
+    b = _filled(POOLS[2], 40, R, 8, 6, [2 * R + 5, R, 7])
+    src, dst = _ints([0, 0, 1]), _ints([3, 4, 5])
+    rows = _ints([40, 40, 40])
+    for lists in (("fork", [0, 0, 1], [3, 4, 5], None), ("reserve", [3, 4, 5], [40, 40, 40]), ("compact",)):
+        b.call(*lists)
+    b.check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.cache.fork(src, dst)
+        b.cache.reserve(dst, rows)
+        b.cache.compact()
+    for turn in range(3):
+        lists = [b.rng.randrange(3) for _ in range(3)]
+        src.copy_(_ints(lists))
+        graph.replay()
+        b.model.fork(lists, [3, 4, 5])
+        b.model.reserve([3, 4, 5], [40, 40, 40])
+        b.model.compact()
+        b.check()
+        b.call("free", [6])
+
+
+def test_a_stream_of_its_own():
+    b = _filled(POOLS[1], 20, 16, 4, 4, [20, 33])
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b.cache.fork(_ints([0]), _ints([2]), stream=st)
+    b.cache.reserve(_ints([2]), _ints([40]), stream=st)
+    b.cache.compact(stream=st)
+    b.model.fork([0], [2])
+    b.model.reserve([2], [40])
+    b.model.compact()
+    b.check()
