@@ -30,6 +30,7 @@ SOURCES = [
     "esda_prefix_tiles.hip",
     "esda_pages.hip",
     "esda_tree.hip",
+    "esda_tree_tiles.hip",
     "es/ESKVCache.cpp",
     "es/ESDecodeAttn.cpp",
     "es/ESSnapshot.cpp",
@@ -49,7 +50,7 @@ HIP_FLAGS = [
 # keeps them overlapped in every copy.  (esda_prefix_tiles.hip: the register allocator crashes on its
 # 512-dim kernel after that strategy.)
 SCHED_FLAGS = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
-DEFAULT_SCHED = {"esda_prefix_tiles.hip"}
+DEFAULT_SCHED = {"esda_prefix_tiles.hip", "esda_tree_tiles.hip"}
 
 # Per-source additions.  The raw-K ring kernel multiplies each row by diag(kw) with MFMAs whose
 # results feed VALU work; the default heuristic gives every MFMA of a kernel that uses the

@@ -1,7 +1,8 @@
 // esda_prefill_kernel.h -- the prefill attention kernel, its split merge and their launch
 // (gfx950), for the sources that build entry points on them: esda_prefill.hip (causal and sliding
 // masks), esda_scored_prefill.hip (capped and biased scores, document and prefix masks) and
-// esda_prefix_tiles.hip (the rows of a decode batch over its shared prefix).  What the kernel does
+// esda_prefix_tiles.hip (the rows of a decode batch over its shared prefix), esda_tree_tiles.hip (steps of
+// many drafted tokens).  What the kernel does
 // is described at the head of esda_prefill.hip.
 #pragma once
 
@@ -17,6 +18,7 @@
 #include "esda_plan.h"
 #include "esda_prefill_plan.h"
 #include "esda_stream.h"
+#include "esda_tree_rows.h"
 
 namespace {
 
@@ -194,6 +196,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     constexpr bool SCORED = std::is_base_of<ScoredParams, P>::value;
     constexpr bool WIDE = std::is_same<P, WideScoredParams>::value || std::is_same<P, WideDocParams>::value;
     constexpr bool PARTS = std::is_same<P, PrefixParams>::value;  // a partial from every split, also one
+    constexpr bool TREE = std::is_same<P, TreeParams>::value;
+    constexpr bool ODD = SCORED || TREE;  // rows whose O^T is not finite are done again
     static_assert(!S2 || !KH, "two stages per iteration: all waves on both");
     static_assert(!PS || (QB == 1 && !KH), "pair split: one block per wave, every wave on every stage");
     constexpr int NQW = KH ? NW / 2 : NW;  // waves with distinct query blocks
@@ -222,7 +226,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     // of each 64 stages, which to compute and which of them without a mask; those past the last
     // of kDocWindows (131,072 keys of a split) are computed with one
     constexpr int kDocWindows = 64;
-    __shared__ unsigned char odd_row[SCORED ? QT : 1];  // tile rows whose O^T is not finite
+    __shared__ unsigned long long paths[TREE ? 64 : 1];  // the nodes'
+    __shared__ unsigned char odd_row[ODD ? QT : 1];  // tile rows whose O^T is not finite
     __shared__ int any_odd;
     // the tile rows' positions, slopes (log2 units) and documents, read where a stage needs them:
     // held in registers they cost the stages reloads of spilled ones, whose waits wait for the DMAs
@@ -231,7 +236,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     __shared__ unsigned long long live_of[DOCS ? kDocWindows : 1], pure_of[DOCS ? kDocWindows : 1];
 
     // (scored: said to be scalar, which frees the registers that the score's form needs)
-    const int lane = threadIdx.x & 63, wave = SCORED ? uniform(threadIdx.x >> 6) : threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = ODD ? uniform(threadIdx.x >> 6) : threadIdx.x >> 6;
     const int li = lane & 15, lg = lane >> 4;
     // Query-block wave and stage parity (both constant for the plain kernel, whose code
     // does not change: a wave-dependent parity there measured 3% slower).
@@ -241,16 +246,42 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     // (dispatch is round-robin over the 8), so the (kv head, split) pair is the fastest
     // index and the workgroups on one XCD share one K / V stream in its L2; tiles run
     // heaviest (latest) first.
-    const int combos = p.Hkv * p.splits;
+    // (TREE: a sequence's splits side by side, too.)
+    int combos = p.Hkv * p.splits;
+    if constexpr (TREE) combos *= p.B;
     const int wg = (int) blockIdx.x;
     const int tile = p.tiles - 1 - wg / combos;
-    const int kvh = (wg % combos) % p.Hkv, split = (wg % combos) / p.Hkv;
-    const long long nrows = (long long) p.Sq * p.Hq;
+    const int kvh = (wg % combos) % p.Hkv;
+    int split = (wg % combos) / p.Hkv, seq = 0;
+    if constexpr (TREE) {
+        seq = split / p.splits;
+        split -= seq * p.splits;
+    }
+    long long nrows = (long long) p.Sq * p.Hq, row0 = 0;  // row0: the sequence's first, of q, out and partials
+    if constexpr (TREE) {
+        row0 = seq * nrows;
+        nrows *= p.B;
+    }
+    const uint16_t *const qb0 = TREE ? p.q + row0 * D : p.q;
+    uint16_t *const out0 = TREE ? p.out + row0 * D : p.out;
 
-    int tj0, tj1;
-    tile_keys(p, tile, QT, tj0, tj1);
-    const int j0 = min(tj1, tj0 + split * p.kps);
-    const int j1 = min(tj1, j0 + p.kps);
+    int j0, j1;
+    TreeView tv{};
+    unsigned long long path = 0ull;
+    if constexpr (TREE) {
+        tv = tree_view(p, seq, lane, path);
+        if (kvh == 0 && split == 0 && tile == 0 && threadIdx.x == 0) {
+            p.views[seq] = tv.ok ? tv.total : -1;
+            if (!tv.ok) __hip_atomic_fetch_add(p.status, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (!tv.ok) return;
+        if (!esda_plan::grid_split(split, p.splits, p.kps, tv.total, &j0, &j1)) j1 = j0;
+    } else {
+        int tj0, tj1;
+        tile_keys(p, tile, QT, tj0, tj1);
+        j0 = min(tj1, tj0 + split * p.kps);
+        j1 = min(tj1, j0 + p.kps);
+    }
 
     // This lane's query row in block qb: tile row wq*16*QB + 16qb + li, global row gr
     // (position gr / G, head kvh*G + gr % G); rows past the end repeat the last row and
@@ -263,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     auto qvalid = [&](int qb) { return (long long) tile * QT + wq * 16 * QB + qb * 16 + li < nq; };
 
     if (j0 >= j1) {  // an empty split: no keys for this tile; the merge skips it
-        if (p.splits > 1 && lg == 0 && kh == 0) {
+        if (!TREE && p.splits > 1 && lg == 0 && kh == 0) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
                 if (qvalid(qb)) {
@@ -274,13 +305,13 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                         f32x2{-INFINITY, 0.0f};
                 }
         }
-        if constexpr (SCORED) {  // unsplit: a tile whose rows see nothing is 0
+        if constexpr (ODD) {  // unsplit: a tile whose rows see nothing is 0
             if (p.splits == 1) {
                 for (int r = wave; r < QT; r += NW) {
                     const long long gr = (long long) tile * QT + r;
                     if (gr >= nq) break;
                     const unsigned qi = position_of(gr, p.G);
-                    uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.o_hs;
+                    uint16_t *o = out0 + (size_t) qi * p.o_rs + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.o_hs;
                     for (int d = 4 * lane; d < D; d += 256) *reinterpret_cast<u32x2 *>(o + d) = u32x2{0u, 0u};
                 }
             }
@@ -295,9 +326,9 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     for (int qb = 0; qb < QB; ++qb) {
         const long long gr = qrow(qb);
         const unsigned qi = position_of(gr, p.G);
-        const uint16_t *qr = p.q + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.q_hs +
+        const uint16_t *qr = qb0 + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.q_hs +
                              (size_t) qi * p.q_rs + lg * 8;
-        if constexpr (!SCORED) qabs[qb] = p.q_pos0 + (int) qi;
+        if constexpr (!ODD) qabs[qb] = p.q_pos0 + (int) qi;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 w = qvalid(qb) ? *reinterpret_cast<const u32x4 *>(qr + ks * 32) : u32x4{0u, 0u, 0u, 0u};
@@ -332,8 +363,38 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     static_assert((NSL & (NSL - 1)) == 0, "stage slots: a power of two");
     auto kslot = [&](int s) { return ring + (s & (NSL - 1)) * 2 * R::HB; };
     auto vslot = [&](int s) { return SH ? kslot(s) : ring + 2 * NSL * R::HB + (s & (NSL - 1)) * 2 * R::HB; };
+    // TREE: this wave's DMAs fill one half of a stage, 16 rows of one page
+    struct None {};
+    std::conditional_t<TREE, TreeRows<D, SH>, None> tr = [&] {
+        if constexpr (TREE) {
+            TreeRows<D, SH> x(p, tv, seq, kvh);
+            x.j0 = j0;
+            x.j1 = j1;
+            return x;
+        } else {
+            return None{};
+        }
+    }();
     auto issue = [&](const uint16_t *head, int s, unsigned char *slot) {
         const int jb = j0 + s * kStageKeys;
+        if constexpr (TREE) {
+            const int half = 16 * (wave / (NW / 2));
+            typename TreeRows<D, SH>::Stage rows;
+            if (tr.dense(jb + half, rows)) {
+                const uint16_t *base = (head == vvb && !SH ? rows.v : rows.k) - half * D;
+#pragma unroll
+                for (int t = 0; t < KPW; ++t) lds_dma16_s<kStreamNT>(base, voff[t], lds_addr(slot) + ldso[t]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < KPW; ++t) {
+                    const uint16_t *kr, *vr;
+                    tr.row(min(jb + vrow[t], j1 - 1), kr, vr);  // rows past the range repeat the last node's
+                    if constexpr (!SH) kr = head == vvb ? vr : kr;
+                    lds_dma16<kStreamNT>(kr + (lane % R::CPR) * 8, lds_addr(slot) + ldso[t]);
+                }
+            }
+            return;
+        }
         if (jb + kStageKeys <= j1) {
             const uint16_t *base = head + (size_t) jb * D;
 #pragma unroll
@@ -347,6 +408,20 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         }
     };
 
+    bool holes = false;  // TREE: some committed row among the keys lies in no page
+    int all_see = 0;     // .. and committed rows from it on are seen by every node
+    if constexpr (TREE) {
+        if (wave == 0) paths[lane] = path;
+        for (int r = threadIdx.x; r < QT; r += 64 * NW) odd_row[r] = 0;
+        if (threadIdx.x == 0) any_odd = 0;
+        if (!p.linear) {
+            const int k0 = (tv.first + j0) >> p.shift, k1 = (min(tv.len, tv.first + j1) - 1) >> p.shift;  // (k1 < k0: none)
+            for (int k = k0 + lane; k <= k1; k += 64) holes = holes || !tree_page(p, tr.table[k]);
+            holes = __builtin_amdgcn_ballot_w64(holes) != 0ull;
+        }
+        if (p.window > 0) all_see = tv.len + p.Sq - p.window;
+        lds_barrier();
+    }
     if constexpr (SCORED) {
         for (int r = threadIdx.x; r < QT; r += 64 * NW) {
             const long long gr = min((long long) tile * QT + r, nq - 1);
@@ -391,8 +466,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         if (lane < 2) *(lds_flag *) (xch + lane * XPAR + NW * XP + wave * 4) = 0u;
     }
     // Positions of the tile's first and last rows (the host keeps positions below 2^31).
-    const int qa_min = p.q_pos0 + (int) position_of((long long) tile * QT, p.G);
-    const int qa_max = p.q_pos0 +
+    const int qa_min = TREE ? 0 : p.q_pos0 + (int) position_of((long long) tile * QT, p.G);
+    const int qa_max = TREE ? 0 : p.q_pos0 +
                        (int) position_of(((long long) tile * QT + QT < nq ? (long long) tile * QT + QT : nq) - 1, p.G);
 
     // S^T[keys x queries] of a stage: s[h][qb] covers keys 16h + 4lg + r of query column li.
@@ -626,7 +701,9 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sv[qb][4 * h + r] = cur.s[h][qb][r];
         const int ka_first = p.k_pos0 + jb, ka_last = ka_first + kStageKeys - 1;
-        const bool full = SCORED ? scored_full(jb, ka_first, ka_last, pure)
+        const int krow = tv.first + jb;  // TREE: the stage's first row
+        const bool full = TREE     ? jb + kStageKeys <= j1 && krow + kStageKeys <= tv.len && krow >= all_see && !holes
+                          : SCORED ? scored_full(jb, ka_first, ka_last, pure)
                                  : jb + kStageKeys <= j1 && ka_last <= qa_min &&
                                        (p.window == 0 || ka_first > qa_max - p.window);
         if constexpr (SCORED) {
@@ -672,7 +749,28 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                 c2 = 1.0f;
             }
         }
-        if (!full) {
+        if constexpr (TREE) {
+            if (!full) {
+                bool held[2] = {true, true};  // the halves' pages
+                if (holes)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (krow + 16 * h < tv.len) held[h] = tr.page_of((krow + 16 * h) >> p.shift) >= 0;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    const unsigned long long sees = paths[position_of(qrow(qb), p.G)];
+                    const int lowest = p.window > 0 ? tv.len + __popcll(sees) - p.window : 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int j = jb + 16 * h + 4 * lg + r, row = tv.first + j;
+                            const bool seen = row < tv.len ? row >= lowest && held[h] : ((sees >> ((row - tv.len) & 63)) & 1) != 0;
+                            if (!(j < j1 && seen)) sv[qb][4 * h + r] = -INFINITY;
+                        }
+                }
+            }
+        } else if (!full) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 const int qa = SCORED ? row_pos[SCORED ? wq * 16 * QB + qb * 16 + li : 0] : qabs[qb];
@@ -832,10 +930,10 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
             }
         }
         lds_barrier();
-        if (!SCORED && kh) return;
+        if (!ODD && kh) return;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            if (SCORED && kh) break;
+            if (ODD && kh) break;
             const f32x2 mlb = *reinterpret_cast<const f32x2 *>(xb + XA + (qb * 64 + lane) * 8);
             const float M = fmaxf(m[qb], mlb[0]);
             const float wa = m[qb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[qb] - M);
@@ -868,8 +966,16 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         // the block's first tile row (PS: the wave's own block, then its partner's)
         const int br = PS ? (nb == 0 ? wave : wave ^ 1) * 16 : wq * 16 * QB + nb * 16;
         const long long gr0 = (long long) tile * QT + br + li;
-        if (gr0 >= nq || (SCORED && KH && kh)) continue;
-        if constexpr (SCORED) {
+        if (gr0 >= nq || (ODD && KH && kh)) continue;
+        if constexpr (TREE) {
+            if (paths[position_of(gr0, p.G)] == 0ull) {  // no node: nothing seen
+                lb[nb] = 0.0f;
+                if (nb < QB) l[nb < QB ? nb : 0] = 0.0f;
+#pragma unroll
+                for (int dt = 0; dt < DW; ++dt) acc[nb][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        if constexpr (ODD) {
             float c = 0.0f;  // NaN where a value is not finite
 #pragma unroll
             for (int dt = 0; dt < DW; ++dt)
@@ -882,12 +988,12 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         }
         const long long gr = gr0;
         const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
-        const long long row = (long long) qi * p.Hq + qh;
+        const long long row = row0 + (long long) qi * p.Hq + qh;
         const int d0 = 16 * DW * hd;  // the wave's first O^T dim
         if (!PARTS && p.splits == 1) {
             float inv = 1.0f / lb[nb];
-            if constexpr (SCORED) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
-            uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
+            if constexpr (ODD) inv = lb[nb] == 0.0f ? 0.0f : inv;  // a row that sees nothing
+            uint16_t *o = out0 + (size_t) qi * p.o_rs + (size_t) qh * p.o_hs + d0 + 4 * lg;
 #pragma unroll
             for (int dt = 0; dt < DW; ++dt) {
                 const f32x4 v4 = acc[nb][dt] * inv;
@@ -908,6 +1014,23 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
             }
             if (lg == 0 && nb < QB)  // (m, l) from the block's owner
                 *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{m[nb < QB ? nb : 0], l[nb < QB ? nb : 0]};
+        }
+    }
+    if constexpr (TREE) {
+        if (tile == 0) append_nodes<D, SH>(tr, paths, j0, j1);
+        ESDA_WAIT_VM(0);  // the rows as written above, before they are written again
+        lds_barrier();
+        if (__builtin_expect(any_odd != 0, 0)) {
+            for (int r = wave; r < QT; r += NW) {
+                if (!odd_row[r]) continue;
+                const long long gr = (long long) tile * QT + r;
+                const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
+                const long long row = row0 + (long long) qi * p.Hq + qh;
+                tree_row_again<D, SH>(tr, p.q + row * D, paths[qi], p.window > 0 ? tv.len + __popcll(paths[qi]) - p.window : 0, j0, j1,
+                                      p.scale_log2e, [&](float mr, float lr, const float(&o)[D / 64]) {
+                                          tree_row_store<D>(p, split, row, lane, mr, lr, o);
+                                      });
+            }
         }
     }
     if constexpr (SCORED) {
@@ -1133,6 +1256,7 @@ void launch_tiles(const P &p, hipStream_t st) {
     const int nw = one ? (shared ? 4 : 8) : p.nw;
     unsigned groups = p.tiles * p.Hkv * p.splits;
     if constexpr (std::is_same<P, PrefixParams>::value) groups += p.own_groups;
+    if constexpr (std::is_same<P, TreeParams>::value) groups *= p.B;
     const dim3 grid(groups), block(64 * nw);
     if constexpr (D == 512) {
         if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);
@@ -1140,16 +1264,23 @@ void launch_tiles(const P &p, hipStream_t st) {
         else if (shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, kWaves, P>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((prefill_kernel<512, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
     }
-    else if constexpr (D == 128 && std::is_base_of<ScoredParams, P>::value)
+    else if constexpr (D == 128 && (std::is_base_of<ScoredParams, P>::value || std::is_same<P, TreeParams>::value))
         hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, 4, P>), grid, block, 0, st, p);
     else if constexpr (D == 128)
         hipLaunchKernelGGL((prefill_kernel<128, 2, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
-    else if (p.qb == 2)
-        hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true, false, kWaves, P>), grid, block, 0, st, p);
-    else if (p.kh)
-        hipLaunchKernelGGL((prefill_kernel<256, 1, true, false, false, false, kWaves, P>), grid, block, 0, st, p);
-    else
-        hipLaunchKernelGGL((prefill_kernel<256, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
+    else {
+        // (a tree's rows of a kv head fill few tiles of 256, whose kernel would spill registers there)
+        if constexpr (!std::is_same<P, TreeParams>::value) {
+            if (p.qb == 2) {
+                hipLaunchKernelGGL((prefill_kernel<256, 2, false, false, true, false, kWaves, P>), grid, block, 0, st, p);
+                return;
+            }
+        }
+        if (p.kh)
+            hipLaunchKernelGGL((prefill_kernel<256, 1, true, false, false, false, kWaves, P>), grid, block, 0, st, p);
+        else
+            hipLaunchKernelGGL((prefill_kernel<256, 1, false, false, false, false, kWaves, P>), grid, block, 0, st, p);
+    }
 }
 
 template <int D, class P = PrefillParams>

@@ -104,8 +104,8 @@ struct PrefixParams : PrefillParams {
 // `splits`, of which those hold keys that its length reaches.
 struct TreeParams : PrefillParams {
     int B;
-    int run_rows;     // > 0: in runs (esda_tree.hip), 16 * this many query rows a workgroup
-    int row_groups;   // .. workgroups of the same keys
+    int run_groups;   // > 0: in runs (esda_tree.hip), 16 * this many query rows a workgroup (else in tiles)
+    int row_groups;   // workgroups of the same keys
     int N, P, shift;  // pages, entries of a sequence's table, log2 of a page's rows
     int linear, cap;  // linear: sequence b in page b, rows below cap
     long long page_stride, table_stride;

@@ -18,6 +18,7 @@
 #include "esda_prefill_kernel.h"
 #include "esda_tree.h"
 #include "esda_tree_rows.h"
+#include "esda_tree_tiles.h"
 
 namespace {
 
@@ -115,18 +116,7 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
             const unsigned long long mine = paths[(r0 + h) / p.G];
             tree_row_again<D, SH>(x, p.q + at(r0 + h) * D, mine, p.window > 0 ? w.len + __popcll(mine) - p.window : 0, x.j0, x.j1,
                                   p.scale_log2e, [&](float m, float l, const float(&o)[D / 64]) {
-                                      constexpr int DPL = D / 64;
-                                      const size_t row = at(r0 + h);
-                                      if (p.splits == 1) {
-                                          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-                                          for (int e = 0; e < DPL; ++e)
-                                              p.out[row * D + lane * DPL + e] = __builtin_bit_cast(uint16_t, (__bf16) (o[e] * inv));
-                                      } else {
-#pragma unroll
-                                          for (int e = 0; e < DPL; ++e) p.part_acc[(part + row) * D + lane * DPL + e] = o[e];
-                                          if (lane == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * (part + row)) = f32x2{m, l};
-                                      }
+                                      tree_row_store<D>(p, split, at(r0 + h), lane, m, l, o);
                                   });
         }
     }
@@ -192,6 +182,84 @@ const char *check_desc(const esda_tree_desc *d) {
     return nullptr;
 }
 
+// How the query rows of a kv head can be laid out: as tiles (nw > 0: a prefill form), or in runs of 16 ng
+// rows.  us of a workgroup: `start`, and `per_kb` per KB of K and V; slots: workgroups the GPU holds at once.
+struct Form {
+    int qb, kh, nw, ng;
+    float start, per_kb;
+    int slots;
+    int rows() const { return ng ? 16 * ng : 16 * qb * (kh ? nw / 2 : nw); }
+};
+
+// The forms a step of `rows` query rows a kv head may take; returns their number.
+int forms_of(int D, int rows, bool shared, Form *f) {
+    int n = 0;
+    const float stage_kb = 32.0f * 2 * D * (shared ? 1 : 2) / 1024;
+    auto tile = [&](const Tiling &t, float more, float times) {
+        f[n++] = {t.qb, t.kh, t.nw, 0, t.wg + t.row * std::min(rows, t.rows()) + more, t.stage / stage_kb * times, 256 * t.occ};
+    };
+    if (D == 512) {
+        if (rows > 64 || shared == false) tile(kTilings512[0], 1.8f, 1.02f);
+        if (rows > 64 || shared) tile(kTilings512[1], 0.0f, 0.96f);  // (launch_tiles' choice for one tile)
+        f[n++] = {0, 0, 0, 1, 8.0f, 1 / 54.0f, 256};
+    } else if (D == 256) {
+        tile(kTilings256[1], -0.7f, 1.47f);
+        tile(kTilings256[2], -1.0f, 1.63f);
+        f[n++] = {0, 0, 0, 1, 4.6f, 1 / 65.0f, 256};
+    } else {
+        tile(kTilings128Scored[0], 0.0f, 1.6f);
+        f[n++] = {0, 0, 0, 1, 5.8f, 1 / 65.0f, 512};
+        if (rows > 16) f[n++] = {0, 0, 0, 2, 13.2f, 1 / 56.0f, 512};
+        if (rows > 32) f[n++] = {0, 0, 0, 4, 13.1f, 1 / 32.0f, 256};
+    }
+    return n;
+}
+
+// Form and splits of a step over at most `most` keys a sequence: the cheapest by the workgroups' time on
+// the GPU, the bytes, and the merge of the partials.
+void choose(const esda_tree_desc *d, long long most, TreeParams *p) {
+    const int D = d->head_dim, rows = p->Sq * p->G;
+    const bool shared = d->kv_shared != 0;
+    const float row_kb = 2.0f * D * (shared ? 1 : 2) / 1024;
+    const long long pairs = (long long) p->B * p->Hkv, out_rows = (long long) p->B * p->Sq * p->Hq;
+    const float floor_us = 4.0f + (float) (most * pairs) * row_kb / 5600.0f;
+    Form f[4];
+    const int nf = forms_of(D, rows, shared, f);
+    float best = INFINITY;
+    auto consider = [&](const Form &form, long long keys) {
+        const long long splits = (most + keys - 1) / keys, tiles = (rows + form.rows() - 1) / form.rows();
+        const long long groups = pairs * tiles * splits;
+        const float us = form.start + (float) std::min(keys, most) * row_kb * form.per_kb;
+        float span = std::max(us, (float) groups / form.slots * us);
+        if (groups > form.slots) span += 0.5f * us;
+        const float cost = std::max(span, floor_us) + 0.13f * std::min(span, floor_us) +
+                           (splits == 1 ? 0.0f : splits <= 8 ? 4.3f : 4.8f) + (splits > 1 ? 2.6e-7f * 4 * D * out_rows * splits : 0.0f);
+        if (cost >= best) return;
+        best = cost;
+        p->qb = form.qb;
+        p->kh = form.kh;
+        p->nw = form.nw;
+        p->run_groups = form.ng;
+        p->tiles = p->row_groups = (int) tiles;
+        p->splits = (int) std::max(1LL, splits);
+        p->kps = (int) keys;
+    };
+    for (int i = 0; i < nf; ++i) {
+        if (d->split_rows > 0) {  // (one longer than the keys is cut to them)
+            consider(f[i], std::min<long long>(d->split_rows, (most + kStageKeys - 1) / kStageKeys * kStageKeys));
+            continue;
+        }
+        long long last = 0;
+        for (int s = 1; s <= 512; s += std::max(1, s / 8)) {
+            const long long keys = std::max(64LL, ((most + s - 1) / s + kStageKeys - 1) / kStageKeys * kStageKeys);
+            if (keys != last) consider(f[i], keys);
+            if (keys == 64) break;
+            last = keys;
+        }
+    }
+    p->part_nt = 4.0f * D * out_rows * p->splits <= kPartNtBytes;
+}
+
 int fresh_plan(const esda_tree_desc *d, TreePlan *pl) {
     if (const char *why = check_desc(d)) return refuse(why);
     const int D = d->head_dim;
@@ -219,20 +287,9 @@ int fresh_plan(const esda_tree_desc *d, TreePlan *pl) {
     long long most = p.linear ? p.cap : (long long) d->max_pages * d->page_rows;
     if (d->max_visible > 0) most = std::min(most, (long long) d->max_visible + p.Sq);
     if (p.window > 0) most = std::min(most, (long long) p.window + p.Sq + kStageKeys);
-    const int rows = p.Sq * p.G;
-    const int ng = D == 128 ? (rows <= 16 ? 1 : rows <= 32 ? 2 : 4) : 1;
-    p.run_rows = ng;
-    p.row_groups = (rows + 16 * ng - 1) / (16 * ng);
+    choose(d, most, &p);
     const long long groups = (long long) p.B * p.Hkv * p.row_groups;
-    long long keys = std::min<long long>(d->split_rows, (most + kStageKeys - 1) / kStageKeys * kStageKeys);
-    if (d->split_rows == 0) {
-        const long long splits = std::max(1LL, (D == 128 ? 512 : 256) / groups);
-        keys = std::max(64LL, ((most + splits - 1) / splits + kStageKeys - 1) / kStageKeys * kStageKeys);
-    }
-    p.kps = (int) keys;
-    const long long splits = std::max(1LL, (most + keys - 1) / keys);
-    if (splits > 4096 || groups * splits >= INT_MAX / 512) return refuse("too many splits");
-    p.splits = (int) splits;
+    if (p.splits > 4096 || groups * p.splits >= INT_MAX / 512) return refuse("too many splits");
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t parts = p.splits > 1 ? (size_t) p.B * p.Sq * p.Hq * p.splits : 0;
     pl->off_views = 256;
@@ -265,6 +322,13 @@ int make_tree_plan(const esda_tree_desc *d, TreePlan *pl) {
 
 template <int D>
 hipError_t launch_step(const TreeParams &p, bool shared, hipStream_t st) {
+    if (!p.run_groups) {
+        esda_detail::tree_tiles(p, D, st);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.splits == 1) return e;
+        launch_parts_merge<D, TreeMergeRow>(p, p.splits, st);
+        return hipGetLastError();
+    }
     const unsigned units = (unsigned) (p.B * p.Hkv * p.splits);
     const dim3 grid((units + 7) / 8 * 8 * p.row_groups), block(256);
     auto run = [&](auto ng) {
@@ -272,10 +336,10 @@ hipError_t launch_step(const TreeParams &p, bool shared, hipStream_t st) {
         if (shared) hipLaunchKernelGGL((tree_run_kernel<D, true, NG>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((tree_run_kernel<D, false, NG>), grid, block, 0, st, p);
     };
-    if (p.run_rows == 1) run(std::integral_constant<int, 1>{});
+    if (p.run_groups == 1) run(std::integral_constant<int, 1>{});
     if constexpr (D == 128) {
-        if (p.run_rows == 2) run(std::integral_constant<int, 2>{});
-        if (p.run_rows == 4) run(std::integral_constant<int, 4>{});
+        if (p.run_groups == 2) run(std::integral_constant<int, 2>{});
+        if (p.run_groups == 4) run(std::integral_constant<int, 4>{});
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;

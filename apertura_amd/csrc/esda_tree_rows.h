@@ -25,7 +25,7 @@ __device__ __forceinline__ bool tree_page(const TreeParams &p, int id) { return 
 // A node's path doubles in length each round: what is above the node that is above it.
 __device__ __forceinline__ TreeView tree_view(const TreeParams &p, int b, int lane, unsigned long long &path) {
     TreeView v;
-    v.len = p.length[b];
+    v.len = uniform(p.length[b]);
     bool node = lane < p.Sq;
     path = node ? (2ull << lane) - 1 : 0ull;
     if (p.parent) {
@@ -82,8 +82,9 @@ struct TreeRows {
         P = p.P;
         shift = p.shift;
         page0 = p.linear ? b : 0;
-        G = j0 = j1 = ids = page = 0;
-        of = -1;
+        G = j0 = j1 = page = 0;
+        ids = page0;  // (linear: every row in entry 0)
+        of = p.linear ? 0 : -1;
     }
 
     struct Stage {
@@ -92,11 +93,11 @@ struct TreeRows {
     };
     // The page of entry n (the same in every lane), 64 entries a load; -1 where it is none.
     __device__ __forceinline__ int page_of(int n) {
-        if (!table) return page0;
-        if (n >> 6 != of) {
-            of = n >> 6;
-            const int i = (of << 6) + (int) (threadIdx.x & 63);
-            ids = i < P ? table[i] : -1;
+        const int block = uniform(n >> 6);
+        if (__builtin_expect(block != of, 0)) {
+            of = block;
+            const int i = (block << 6) + (int) (threadIdx.x & 63);
+            ids = table[min(i, P - 1)];  // (entries past the last are not asked for)
             if ((unsigned) ids >= (unsigned) N) ids = -1;
         }
         return __builtin_amdgcn_readlane(ids, n & 63);
@@ -211,6 +212,23 @@ __device__ __forceinline__ void tree_row_again(const TreeRows<D, SH> &x, const u
         }
     }
     store(m, l, o);
+}
+
+// .. and its place in out or among the partials.
+template <int D>
+__device__ __forceinline__ void tree_row_store(const TreeParams &p, int split, long long row, int lane, float m, float l,
+                                               const float (&o)[D / 64]) {
+    constexpr int DPL = D / 64;
+    if (p.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) p.out[row * D + lane * DPL + e] = __builtin_bit_cast(uint16_t, (__bf16) (o[e] * inv));
+        return;
+    }
+    const long long at = (long long) split * p.B * p.Sq * p.Hq + row;
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) p.part_acc[at * D + lane * DPL + e] = o[e];
+    if (lane == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * at) = f32x2{m, l};
 }
 
 }  // namespace
