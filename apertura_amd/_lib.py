@@ -236,8 +236,7 @@ class TreeDesc(ctypes.Structure):
         ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("kv_shared", ctypes.c_int32),
         ("window", ctypes.c_int32), ("num_pages", ctypes.c_int32), ("page_rows", ctypes.c_int32),
         ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
-        ("head_stride", ctypes.c_int64), ("max_visible", ctypes.c_int32), ("split_rows", ctypes.c_int32),
-        ("scale", ctypes.c_float), ("pad", ctypes.c_int32),
+        ("head_stride", ctypes.c_int64), ("split_rows", ctypes.c_int32), ("scale", ctypes.c_float),
     ]
 
 

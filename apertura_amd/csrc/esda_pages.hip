@@ -47,7 +47,7 @@ struct Entry {
 };
 
 struct Header {
-    int left_out, ticket, moves, live;
+    int left_out, moves, live;  // 256 bytes, then a ticket of each slot
 };
 
 struct Params {
@@ -299,7 +299,8 @@ __global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, con
     }
 }
 
-// .. second launch, one workgroup: a free page for every entry that copies.
+// .. second launch, one workgroup: a free page for every entry that copies.  (As the work of the first
+// launch's last workgroup, behind fences for what the others wrote, a fork of 4 took 5 us more, of 32 10.)
 __global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) {
     __shared__ int ids[ESDA_MAX_ENTRIES];
     const int t = threadIdx.x;
@@ -449,6 +450,11 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsParams p) {
 
 // ---- accepted rows
 
+constexpr int kCommitParts = 2;  // times 256 lanes of rows a workgroup
+__host__ __device__ inline unsigned commit_groups(const Pool &o) {
+    return (unsigned) (((long long) o.planes * o.heads * (o.D / 8) + 256 * kCommitParts - 1) / (256 * kCommitParts));
+}
+
 struct CommitParams {
     int N, shift, S, P, cap, linear;  // linear: slot s in page s, rows below cap
     long long table_stride, accept_stride;
@@ -488,16 +494,18 @@ __device__ __forceinline__ bool accepted(const CommitParams &p, int s, int lane,
 
 // Groups of D / 8 lanes, each a (plane, kv head) of one slot: they take the moved rows in order, eight
 // at a time.  The rows rise, so that a row is written after it was read: row i becomes accept[i] >= i,
-// and what is read later lies above accept[i].  The workgroup that is the last to have read its slot's
-// list moves the lengths on.  Bound by the latency of the list, its pages and the rows.
+// and what is read later lies above accept[i].  Of a slot's workgroups the last to have read its list
+// moves its length on.  Bound by the latency of the list, its pages and the rows.
 __global__ __launch_bounds__(256) void commit_kernel(CommitParams p) {
     __shared__ int2 from[64], to[64];
-    __shared__ int moved, last;
+    __shared__ int moved;
     const int s = (int) (blockIdx.x / p.groups), lane = threadIdx.x & 63;
+    int n = 0, c = 0;
+    bool ok = false;
     if (threadIdx.x < 64) {
-        int n, take, c;
+        int take;
         int2 a{0, 0}, b{0, 0};
-        const bool ok = accepted(p, s, lane, n, take, c, a, b);
+        ok = accepted(p, s, lane, n, take, c, a, b);
         const bool moves = ok && lane < c && take != lane;
         const unsigned long long who = __builtin_amdgcn_ballot_w64(moves);
         if (moves) {
@@ -508,18 +516,26 @@ __global__ __launch_bounds__(256) void commit_kernel(CommitParams p) {
         if (lane == 0) moved = __popcll(who);
     }
     __syncthreads();  // the list was read
-    if (threadIdx.x == 0)
-        last = __hip_atomic_fetch_add(&p.head->ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int) gridDim.x - 1;
+    if (threadIdx.x == 0) {
+        int *const ticket = reinterpret_cast<int *>(p.head) + 64 + s;
+        if (__hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int) p.groups - 1) {
+            *ticket = 0;
+            if (ok) p.length[s] = n + c;
+            else add(&p.head->left_out, 1);
+        }
+    }
     unsigned g = blockIdx.x % p.groups;
     int k = 0;
     for (; k + 1 < p.num_pools; ++k) {
-        const unsigned of = (unsigned) (p.pools[k].planes * p.pools[k].heads * (p.pools[k].D / 8) + 255) / 256;
+        const unsigned of = commit_groups(p.pools[k]);
         if (g < of) break;
         g -= of;
     }
     const Pool &o = p.pools[k];
-    const unsigned lanes = (unsigned) o.D / 8, block = (g * 256 + threadIdx.x) / lanes;
-    if (block < (unsigned) (o.planes * o.heads)) {
+    const unsigned lanes = (unsigned) o.D / 8;
+    for (int part = 0; part < kCommitParts; ++part) {
+        const unsigned block = ((g * kCommitParts + part) * 256 + threadIdx.x) / lanes;
+        if (moved == 0 || block >= (unsigned) (o.planes * o.heads)) break;
         constexpr int U = 8;
         uint16_t *const base = o.data + (long long) (block / (unsigned) o.heads) * o.plane_stride +
                                (long long) (block % (unsigned) o.heads) * o.head_stride + 8 * (threadIdx.x % lanes);
@@ -534,18 +550,6 @@ __global__ __launch_bounds__(256) void commit_kernel(CommitParams p) {
                 if (i + u < moved) *at(to[i + u]) = v[u];
         }
     }
-    __syncthreads();
-    if (!last) return;
-    for (int x = threadIdx.x >> 6; x < p.S; x += 4) {
-        int n, take, c;
-        int2 a, b;
-        const bool ok = accepted(p, x, lane, n, take, c, a, b);
-        if (lane == 0) {
-            if (ok) p.length[x] = n + c;
-            else add(&p.head->left_out, 1);
-        }
-    }
-    if (threadIdx.x == 0) p.head->ticket = 0;
 }
 
 // ------------------------------------------------------------------------ host side
@@ -568,10 +572,13 @@ struct Layout {
     size_t entries, moves, ids, rows, bytes;
 };
 
+// The status word and the tickets, zeroed once: each call leaves the tickets as it finds them.
+size_t zeroed(int slots) { return 256 + (sizeof(int) * (size_t) slots + 255) / 256 * 256; }
+
 Layout layout(int num_pages, int slots, int max_pages) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Layout l;
-    l.entries = 256;
+    l.entries = zeroed(slots);
     l.moves = l.entries + sizeof(Entry) * ESDA_MAX_ENTRIES;
     l.ids = l.moves + sizeof(Move) * std::max<size_t>(ESDA_MAX_ENTRIES, num_pages / 2 + 1);
     l.rows = l.ids + up(sizeof(int) * (size_t) num_pages);
@@ -781,8 +788,8 @@ int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_
         return refuse(call, "max_accept must be 1 .. 64, accept_stride at least that");
     if (!accept || !count || !aligned(accept, 4) || !aligned(count, 4))
         return refuse(call, "accept and count must be 4-byte aligned device memory");
-    if (!c->workspace || c->workspace_bytes < 256 || !aligned(c->workspace, 16))
-        return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: a workspace of 256 bytes or more is needed");
+    if (!c->workspace || c->workspace_bytes < zeroed(c->slots) || !aligned(c->workspace, 16))
+        return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: workspace missing or smaller than esda_pages_workspace_size");
     CommitParams p{};
     p.N = c->num_pages;
     p.linear = linear;
@@ -802,7 +809,7 @@ int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_
     long long groups = 0;
     for (int i = 0; i < c->num_pools; ++i) {
         p.pools[i] = pool_params(c->pools[i], c->page_rows);
-        groups += ((long long) p.pools[i].planes * p.pools[i].heads * (p.pools[i].D / 8) + 255) / 256;
+        groups += commit_groups(p.pools[i]);
     }
     groups = std::max(1LL, groups);
     if (groups * c->slots > 1LL << 23) return refuse(call, "too many slots, planes and heads");

@@ -246,36 +246,32 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     // (dispatch is round-robin over the 8), so the (kv head, split) pair is the fastest
     // index and the workgroups on one XCD share one K / V stream in its L2; tiles run
     // heaviest (latest) first.
-    // (TREE: a sequence's splits side by side, too.)
+    // (TREE: units of one piece of keys and one kv head.)
     int combos = p.Hkv * p.splits;
-    if constexpr (TREE) combos *= p.B;
+    if constexpr (TREE) combos = p.units;
     const int wg = (int) blockIdx.x;
     const int tile = p.tiles - 1 - wg / combos;
-    const int kvh = (wg % combos) % p.Hkv;
-    int split = (wg % combos) / p.Hkv, seq = 0;
+    TreeUnit tu{};
+    int tree_first = -1;
     if constexpr (TREE) {
-        seq = split / p.splits;
-        split -= seq * p.splits;
+        tree_first = tree_ids(p, lane);
+        tu = tree_unit(p, (unsigned) (wg % combos), lane);
+        if (!tu.there) return;
     }
-    long long nrows = (long long) p.Sq * p.Hq, row0 = 0;  // row0: the sequence's first, of q, out and partials
-    if constexpr (TREE) {
-        row0 = seq * nrows;
-        nrows *= p.B;
-    }
+    const int kvh = TREE ? tu.kvh : (wg % combos) % p.Hkv, split = TREE ? tu.piece : (wg % combos) / p.Hkv;
+    const long long nrows = (long long) p.Sq * p.Hq;
+    const long long row0 = TREE ? tu.b * nrows : 0;  // the sequence's first row of q and out
     const uint16_t *const qb0 = TREE ? p.q + row0 * D : p.q;
     uint16_t *const out0 = TREE ? p.out + row0 * D : p.out;
 
     int j0, j1;
-    TreeView tv{};
-    unsigned long long path = 0ull;
     if constexpr (TREE) {
-        tv = tree_view(p, seq, lane, path);
-        if (kvh == 0 && split == 0 && tile == 0 && threadIdx.x == 0) {
-            p.views[seq] = tv.ok ? tv.total : -1;
-            if (!tv.ok) __hip_atomic_fetch_add(p.status, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        j0 = tu.j0;
+        j1 = tu.j1;
+        if (tu.keys == 0) {  // no length: skipped
+            if (kvh == 0 && tile == 0 && threadIdx.x == 0) tree_report(p, tu, false);
+            return;
         }
-        if (!tv.ok) return;
-        if (!esda_plan::grid_split(split, p.splits, p.kps, tv.total, &j0, &j1)) j1 = j0;
     } else {
         int tj0, tj1;
         tile_keys(p, tile, QT, tj0, tj1);
@@ -293,8 +289,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     };
     auto qvalid = [&](int qb) { return (long long) tile * QT + wq * 16 * QB + qb * 16 + li < nq; };
 
-    if (j0 >= j1) {  // an empty split: no keys for this tile; the merge skips it
-        if (!TREE && p.splits > 1 && lg == 0 && kh == 0) {
+    if (!TREE && j0 >= j1) {  // an empty split: no keys for this tile; the merge skips it
+        if (p.splits > 1 && lg == 0 && kh == 0) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
                 if (qvalid(qb)) {
@@ -305,13 +301,13 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                         f32x2{-INFINITY, 0.0f};
                 }
         }
-        if constexpr (ODD) {  // unsplit: a tile whose rows see nothing is 0
+        if constexpr (SCORED) {  // unsplit: a tile whose rows see nothing is 0
             if (p.splits == 1) {
                 for (int r = wave; r < QT; r += NW) {
                     const long long gr = (long long) tile * QT + r;
                     if (gr >= nq) break;
                     const unsigned qi = position_of(gr, p.G);
-                    uint16_t *o = out0 + (size_t) qi * p.o_rs + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.o_hs;
+                    uint16_t *o = p.out + (size_t) qi * p.o_rs + (size_t) (kvh * p.G + (int) ((unsigned) gr - qi * p.G)) * p.o_hs;
                     for (int d = 4 * lane; d < D; d += 256) *reinterpret_cast<u32x2 *>(o + d) = u32x2{0u, 0u};
                 }
             }
@@ -367,10 +363,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
     struct None {};
     std::conditional_t<TREE, TreeRows<D, SH>, None> tr = [&] {
         if constexpr (TREE) {
-            TreeRows<D, SH> x(p, tv, seq, kvh);
-            x.j0 = j0;
-            x.j1 = j1;
-            return x;
+            return TreeRows<D, SH>(p, tu, tree_first);
         } else {
             return None{};
         }
@@ -408,20 +401,6 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         }
     };
 
-    bool holes = false;  // TREE: some committed row among the keys lies in no page
-    int all_see = 0;     // .. and committed rows from it on are seen by every node
-    if constexpr (TREE) {
-        if (wave == 0) paths[lane] = path;
-        for (int r = threadIdx.x; r < QT; r += 64 * NW) odd_row[r] = 0;
-        if (threadIdx.x == 0) any_odd = 0;
-        if (!p.linear) {
-            const int k0 = (tv.first + j0) >> p.shift, k1 = (min(tv.len, tv.first + j1) - 1) >> p.shift;  // (k1 < k0: none)
-            for (int k = k0 + lane; k <= k1; k += 64) holes = holes || !tree_page(p, tr.table[k]);
-            holes = __builtin_amdgcn_ballot_w64(holes) != 0ull;
-        }
-        if (p.window > 0) all_see = tv.len + p.Sq - p.window;
-        lds_barrier();
-    }
     if constexpr (SCORED) {
         for (int r = threadIdx.x; r < QT; r += 64 * NW) {
             const long long gr = min((long long) tile * QT + r, nq - 1);
@@ -611,6 +590,27 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         }
     }
 
+    bool holes = false;  // TREE: some committed row among the keys lies in no page
+    int all_see = 0;     // .. and committed rows from it on are seen by every node
+    bool is_seq = true;
+    if constexpr (TREE) {  // beside the first stage's loads
+        unsigned long long path;
+        is_seq = tree_paths(p, tu.b, tu.len, lane, path);
+        if (wave == 0) paths[lane] = path;
+        for (int r = threadIdx.x; r < QT; r += 64 * NW) odd_row[r] = 0;
+        if (threadIdx.x == 0) any_odd = 0;
+        if (!p.linear) {
+            const int k0 = (tu.first + j0) >> p.shift, k1 = (min(tu.len, tu.first + j1) - 1) >> p.shift;  // (k1 < k0: none)
+            for (int k = k0 + lane; k <= k1; k += 64) holes = holes || !tree_page(p, tr.table[k]);
+            holes = __builtin_amdgcn_ballot_w64(holes) != 0ull;
+        }
+        if (p.window > 0) all_see = tu.len + p.Sq - p.window;
+        if (kvh == 0 && split == 0 && tile == 0 && threadIdx.x == 0) tree_report(p, tu, is_seq);
+        if (!is_seq) {  // (its DMAs end before the workgroup's LDS is another's)
+            ESDA_WAIT_VM(0);
+            return;
+        }
+    }
     auto shift = [&]() {
         if constexpr (DOCS) {
 #pragma unroll
@@ -701,8 +701,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sv[qb][4 * h + r] = cur.s[h][qb][r];
         const int ka_first = p.k_pos0 + jb, ka_last = ka_first + kStageKeys - 1;
-        const int krow = tv.first + jb;  // TREE: the stage's first row
-        const bool full = TREE     ? jb + kStageKeys <= j1 && krow + kStageKeys <= tv.len && krow >= all_see && !holes
+        const int krow = tu.first + jb;  // TREE: the stage's first row
+        const bool full = TREE     ? jb + kStageKeys <= j1 && krow + kStageKeys <= tu.len && krow >= all_see && !holes
                           : SCORED ? scored_full(jb, ka_first, ka_last, pure)
                                  : jb + kStageKeys <= j1 && ka_last <= qa_min &&
                                        (p.window == 0 || ka_first > qa_max - p.window);
@@ -755,17 +755,17 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                 if (holes)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        if (krow + 16 * h < tv.len) held[h] = tr.page_of((krow + 16 * h) >> p.shift) >= 0;
+                        if (krow + 16 * h < tu.len) held[h] = tr.page_of((krow + 16 * h) >> p.shift) >= 0;
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb) {
                     const unsigned long long sees = paths[position_of(qrow(qb), p.G)];
-                    const int lowest = p.window > 0 ? tv.len + __popcll(sees) - p.window : 0;
+                    const int lowest = p.window > 0 ? tu.len + __popcll(sees) - p.window : 0;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int j = jb + 16 * h + 4 * lg + r, row = tv.first + j;
-                            const bool seen = row < tv.len ? row >= lowest && held[h] : ((sees >> ((row - tv.len) & 63)) & 1) != 0;
+                            const int j = jb + 16 * h + 4 * lg + r, row = tu.first + j;
+                            const bool seen = row < tu.len ? row >= lowest && held[h] : ((sees >> ((row - tu.len) & 63)) & 1) != 0;
                             if (!(j < j1 && seen)) sv[qb][4 * h + r] = -INFINITY;
                         }
                 }
@@ -988,7 +988,9 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         }
         const long long gr = gr0;
         const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
-        const long long row = row0 + (long long) qi * p.Hq + qh;
+        const long long row = (long long) qi * p.Hq + qh;
+        long long part = (long long) split * nrows + row;  // its partial
+        if constexpr (TREE) part = tree_part(p, tu) + gr;
         const int d0 = 16 * DW * hd;  // the wave's first O^T dim
         if (!PARTS && p.splits == 1) {
             float inv = 1.0f / lb[nb];
@@ -1001,7 +1003,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                 *reinterpret_cast<bf16x4 *>(o + 16 * dt) = b4;
             }
         } else {
-            float *pa = p.part_acc + ((long long) split * nrows + row) * D + d0 + 4 * lg;
+            float *pa = p.part_acc + part * D + d0 + 4 * lg;
             if (p.part_nt) {
                 // (the barriers keep the two branches' stores from being merged into plain ones)
                 asm volatile("" ::: "memory");
@@ -1013,7 +1015,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                 for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4 *>(pa + 16 * dt) = acc[nb][dt];
             }
             if (lg == 0 && nb < QB)  // (m, l) from the block's owner
-                *reinterpret_cast<f32x2 *>(p.part_ml + 2 * ((long long) split * nrows + row)) = f32x2{m[nb < QB ? nb : 0], l[nb < QB ? nb : 0]};
+                *reinterpret_cast<f32x2 *>(p.part_ml + 2 * part) = f32x2{m[nb < QB ? nb : 0], l[nb < QB ? nb : 0]};
         }
     }
     if constexpr (TREE) {
@@ -1026,9 +1028,9 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
                 const long long gr = (long long) tile * QT + r;
                 const int qi = (int) position_of(gr, p.G), qh = kvh * p.G + (int) ((unsigned) gr - (unsigned) qi * p.G);
                 const long long row = row0 + (long long) qi * p.Hq + qh;
-                tree_row_again<D, SH>(tr, p.q + row * D, paths[qi], p.window > 0 ? tv.len + __popcll(paths[qi]) - p.window : 0, j0, j1,
+                tree_row_again<D, SH>(tr, p.q + row * D, paths[qi], p.window > 0 ? tu.len + __popcll(paths[qi]) - p.window : 0, j0, j1,
                                       p.scale_log2e, [&](float mr, float lr, const float(&o)[D / 64]) {
-                                          tree_row_store<D>(p, split, row, lane, mr, lr, o);
+                                          tree_row_store<D>(p, row, tree_part(p, tu) + gr, lane, mr, lr, o);
                                       });
             }
         }
@@ -1256,7 +1258,7 @@ void launch_tiles(const P &p, hipStream_t st) {
     const int nw = one ? (shared ? 4 : 8) : p.nw;
     unsigned groups = p.tiles * p.Hkv * p.splits;
     if constexpr (std::is_same<P, PrefixParams>::value) groups += p.own_groups;
-    if constexpr (std::is_same<P, TreeParams>::value) groups *= p.B;
+    if constexpr (std::is_same<P, TreeParams>::value) groups = p.tiles * p.units;
     const dim3 grid(groups), block(64 * nw);
     if constexpr (D == 512) {
         if (nw == 4 && shared) hipLaunchKernelGGL((prefill_kernel<512, 1, false, true, true, true, 4, P>), grid, block, 0, st, p);

@@ -100,10 +100,14 @@ struct PrefixParams : PrefillParams {
 
 // A step of drafted tokens (esda_tree.h): Sq nodes of each of B sequences, whose keys are the rows of a
 // cache in pages (kv_hs: between the heads of a page) or linear, and the nodes' own.  Keys are counted
-// from the first one that any node sees; `kps` of them a split, and every (sequence, kv head) has
-// `splits`, of which those hold keys that its length reaches.
+// from the first one that any node sees.  Which pieces of them a workgroup takes follows from the
+// lengths (esda_tree_plan.h): `splits` is the most pieces of a (sequence, kv head); partials are
+// [piece of the batch][kv head][Sq * G rows].
 struct TreeParams : PrefillParams {
     int B;
+    int units;        // workgroups of a row group or tile: (piece, kv head), some of them without work
+    int share, least; // pieces of a kv head's keys over the batch; shortest piece, in blocks
+    int forced;       // > 0: blocks of every piece
     int run_groups;   // > 0: in runs (esda_tree.hip), 16 * this many query rows a workgroup (else in tiles)
     int row_groups;   // workgroups of the same keys
     int N, P, shift;  // pages, entries of a sequence's table, log2 of a page's rows
@@ -112,7 +116,7 @@ struct TreeParams : PrefillParams {
     const int *table, *length, *parent;
     const uint16_t *k_new, *v_new;
     int *status;
-    int *views;       // [B]: keys of a sequence, -1 where it is skipped, for the merge
+    int *views;       // [B][2]: first piece of a sequence, and pieces (0: skipped), for the merge
 };
 
 // A kernel form of one head dim: 16-query blocks per wave, stage halves or not, waves, and

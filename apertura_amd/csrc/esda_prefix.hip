@@ -25,7 +25,6 @@
 #include "esda.h"
 #include "esda_attend.h"
 #include "esda_internal.h"
-#include "esda_parts_merge.h"
 #include "esda_prefill_kernel.h"
 #include "esda_prefix.h"
 #include "esda_prefix_tiles.h"
@@ -40,19 +39,15 @@ struct PrefixMergeParams {
     int B, Hq, Hkv, G, base, cap, splits, own_splits, own_chunk;
 };
 
-// A row's partials for esda_parts_merge.h: its prefix splits, then the own splits that hold rows.
+// out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the n partials of a row: its prefix
+// splits, then the own splits that hold rows.
 struct MergeRow {
-    using Params = PrefixMergeParams;
-    static constexpr bool EMPTY = false;
     const PrefixMergeParams &p;
     int row, b, h, n;
     __device__ MergeRow(const PrefixMergeParams &q, int r) : p(q), row(r), b(r / q.Hq), h(r % q.Hq) {
         const SeqView sv = seq_view(p.pos[b], p.base, p.cap, 0, 0);
         n = sv.ok ? p.splits + esda_plan::grid_splits(sv.nvis, p.own_chunk, p.own_splits) : 0;
     }
-    static __host__ __device__ int rows(const PrefixMergeParams &q) { return q.B * q.Hq; }
-    __device__ int most() const { return p.splits + p.own_splits; }
-    __device__ bool write() const { return n > 0; }  // (else skipped: its position lies outside its cache)
     // partial j's row among its kind's
     __device__ size_t at(int j) const {
         if (j < p.splits) return (size_t) j * ((size_t) p.B * p.Hq) + row;
@@ -61,6 +56,104 @@ struct MergeRow {
     __device__ f32x2 ml(int j) const { return *reinterpret_cast<const f32x2 *>((j < p.splits ? p.pre_ml : p.own_ml) + 2 * at(j)); }
     __device__ const float *acc(int j) const { return j < p.splits ? p.pre_acc : p.own_acc; }
 };
+
+// A thread per row and 4 dims: plans of at most NS partials a row.  Every partial is loaded at once,
+// beside the position that says how many of the own ones count (the others are dropped by a select).
+template <int D, int NS>
+__global__ __launch_bounds__(256) void prefix_merge_few_kernel(PrefixMergeParams p) {
+    const long long t = (long long) blockIdx.x * 256 + threadIdx.x;
+    const int row = (int) (t / (D / 4)), d = (int) (t % (D / 4)) * 4;
+    if (row >= p.B * p.Hq) return;
+    const MergeRow r(p, row);
+    f32x2 ml[NS];
+    f32x4 a[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        ml[j] = f32x2{-INFINITY, 0.0f};
+        a[j] = 0.0f;
+        if (j < p.splits + p.own_splits) {
+            ml[j] = r.ml(j);
+            a[j] = *reinterpret_cast<const f32x4 *>(r.acc(j) + r.at(j) * D + d);
+        }
+    }
+    if (r.n == 0) return;  // skipped: its position lies outside its cache
+    float M = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) M = j < r.n ? fmaxf(M, ml[j][0]) : M;
+    float den = 0.0f;
+    f32x4 num = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+        if (j < r.n) {
+            const float w = __builtin_amdgcn_exp2f(ml[j][0] - M);
+            den = __builtin_fmaf(ml[j][1], w, den);
+            num += a[j] * w;
+        }
+    bf16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (__bf16) (num[e] / den);
+    *reinterpret_cast<bf16x4 *>(p.out + (size_t) row * D + d) = o;
+}
+
+// A workgroup per row and 64 dims: 16 groups of 16 lanes x 4 dims take the partials in turn, U of
+// them in flight, each against its own maximum; the groups meet in LDS.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_merge_many_kernel(PrefixMergeParams p) {
+    constexpr int U = 4;
+    __shared__ f32x4 part[16][16];
+    __shared__ f32x2 gml[16];
+    const int row = blockIdx.x / (D / 64), lane = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int d = (int) (blockIdx.x % (D / 64)) * 64 + lane * 4;
+    const MergeRow r(p, row);
+    if (r.n == 0) return;  // skipped
+    float M = -INFINITY, den = 0.0f;
+    f32x4 num = 0.0f;
+    for (int j0 = g; j0 < r.n; j0 += 16 * U) {
+        f32x2 ml[U];
+        f32x4 a[U];
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + 16 * u;
+            ml[u] = f32x2{-INFINITY, 0.0f};
+            a[u] = 0.0f;
+            if (j < r.n) {
+                ml[u] = r.ml(j);
+                a[u] = *reinterpret_cast<const f32x4 *>(r.acc(j) + r.at(j) * D + d);
+            }
+            top = fmaxf(top, ml[u][0]);
+        }
+        const float c = __builtin_amdgcn_exp2f(M - (top == -INFINITY ? 0.0f : top));
+        num *= c;
+        den *= c;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = __builtin_amdgcn_exp2f(ml[u][0] - (top == -INFINITY ? 0.0f : top));
+            den = __builtin_fmaf(ml[u][1], w, den);
+            num += a[u] * w;
+        }
+        M = top;
+    }
+    part[g][lane] = num;
+    if (lane == 0) gml[g] = f32x2{M, den};
+    __syncthreads();
+    if (g == 0) {
+        float top = gml[0][0], l = 0.0f;
+#pragma unroll
+        for (int u = 1; u < 16; ++u) top = fmaxf(top, gml[u][0]);
+        f32x4 o = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const float w = gml[u][0] == -INFINITY && gml[u][1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(gml[u][0] - top);
+            l = __builtin_fmaf(gml[u][1], w, l);
+            o += part[u][lane] * w;
+        }
+        bf16x4 b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = (__bf16) (o[e] / l);
+        *reinterpret_cast<bf16x4 *>(p.out + (size_t) row * D + d) = b;
+    }
+}
 
 // ------------------------------------------------------------------------ host side
 
@@ -295,7 +388,20 @@ hipError_t launch_step(const PrefixParams &p, const PrefixMergeParams &m, bool s
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    launch_parts_merge<D, MergeRow>(m, m.splits + m.own_splits, st);
+    // The threads of the first form hold a row's partials side by side: up to 8 of them always, up to 40
+    // where there are threads to cover the loads.  64 rows (2,048 .. 8,192 threads) in 21 partials, first
+    // form / second: 10.5 / 8.9, 19.0 / 17.5, 15.4 / 14.1 us a step (D = 128, 256, 512); 32,768 threads, 11
+    // 15.3 / 16.3 and 20.9 / 21.8, 21 20.7 / 20.5 and 22.2 / 22.3; 65,536 20.1 / 23.7 and 24.7 / 28.4, 31
+    // 33.6 / 35.5 and 41.3 / 43.6; 262,144 in 11 37.6 / 48.5, in 31 77.4 / 79.6.
+    const int rows = m.B * m.Hq, n = m.splits + m.own_splits;
+    const long long threads = (long long) rows * (D / 4);
+    const unsigned few = (unsigned) ((threads + 255) / 256);
+    if (n <= 4) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 4>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 8) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 8>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 16 && threads >= 1 << 15) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 16>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 24 && threads >= 1 << 15) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 24>), dim3(few), dim3(256), 0, st, m);
+    else if (n <= 40 && threads >= 1 << 16) hipLaunchKernelGGL((prefix_merge_few_kernel<D, 40>), dim3(few), dim3(256), 0, st, m);
+    else hipLaunchKernelGGL(prefix_merge_many_kernel<D>, dim3(rows * (D / 64)), dim3(256), 0, st, m);
     return hipGetLastError();
 }
 

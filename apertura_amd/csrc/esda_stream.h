@@ -20,6 +20,7 @@ namespace esda_stream {
 //                        every wave calls it for its stages in order, before their loads
 //   row(j, k, v)         where row j lies, for stages that are not dense
 //   Stage::end           rows of the stage from it on have no weight
+//   begun()              called once by every wave after its first loads
 //   appended(wave, lane) called once by every wave after its last stage
 // A run of linear or ring rows, the last one maybe new: rows [j0, j1) of a kv head's nvis visible ones.
 template <int D, bool SH>
@@ -45,6 +46,7 @@ struct RunOf {
         kr = is_new ? k_new : k + (size_t) r * D;
         if constexpr (!SH) vr = is_new ? v_new : v + (size_t) r * D;
     }
+    __device__ __forceinline__ void begun() const {}
     // The new row into the cache (bit-exact) by the run that ends with it; no other run reads it.
     __device__ __forceinline__ void appended(int wave, int lane) const {
         if (k_new != nullptr && j1 == nvis && wave == 0)
@@ -129,6 +131,7 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, Run &x, Query &&q
 
     int end = 0, next_end = 0;  // of this stage and the next
     if (wave < nst) end = dma(wave, ring);
+    x.begun();
     bf16x8 qv[NG][KS];  // B operands: query row 16 g + li, dims 32 ks + 8 lg ..
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -338,6 +341,7 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, Run &x, Query 
 
     dma(0);
     end = next_end;
+    x.begun();
     u32x4 qv[KS];  // B operands: query row li, dims 32 ks + 8 lg ..
     const bool there = scores && li < x.G;
     const uint16_t *const qr = query(there ? li : 0) + 8 * lg;

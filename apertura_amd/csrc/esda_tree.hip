@@ -14,7 +14,6 @@
 #include "esda.h"
 #include "esda_internal.h"
 #include "esda_page_view.h"
-#include "esda_parts_merge.h"
 #include "esda_prefill_kernel.h"
 #include "esda_tree.h"
 #include "esda_tree_rows.h"
@@ -22,7 +21,15 @@
 
 namespace {
 
-// Query rows r0 .. of a (sequence, kv head) over one split of its keys, in a run (esda_stream.h).
+// A run's rows with what is to be done once its first loads are under way.
+template <int D, bool SH, class Begin>
+struct BegunRows : TreeRows<D, SH> {
+    Begin &begin;
+    __device__ __forceinline__ BegunRows(const TreeParams &p, const TreeUnit &t, int ids, Begin &f) : TreeRows<D, SH>(p, t, ids), begin(f) {}
+    __device__ __forceinline__ void begun() const { begin(); }
+};
+
+// 16 NG query rows of a (sequence, kv head) over one piece of its keys, in a run (esda_stream.h).
 template <int D, bool SH, int NG>
 __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
     using Own = OwnRows<D, SH, 4, NG>;
@@ -34,52 +41,49 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
     // the first read.
     const unsigned i = blockIdx.x >> 3, unit = i / (unsigned) p.row_groups * 8 + (blockIdx.x & 7);
     const int r0 = (int) (i % (unsigned) p.row_groups) * 16 * NG;
-    const int split = (int) (unit % (unsigned) p.splits), pair = (int) (unit / (unsigned) p.splits);
-    if (pair >= p.B * p.Hkv) return;
-    const int b = pair / p.Hkv, kvh = pair % p.Hkv;
-    unsigned long long path;
-    const TreeView w = tree_view(p, b, lane, path);
-    if (kvh == 0 && split == 0 && r0 == 0 && threadIdx.x == 0) {
-        p.views[b] = w.ok ? w.total : -1;
-        if (!w.ok) __hip_atomic_fetch_add(p.status, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (!w.ok) return;
-    const int rows = p.Sq * p.G;
-    const size_t head = ((size_t) b * p.Sq * p.Hq + (size_t) kvh * p.G);  // of q and out, in rows
-    auto at = [&](int r) { return head + (size_t) (r / p.G) * p.Hq + r % p.G; };
-    TreeRows<D, SH> x(p, w, b, kvh);
-    if (!esda_plan::grid_split(split, p.splits, p.kps, w.total, &x.j0, &x.j1)) {
-        if (split == 0 && p.splits == 1)  // no node at all
-            for (int t = threadIdx.x; t < min(16 * NG, rows - r0) * (D / 8); t += 256)
-                *reinterpret_cast<u32x4 *>(p.out + at(r0 + t / (D / 8)) * D + t % (D / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
+    const int ids = tree_ids(p, lane);
+    const TreeUnit t = tree_unit(p, unit, lane);
+    if (!t.there) return;
+    const bool reports = t.piece == 0 && t.kvh == 0 && r0 == 0 && threadIdx.x == 0;
+    if (t.keys == 0) {  // no length: skipped
+        if (reports) tree_report(p, t, false);
         return;
     }
-    x.G = min(rows - r0, 16 * NG);
-    if (wave == 0) paths[lane] = path;
-    for (int t = threadIdx.x; t < 16 * NG; t += 256) odd[t] = 0;
-    if (threadIdx.x == 0) any_odd = 0;
-    lds_barrier();
+    const int rows = p.Sq * p.G;
+    const size_t head = ((size_t) t.b * p.Sq * p.Hq + (size_t) t.kvh * p.G);  // of q and out, in rows
+    auto at = [&](int r) { return head + (size_t) (r / p.G) * p.Hq + r % p.G; };
     unsigned long long sees[NG];
     int lowest[NG];
+    bool ok = false;
+    auto begin = [&]() {  // beside the first stage's loads; the workgroup meets again before its rows are written
+        unsigned long long path;
+        ok = tree_paths(p, t.b, t.len, lane, path);
+        if (wave == 0) paths[lane] = path;
+        for (int e = threadIdx.x; e < 16 * NG; e += 256) odd[e] = 0;
+        if (threadIdx.x == 0) any_odd = 0;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const int r = r0 + 16 * g + li;
-        sees[g] = r < rows ? paths[r / p.G] : 0ull;
-        lowest[g] = p.window > 0 ? w.len + __popcll(sees[g]) - p.window : 0;
-    }
-    const int all_see = p.window > 0 ? w.len + p.Sq - p.window : 0;  // committed rows from it on: every node
+        for (int g = 0; g < NG; ++g) {
+            const int r = min(r0 + 16 * g + li, rows - 1);
+            sees[g] = __shfl(path, r / p.G);
+            lowest[g] = p.window > 0 ? t.len + __popcll(sees[g]) - p.window : 0;
+        }
+        if (reports) tree_report(p, t, ok);
+    };
+    BegunRows<D, SH, decltype(begin)> x(p, t, ids, begin);
+    x.G = min(rows - r0, 16 * NG);
+    const int all_see = p.window > 0 ? t.len + p.Sq - p.window : 0;  // committed rows from it on: every node
     auto score = [&](f32x4 &s, int jst, int end, int g) {
         s *= p.scale_log2e;
-        const int row = x.first + jst;
-        if (row >= all_see && row + 16 <= w.len && jst + 16 <= end) return;
+        const int row = t.first + jst;
+        if (row >= all_see && row + 16 <= t.len && jst + 16 <= end) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int j = jst + 4 * lg + e, r = x.first + j;
-            const bool seen = r < w.len ? r >= lowest[g] : ((sees[g] >> ((r - w.len) & 63)) & 1) != 0;
+            const int j = jst + 4 * lg + e, r = t.first + j;
+            const bool seen = r < t.len ? r >= lowest[g] : ((sees[g] >> ((r - t.len) & 63)) & 1) != 0;
             if (j >= end || !seen) s[e] = -INFINITY;
         }
     };
-    const size_t nrows = (size_t) p.B * p.Sq * p.Hq, part = (size_t) split * nrows;
+    const size_t part = (size_t) tree_part(p, t);
     auto finish = [&](int r, int d, f32x4 o, float m, float l) {  // dims d .. d + 3 of query row r
         if (paths[r / p.G] == 0ull) {  // no node: nothing seen
             o = 0.0f;
@@ -90,9 +94,9 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
             bf16x4 y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (__bf16) (o[e] * inv);
-            *reinterpret_cast<bf16x4 *>(p.out + at(r) * D + d) = y;
+            if (ok) *reinterpret_cast<bf16x4 *>(p.out + at(r) * D + d) = y;
         } else {
-            Own::store(p.part_acc, p.part_ml, part + at(r), d, o, m, l);
+            Own::store(p.part_acc, p.part_ml, part + r, d, o, m, l);
         }
     };
     Own::attend(
@@ -107,6 +111,7 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
                 any_odd = 1;
             }
         });
+    if (!ok) return;
     if (r0 == 0) append_nodes<D, SH>(x, paths, x.j0, x.j1);
     ESDA_WAIT_VM(0);  // the rows as written above, before they are written again
     lds_barrier();
@@ -114,31 +119,85 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
         for (int h = wave; h < x.G; h += 4) {
             if (!odd[h]) continue;
             const unsigned long long mine = paths[(r0 + h) / p.G];
-            tree_row_again<D, SH>(x, p.q + at(r0 + h) * D, mine, p.window > 0 ? w.len + __popcll(mine) - p.window : 0, x.j0, x.j1,
+            tree_row_again<D, SH>(x, p.q + at(r0 + h) * D, mine, p.window > 0 ? t.len + __popcll(mine) - p.window : 0, x.j0, x.j1,
                                   p.scale_log2e, [&](float m, float l, const float(&o)[D / 64]) {
-                                      tree_row_store<D>(p, split, at(r0 + h), lane, m, l, o);
+                                      tree_row_store<D>(p, at(r0 + h), part + r0 + h, lane, m, l, o);
                                   });
         }
     }
 }
 
-// A row's partials for esda_parts_merge.h: the splits that its sequence's keys reach.
-struct TreeMergeRow {
-    using Params = TreeParams;
-    static constexpr bool EMPTY = true;
-    const TreeParams &p;
-    int row, view, n;
-    __device__ TreeMergeRow(const TreeParams &q, int r) : p(q), row(r) {
-        view = q.views[r / (q.Sq * q.Hq)];
-        n = view > 0 ? esda_plan::grid_splits(view, q.kps, q.splits) : 0;
+// out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the pieces of a row's sequence; 0 where it
+// saw no key.  A workgroup takes 256 / GR lanes of 4 dims, and its GR groups of threads the pieces in
+// turn, U of them in flight, each against its own maximum; the groups meet in LDS.
+template <int D, int GR>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
+    constexpr int U = 4, LANES = 256 / GR;
+    __shared__ f32x4 part[GR > 1 ? GR : 1][LANES];
+    __shared__ f32x2 gml[GR > 1 ? GR : 1][LANES];
+    const int lane = threadIdx.x % LANES, g = threadIdx.x / LANES;
+    const long long x = (long long) blockIdx.x * LANES + lane;
+    const int row = (int) (x / (D / 4)), d = (int) (x % (D / 4)) * 4;
+    const bool there = row < p.B * p.Sq * p.Hq;
+    const int i = (there ? row : 0) / p.Hq, h = (there ? row : 0) % p.Hq, b = i / p.Sq;
+    const int base = p.views[2 * b], n = there ? p.views[2 * b + 1] : 0;  // 0: skipped, and left as it is
+    const size_t first = ((size_t) base * p.Hkv + h / p.G) * (p.Sq * p.G) + (i - b * p.Sq) * p.G + h % p.G;
+    const size_t step = (size_t) p.Hkv * p.Sq * p.G;
+    float M = -INFINITY, den = 0.0f;
+    f32x4 num = 0.0f;
+    for (int j0 = g; j0 < n; j0 += GR * U) {
+        f32x2 ml[U];
+        f32x4 a[U];
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + GR * u;
+            ml[u] = f32x2{-INFINITY, 0.0f};
+            a[u] = 0.0f;
+            if (j < n) {
+                ml[u] = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * (first + j * step));
+                a[u] = *reinterpret_cast<const f32x4 *>(p.part_acc + (first + j * step) * D + d);
+            }
+            top = fmaxf(top, ml[u][0]);
+        }
+        const float at = top == -INFINITY ? 0.0f : top;
+        const float c = __builtin_amdgcn_exp2f(M - at);
+        num *= c;
+        den *= c;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = __builtin_amdgcn_exp2f(ml[u][0] - at);
+            den = __builtin_fmaf(ml[u][1], w, den);
+            num += a[u] * w;
+        }
+        M = top;
     }
-    static __host__ __device__ int rows(const TreeParams &q) { return q.B * q.Sq * q.Hq; }
-    __device__ int most() const { return p.splits; }
-    __device__ bool write() const { return view >= 0; }
-    __device__ size_t at(int j) const { return (size_t) j * rows(p) + row; }
-    __device__ f32x2 ml(int j) const { return *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * at(j)); }
-    __device__ const float *acc(int) const { return p.part_acc; }
-};
+    if constexpr (GR > 1) {
+        part[g][lane] = num;
+        gml[g][lane] = f32x2{M, den};
+        __syncthreads();
+        if (g != 0) return;
+        float top = M;
+#pragma unroll
+        for (int u = 1; u < GR; ++u) top = fmaxf(top, gml[u][lane][0]);
+        if (top == -INFINITY) top = 0.0f;
+        num = 0.0f;
+        den = 0.0f;
+#pragma unroll
+        for (int u = 0; u < GR; ++u) {
+            const f32x2 ml = gml[u][lane];
+            const float w = __builtin_amdgcn_exp2f(ml[0] - top);
+            den = __builtin_fmaf(ml[1], w, den);
+            num += part[u][lane] * w;
+        }
+    }
+    if (n == 0) return;
+    if (den == 0.0f) den = 1.0f;
+    bf16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (__bf16) (num[e] / den);
+    *reinterpret_cast<bf16x4 *>(p.out + (size_t) row * D + d) = o;
+}
 
 // ------------------------------------------------------------------------ host side
 
@@ -175,7 +234,7 @@ const char *check_desc(const esda_tree_desc *d) {
     if (!whole16(d->page_stride) || !whole16(d->head_stride)) return "strides must be non-negative multiples of 8";
     if (!blocks_apart({1, d->num_pages, d->num_kv_heads}, {0, d->page_stride, d->head_stride}, (long long) d->page_rows * d->head_dim))
         return "the pages overlap";
-    if (d->max_visible < 0) return "max_visible must not be negative";
+    if (d->max_pages != 0 && (long long) d->max_pages * d->page_rows > (1LL << 31) - 256) return "a table holds fewer than 2^31 - 256 rows";
     if (d->split_rows < 0 || d->split_rows % kStageKeys) return "split_rows must be a multiple of 32";
     if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return "scale must be positive and finite";
     if ((long long) d->batch * d->nodes * d->num_q_heads * (d->head_dim / 64) >= 1 << 24) return "too many query rows";
@@ -215,49 +274,48 @@ int forms_of(int D, int rows, bool shared, Form *f) {
     return n;
 }
 
-// Form and splits of a step over at most `most` keys a sequence: the cheapest by the workgroups' time on
-// the GPU, the bytes, and the merge of the partials.
+// Runs up to 16 query rows, ..
+int pick(int D, int rows, bool shared, const Form *f, int nf) {
+    (void) shared;
+    auto find = [&](int ng, int rows_of) {
+        for (int i = 0; i < nf; ++i)
+            if (f[i].ng == ng && (ng || f[i].rows() == rows_of)) return i;
+        return 0;
+    };
+    if (rows <= 16) return find(1, 0);
+    if (D == 128) return rows <= 32 ? find(2, 0) : find(0, 128);
+    if (D == 256) return rows <= 64 ? find(0, 64) : find(0, 128);
+    return rows <= 32 ? find(1, 0) : find(0, rows > 64 || !shared ? 128 : 64);
+}
+
+// The form of a step, and how many pieces its keys are to make: the host does not know the lengths, so
+// it asks for as many workgroups as the GPU holds at once (esda_tree_plan.h shares the keys out).
 void choose(const esda_tree_desc *d, long long most, TreeParams *p) {
     const int D = d->head_dim, rows = p->Sq * p->G;
-    const bool shared = d->kv_shared != 0;
-    const float row_kb = 2.0f * D * (shared ? 1 : 2) / 1024;
-    const long long pairs = (long long) p->B * p->Hkv, out_rows = (long long) p->B * p->Sq * p->Hq;
-    const float floor_us = 4.0f + (float) (most * pairs) * row_kb / 5600.0f;
+    const long long pairs = (long long) p->B * p->Hkv;
     Form f[4];
-    const int nf = forms_of(D, rows, shared, f);
-    float best = INFINITY;
-    auto consider = [&](const Form &form, long long keys) {
-        const long long splits = (most + keys - 1) / keys, tiles = (rows + form.rows() - 1) / form.rows();
-        const long long groups = pairs * tiles * splits;
-        const float us = form.start + (float) std::min(keys, most) * row_kb * form.per_kb;
-        float span = std::max(us, (float) groups / form.slots * us);
-        if (groups > form.slots) span += 0.5f * us;
-        const float cost = std::max(span, floor_us) + 0.13f * std::min(span, floor_us) +
-                           (splits == 1 ? 0.0f : splits <= 8 ? 4.3f : 4.8f) + (splits > 1 ? 2.6e-7f * 4 * D * out_rows * splits : 0.0f);
-        if (cost >= best) return;
-        best = cost;
-        p->qb = form.qb;
-        p->kh = form.kh;
-        p->nw = form.nw;
-        p->run_groups = form.ng;
-        p->tiles = p->row_groups = (int) tiles;
-        p->splits = (int) std::max(1LL, splits);
-        p->kps = (int) keys;
-    };
-    for (int i = 0; i < nf; ++i) {
-        if (d->split_rows > 0) {  // (one longer than the keys is cut to them)
-            consider(f[i], std::min<long long>(d->split_rows, (most + kStageKeys - 1) / kStageKeys * kStageKeys));
-            continue;
-        }
-        long long last = 0;
-        for (int s = 1; s <= 512; s += std::max(1, s / 8)) {
-            const long long keys = std::max(64LL, ((most + s - 1) / s + kStageKeys - 1) / kStageKeys * kStageKeys);
-            if (keys != last) consider(f[i], keys);
-            if (keys == 64) break;
-            last = keys;
-        }
+    const int nf = forms_of(D, rows, d->kv_shared != 0, f);
+    const Form &x = f[pick(D, rows, d->kv_shared != 0, f, nf)];
+    p->qb = x.qb;
+    p->kh = x.kh;
+    p->nw = x.nw;
+    p->run_groups = x.ng;
+    p->tiles = p->row_groups = (rows + x.rows() - 1) / x.rows();
+    long long units;
+    if (d->split_rows > 0) {
+        p->forced = (int) std::min<long long>(d->split_rows / kStageKeys, (most + kStageKeys - 1) / kStageKeys);
+        p->splits = (int) std::min<long long>((most + d->split_rows - 1) / d->split_rows, INT_MAX);
+        p->share = 1;
+        units = pairs * p->splits;
+    } else {
+        p->least = 2;
+        p->share = std::max(1, (int) (x.slots / ((long long) p->Hkv * p->tiles)));
+        const bool split = p->share > p->B;
+        if (!split) p->share = p->B;
+        p->splits = split ? p->share : 1;
+        units = split ? (long long) p->share * p->Hkv : pairs;
     }
-    p->part_nt = 4.0f * D * out_rows * p->splits <= kPartNtBytes;
+    p->units = (int) std::min<long long>((units + 7) / 8 * 8, INT_MAX);
 }
 
 int fresh_plan(const esda_tree_desc *d, TreePlan *pl) {
@@ -282,18 +340,14 @@ int fresh_plan(const esda_tree_desc *d, TreePlan *pl) {
     p.scale_log2e = d->scale * kLog2e;
     p.q_hs = p.o_hs = D;
     p.q_rs = p.o_rs = (long long) p.Hq * D;
-    // most keys of a sequence: what its pages hold, the bound that is given, its window (from a multiple
-    // of 32 on); longer ones only lengthen the last split
-    long long most = p.linear ? p.cap : (long long) d->max_pages * d->page_rows;
-    if (d->max_visible > 0) most = std::min(most, (long long) d->max_visible + p.Sq);
-    if (p.window > 0) most = std::min(most, (long long) p.window + p.Sq + kStageKeys);
-    choose(d, most, &p);
-    const long long groups = (long long) p.B * p.Hkv * p.row_groups;
-    if (p.splits > 4096 || groups * p.splits >= INT_MAX / 512) return refuse("too many splits");
+    const long long most = (p.linear ? p.cap : (long long) d->max_pages * d->page_rows) + p.Sq;  // keys of a sequence
+    choose(d, p.window > 0 ? std::min(most, (long long) p.window + p.Sq + kStageKeys) : most, &p);
+    if (p.splits > 4096 || (long long) p.units * p.tiles >= INT_MAX / 512) return refuse("too many splits");
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t parts = p.splits > 1 ? (size_t) p.B * p.Sq * p.Hq * p.splits : 0;
+    const size_t parts = p.splits > 1 ? (size_t) p.units * p.Sq * p.G : 0;
+    p.part_nt = 4.0f * D * parts <= kPartNtBytes;
     pl->off_views = 256;
-    pl->off_ml = pl->off_views + up((size_t) p.B * 4);
+    pl->off_ml = pl->off_views + up((size_t) p.B * 8);
     pl->off_acc = pl->off_ml + up(parts * 8);
     pl->bytes = pl->off_acc + parts * D * sizeof(float);
     return ESDA_OK;
@@ -322,28 +376,31 @@ int make_tree_plan(const esda_tree_desc *d, TreePlan *pl) {
 
 template <int D>
 hipError_t launch_step(const TreeParams &p, bool shared, hipStream_t st) {
-    if (!p.run_groups) {
+    if (p.run_groups) {
+        const dim3 grid(p.units * p.row_groups), block(256);
+        auto run = [&](auto ng) {
+            constexpr int NG = decltype(ng)::value;
+            if (shared) hipLaunchKernelGGL((tree_run_kernel<D, true, NG>), grid, block, 0, st, p);
+            else hipLaunchKernelGGL((tree_run_kernel<D, false, NG>), grid, block, 0, st, p);
+        };
+        if (p.run_groups == 1) run(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            if (p.run_groups == 2) run(std::integral_constant<int, 2>{});
+            if (p.run_groups == 4) run(std::integral_constant<int, 4>{});
+        }
+    } else {
         esda_detail::tree_tiles(p, D, st);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess || p.splits == 1) return e;
-        launch_parts_merge<D, TreeMergeRow>(p, p.splits, st);
-        return hipGetLastError();
-    }
-    const unsigned units = (unsigned) (p.B * p.Hkv * p.splits);
-    const dim3 grid((units + 7) / 8 * 8 * p.row_groups), block(256);
-    auto run = [&](auto ng) {
-        constexpr int NG = decltype(ng)::value;
-        if (shared) hipLaunchKernelGGL((tree_run_kernel<D, true, NG>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((tree_run_kernel<D, false, NG>), grid, block, 0, st, p);
-    };
-    if (p.run_groups == 1) run(std::integral_constant<int, 1>{});
-    if constexpr (D == 128) {
-        if (p.run_groups == 2) run(std::integral_constant<int, 2>{});
-        if (p.run_groups == 4) run(std::integral_constant<int, 4>{});
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    launch_parts_merge<D, TreeMergeRow>(p, p.splits, st);
+    const long long lanes = (long long) p.B * p.Sq * p.Hq * (D / 4);
+    auto merge = [&](auto gr) {
+        constexpr int GR = decltype(gr)::value;
+        hipLaunchKernelGGL((tree_merge_kernel<D, GR>), dim3((unsigned) ((lanes + 256 / GR - 1) / (256 / GR))), dim3(256), 0, st, p);
+    };
+    if (lanes <= 1 << 14) merge(std::integral_constant<int, 16>{});
+    else if (lanes <= 1 << 16) merge(std::integral_constant<int, 4>{});
+    else merge(std::integral_constant<int, 1>{});
     return hipGetLastError();
 }
 

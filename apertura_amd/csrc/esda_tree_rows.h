@@ -9,25 +9,119 @@
 
 #include "esda_device.h"
 #include "esda_prefill_plan.h"
+#include "esda_tree_plan.h"
 
 namespace {
 
 using esda_prefill_plan::TreeParams;
 
-// A sequence's keys: `total` of them from row `first` on (0: it has no node; then it is done).
-struct TreeView {
-    int ok, len, nodes, first, total;
-};
-
 __device__ __forceinline__ bool tree_page(const TreeParams &p, int id) { return (unsigned) id < (unsigned) p.N; }
 
-// Sequence b as a wave: lane i < 64 gets node i's path (bit j: node j is above it, or is it; 0: no node).
-// A node's path doubles in length each round: what is above the node that is above it.
-__device__ __forceinline__ TreeView tree_view(const TreeParams &p, int b, int lane, unsigned long long &path) {
-    TreeView v;
-    v.len = uniform(p.length[b]);
+// A workgroup's piece: keys [j0, j1) of sequence b and kv head kvh, counted from row `first` on; the
+// sequence's pieces are base .. base + pieces - 1 of the batch's.
+struct TreeUnit {
+    int there, b, kvh, len, first, keys, piece, pieces, base, j0, j1;
+};
+
+// Keys of a sequence of len rows, and the first row that any node sees (a multiple of 32); 0 keys where
+// the length is none (every node's row is counted, whether it is one or not).
+__device__ __forceinline__ int tree_keys(const TreeParams &p, int len, int &first) {
+    const long long most = p.linear ? (long long) p.cap : (long long) p.P << p.shift;
+    first = p.window > 0 ? max(0, len - p.window + 1) & ~31 : 0;
+    return len >= 0 && len <= most ? len - first + p.Sq : 0;
+}
+
+// Unit u as a wave: the pieces that the batch's lengths make, and which of them it is.
+__device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, unsigned u, int lane) {
+    using namespace esda_tree_plan;
+    TreeUnit t;
+    t.kvh = (int) (u % (unsigned) p.Hkv);
+    const int g = (int) (u / (unsigned) p.Hkv);  // piece of the batch
+    t.there = 0;
+    if (p.B == 1) {
+        t.b = t.base = 0;
+        t.len = uniform(p.length[0]);
+        t.keys = tree_keys(p, t.len, t.first);
+        const int n = blocks_of(t.keys);
+        const int chunk = p.forced ? p.forced : chunk_of(n, p.share, 1, p.least, 0);
+        t.pieces = pieces_of(n, chunk, p.splits);
+        t.piece = g;
+        t.there = g < t.pieces;
+        piece_keys(g, t.pieces, chunk, t.keys, &t.j0, &t.j1);
+        return t;
+    }
+    constexpr int K = 4;  // sequences a lane: 64 k + lane
+    int len[K], n[K], first, sum = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int s = 64 * k + lane;
+        len[k] = s < p.B ? p.length[s] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        n[k] = blocks_of(tree_keys(p, len[k], first));
+        sum += n[k];
+    }
+    int chunk = p.forced;
+    if (!p.forced) {
+        auto total = [](int x) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+            return uniform(x);
+        };
+        sum = total(sum);
+        for (int i = 0; i <= kTries; ++i) {
+            chunk = chunk_of(sum, p.share, p.B, p.least, i);
+            int count = 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (64 * k + lane < p.B) count += pieces_of(n[k], chunk, p.splits);
+            if (total(count) <= p.share) break;
+        }
+    }
+    int before = 0;  // pieces of the sequences of the rounds before
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (64 * k >= p.B) break;
+        const bool mine = 64 * k + lane < p.B;
+        const int count = mine ? pieces_of(n[k], chunk, p.splits) : 0;
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o);
+            if (lane >= o) upto += y;
+        }
+        upto += before;
+        const int from = upto - count;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(from <= g && g < upto);
+        if (who) {
+            const int l = __builtin_ctzll(who);
+            t.there = 1;
+            t.b = 64 * k + l;
+            t.base = __builtin_amdgcn_readlane(from, l);
+            t.len = __builtin_amdgcn_readlane(len[k], l);
+            t.pieces = __builtin_amdgcn_readlane(count, l);
+            t.keys = tree_keys(p, t.len, t.first);
+            t.piece = g - t.base;
+            piece_keys(t.piece, t.pieces, chunk, t.keys, &t.j0, &t.j1);
+            return t;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return t;
+}
+
+// Sequence b's nodes as a wave: lane i < 64 gets node i's path (bit j: node j is above it, or is it; 0: no
+// node), and whether the sequence is one: its length and its nodes' rows lie in its cache.  A node's path
+// doubles in length each round: what is above the node that is above it.
+__device__ __forceinline__ bool tree_paths(const TreeParams &p, int b, int len, int lane, unsigned long long &path) {
     bool node = lane < p.Sq;
     path = node ? (2ull << lane) - 1 : 0ull;
+    const long long most = p.linear ? (long long) p.cap : (long long) p.P << p.shift;
+    const long long row = (long long) len + lane;
+    const bool within = len >= 0 && row < most;
+    int id = 0;
+    if (node && within && !p.linear) id = p.table[b * p.table_stride + (row >> p.shift)];
     if (p.parent) {
         int above = node ? p.parent[(size_t) b * p.Sq + lane] : -2;
         if (above < -1 || above >= lane) above = -2;  // on no node
@@ -45,14 +139,23 @@ __device__ __forceinline__ TreeView tree_view(const TreeParams &p, int b, int la
         node = above == -1;
         if (!node) path = 0ull;
     }
-    const unsigned long long there = __builtin_amdgcn_ballot_w64(node);
-    v.nodes = there ? 64 - __builtin_clzll(there) : 0;
-    bool ok = v.len >= 0 && (long long) v.len + v.nodes <= (p.linear ? (long long) p.cap : (long long) p.P << p.shift);
-    if (ok && node && !p.linear) ok = tree_page(p, p.table[b * p.table_stride + ((v.len + lane) >> p.shift)]);
-    v.ok = __builtin_amdgcn_ballot_w64(!ok) == 0ull;
-    v.first = p.window > 0 ? max(0, v.len - p.window + 1) & ~31 : 0;
-    v.total = v.nodes ? v.len + v.nodes - v.first : 0;
-    return v;
+    const bool ok = len >= 0 && len <= most && (!node || (within && (p.linear || tree_page(p, id))));
+    return __builtin_amdgcn_ballot_w64(!ok) == 0ull;
+}
+
+// The first partial of a unit, and what the merge is told of its sequence (by one thread of them all).
+__device__ __forceinline__ long long tree_part(const TreeParams &p, const TreeUnit &t) {
+    return ((long long) (t.base + t.piece) * p.Hkv + t.kvh) * (p.Sq * p.G);
+}
+__device__ __forceinline__ void tree_report(const TreeParams &p, const TreeUnit &t, bool ok) {
+    p.views[2 * t.b] = t.base;
+    p.views[2 * t.b + 1] = ok ? t.pieces : 0;
+    if (!ok) __hip_atomic_fetch_add(p.status, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The first entries of a single sequence's table, read beside its length (0.5 us of a step's 11).
+__device__ __forceinline__ int tree_ids(const TreeParams &p, int lane) {
+    return p.B == 1 && !p.linear ? p.table[min(lane, p.P - 1)] : -1;
 }
 
 // The rows of one (sequence, kv head) as esda_stream.h's runs take them.
@@ -67,7 +170,9 @@ struct TreeRows {
     int ids, of;                    // lane i: page 64 of + i of the table
     int page;                       // of the last stage
 
-    __device__ __forceinline__ TreeRows(const TreeParams &p, const TreeView &w, int b, int kvh) {
+    // ids0: the first 64 entries of the table (tree_ids), or anything
+    __device__ __forceinline__ TreeRows(const TreeParams &p, const TreeUnit &w, int ids0) {
+        const int b = w.b, kvh = w.kvh;
         k = const_cast<uint16_t *>(p.k) + kvh * p.kv_hs;
         v = const_cast<uint16_t *>(p.v) + kvh * p.kv_hs;
         const size_t at = ((size_t) b * p.Sq * p.Hkv + kvh) * D;
@@ -82,9 +187,11 @@ struct TreeRows {
         P = p.P;
         shift = p.shift;
         page0 = p.linear ? b : 0;
-        G = j0 = j1 = page = 0;
-        ids = page0;  // (linear: every row in entry 0)
-        of = p.linear ? 0 : -1;
+        G = page = 0;
+        j0 = w.j0;
+        j1 = w.j1;
+        ids = p.linear ? page0 : (unsigned) ids0 < (unsigned) N ? ids0 : -1;  // (linear: every row in entry 0)
+        of = p.linear || p.B == 1 ? 0 : -1;
     }
 
     struct Stage {
@@ -125,6 +232,7 @@ struct TreeRows {
         kr = (r < len ? k : k_new) + at;
         if constexpr (!SH) vr = (r < len ? v : v_new) + at;
     }
+    __device__ __forceinline__ void begun() const {}
     __device__ __forceinline__ void appended(int, int) const {}
 };
 
@@ -214,9 +322,9 @@ __device__ __forceinline__ void tree_row_again(const TreeRows<D, SH> &x, const u
     store(m, l, o);
 }
 
-// .. and its place in out or among the partials.
+// .. and into out, row `row`, or its partial, number `at`.
 template <int D>
-__device__ __forceinline__ void tree_row_store(const TreeParams &p, int split, long long row, int lane, float m, float l,
+__device__ __forceinline__ void tree_row_store(const TreeParams &p, long long row, long long at, int lane, float m, float l,
                                                const float (&o)[D / 64]) {
     constexpr int DPL = D / 64;
     if (p.splits == 1) {
@@ -225,7 +333,6 @@ __device__ __forceinline__ void tree_row_store(const TreeParams &p, int split, l
         for (int e = 0; e < DPL; ++e) p.out[row * D + lane * DPL + e] = __builtin_bit_cast(uint16_t, (__bf16) (o[e] * inv));
         return;
     }
-    const long long at = (long long) split * p.B * p.Sq * p.Hq + row;
 #pragma unroll
     for (int e = 0; e < DPL; ++e) p.part_acc[at * D + lane * DPL + e] = o[e];
     if (lane == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * at) = f32x2{m, l};

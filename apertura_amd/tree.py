@@ -32,7 +32,6 @@ class TreeStep:
     window: int = 0
     kv_shared: bool = False
     scale: float = 1.0
-    max_visible: int = 0
     split_rows: int = 0
     table_stride: int | None = None
     page_stride: int | None = None
@@ -44,10 +43,10 @@ class TreeStep:
         ts = self.table_stride if self.table_stride is not None else self.max_pages
         check_int32(batch=self.batch, nodes=self.nodes, num_q_heads=self.num_q_heads, num_kv_heads=self.num_kv_heads,
                     head_dim=self.head_dim, num_pages=self.num_pages, page_rows=self.page_rows, max_pages=self.max_pages,
-                    window=self.window, max_visible=self.max_visible, split_rows=self.split_rows)
+                    window=self.window, split_rows=self.split_rows)
         return TreeDesc(self.batch, self.nodes, self.num_q_heads, self.num_kv_heads, self.head_dim, int(bool(self.kv_shared)),
-                        self.window, self.num_pages, self.page_rows, self.max_pages, ts, ps, hs, self.max_visible,
-                        self.split_rows, self.scale, 0)
+                        self.window, self.num_pages, self.page_rows, self.max_pages, ts, ps, hs, self.split_rows,
+                        self.scale)
 
     @classmethod
     def for_pages(cls, pages: torch.Tensor, table: torch.Tensor, num_q_heads: int, nodes: int, **kw) -> "TreeStep":

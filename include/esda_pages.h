@@ -60,7 +60,7 @@ typedef struct esda_pages {
     int32_t num_pools;    /* 0 .. ESDA_MAX_POOLS                        */
     int32_t pad;          /* 0                                          */
     esda_pool pools[ESDA_MAX_POOLS]; /* one table for all of them       */
-    void *workspace;      /* esda_pages_workspace_size bytes, 16-byte aligned; first 256 zeroed once */
+    void *workspace;      /* esda_pages_workspace_size bytes, 16-byte aligned; zeroed once */
     size_t workspace_bytes;
 } esda_pages;
 

@@ -48,11 +48,8 @@ typedef struct esda_tree_desc {
     int64_t table_stride; /* ints; >= max_pages                                     */
     int64_t page_stride;  /* elements: (page, kvh, row, d) at page*page_stride + kvh*head_stride + row*head_dim + d */
     int64_t head_stride;  /* both multiples of 8; blocks of page_rows * head_dim elements must not overlap */
-    int32_t max_visible;  /* expected bound on committed rows, sizes the split (0: what the table holds);
-                             rows beyond it are still attended                     */
-    int32_t split_rows;   /* rows per split (0 = automatic; multiple of 32)         */
+    int32_t split_rows;   /* rows per split (0: from the lengths, on the device; multiple of 32) */
     float scale;          /* softmax scale, positive                                */
-    int32_t pad;          /* 0                                                      */
 } esda_tree_desc;
 
 typedef struct esda_tree_args {
@@ -78,7 +75,7 @@ int esda_tree_decode(const esda_tree_desc *desc, const esda_tree_args *args, voi
  * entries rise and lie in 0 .. 63.  A slot with another list, a count outside 0 .. max_accept or rows
  * that lie in no page is left as it was and counted.  max_accept: 1 .. 64.
  * cache->table NULL: linear caches, slot s in page s (num_pages == slots, max_pages 1, page_rows any
- * 1 .. 2^30); refs is not used. */
+ * 1 .. 2^30); refs is not used.  The workspace is esda_pages.h's, zeroed once. */
 int esda_tree_commit(const esda_pages *cache, const int32_t *accept, int64_t accept_stride, int32_t max_accept,
                      const int32_t *count, void *stream);
 

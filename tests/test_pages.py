@@ -102,7 +102,7 @@ def test_workspaces_grow_with_the_cache():
         return n.value
 
     base = size()
-    assert base >= 256 + 1024 * (16 + 16) + 20 * 4 + 6 * 5 * 4
+    assert base >= 256 + 6 * 4 + 1024 * (16 + 16) + 20 * 4 + 6 * 5 * 4
     assert size(num_pages=2 ** 22) >= 2 ** 22 * 4 + 2 ** 21 * 16
     assert size(slots=2000, max_pages=100) >= 1024 * 100 * 4 + base - 6 * 5 * 4
     n = ctypes.c_size_t(0)

@@ -227,9 +227,9 @@ def test_commit_over_linear_caches():
     B, cap = 3, 50
     pool = torch.randint(0, 2 ** 15, (2, B, 3, cap, 128), dtype=torch.int16, device=DEV)
     first = pool.clone()
-    length, ws = _ints([10, 44, 47]), torch.zeros(256, dtype=torch.uint8, device=DEV)
+    length, ws = _ints([10, 44, 47]), torch.zeros(512, dtype=torch.uint8, device=DEV)
     c = _lib.Pages(num_pages=B, page_rows=cap, slots=B, max_pages=1, length=length.data_ptr(), num_pools=1,
-                   workspace=ws.data_ptr(), workspace_bytes=256)
+                   workspace=ws.data_ptr(), workspace_bytes=512)
     c.pools[0] = _lib.Pool(pool.data_ptr(), 2, 3, 128, 0, *pool.stride()[:3])
     accept, count = _ints([[1, 4, 8], [0, 3, 5], [0, 1, 3]]), _ints([3, 3, 3])
     _lib.check(_lib.lib().esda_tree_commit(ctypes.byref(c), accept.data_ptr(), 3, 3, count.data_ptr(), None))
@@ -240,6 +240,7 @@ def test_commit_over_linear_caches():
             assert torch.equal(pool[:, b, :, n + i], pool_want)
     assert torch.equal(pool[:, 2], first[:, 2])
     assert length.tolist() == [13, 47, 47] and ws[:4].view(torch.int32).item() == 1
+    assert not bool(ws[256:].any())  # the tickets are back
 
 
 @pytest.mark.parametrize("planes,hkv,D", [(1, 1, 128), (2, 3, 256), (1, 2, 512)])

@@ -24,29 +24,31 @@ def _linear(**kw):
 
 
 def test_workspace_holds_every_partial():
-    """The status word, the sequences' keys, then (m, l) and O of every split of the query rows."""
-    up = lambda n: (n + 255) // 256 * 256
-    for rows, splits in ((32, 5), (64, 3), (96, 2)):
-        parts = splits * 4 * 5 * 8
-        assert tree_workspace_bytes(_step(split_rows=rows)) == 256 + up(16) + up(parts * 8) + parts * 128 * 4
-    for rows in (160, 320, 2 ** 31 - 32):  # one split: no partials
+    """The status word, the sequences' pieces, then (m, l) and O of every piece of the query rows (a sequence
+    has 165 keys at most; pieces of all heads in eights)."""
+    up = lambda n, of=256: (n + of - 1) // of * of
+    for rows, splits in ((32, 6), (64, 3), (96, 2)):
+        parts = up(splits * 4 * 2, 8) * 5 * 4
+        assert tree_workspace_bytes(_step(split_rows=rows)) == 256 + up(32) + up(parts * 8) + parts * 128 * 4
+    for rows in (192, 320, 2 ** 31 - 32):  # one split: no partials
         assert tree_workspace_bytes(_step(split_rows=rows)) == 512
 
 
 def test_bounds_on_rows_size_the_splits():
-    """A bound that is given, and a window, of which a sequence sees no more."""
+    """A window, of which a sequence sees no more; automatic splits do not go by the room for rows."""
     long = dict(max_pages=4000, split_rows=64)
-    assert tree_workspace_bytes(_step(max_visible=200, **long)) < tree_workspace_bytes(_step(**long))
     assert tree_workspace_bytes(_step(window=200, **long)) < tree_workspace_bytes(_step(**long))
+    assert tree_workspace_bytes(_step(max_pages=4000)) == tree_workspace_bytes(_step())
     assert tree_workspace_bytes(_linear(split_rows=32)) > tree_workspace_bytes(_linear(split_rows=64))
 
 
 @pytest.mark.parametrize("kw", [
     dict(batch=0), dict(batch=257), dict(nodes=0), dict(nodes=65), dict(num_q_heads=9), dict(num_q_heads=34), dict(num_kv_heads=0),
     dict(head_dim=64), dict(window=-1), dict(window=4), dict(num_pages=0), dict(num_pages=2 ** 22 + 1), dict(page_rows=8),
-    dict(page_rows=24), dict(page_rows=8192), dict(max_pages=-1), dict(max_pages=2 ** 20 + 1), dict(table_stride=9),
+    dict(page_rows=24), dict(page_rows=8192), dict(max_pages=-1), dict(max_pages=2 ** 19, page_rows=4096),
+    dict(max_pages=2 ** 19 - 1, page_rows=4096, split_rows=32), dict(max_pages=2 ** 20 + 1), dict(table_stride=9),
     dict(page_stride=2 * 16 * 128 - 8), dict(head_stride=16 * 128 + 4), dict(head_stride=8), dict(page_stride=-8),
-    dict(page_stride=2 ** 60), dict(max_visible=-1), dict(split_rows=16), dict(split_rows=-32), dict(scale=0.0),
+    dict(page_stride=2 ** 60), dict(split_rows=16), dict(split_rows=-32), dict(scale=0.0),
     dict(scale=math.nan), dict(scale=math.inf), dict(batch=256, nodes=64, num_q_heads=16 * 64, num_kv_heads=64),
 ])
 def test_bad_descriptions_are_refused(kw):
@@ -112,8 +114,7 @@ def test_front_end_refuses_wrong_tensors():
         TreeCall(linear, **good)
 
 
-@pytest.mark.parametrize("kw", [dict(page_rows=2 ** 32 + 16), dict(max_pages=2 ** 32), dict(window=2 ** 32 + 64), dict(split_rows=2 ** 32),
-                                dict(max_visible=2 ** 32 + 1)])
+@pytest.mark.parametrize("kw", [dict(page_rows=2 ** 32 + 16), dict(max_pages=2 ** 32), dict(window=2 ** 32 + 64), dict(split_rows=2 ** 32)])
 def test_values_that_a_description_would_wrap_are_refused(kw):
     with pytest.raises(ValueError):
         _step(**kw).desc()
@@ -121,6 +122,7 @@ def test_values_that_a_description_would_wrap_are_refused(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(batch=256, nodes=64, num_q_heads=32, num_kv_heads=4, head_dim=512, max_pages=2 ** 18, num_pages=2 ** 22, page_rows=4096),
+    dict(max_pages=2 ** 19 - 1, page_rows=4096, split_rows=2 ** 23),
     dict(batch=1, nodes=1, num_q_heads=1, num_kv_heads=1, max_pages=1), dict(max_pages=2 ** 20, page_rows=1024),
     dict(batch=256, num_q_heads=512, num_kv_heads=32, max_pages=2 ** 16), dict(batch=1, nodes=64, max_pages=2 ** 20, window=2 ** 30),
     dict(batch=1, num_pages=1, page_rows=2 ** 30, max_pages=0),
@@ -131,3 +133,18 @@ def test_extreme_descriptions_plan_quickly(kw):
     n = tree_workspace_bytes(step)
     assert time.perf_counter() - t < 0.25
     assert 512 <= n <= 4096 + step.batch * 4 + 600 * step.batch * step.nodes * step.num_q_heads * (4 * step.head_dim + 8)
+
+
+def test_the_pieces_of_random_batches(tmp_path):
+    """esda_tree_plan.h: every key in one piece, and no more pieces than the host makes room for."""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "tree_plan_check"
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
+                        os.path.join(root, "apertura_amd", "csrc"), os.path.join(root, "tests", "tree_plan_check.cpp"), "-o", str(exe)],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr

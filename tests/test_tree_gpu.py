@@ -50,7 +50,7 @@ class Case:
     """lengths: committed rows of each sequence.  page 0: linear caches of `cap` rows."""
 
     def __init__(self, T, hq, hkv, D, lengths, page=16, shared=False, window=0, parent=None, cap=0, split_rows=0,
-                 max_visible=0, spare=0, gap=0, seed=0):
+                 spare=0, gap=0, seed=0):
         g = _gen(seed)
         B = len(lengths)
         self.B, self.T, self.hq, self.hkv, self.D, self.page, self.shared, self.window = B, T, hq, hkv, D, page, shared, window
@@ -79,7 +79,7 @@ class Case:
                     part = rows[:, k * R:min(n, (k + 1) * R)]
                     plane[int(self.table[b, k]) if page else b, :, :part.shape[1]] = part
         self.length = torch.tensor(lengths, dtype=torch.int32, device=DEV)
-        kw = dict(window=window, kv_shared=shared, scale=D ** -0.5, split_rows=split_rows, max_visible=max_visible)
+        kw = dict(window=window, kv_shared=shared, scale=D ** -0.5, split_rows=split_rows)
         self.step = TreeStep.for_pages(self.pool[0], self.table, hq, T, **kw) if page else \
             TreeStep.for_cache(self.pool[0], hq, T, **kw)
 
@@ -194,9 +194,13 @@ def test_long_sequences(D, hq, hkv, shared, T):
     Case(T, hq, hkv, D, [5000, 2111], 16, shared, split_rows=64, gap=1, seed=T).run()
 
 
-@pytest.mark.parametrize("D,hq,hkv,shared", [(128, 8, 2, False), (512, 8, 1, True)])
-def test_a_low_estimate_of_rows(D, hq, hkv, shared):
-    Case(3, hq, hkv, D, [900, 20], 16, shared, max_visible=40, seed=1).run()
+@pytest.mark.parametrize("T", [1, 3, 30])
+@pytest.mark.parametrize("D,hq,hkv,shared", [(128, 8, 2, False), (256, 4, 2, False), (512, 8, 1, True)])
+def test_ragged_batches(D, hq, hkv, shared, T):
+    """One sequence far longer than the others; tables with much more room than rows; more than 64
+    sequences, the long one among the last."""
+    Case(T, hq, hkv, D, [9000, 2, 20, 0, 77], 16, shared, parent=random_parents(5, T, 1), spare=300, seed=1).run()
+    Case(T, hq, hkv, D, [n % 37 for n in range(130)] + [4000, 1], 16, shared, seed=2).run()
 
 
 @pytest.mark.parametrize("D,hq,hkv,shared", [(128, 8, 8, False), (256, 8, 4, False), (512, 8, 1, True)])
