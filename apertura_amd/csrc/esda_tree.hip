@@ -242,60 +242,60 @@ const char *check_desc(const esda_tree_desc *d) {
 }
 
 // How the query rows of a kv head can be laid out: as tiles (nw > 0: a prefill form), or in runs of 16 ng
-// rows.  us of a workgroup: `start`, and `per_kb` per KB of K and V; slots: workgroups the GPU holds at once.
+// rows.  slots: workgroups the GPU holds at once; stage: us of one for 32 keys.
 struct Form {
-    int qb, kh, nw, ng;
-    float start, per_kb;
-    int slots;
+    int qb, kh, nw, ng, slots;
+    float stage;
     int rows() const { return ng ? 16 * ng : 16 * qb * (kh ? nw / 2 : nw); }
 };
+constexpr Form kRun128 = {0, 0, 0, 1, 512, 0.25f}, kRun128x2 = {0, 0, 0, 2, 512, 0.3f}, kTile128 = {2, 0, 4, 0, 512, 1.2f};
+constexpr Form kRun256 = {0, 0, 0, 1, 256, 0.5f}, kTile256 = {1, 0, 8, 0, 256, 1.0f}, kTile256Half = {1, 1, 8, 0, 256, 0.8f};
+constexpr Form kRun512 = {0, 0, 0, 1, 256, 0.8f}, kTile512 = {1, 0, 8, 0, 256, 1.6f}, kTile512Half = {1, 0, 4, 0, 256, 1.6f};
 
-// The forms a step of `rows` query rows a kv head may take; returns their number.
-int forms_of(int D, int rows, bool shared, Form *f) {
-    int n = 0;
-    const float stage_kb = 32.0f * 2 * D * (shared ? 1 : 2) / 1024;
-    auto tile = [&](const Tiling &t, float more, float times) {
-        f[n++] = {t.qb, t.kh, t.nw, 0, t.wg + t.row * std::min(rows, t.rows()) + more, t.stage / stage_kb * times, 256 * t.occ};
-    };
-    if (D == 512) {
-        if (rows > 64 || shared == false) tile(kTilings512[0], 1.8f, 1.02f);
-        if (rows > 64 || shared) tile(kTilings512[1], 0.0f, 0.96f);  // (launch_tiles' choice for one tile)
-        f[n++] = {0, 0, 0, 1, 8.0f, 1 / 54.0f, 256};
-    } else if (D == 256) {
-        tile(kTilings256[1], -0.7f, 1.47f);
-        tile(kTilings256[2], -1.0f, 1.63f);
-        f[n++] = {0, 0, 0, 1, 4.6f, 1 / 65.0f, 256};
-    } else {
-        tile(kTilings128Scored[0], 0.0f, 1.6f);
-        f[n++] = {0, 0, 0, 1, 5.8f, 1 / 65.0f, 512};
-        if (rows > 16) f[n++] = {0, 0, 0, 2, 13.2f, 1 / 56.0f, 512};
-        if (rows > 32) f[n++] = {0, 0, 0, 4, 13.1f, 1 / 32.0f, 256};
+// The form of a step of `rows` query rows a kv head over caches with room for `room` bytes of keys and
+// values (the host does not know how many are there).  Up to 16 rows a run reads every key once; more
+// take a run's rows again for each 16, or fill a tile, which starts later.  Of 2,170 random steps (1 .. 64
+// sequences and nodes, 32 .. 49,152 rows, a quarter to all of the room filled), times over the fastest
+// form's, below 10 MB / below 100 / above:
+//   D = 128  17 .. 32 rows   run 1.00 / 1.06 / 1.21   two blocks a run 1.15 / 1.03 / 1.00   tile 1.15 / 1.12 / 1.13
+//            33 .. 64            1.00 / 1.07 / 1.40                    1.16 / 1.04 / 1.06        1.22 / 1.09 / 1.01
+//            65 .. 256           1.05 / 1.27 / 1.8                     1.16 / 1.09 / 1.2         1.33 / 1.03 / 1.00
+//            more                1.14 / 1.47                           1.10 / 1.21               1.21 / 1.00
+//   D = 256  up to 16        run 1.01 / 1.00 / 1.00   tile of 64 rows 1.06 / 1.09 / 1.14    of 128 1.03 / 1.10 / 1.26
+//            17 .. 64            1.05 / 1.07 / 1.30                   1.09 / 1.02 / 1.00           1.06 / 1.03 / 1.10
+//            more                1.26 / 1.65 / 2.0                    1.06 / 1.03 / 1.09           1.18 / 1.07 / 1.00
+//   D = 512  up to 16        run 1.00 / 1.00 / 1.00   tile of 64 rows 1.11 / 1.16 / 1.32
+//            17 .. 32            1.03 / 1.00 / 1.02                   1.18 / 1.10 / 1.05   (K and V apart, tile of 128: 1.00, run 1.2)
+//            33 .. 64            1.05 / 1.18 / 1.50                   1.23 / 1.03 / 1.00
+//            65 .. 128           1.08 / 1.3  / 1.8                    1.17 / 1.02 / 1.25    of 128 1.31 / 1.05 / 1.00
+//            more                1.1  / 1.7  / 2.3                    1.15 / 1.2  / 1.5            1.3  / 1.00 / 1.00
+Form pick(int D, int rows, bool shared, float room) {
+    const bool small = room <= 1e7f, large = room > 1e8f;
+    if (D == 128) {
+        if (rows <= 16) return kRun128;
+        if (small) return rows <= 256 ? kRun128 : kRun128x2;
+        return rows <= (large ? 32 : 64) ? kRun128x2 : kTile128;
     }
-    return n;
+    if (D == 256) {
+        if (rows <= 16) return kRun256;
+        return rows <= 64 || !large ? kTile256Half : kTile256;
+    }
+    if (rows <= 16 || (small && rows <= 256) || (rows <= 32 && shared)) return kRun512;
+    if (rows <= 64) return shared ? kTile512Half : kTile512;  // (launch_tiles' choice for one tile)
+    return small || (rows <= 128 && !large) ? kTile512Half : kTile512;
 }
 
-// Runs up to 16 query rows, ..
-int pick(int D, int rows, bool shared, const Form *f, int nf) {
-    (void) shared;
-    auto find = [&](int ng, int rows_of) {
-        for (int i = 0; i < nf; ++i)
-            if (f[i].ng == ng && (ng || f[i].rows() == rows_of)) return i;
-        return 0;
-    };
-    if (rows <= 16) return find(1, 0);
-    if (D == 128) return rows <= 32 ? find(2, 0) : find(0, 128);
-    if (D == 256) return rows <= 64 ? find(0, 64) : find(0, 128);
-    return rows <= 32 ? find(1, 0) : find(0, rows > 64 || !shared ? 128 : 64);
-}
-
-// The form of a step, and how many pieces its keys are to make: the host does not know the lengths, so
-// it asks for as many workgroups as the GPU holds at once (esda_tree_plan.h shares the keys out).
+// The form of a step, and how many pieces its keys are to make (esda_tree_plan.h shares them out): at most
+// as many workgroups as the GPU holds at once.  Fewer where the room for keys is little: k pieces of a full
+// sequence take t / k, but a second launch (4 us) and k partials of every row, written and read back (at 4
+// TB/s); then k = sqrt(t / what one partial of all rows takes), or a single piece.  (As many pieces as
+// fit, whatever the room: 12 sequences of 39 rows, 64 nodes, D = 128, 32.8 us, with one each 19.7.)
 void choose(const esda_tree_desc *d, long long most, TreeParams *p) {
     const int D = d->head_dim, rows = p->Sq * p->G;
+    const bool shared = d->kv_shared != 0;
     const long long pairs = (long long) p->B * p->Hkv;
-    Form f[4];
-    const int nf = forms_of(D, rows, d->kv_shared != 0, f);
-    const Form &x = f[pick(D, rows, d->kv_shared != 0, f, nf)];
+    const float room = (float) (most * pairs) * 2.0f * D * (shared ? 1 : 2);
+    const Form x = pick(D, rows, shared, room);
     p->qb = x.qb;
     p->kh = x.kh;
     p->nw = x.nw;
@@ -308,12 +308,13 @@ void choose(const esda_tree_desc *d, long long most, TreeParams *p) {
         p->share = 1;
         units = pairs * p->splits;
     } else {
-        p->least = 2;
-        p->share = std::max(1, (int) (x.slots / ((long long) p->Hkv * p->tiles)));
-        const bool split = p->share > p->B;
-        if (!split) p->share = p->B;
+        p->least = rows <= 64 ? 2 : rows <= 256 ? 4 : 8;
+        const float t = (float) most / kStageKeys * x.stage, part = 5.0e-7f * 4 * D * (float) (pairs * rows);
+        const float k = std::min((float) x.slots / (float) (pairs * p->tiles), std::sqrt(t / part));
+        const bool split = k > 1.0f && t / k + 4.0f + part * k < t;
+        p->share = split ? std::max(p->B + 1, (int) (k * p->B)) : p->B;
         p->splits = split ? p->share : 1;
-        units = split ? (long long) p->share * p->Hkv : pairs;
+        units = (long long) p->share * p->Hkv;
     }
     p->units = (int) std::min<long long>((units + 7) / 8 * 8, INT_MAX);
 }
@@ -386,7 +387,6 @@ hipError_t launch_step(const TreeParams &p, bool shared, hipStream_t st) {
         if (p.run_groups == 1) run(std::integral_constant<int, 1>{});
         if constexpr (D == 128) {
             if (p.run_groups == 2) run(std::integral_constant<int, 2>{});
-            if (p.run_groups == 4) run(std::integral_constant<int, 4>{});
         }
     } else {
         esda_detail::tree_tiles(p, D, st);

@@ -35,10 +35,10 @@ def test_workspace_holds_every_partial():
 
 
 def test_bounds_on_rows_size_the_splits():
-    """A window, of which a sequence sees no more; automatic splits do not go by the room for rows."""
+    """A window, of which a sequence sees no more; automatic splits of long caches do not go by the room for rows."""
     long = dict(max_pages=4000, split_rows=64)
     assert tree_workspace_bytes(_step(window=200, **long)) < tree_workspace_bytes(_step(**long))
-    assert tree_workspace_bytes(_step(max_pages=4000)) == tree_workspace_bytes(_step())
+    assert tree_workspace_bytes(_step(nodes=4, max_pages=8000)) == tree_workspace_bytes(_step(nodes=4, max_pages=4000))
     assert tree_workspace_bytes(_linear(split_rows=32)) > tree_workspace_bytes(_linear(split_rows=64))
 
 
