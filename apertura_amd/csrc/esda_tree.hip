@@ -268,21 +268,25 @@ constexpr Form kRun512 = {0, 0, 0, 1, 256, 0.8f}, kTile512 = {1, 0, 8, 0, 256, 1
 //            17 .. 32            1.03 / 1.00 / 1.02                   1.18 / 1.10 / 1.05   (K and V apart, tile of 128: 1.00, run 1.2)
 //            33 .. 64            1.05 / 1.18 / 1.50                   1.23 / 1.03 / 1.00
 //            65 .. 128           1.08 / 1.3  / 1.8                    1.17 / 1.02 / 1.25    of 128 1.31 / 1.05 / 1.00
-//            more                1.1  / 1.7  / 2.3                    1.15 / 1.2  / 1.5            1.3  / 1.00 / 1.00
-Form pick(int D, int rows, bool shared, float room) {
+//            more                1.1  / 1.7  / 2.3                    1.15 / 1.2  / 1.5            1.3  / 1.00 / 1.00;
+// and a form whose workgroups do not fit the GPU at once, for `pairs` sequences and kv heads, gives way to
+// one of more rows (12 sequences of 59 rows, 64 nodes, D = 128: 31.4 us in runs, 19.1 in tiles).
+Form pick(int D, int rows, bool shared, float room, long long pairs) {
     const bool small = room <= 1e7f, large = room > 1e8f;
+    auto fits = [&](const Form &f) { return pairs * ((rows + f.rows() - 1) / f.rows()) <= f.slots; };
     if (D == 128) {
         if (rows <= 16) return kRun128;
-        if (small) return rows <= 256 ? kRun128 : kRun128x2;
+        if (small && rows <= 256 && fits(kRun128)) return kRun128;
+        if (small && fits(kRun128x2)) return kRun128x2;
         return rows <= (large ? 32 : 64) ? kRun128x2 : kTile128;
     }
     if (D == 256) {
         if (rows <= 16) return kRun256;
-        return rows <= 64 || !large ? kTile256Half : kTile256;
+        return rows <= 64 || (!large && fits(kTile256Half)) ? kTile256Half : kTile256;
     }
-    if (rows <= 16 || (small && rows <= 256) || (rows <= 32 && shared)) return kRun512;
+    if (rows <= 16 || (rows <= 32 && shared) || (small && rows <= 256 && fits(kRun512))) return kRun512;
     if (rows <= 64) return shared ? kTile512Half : kTile512;  // (launch_tiles' choice for one tile)
-    return small || (rows <= 128 && !large) ? kTile512Half : kTile512;
+    return (small || (rows <= 128 && !large)) && fits(kTile512Half) ? kTile512Half : kTile512;
 }
 
 // The form of a step, and how many pieces its keys are to make (esda_tree_plan.h shares them out): at most
@@ -295,7 +299,7 @@ void choose(const esda_tree_desc *d, long long most, TreeParams *p) {
     const bool shared = d->kv_shared != 0;
     const long long pairs = (long long) p->B * p->Hkv;
     const float room = (float) (most * pairs) * 2.0f * D * (shared ? 1 : 2);
-    const Form x = pick(D, rows, shared, room);
+    const Form x = pick(D, rows, shared, room, pairs);
     p->qb = x.qb;
     p->kh = x.kh;
     p->nw = x.nw;
