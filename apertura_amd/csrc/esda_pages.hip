@@ -76,7 +76,13 @@ __device__ __forceinline__ bool named_before(const int *list, int i) {
     return __syncthreads_or(found);
 }
 
-// `chunks` 16-byte pieces by the lanes of a wave, eight loads in flight each.
+// `chunks` 16-byte pieces by the lanes of a wave, eight loads in flight each.  LOADED / STORED: past the
+// caches.  Pages are written so: nothing reads them soon, and they push out what is (a prompt's 4095 rows of
+// 16 heads x 256, K and V, 134 MB, 32.0 us with plain stores, 23.4); rows that are read out are used next,
+// and written plainly (32,767 of 4 x 512, 268 MB, 45.6 us, 54.1 past the caches).  Pages that move are not
+// read again (16 slots' pool, 473 MB: 104.8 us plain, 101.8 with such stores, 98.3 with such loads too);
+// those that are forked are, by the next child.
+template <bool LOADED, bool STORED>
 __device__ __forceinline__ void wave_copy(uint16_t *dst, const uint16_t *src, int chunks, int lane) {
     constexpr int U = 8;
     const u32x4 *s = reinterpret_cast<const u32x4 *>(src);
@@ -85,10 +91,13 @@ __device__ __forceinline__ void wave_copy(uint16_t *dst, const uint16_t *src, in
         u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c + 64 * u < chunks) v[u] = s[c + 64 * u];
+            if (c + 64 * u < chunks) v[u] = LOADED ? __builtin_nontemporal_load(s + c + 64 * u) : s[c + 64 * u];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c + 64 * u < chunks) d[c + 64 * u] = v[u];
+            if (c + 64 * u < chunks) {
+                if constexpr (STORED) __builtin_nontemporal_store(v[u], d + c + 64 * u);
+                else d[c + 64 * u] = v[u];
+            }
     }
 }
 
@@ -113,6 +122,7 @@ __device__ __forceinline__ Piece piece_of(const Params &p, unsigned i) {
 }
 
 // The listed moves, a wave to a piece.
+template <bool LOADED>
 __device__ void carry_out(const Params &p) {
     if (p.num_pools == 0) return;
     const int lane = threadIdx.x & 63;
@@ -125,7 +135,7 @@ __device__ void carry_out(const Params &p) {
         const int rows = min(mv[2] - x.row, min(p.R, x.pool->rows_per_piece()));
         if (rows <= 0) continue;
         uint16_t *const base = x.pool->data + x.at;
-        wave_copy(base + (long long) mv[1] * x.pool->page_stride, base + (long long) mv[0] * x.pool->page_stride, rows * x.pool->D / 8, lane);
+        wave_copy<LOADED, true>(base + (long long) mv[1] * x.pool->page_stride, base + (long long) mv[0] * x.pool->page_stride, rows * x.pool->D / 8, lane);
     }
 }
 
@@ -344,7 +354,7 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(Params p, int n) {
         for (int k = threadIdx.x; k < p.P; k += 256) to[k] = row[k];
         if (threadIdx.x == 0) p.length[e.dst] = e.state == kFailed ? 0 : e.rows;
     }
-    carry_out(p);
+    carry_out<false>(p);
 }
 
 // Compaction, first launch, one workgroup: the pages in use at or above their number, and the free ones
@@ -401,7 +411,7 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(Params p) {
         const int id = *at;
         if (id >= live && id < p.N) *at = p.ids[id];
     }
-    carry_out(p);
+    carry_out<true>(p);
 }
 
 // ---- rows in and out
@@ -444,7 +454,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsParams p) {
         uint16_t *const page = p.pool.data + plane * p.pool.plane_stride + (long long) id * p.pool.page_stride +
                                head * p.pool.head_stride + (i & (p.R - 1)) * p.pool.D;
         uint16_t *const rows = p.linear + plane * p.plane_stride + b * p.seq_stride + head * p.head_stride + (i - first) * p.pool.D;
-        wave_copy(WRITE ? page : rows, WRITE ? rows : page, (int) (j - i) * p.pool.D / 8, lane);
+        wave_copy<false, WRITE>(WRITE ? page : rows, WRITE ? rows : page, (int) (j - i) * p.pool.D / 8, lane);
     }
 }
 
