@@ -68,12 +68,19 @@ __device__ __forceinline__ bool is_page(int id, int N) { return (unsigned) id < 
 
 __device__ __forceinline__ void add(int *at, int by) { __hip_atomic_fetch_add(at, by, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// Whether list[i] stands in list before i; every thread of the workgroup calls it.
-__device__ __forceinline__ bool named_before(const int *list, int i) {
+// W threads that work on an entry: a wave, or a workgroup of 256.
+template <int W>
+__device__ __forceinline__ bool any_of(bool x) {
+    if constexpr (W == 64) return __builtin_amdgcn_ballot_w64(x) != 0ull;
+    else return __syncthreads_or(x);
+}
+// Whether list[i] stands in list before i; every one of the W threads, numbers t, calls it.
+template <int W>
+__device__ __forceinline__ bool named_before(const int *list, int i, int t) {
     const int x = list[i];
     bool found = false;
-    for (int j = threadIdx.x; j < i; j += blockDim.x) found = found || list[j] == x;
-    return __syncthreads_or(found);
+    for (int j = t; j < i; j += W) found = found || list[j] == x;
+    return any_of<W>(found);
 }
 
 // `chunks` 16-byte pieces by the lanes of a wave, eight loads in flight each.  LOADED / STORED: past the
@@ -164,6 +171,11 @@ __device__ __forceinline__ Scan scan(int x) {
     return {before + in - x, total};
 }
 
+// A page's references as the atomics have left them, past the caches of this CU.
+__device__ __forceinline__ int references(const Params &p, int id) {
+    return __hip_atomic_load(p.refs + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // The lowest `need` free pages in order, put(rank, page) for each; how many there are (at most need).
 template <class Put>
 __device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put) {
@@ -174,7 +186,7 @@ __device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int id = base + 4 * (int) threadIdx.x + e;
-            free[e] = id < p.N && p.refs[id] == 0;
+            free[e] = id < p.N && references(p, id) == 0;
             n += free[e];
         }
         const Scan s = scan(n);
@@ -195,7 +207,7 @@ __device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put)
 // A workgroup per entry.
 __global__ __launch_bounds__(256) void free_kernel(Params p, const int *slots) {
     const int i = blockIdx.x, s = slots[i];
-    const bool twice = named_before(slots, i);
+    const bool twice = named_before<256>(slots, i, threadIdx.x);
     if (twice || (unsigned) s >= (unsigned) p.S) {
         if (threadIdx.x == 0) add(&p.head->left_out, 1);
         return;
@@ -262,13 +274,13 @@ __global__ __launch_bounds__(kOneGroup) void reserve_kernel(Params p, const int 
     }
 }
 
-// A fork, first launch: a workgroup per entry.  References of what it shares and gives up, the new row
-// of its table (dst's may be another's source), and what is left to copy.  The page to copy from holds a
-// reference more until the free pages are given out, so that it is none of them.
-__global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, const int *dst, const int *rows) {
-    const int i = blockIdx.x, s = src[i], d = dst[i];
-    Entry &entry = p.entries[i];
-    const bool twice = named_before(dst, i);
+// An entry of a fork, by W threads: references of what it shares and gives up, the new row of its table
+// (dst's may be another's source), and what is left to copy.  The page to copy from holds a reference more
+// until the free pages are given out, so that it is none of them.
+template <int W>
+__device__ Entry fork_entry(const Params &p, const int *src, const int *dst, const int *rows, int i, int t) {
+    const int s = src[i], d = dst[i];
+    const bool twice = named_before<W>(dst, i, t);
     bool ok = !twice && (unsigned) s < (unsigned) p.S && (unsigned) d < (unsigned) p.S;
     int len = 0, r = 0;
     if (ok) {
@@ -280,19 +292,16 @@ __global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, con
     const int *const from = p.table + (long long) (ok ? s : 0) * p.table_stride;
     bool there = true;
     if (ok)
-        for (int k = threadIdx.x; k < full + (part > 0); k += 256) there = there && is_page(from[k], p.N);
-    if (__syncthreads_or(!there) || !ok) {
-        if (threadIdx.x == 0) {
-            add(&p.head->left_out, 1);
-            entry = Entry{kLeftOut, 0, 0, 0};
-        }
-        return;
+        for (int k = t; k < full + (part > 0); k += W) there = there && is_page(from[k], p.N);
+    if (any_of<W>(!there) || !ok) {
+        if (t == 0) add(&p.head->left_out, 1);
+        return Entry{kLeftOut, 0, 0, 0};
     }
     // a cut within the page of the sequence's own last rows keeps that page
     const bool keep = s == d && part > 0 && full == len >> p.shift;
     const int *const old = p.table + (long long) d * p.table_stride;
     int *const row = p.rows + (long long) i * p.P;
-    for (int k = threadIdx.x; k < p.P; k += 256) {
+    for (int k = t; k < p.P; k += W) {
         const int was = old[k];
         int is = -1;
         if (k < full || (keep && k == full)) {
@@ -302,23 +311,21 @@ __global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, con
         if (is_page(was, p.N) && !(s == d && is >= 0)) add(p.refs + was, -1);
         row[k] = is;
     }
-    if (threadIdx.x == 0) {
-        const bool copies = part > 0 && !keep;
-        entry = Entry{copies ? kNeedsPage : kShared, d, r, copies ? (s == d ? ~from[full] : from[full]) : 0};
-        if (copies) add(p.refs + from[full], 1);
-    }
+    const bool copies = part > 0 && !keep;
+    const int tail = copies ? from[full] : 0;
+    if (copies && t == 0) add(p.refs + tail, 1);
+    return Entry{copies ? kNeedsPage : kShared, d, r, copies && s == d ? ~tail : tail};
 }
 
-// .. second launch, one workgroup: a free page for every entry that copies.  (As the work of the first
-// launch's last workgroup, behind fences for what the others wrote, a fork of 4 took 5 us more, of 32 10.)
-__global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) {
+// A free page for every entry that copies, by a workgroup of kOneGroup; the entries as the copy takes them.
+__device__ void fork_pages(const Params &p, const Entry *entries, int n) {
     __shared__ int ids[ESDA_MAX_ENTRIES];
     const int t = threadIdx.x;
-    const Entry e = t < n ? p.entries[t] : Entry{kLeftOut, 0, 0, 0};
+    Entry e = t < n ? entries[t] : Entry{kLeftOut, 0, 0, 0};
     const int tail = e.tail < 0 ? ~e.tail : e.tail, full = e.rows >> p.shift;
     int *const row = p.rows + (long long) t * p.P;
     bool needs = e.state == kNeedsPage;
-    if (needs && e.tail < 0 && p.refs[tail] == 1) {  // a sequence cut within a page that nobody else holds or copies
+    if (needs && e.tail < 0 && references(p, tail) == 1) {  // a sequence cut within a page that nobody else holds or copies
         row[full] = tail;
         needs = false;
     }
@@ -338,13 +345,36 @@ __global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) 
                 add(p.refs + row[k], -1);
                 row[k] = -1;
             }
-            p.entries[t].state = kFailed;
+            e.state = kFailed;
         }
     }
+    if (t < n) p.entries[t] = e;
     if (t == 0) p.head->moves = got;
 }
 
-// .. third: the tables, and the rows of the last pages.
+// A fork's decisions: of a small one in one launch, a wave to an entry; else in two, a workgroup to an
+// entry and then one for the free pages.  (4 children of 32 pages, and their next page: 15.0 us in two, 13.9
+// in one; 32 children of 79, two to a wave: 19.5 and 25.6.  As the work of the last workgroup of the first of
+// two, behind fences for what the others wrote, the free pages took 5 and 10 us more.)
+constexpr int kSmallFork = kOneGroup / 64, kSmallForkTable = 256;  // entries, pages of each
+__global__ __launch_bounds__(kOneGroup) void fork_small_kernel(Params p, const int *src, const int *dst, const int *rows, int n) {
+    __shared__ Entry entries[kSmallFork];
+    const int lane = threadIdx.x & 63;
+    for (int i = uniform(threadIdx.x >> 6); i < n; i += kOneGroup / 64) {
+        const Entry e = fork_entry<64>(p, src, dst, rows, i, lane);
+        if (lane == 0) entries[i] = e;
+    }
+    ESDA_WAIT_VM(0);  // references and rows are written
+    __syncthreads();
+    fork_pages(p, entries, n);
+}
+__global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, const int *dst, const int *rows) {
+    const Entry e = fork_entry<256>(p, src, dst, rows, blockIdx.x, threadIdx.x);
+    if (threadIdx.x == 0) p.entries[blockIdx.x] = e;
+}
+__global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) { fork_pages(p, p.entries, n); }
+
+// .. and what follows from them: the tables, and the rows of the last pages.
 __global__ __launch_bounds__(256) void fork_copy_kernel(Params p, int n) {
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         const Entry e = p.entries[i];
@@ -746,8 +776,12 @@ int esda_pages_fork(const esda_pages *c, const int32_t *src, const int32_t *dst,
     if (const int rc = esda_detail::check_device()) return rc;
     if (n == 0) return ESDA_OK;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(fork_kernel, dim3(n), dim3(256), 0, st, p, src, dst, rows);
-    hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kOneGroup), 0, st, p, n);
+    if (n <= kSmallFork && p.P <= kSmallForkTable) {
+        hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kOneGroup), 0, st, p, src, dst, rows, n);
+    } else {
+        hipLaunchKernelGGL(fork_kernel, dim3(n), dim3(256), 0, st, p, src, dst, rows);
+        hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kOneGroup), 0, st, p, n);
+    }
     hipLaunchKernelGGL(fork_copy_kernel, dim3(std::max<unsigned>(n, copy_groups(p, n))), dim3(256), 0, st, p, n);
     return launched(call);
 }

@@ -360,3 +360,26 @@ def test_a_stream_of_its_own():
     b.model.reserve([2], [40])
     b.model.compact()
     b.check()
+
+
+@pytest.mark.parametrize("S,most,n", [(200, 8, 90), (200, 8, 17), (200, 8, 16), (12, 300, 8), (12, 255, 9), (1100, 3, 1024)])
+def test_forks_of_many_entries_and_pages(S, most, n):
+    """More than 16 entries or 256 pages a slot, where the decisions take two launches, and fewer; entries that
+    are left out among them."""
+    R, held = 16, 40 if most > 8 else 6
+    rng = random.Random(n)
+    lengths = [rng.randrange(0, (most - 1) * R) if s < held else 0 for s in range(S)]
+    N = sum((x + R - 1) // R for x in lengths) + n // 2 + 3
+    b = _filled(POOLS[0], N, R, S, most, lengths[:held])
+    src = [rng.randrange(-1, held) for _ in range(n)]
+    dst = rng.sample(range(-2, S), n)
+    dst[3] = dst[1]
+    b.call("fork", src, dst, [rng.randrange(-2, most * R) for _ in range(n)])
+    b.check()
+    b.call("fork", dst[:held], src[:held], None)
+    b.check()
+    slots = rng.sample(range(S), min(n, S))
+    b.call("reserve", slots, [rng.randrange(0, 60) for _ in slots])
+    b.check()
+    b.call("free", [s for s in range(S) if s % 3][:1024])
+    b.check()
