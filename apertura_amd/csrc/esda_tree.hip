@@ -434,6 +434,25 @@ int esda_tree_decode(const esda_tree_desc *d, const esda_tree_args *a, void *str
     if ((d->max_pages == 0) != (a->table == nullptr)) return refuse("a table goes with pages, and only with them");
     if (!a->length || !aligned(a->length, 4) || !aligned(a->table, 4) || !aligned(a->parent, 4))
         return refuse("table, length and parent must be 4-byte aligned device memory");
+    // What is written must not be what is read: rows of q are read again after rows of out are written, and
+    // the new rows while they are written to the pages.
+    struct Range {
+        const void *at;
+        size_t bytes;
+        bool meets(const Range &o) const {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+            return a < b + o.bytes && b < a + bytes;
+        }
+    };
+    const size_t token = (size_t) d->batch * d->nodes * d->head_dim * 2;
+    const size_t extent = 2 * ((size_t) (d->num_pages - 1) * d->page_stride + (size_t) (d->num_kv_heads - 1) * d->head_stride +
+                               (size_t) d->page_rows * d->head_dim);
+    const Range out{a->out, token * d->num_q_heads}, k_new{a->k_new, token * d->num_kv_heads},
+        v_new{shared ? a->k_new : a->v_new, token * d->num_kv_heads}, k_pages{a->k_pages, extent}, v_pages{a->v_pages, extent};
+    for (const Range &x : {Range{a->q, out.bytes}, k_new, v_new, k_pages, v_pages})
+        if (out.meets(x)) return refuse("out must not overlap q, the new rows or the pages");
+    for (const Range &x : {k_new, v_new})
+        if (x.meets(k_pages) || x.meets(v_pages)) return refuse("the new rows must not overlap the pages");
     if (!a->workspace || a->workspace_bytes < pl.bytes || !aligned(a->workspace, 16))
         return fail(ESDA_ERR_WORKSPACE, "esda_tree_decode: workspace missing or smaller than esda_tree_workspace_size");
     rc = esda_detail::check_device();

@@ -170,6 +170,7 @@ class PagedCache:
 def pages_status(workspace: torch.Tensor, stream=None) -> int:
     """Reads (synchronously) and clears the status word of a workspace of esda_pages.h or esda_tree.h."""
     n = ctypes.c_int32(0)
+    _same_device({"workspace": workspace})
     check(lib().esda_pages_status(workspace.data_ptr(), ctypes.byref(n), _stream_ptr(stream)))
     return int(n.value)
 

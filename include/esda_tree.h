@@ -19,7 +19,8 @@
  * step is given the same; esda_tree_commit moves it on.
  * A committed row whose table entry is no page is left out.  A sequence with a negative length, or one
  * whose nodes' rows do not all lie in its pages, is skipped: nothing is written for it, and it is
- * counted (esda_pages_status).  A value of k or v that is not finite reaches only the queries that see
+ * counted (esda_pages_status).  Pages of the nodes' rows belong to one sequence.  Calls that overlap need
+ * workspaces of their own.  A value of k or v that is not finite reaches only the queries that see
  * its row. */
 #ifndef APERTURA_ESDA_TREE_H
 #define APERTURA_ESDA_TREE_H
@@ -61,7 +62,8 @@ typedef struct esda_tree_args {
     const int32_t *table;  /* [B][max_pages] int32, device memory (linear: NULL)     */
     const int32_t *length; /* [B] int32, device memory: committed rows               */
     const int32_t *parent; /* [B, nodes] int32, device memory, or NULL: a chain      */
-    void *out;             /* [B, nodes, Hq, D] bf16; no overlap with the others     */
+    void *out;             /* [B, nodes, Hq, D] bf16; must not overlap q, the new rows or the pages, nor
+                              the new rows the pages                                 */
     void *workspace;       /* esda_tree_workspace_size bytes, 16-byte aligned; first 256 zeroed once */
     size_t workspace_bytes;
 } esda_tree_args;

@@ -67,15 +67,18 @@ def test_bad_linear_caches_are_refused(kw):
 def _call(step=None, nbytes=None, **kw):
     step = step or _step()
     d = step.desc()
-    a = dict(q=FAKE, k_new=FAKE, v_new=FAKE, k_pages=FAKE, v_pages=FAKE + (1 << 24), table=FAKE, length=FAKE, parent=None,
-             out=FAKE, workspace=FAKE, workspace_bytes=tree_workspace_bytes(step) if nbytes is None else nbytes)
+    a = dict(q=FAKE, k_new=FAKE + (1 << 22), v_new=FAKE + (2 << 22), k_pages=FAKE + (1 << 24), v_pages=FAKE + (2 << 24),
+             table=FAKE, length=FAKE, parent=None, out=FAKE + (3 << 22), workspace=FAKE, workspace_bytes=tree_workspace_bytes(step) if nbytes is None else nbytes)
     a.update(kw)
     return _lib.lib().esda_tree_decode(ctypes.byref(d), ctypes.byref(_lib.TreeArgs(**a)), None)
 
 
 @pytest.mark.parametrize("kw", [
     dict(q=None), dict(k_new=None), dict(v_new=None), dict(k_pages=None), dict(v_pages=None), dict(out=None), dict(length=None),
-    dict(table=None), dict(v_pages=FAKE), dict(q=FAKE + 8), dict(out=FAKE + 4), dict(v_new=FAKE + 2), dict(k_pages=FAKE + 8),
+    dict(table=None), dict(v_pages=FAKE + (1 << 24)), dict(q=FAKE + 8), dict(out=FAKE + 4),
+    dict(out=FAKE), dict(out=FAKE + 4 * 5 * 8 * 128 * 2 - 16), dict(out=FAKE + (1 << 22)), dict(out=FAKE + (2 << 22)),
+    dict(out=FAKE + (1 << 24) + 4096), dict(out=FAKE + (2 << 24) + 40 * 2 * 16 * 128 * 2 - 16), dict(k_new=FAKE + (1 << 24)),
+    dict(v_new=FAKE + (2 << 24) - 16), dict(v_new=FAKE + (1 << 24)), dict(v_new=FAKE + 2), dict(k_pages=FAKE + (1 << 24) + 8),
     dict(length=FAKE + 2), dict(table=FAKE + 2), dict(parent=FAKE + 1), dict(step=_linear()),
     dict(step=_step(kv_shared=True)),
 ])
@@ -84,6 +87,7 @@ def test_bad_arguments_are_refused(kw):
 
 
 def test_the_workspace_is_needed():
+    assert _call(out=FAKE + 4 * 5 * 8 * 128 * 2, workspace=None) == 4  # right behind q
     assert _call(workspace=None) == 4
     assert _call(workspace=FAKE + 8) == 4
     assert _call(nbytes=tree_workspace_bytes(_step()) - 1) == 4

@@ -367,3 +367,56 @@ def test_pages_past_32_bit_offsets():
         o, bound = attend64(q[0, :, h], k, k, seen, D ** -0.5)
         check(out[0, :, h], o, bound, f"head {h}")
     assert torch.equal(pool[0, N - 3, :, R - 4:R - 1], kn[0].transpose(0, 1))
+
+
+@pytest.mark.parametrize("D,hq,hkv,shared,T,lengths", [
+    (128, 32, 8, False, 1, [4000]), (128, 32, 8, False, 6, [4000, 900]), (128, 32, 8, False, 6, [300, 9]), (128, 16, 2, False, 64, [600] * 20),
+    (128, 32, 8, False, 16, [8000, 5000]), (128, 32, 8, False, 40, [9000, 100]), (128, 16, 16, True, 64, [3000]),
+    (256, 32, 16, False, 4, [5000, 11]), (256, 32, 16, False, 20, [6000, 3]), (256, 32, 16, False, 64, [9000, 4000]), (256, 16, 1, True, 64, [500, 2]),
+    (512, 32, 4, True, 2, [6000, 70]), (512, 32, 4, True, 4, [6000, 70]), (512, 32, 4, True, 8, [6000, 70]), (512, 32, 4, True, 12, [9000, 70]),
+    (512, 32, 4, True, 12, [20000, 13000]), (512, 32, 4, True, 64, [200] * 9), (512, 8, 8, False, 64, [3000, 17]), (512, 16, 2, False, 4, [9000]),
+    (512, 16, 4, False, 64, [700, 4000]), (512, 32, 4, True, 30, [300])])
+@pytest.mark.parametrize("window", [0, 1024])
+def test_every_form(D, hq, hkv, shared, T, lengths, window):
+    """The forms and splits that the rules choose between, with holes in the trees."""
+    Case(T, hq, hkv, D, lengths, 32, shared, window, parent=random_parents(len(lengths), T, T, 0.1), seed=T + D).run()
+
+
+@pytest.mark.parametrize("D,hq,hkv,shared,T,cap", [(128, 32, 8, False, 40, 20000), (256, 32, 16, False, 64, 9000), (256, 32, 16, False, 20, 9000),
+                                                   (512, 32, 4, True, 8, 9000), (512, 32, 4, True, 64, 9000), (512, 8, 4, False, 64, 9000)])
+def test_tiles_over_bad_pages_and_values(D, hq, hkv, shared, T, cap):
+    """What the tiles do about pages that are none and values that are not finite."""
+    parent = random_parents(2, T, 5)
+    parent[:, T - 3:] = torch.tensor([-2, T, T - 2], dtype=torch.int32)  # no nodes: two that are told so, one on such
+    c = Case(T, hq, hkv, D, [700, 90], 16, shared, parent=parent, spare=(cap - 700) // 16, seed=T)
+    G, before = hq // hkv, c.full.clone()
+    bad = 2
+    clean, clean_bound = c.exact(before, 1)
+    (c.kn if shared else c.vn)[0, bad, 1] = float("inf")
+    c.kn[1, 1, 0, 3] = float("nan")
+    held = c.table[0, 7].item()
+    c.table[0, 7] = -7
+    out = tree_decode(c.step, **c.args())
+    c.table[0, 7] = held
+    k = [torch.cat([p[c.table[0, :44].long()].transpose(0, 1).reshape(hkv, -1, D)[:, :700], n[0].transpose(0, 1)], 1)
+         for p, n in ((before[0], c.kn), (before[-1], c.kn if shared else c.vn))]
+    seen = torch.zeros((T, 700 + T), dtype=torch.bool, device=DEV)
+    for i, path in enumerate(c.paths[0]):
+        if path:
+            seen[i, :700] = True
+            seen[i, [700 + j for j in path]] = True
+    seen[:, 112:128] = False
+    for h in range(hkv):
+        sees = torch.tensor([h == 1 and bad in path for path in c.paths[0]], device=DEV)
+        kk, vv = k[0][h].clone(), k[1][h].clone()
+        if h == 1:  # (clean where the others look)
+            kk[700 + bad], vv[700 + bad] = 0.0, 0.0
+        o, bound = attend64(c.q[0, :, h * G:(h + 1) * G].reshape(T * G, D), kk, vv, seen.repeat_interleave(G, 0), D ** -0.5)
+        got = out[0, :, h * G:(h + 1) * G].reshape(T * G, D)
+        rest = (~sees).repeat_interleave(G)
+        check(got[rest], o[rest], bound[rest], f"kv head {h}")
+        assert not bool(torch.isfinite(got[~rest]).any())
+    for i, path in enumerate(c.paths[1]):
+        for h in range(hkv):
+            if 1 not in path or h != 0:
+                check(out[1, i, h * G:(h + 1) * G], clean[h, i], clean_bound[h, i], f"node {i} kv head {h}")
