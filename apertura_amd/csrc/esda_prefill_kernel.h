@@ -188,6 +188,9 @@ struct PRing {
 // read the range of ids of every 32-key stage: stages that hold no id of the tile's range are never
 // loaded, those that hold nothing but the tile's one id need no mask, and the ids of the others
 // come with their keys by DMA.
+// P = TreeParams (esda_tree.h): a unit of workgroups is one piece of the keys of one sequence and kv head
+// (tree_unit), its query rows the nodes' heads; a wave's DMAs fill one half of a stage, 16 rows of one page.
+// Stages that hold nodes, the window's edge or a page that is none are masked by the nodes' paths.
 template <int D, int QB, bool KH = false, bool SH = false, bool S2 = false, bool PS = false, int NW = kWaves,
           class P = PrefillParams>
 // (D == 128 on four waves: two workgroups per CU)

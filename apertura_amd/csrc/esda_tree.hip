@@ -1,5 +1,20 @@
 // esda_tree.hip -- the step of drafted tokens over a cache in pages, or a linear one, for MI355X
 // (gfx950).  The C ABI is include/esda_tree.h.
+//
+//   out_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i),  s_ij = scale log2 e q_i.k_j,
+// over the committed rows within node i's window and the nodes on its path.  A path is 64 bits, bit j for
+// node j; a wave works them out with a node to a lane, doubling the paths' length in each of six rounds,
+// and a node's depth is the number of its bits.  Only stages that hold nodes, the window's edge or a page
+// that is none look at them; the others are plain attention.
+//
+// A launch of pieces (one kv head, one sequence, a share of its keys) and one that merges them.  Few query
+// rows a kv head take runs (tree_run_kernel), bound by memory: 32 sequences of 1,024 .. 8,192 rows of 128
+// dims, K and V of 8 heads in 16-row pages, 608 MB read in 102 us (6.0 TB/s; a read of a large buffer
+// reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 133 (6.2).  More take query tiles (prefill_kernel with
+// TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes over 16,384 and
+// 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 150 us with the merge (0.87 PFLOP/s), the matrix
+// pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
+// 3.7 us each by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
 
 #include <hip/hip_runtime.h>
 
@@ -21,7 +36,7 @@
 
 namespace {
 
-// A run's rows with what is to be done once its first loads are under way.
+// A run's rows (esda_tree_rows.h) with what is to be done once its first loads are under way.
 template <int D, bool SH, class Begin>
 struct BegunRows : TreeRows<D, SH> {
     Begin &begin;
@@ -29,7 +44,12 @@ struct BegunRows : TreeRows<D, SH> {
     __device__ __forceinline__ void begun() const { begin(); }
 };
 
-// 16 NG query rows of a (sequence, kv head) over one piece of its keys, in a run (esda_stream.h).
+// 16 NG query rows of a (sequence, kv head) over one piece of its keys, in a run (esda_stream.h): four waves
+// that stream 16-row stages of their own, each row read once for all 16 NG query rows.  The page of a stage
+// comes from a register that holds the next 64 entries of the table, a lane each.  Tried and not kept: two
+// stages of a wave under way at once and the entries by DMA (token of 32 sequences 104.0 -> 105.5 us), shares
+// that go on from one sequence to the next (104.0 -> 102.9, but 8 sequences of 5 nodes 135 -> 138 and one
+// token 11.0 -> 12.3), q's loads before the nodes' paths (no difference).
 template <int D, bool SH, int NG>
 __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
     using Own = OwnRows<D, SH, 4, NG>;
@@ -129,7 +149,9 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
 
 // out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the pieces of a row's sequence; 0 where it
 // saw no key.  A workgroup takes 256 / GR lanes of 4 dims, and its GR groups of threads the pieces in
-// turn, U of them in flight, each against its own maximum; the groups meet in LDS.
+// turn, U of them in flight, each against its own maximum; the groups meet in LDS.  Few rows take many
+// groups (launch_step), which cover the loads' latency; many rows are bound by the partials' bytes (4,032
+// rows of 512 dims, 67 MB in 12.5 us, 5.4 TB/s).
 template <int D, int GR>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     constexpr int U = 4, LANES = 256 / GR;
