@@ -29,6 +29,12 @@ inline bool blocks_apart(const long long (&count)[3], const long long (&stride)[
 inline bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
 inline bool whole16(long long a) { return a >= 0 && a % 8 == 0; }
 
+// Whether the na elements from a on meet the nb from b on.
+inline bool meet(const void *a, long long na, const void *b, long long nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + 2 * (uintptr_t) nb && y < x + 2 * (uintptr_t) na;
+}
+
 // What is wrong with a pool of pages of page_rows rows, or null.
 inline const char *check_pool(const esda_pool &p, int num_pages, int page_rows) {
     if (!p.data || (reinterpret_cast<uintptr_t>(p.data) & 15u)) return "a pool must be 16-byte aligned device memory";

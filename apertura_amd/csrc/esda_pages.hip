@@ -708,6 +708,13 @@ int rows_call(const char *call, bool write, const esda_page_rows_desc *d, const 
     if (!write && !blocks_apart({d->pool.planes, d->batch, d->pool.num_kv_heads},
                                 {d->linear_plane_stride, d->linear_seq_stride, d->linear_head_stride}, (long long) d->rows * d->pool.head_dim))
         return refuse(call, "the linear rows overlap");
+    const __int128 reach = (__int128) (d->pool.planes - 1) * d->linear_plane_stride + (__int128) (d->batch - 1) * d->linear_seq_stride +
+                           (__int128) (d->pool.num_kv_heads - 1) * d->linear_head_stride + (__int128) d->rows * d->pool.head_dim;
+    if (reach > (__int128) 1 << 60) return refuse(call, "the linear rows reach too far");
+    if (d->rows > 0 && meet(linear, (long long) reach, d->pool.data,
+                            (d->pool.planes - 1) * d->pool.plane_stride + (d->num_pages - 1) * d->pool.page_stride +
+                                (d->pool.num_kv_heads - 1) * d->pool.head_stride + (long long) d->page_rows * d->pool.head_dim))
+        return refuse(call, "the linear rows must not overlap the pool");
     const int rc = esda_detail::check_device();
     if (rc || d->rows == 0) return rc;
     RowsParams p{};

@@ -10,10 +10,10 @@
 // A launch of pieces (one kv head, one sequence, a share of its keys) and one that merges them.  Few query
 // rows a kv head take runs (tree_run_kernel), bound by memory: 32 sequences of 1,024 .. 8,192 rows of 128
 // dims, K and V of 8 heads in 16-row pages, 608 MB read in 102 us (6.0 TB/s; a read of a large buffer
-// reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 133 (6.2).  More take query tiles (prefill_kernel with
-// TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes over 16,384 and
-// 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 150 us with the merge (0.87 PFLOP/s), the matrix
-// pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
+// reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 133 (6.2).  More take query tiles
+// (prefill_kernel with TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes
+// over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 150 us with the merge
+// (0.87 PFLOP/s), the matrix pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
 // 3.7 us each by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
 
 #include <hip/hip_runtime.h>
@@ -460,18 +460,14 @@ int esda_tree_decode(const esda_tree_desc *d, const esda_tree_args *a, void *str
     // the new rows while they are written to the pages.
     struct Range {
         const void *at;
-        size_t bytes;
-        bool meets(const Range &o) const {
-            const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
-            return a < b + o.bytes && b < a + bytes;
-        }
+        long long n;
+        bool meets(const Range &o) const { return esda_page_view::meet(at, n, o.at, o.n); }
     };
-    const size_t token = (size_t) d->batch * d->nodes * d->head_dim * 2;
-    const size_t extent = 2 * ((size_t) (d->num_pages - 1) * d->page_stride + (size_t) (d->num_kv_heads - 1) * d->head_stride +
-                               (size_t) d->page_rows * d->head_dim);
+    const long long token = (long long) d->batch * d->nodes * d->head_dim;
+    const long long extent = (d->num_pages - 1) * d->page_stride + (d->num_kv_heads - 1) * d->head_stride + (long long) d->page_rows * d->head_dim;
     const Range out{a->out, token * d->num_q_heads}, k_new{a->k_new, token * d->num_kv_heads},
         v_new{shared ? a->k_new : a->v_new, token * d->num_kv_heads}, k_pages{a->k_pages, extent}, v_pages{a->v_pages, extent};
-    for (const Range &x : {Range{a->q, out.bytes}, k_new, v_new, k_pages, v_pages})
+    for (const Range &x : {Range{a->q, out.n}, k_new, v_new, k_pages, v_pages})
         if (out.meets(x)) return refuse("out must not overlap q, the new rows or the pages");
     for (const Range &x : {k_new, v_new})
         if (x.meets(k_pages) || x.meets(v_pages)) return refuse("the new rows must not overlap the pages");

@@ -20,7 +20,8 @@
  * taken lowest number first, so the outcome depends on the table, refs and the lists alone.  Nothing
  * is read back: what cannot be done is left out and counted in the workspace's status word
  * (esda_pages_status).  Calls may be captured in a graph; calls on one cache are ordered on one
- * stream, and calls that overlap need workspaces of their own. */
+ * stream, and calls that overlap need workspaces of their own.  What a workspace holds between calls
+ * lies where num_pages, slots and max_pages put it: another cache's sizes need another workspace. */
 #ifndef APERTURA_ESDA_PAGES_H
 #define APERTURA_ESDA_PAGES_H
 
@@ -80,10 +81,9 @@ int esda_pages_free(const esda_pages *cache, const int32_t *slots, int32_t n, vo
 /* Slot dst[i] becomes the first rows[i] rows of slot src[i] (rows NULL, or more than it holds: all of
  * them).  What dst[i] held is given up; full pages are shared; the rows of a last page that is not full
  * are copied to a page of dst[i]'s own in every pool.  dst[i] == src[i] cuts a sequence, which keeps a
- * last page that nobody else holds.  Entries
- * outside the cache, with rows below 0, with rows that lie in no page, and slots named before in dst
- * are left out and counted; an entry that finds no free page leaves its dst empty and is counted.
- * n <= slots. */
+ * last page that nobody else holds.  Entries outside the cache, with rows below 0, with rows that lie in
+ * no page, and slots named before in dst are left out and counted; an entry that finds no free page
+ * leaves its dst empty and is counted.  n <= slots. */
 int esda_pages_fork(const esda_pages *cache, const int32_t *src, const int32_t *dst, const int32_t *rows, int32_t n,
                     void *stream);
 
@@ -98,8 +98,8 @@ int esda_pages_status(void *workspace, int32_t *left_out, void *stream);
 /* ------------------------------------------------------------ rows in and out
  * Rows row0[b] .. row0[b] + rows - 1 of sequence b < batch between its pages and a linear buffer, in
  * every plane: element (plane, b, kvh, i, d) at linear[plane*linear_plane_stride + b*linear_seq_stride +
- * kvh*linear_head_stride + i*head_dim + d].  Rows that lie in no page are
- * not written, and read as 0. */
+ * kvh*linear_head_stride + i*head_dim + d].  Rows that lie in no page are not written, and read as 0.
+ * The linear rows must not overlap the pool. */
 typedef struct esda_page_rows_desc {
     esda_pool pool;
     int32_t num_pages, page_rows; /* as in esda_pages                         */

@@ -136,6 +136,11 @@ def test_bad_row_copy_arguments_are_refused():
         for args in ((None, FAKE, FAKE), (FAKE, None, FAKE), (FAKE, FAKE, None), (FAKE + 2, FAKE, FAKE), (FAKE, FAKE, FAKE + 8)):
             assert f(d, *args, None) == 1
         assert f(None, FAKE, FAKE, FAKE, None) == 1
+    # linear rows that meet the pool's, at either end
+    reach, pool = 2 * (2 * 6 * 3 * 40 * 128), 2 * (2 * 20 * 3 * 16 * 128)
+    for f in (L.esda_pages_write, L.esda_pages_read):
+        for at in (0, pool - 16, 16 - reach):
+            assert f(d, FAKE, FAKE, FAKE + at, None) == 1 and b"overlap the pool" in L.esda_last_error()
     # linear rows that overlap may be read from, not written to
     assert L.esda_pages_read(ctypes.byref(_rows(linear_head_stride=39 * 128)), FAKE, FAKE, FAKE, None) == 1
 

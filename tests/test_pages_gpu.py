@@ -273,6 +273,19 @@ def test_rows_in_and_out(planes, hkv, D, R, n):
     assert bool((out[:, :, :, n:] == 3.0).all())
 
 
+def test_rows_right_beside_the_pool():
+    """Linear rows of the pool's own allocation, before and behind it."""
+    R, N, rows = 16, 3, 2 * 128 * 40
+    memory = torch.randn(2 * rows + 2 * N * R * 128, device=DEV).to(BF)
+    pool = memory[rows:-rows].view(2, N, 1, R, 128)
+    before, behind = memory[:rows].view(2, 1, 1, 40, 128), memory[-rows:].view(2, 1, 1, 40, 128)
+    table, row0 = _ints([2, 0, 1]).view(1, 3), _ints([5])
+    held = before.clone()
+    pages_write(pool, table, row0, before)
+    pages_read(pool, table, row0, 40, out=behind)
+    assert torch.equal(before, held) and torch.equal(behind, held)
+
+
 def test_rows_before_the_first_and_behind_the_last_page():
     pool = _make([(1, 2, 128)], 4, 16)[0]
     table, row0 = _ints([[0, 1], [2, 3]]), _ints([-5, 20])
