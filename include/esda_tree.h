@@ -19,7 +19,8 @@
  * step is given the same; esda_tree_commit moves it on.
  * A committed row whose table entry is no page is left out.  A sequence with a negative length, or one
  * whose nodes' rows do not all lie in its pages, is skipped: nothing is written for it, and it is
- * counted (esda_pages_status).  Pages of the nodes' rows belong to one sequence.  Calls that overlap need
+ * counted (esda_pages_status); one of length 0 whose nodes are all none is a batch's padding: it needs no
+ * pages and gives 0.  Pages of the nodes' rows belong to one sequence.  Calls that overlap need
  * workspaces of their own.  A value of k or v that is not finite reaches only the queries that see
  * its row. */
 #ifndef APERTURA_ESDA_TREE_H

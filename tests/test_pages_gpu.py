@@ -362,6 +362,35 @@ def test_graph_replays():
         b.call("free", [6])
 
 
+def test_pages_past_32_bit_offsets():
+    """As many pages as a cache can have, 16 GiB a plane: those in use are the last of them."""
+    N, R, D = 2 ** 22, 16, 128
+    pool = torch.empty((1, N, 1, R, D), dtype=BF, device=DEV)
+    table = torch.full((3, 4), -1, dtype=torch.int32, device=DEV)
+    refs = torch.ones(N, dtype=torch.int32, device=DEV)  # (the others are somebody's)
+    refs[-8:] = 0
+    cache = PagedCache([pool], table, torch.zeros(3, dtype=torch.int32, device=DEV), refs)
+    cache.reserve(_ints([0]), _ints([60]))
+    assert table[0].tolist() == [N - 8, N - 7, N - 6, N - 5]
+    rows = torch.randn((1, 1, 1, 60, D), device=DEV).to(BF)
+    pages_write(pool, table[:1], _ints([0]), rows)
+    assert torch.equal(pool[0, N - 5, 0, :12], rows[0, 0, 0, 48:])
+    cache.length[0] = 40
+    cache.fork(_ints([0]), _ints([1]))
+    assert table[1].tolist() == [N - 8, N - 7, N - 4, -1]
+    assert torch.equal(pool[0, N - 4, 0, :8], rows[0, 0, 0, 32:40])
+    cache.commit(torch.tensor([[1, 9], [0, 0], [0, 0]], dtype=torch.int32, device=DEV), _ints([2, 0, 0]))
+    assert cache.length.tolist() == [42, 40, 0] and cache.left_out() == 0
+    want = torch.cat([rows[:, :, :, :40], rows[:, :, :, [41, 49]]], dim=3)
+    assert torch.equal(pages_read(pool, table[:1], _ints([0]), 42), want)
+    refs[:-8] = 0
+    cache.compact()
+    assert table.tolist() == [[0, 1, 2, 3], [0, 1, 4, -1], [-1] * 4] and refs.tolist()[:6] == [2, 2, 1, 1, 1, 0]
+    assert refs.sum().item() == 7
+    assert torch.equal(pages_read(pool, table[:1], _ints([0]), 42), want)
+    assert torch.equal(pages_read(pool, table[1:2], _ints([0]), 40), want[:, :, :, :40])
+
+
 def test_a_stream_of_its_own():
     b = _filled(POOLS[1], 20, 16, 4, 4, [20, 33])
     st = torch.cuda.Stream()

@@ -348,6 +348,21 @@ def test_two_streams():
     b.check(outs[1], before[1])
 
 
+@pytest.mark.parametrize("T", [1, 4, 20, 64])
+@pytest.mark.parametrize("D,hq,hkv,shared", [(128, 8, 2, False), (256, 4, 2, False), (512, 8, 1, True)])
+def test_padded_batches(D, hq, hkv, shared, T):
+    """Sequences of no rows, no pages and no nodes beside real ones give zeros and are not counted."""
+    parent = random_parents(5, T, T)
+    parent[1::2] = -2
+    c = Case(T, hq, hkv, D, [70, 0, 500, 0, 3], 16, shared, parent=parent, seed=T)
+    c.table[1::2] = -1
+    out = torch.full_like(c.q, float("nan"))
+    workspace = new_tree_workspace(c.step, DEV)
+    c.run(out=out, workspace=workspace)
+    assert (out[1::2] == 0).all()
+    assert pages_status(workspace) == 0
+
+
 def test_pages_past_32_bit_offsets():
     """A pool of more than 2^32 elements; the sequence's pages lie at its end."""
     D, hq, hkv, R = 128, 8, 8, 1024
