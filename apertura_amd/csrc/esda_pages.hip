@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdint>
 #include <string>
 
@@ -191,12 +192,14 @@ template <class Put>
 __device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put) {
     int got = 0;
     for (int base = 0; base < p.N && got < need; base += 4 * kOneGroup) {
+        const int id0 = base + 4 * (int) threadIdx.x;
+        int of[4], n = 0;
         bool free[4];
-        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) of[e] = references(p, min(id0 + e, p.N - 1));  // (no branch: all under way at once)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int id = base + 4 * (int) threadIdx.x + e;
-            free[e] = id < p.N && references(p, id) == 0;
+            free[e] = id0 + e < p.N && of[e] == 0;
             n += free[e];
         }
         const Scan s = scan(n);
@@ -204,7 +207,7 @@ __device__ __forceinline__ int lowest_free(const Params &p, int need, Put &&put)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (free[e]) {
-                if (rank < need) put(rank, base + 4 * (int) threadIdx.x + e);
+                if (rank < need) put(rank, id0 + e);
                 ++rank;
             }
         got += s.total;
@@ -235,28 +238,29 @@ __global__ __launch_bounds__(256) void free_kernel(Params p, const int *slots) {
 // the lowest pages.  A scan takes 4,096 pages' references a step and ends with the last page that is needed.)
 __global__ __launch_bounds__(kOneGroup) void reserve_kernel(Params p, const int *slots, const int *rows, int n) {
     __shared__ int slot[ESDA_MAX_ENTRIES], first[ESDA_MAX_ENTRIES], last[ESDA_MAX_ENTRIES], lack[ESDA_MAX_ENTRIES], from[ESDA_MAX_ENTRIES];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    if (t < n) slot[t] = slots[t];
-    __syncthreads();
+    const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
     if (t < n) {
-        const int s = slot[t], r = rows[t];
-        bool ok = (unsigned) s < (unsigned) p.S && r >= 0 && r <= (long long) p.P * p.R;
-        for (int j = 0; j < t; ++j) ok = ok && slot[j] != s;
-        int len = 0;
-        if (ok) {
-            len = p.length[s];
-            ok = len >= 0;
-        }
-        if (!ok) add(&p.head->left_out, 1);
+        const int s = slots[t], r = rows[t];
+        const bool there = (unsigned) s < (unsigned) p.S;
+        const int len = p.length[there ? s : 0];
+        const bool ok = there && r >= 0 && r <= (long long) p.P * p.R && len >= 0;
+        slot[t] = s;
         first[t] = ok ? len >> p.shift : 0;
-        last[t] = ok ? (int) (((long long) r + p.R - 1) >> p.shift) : 0;
+        last[t] = ok ? (int) (((long long) r + p.R - 1) >> p.shift) : -1;  // (-1: left out)
     }
     __syncthreads();
     for (int i = wave; i < n; i += kOneGroup / 64) {
-        const int *const row = p.table + (long long) slot[i] * p.table_stride;
-        int sum = 0;
-        for (int k = first[i]; k < last[i]; k += 64)
-            sum += __popcll(__builtin_amdgcn_ballot_w64(k + lane < last[i] && !is_page(row[k + lane], p.N)));
+        const int s = slot[i];
+        bool twice = false;
+        for (int j = lane; j < i; j += 64) twice = twice || slot[j] == s;
+        int to = last[i], sum = 0;
+        if (to < 0 || any_of<64>(twice)) {
+            if (lane == 0) add(&p.head->left_out, 1);
+            to = 0;
+        }
+        const int *const row = p.table + (long long) s * p.table_stride;
+        for (int k = first[i]; k < to; k += 64)
+            sum += __popcll(__builtin_amdgcn_ballot_w64(k + lane < to && !is_page(row[k + lane], p.N)));
         if (lane == 0) lack[i] = sum;
     }
     __syncthreads();
@@ -290,15 +294,10 @@ __global__ __launch_bounds__(kOneGroup) void reserve_kernel(Params p, const int 
 // until the free pages are given out, so that it is none of them.
 template <int W>
 __device__ Entry fork_entry(const Params &p, const int *src, const int *dst, const int *rows, int i, int t) {
-    const int s = src[i], d = dst[i];
-    const bool twice = named_before<W>(dst, i, t);
-    bool ok = !twice && (unsigned) s < (unsigned) p.S && (unsigned) d < (unsigned) p.S;
-    int len = 0, r = 0;
-    if (ok) {
-        len = p.length[s];
-        r = rows ? min(rows[i], len) : len;
-        ok = r >= 0 && len <= (long long) p.P * p.R;
-    }
+    const int s = src[i], d = dst[i], most = rows ? rows[i] : INT_MAX;
+    bool ok = (unsigned) s < (unsigned) p.S && (unsigned) d < (unsigned) p.S;
+    const int len = p.length[ok ? s : 0], r = min(most, len);
+    ok = ok && r >= 0 && len <= (long long) p.P * p.R && !named_before<W>(dst, i, t);
     const int full = r >> p.shift, part = r & (p.R - 1);
     const int *const from = p.table + (long long) (ok ? s : 0) * p.table_stride;
     bool there = true;
@@ -402,17 +401,27 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(Params p, int n) {
 // below it, both in order; references and the way of each page that moves.
 __global__ __launch_bounds__(kOneGroup) void compact_kernel(Params p) {
     const int t = threadIdx.x;
-    int n = 0;
-    for (int id = t; id < p.N; id += kOneGroup) n += p.refs[id] != 0;
+    // references of pages id0 .. id0 + 3 (past the last: of that; no branch: all under way at once)
+    auto four = [&](int id0, int (&of)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) of[e] = p.refs[min(id0 + e, p.N - 1)];
+    };
+    int n = 0, of[4];
+    for (int id0 = 4 * t; id0 < p.N; id0 += 4 * kOneGroup) {
+        four(id0, of);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n += id0 + e < p.N && of[e] != 0;
+    }
     const int live = scan(n).total;
     int moves = 0, holes = 0;
     for (int base = 0; base < p.N; base += 4 * kOneGroup) {
         bool mover[4], hole[4];
         int m = 0, h = 0;
+        four(base + 4 * t, of);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int id = base + 4 * t + e;
-            const bool used = id < p.N && p.refs[id] != 0;
+            const bool used = id < p.N && of[e] != 0;
             mover[e] = used && id >= live;
             hole[e] = !used && id < live;
             m += mover[e];
