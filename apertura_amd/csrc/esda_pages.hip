@@ -60,7 +60,8 @@ struct Params {
     long long table_stride;
     int *table, *refs, *length;
     int num_pools;
-    unsigned pieces;  // of one move, over all pools
+    unsigned pieces;     // of one move, over all pools
+    unsigned last_move;  // moves' room - 1
     Header *head;
     Entry *entries;
     Move *moves;
@@ -133,21 +134,30 @@ __device__ __forceinline__ Piece piece_of(const Params &p, unsigned i) {
                     (long long) row * o.D, row};
 }
 
-// The listed moves, a wave to a piece.
+// The listed moves, a wave to a piece.  (The first is read beside their number; moves has room for it.)
 template <bool LOADED>
-__device__ void carry_out(const Params &p) {
+__device__ __forceinline__ void carry_out(const Params &p) {
     if (p.num_pools == 0) return;
     const int lane = threadIdx.x & 63;
-    const unsigned waves = gridDim.x * (blockDim.x / 64);
-    const unsigned long long all = (unsigned long long) (unsigned) p.head->moves * p.pieces;
-    for (unsigned long long u = blockIdx.x * (blockDim.x / 64) + (unsigned) uniform(threadIdx.x >> 6); u < all; u += waves) {
-        const unsigned m = (unsigned) (u / p.pieces);
-        const Piece x = piece_of(p, (unsigned) (u - (unsigned long long) m * p.pieces));
-        const Move mv = p.moves[m];
+    const unsigned waves = gridDim.x * (blockDim.x / 64), u = blockIdx.x * (blockDim.x / 64) + (unsigned) uniform(threadIdx.x >> 6);
+    unsigned m = u / p.pieces, i = u % p.pieces;
+    const unsigned step = waves / p.pieces, over = waves % p.pieces;
+    Move mv = p.moves[min(m, p.last_move)];
+    const unsigned moves = (unsigned) p.head->moves;
+    while (m < moves) {
+        const Piece x = piece_of(p, i);
         const int rows = min(mv[2] - x.row, min(p.R, x.pool->rows_per_piece()));
-        if (rows <= 0) continue;
         uint16_t *const base = x.pool->data + x.at;
-        wave_copy<LOADED, true>(base + (long long) mv[1] * x.pool->page_stride, base + (long long) mv[0] * x.pool->page_stride, rows * x.pool->D / 8, lane);
+        if (rows > 0)
+            wave_copy<LOADED, true>(base + (long long) mv[1] * x.pool->page_stride, base + (long long) mv[0] * x.pool->page_stride,
+                                    rows * x.pool->D / 8, lane);
+        m += step;
+        i += over;
+        if (i >= p.pieces) {
+            i -= p.pieces;
+            ++m;
+        }
+        mv = p.moves[min(m, p.last_move)];
     }
 }
 
@@ -384,15 +394,17 @@ __global__ __launch_bounds__(256) void fork_kernel(Params p, const int *src, con
 }
 __global__ __launch_bounds__(kOneGroup) void fork_pages_kernel(Params p, int n) { fork_pages(p, p.entries, n); }
 
-// .. and what follows from them: the tables, and the rows of the last pages.
+// .. and what follows from them: the tables, by the last n workgroups, and the rows of the last pages.
 __global__ __launch_bounds__(256) void fork_copy_kernel(Params p, int n) {
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int i = (int) (blockIdx.x + n - gridDim.x);
+    if (i >= 0) {
         const Entry e = p.entries[i];
-        if (e.state == kLeftOut) continue;
-        int *const to = p.table + (long long) e.dst * p.table_stride;
-        const int *const row = p.rows + (long long) i * p.P;
-        for (int k = threadIdx.x; k < p.P; k += 256) to[k] = row[k];
-        if (threadIdx.x == 0) p.length[e.dst] = e.state == kFailed ? 0 : e.rows;
+        if (e.state != kLeftOut) {
+            int *const to = p.table + (long long) e.dst * p.table_stride;
+            const int *const row = p.rows + (long long) i * p.P;
+            for (int k = threadIdx.x; k < p.P; k += 256) to[k] = row[k];
+            if (threadIdx.x == 0) p.length[e.dst] = e.state == kFailed ? 0 : e.rows;
+        }
     }
     carry_out<false>(p);
 }
@@ -635,12 +647,14 @@ struct Layout {
 // The status word and the tickets, zeroed once: each call leaves the tickets as it finds them.
 size_t zeroed(int slots) { return 256 + (sizeof(int) * (size_t) slots + 255) / 256 * 256; }
 
+size_t most_moves(int num_pages) { return std::max<size_t>(ESDA_MAX_ENTRIES, num_pages / 2 + 1); }
+
 Layout layout(int num_pages, int slots, int max_pages) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Layout l;
     l.entries = zeroed(slots);
     l.moves = l.entries + sizeof(Entry) * ESDA_MAX_ENTRIES;
-    l.ids = l.moves + sizeof(Move) * std::max<size_t>(ESDA_MAX_ENTRIES, num_pages / 2 + 1);
+    l.ids = l.moves + sizeof(Move) * most_moves(num_pages);
     l.rows = l.ids + up(sizeof(int) * (size_t) num_pages);
     l.bytes = l.rows + sizeof(int) * (size_t) std::min(slots, ESDA_MAX_ENTRIES) * max_pages;
     return l;
@@ -684,6 +698,7 @@ int page_params(const char *call, const esda_pages *c, Params *p) {
     p->refs = c->refs;
     p->length = c->length;
     p->num_pools = c->num_pools;
+    p->last_move = (unsigned) most_moves(c->num_pages) - 1;
     p->head = reinterpret_cast<Header *>(ws);
     p->entries = reinterpret_cast<Entry *>(ws + l.entries);
     p->moves = reinterpret_cast<Move *>(ws + l.moves);
@@ -809,7 +824,7 @@ int esda_pages_fork(const esda_pages *c, const int32_t *src, const int32_t *dst,
         hipLaunchKernelGGL(fork_kernel, dim3(n), dim3(256), 0, st, p, src, dst, rows);
         hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kOneGroup), 0, st, p, n);
     }
-    hipLaunchKernelGGL(fork_copy_kernel, dim3(std::max<unsigned>(n, copy_groups(p, n))), dim3(256), 0, st, p, n);
+    hipLaunchKernelGGL(fork_copy_kernel, dim3(n + copy_groups(p, n)), dim3(256), 0, st, p, n);
     return launched(call);
 }
 
