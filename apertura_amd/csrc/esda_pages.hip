@@ -373,8 +373,8 @@ __device__ void fork_pages(const Params &p, const Entry *entries, int n) {
 }
 
 // A fork's decisions: of a small one in one launch, a wave to an entry; else in two, a workgroup to an
-// entry and then one for the free pages.  (4 children of 32 pages, and their next page: 15.0 us in two, 13.9
-// in one; 32 children of 79, two to a wave: 19.5 and 25.6.  As the work of the last workgroup of the first of
+// entry and then one for the free pages.  (4 children of 32 pages, and their next page: 13.7 us in two, 11.3
+// in one; 32 children of 79, two to a wave: 17.1 and 19.2.  As the work of the last workgroup of the first of
 // two, behind fences for what the others wrote, the free pages took 5 and 10 us more.)
 constexpr int kSmallFork = kOneGroup / 64, kSmallForkTable = 256;  // entries, pages of each
 __global__ __launch_bounds__(kOneGroup) void fork_small_kernel(Params p, const int *src, const int *dst, const int *rows, int n) {
@@ -541,27 +541,26 @@ struct CommitParams {
 // Slot s's list, as a wave: lane i has the place of the row to take (page, row) and of the one it becomes.
 // False where the slot is left as it was.
 __device__ __forceinline__ bool accepted(const CommitParams &p, int s, int lane, int &n, int &take, int &c, int2 &from, int2 &to) {
+    // (every lane loads, within the list and the table: a branch would wait for each load)
     n = p.length[s];
     c = p.count[s];
-    bool ok = n >= 0 && c >= 0 && c <= p.max_accept;
-    take = ok && lane < c ? p.accept[s * p.accept_stride + lane] : -1;
+    take = p.accept[s * p.accept_stride + min(lane, p.max_accept - 1)];
     const int before = __shfl_up(take, 1);
-    if (ok && lane < c) ok = take >= 0 && take < 64 && (lane == 0 || take > before);
-    if (ok && lane < c) {
-        auto place = [&](long long row, int2 &at) {
-            const long long k = row >> p.shift;
-            if (p.linear) {
-                at = int2{s, (int) row};
-                return row < p.cap;
-            }
-            if (k >= p.P) return false;
-            at = int2{p.table[s * p.table_stride + k], (int) (row & ((1 << p.shift) - 1))};
-            return is_page(at.x, p.N);
-        };
-        const bool a = place((long long) n + take, from), b = place((long long) n + lane, to);
-        ok = a && b;
+    const bool listed = n >= 0 && c >= 0 && c <= p.max_accept, mine = listed && lane < c;
+    bool ok = take >= 0 && take < 64 && (lane == 0 || take > before);
+    const unsigned a = (unsigned) max(n, 0) + (take & 63), b = (unsigned) max(n, 0) + lane;
+    if (p.linear) {
+        from = int2{s, (int) a};
+        to = int2{s, (int) b};
+        ok = ok && max(a, b) < (unsigned) p.cap;
+    } else {
+        const int *const row = p.table + s * p.table_stride;
+        const unsigned ka = a >> p.shift, kb = b >> p.shift, within = (1u << p.shift) - 1;
+        from = int2{row[min(ka, p.P - 1u)], (int) (a & within)};
+        to = int2{row[min(kb, p.P - 1u)], (int) (b & within)};
+        ok = ok && max(ka, kb) < (unsigned) p.P && is_page(from.x, p.N) && is_page(to.x, p.N);
     }
-    return __builtin_amdgcn_ballot_w64(!ok) == 0ull;
+    return listed && __builtin_amdgcn_ballot_w64(mine && !ok) == 0ull;
 }
 
 // Groups of D / 8 lanes, each a (plane, kv head) of one slot: they take the moved rows in order, eight
