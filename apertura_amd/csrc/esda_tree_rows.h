@@ -54,8 +54,8 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, unsigned u, i
     int len[K], n[K], first, sum = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int s = 64 * k + lane;
-        len[k] = s < p.B ? p.length[s] : -1;
+        const int s = 64 * k + lane, n = p.length[min(s, p.B - 1)];
+        len[k] = s < p.B ? n : -1;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -121,10 +121,10 @@ __device__ __forceinline__ bool tree_paths(const TreeParams &p, int b, int len, 
     const long long row = (long long) len + lane;
     const bool within = len >= 0 && row < most;
     int id = 0;
-    if (node && within && !p.linear) id = p.table[b * p.table_stride + (row >> p.shift)];
+    if (!p.linear) id = p.table[b * p.table_stride + (node && within ? row >> p.shift : 0)];
     if (p.parent) {
-        int above = node ? p.parent[(size_t) b * p.Sq + lane] : -2;
-        if (above < -1 || above >= lane) above = -2;  // on no node
+        int above = p.parent[(size_t) b * p.Sq + min(lane, p.Sq - 1)];
+        if (!node || above < -1 || above >= lane) above = -2;  // on no node
         path = 1ull << lane;
 #pragma unroll
         for (int i = 0; i < 6; ++i) {
