@@ -173,6 +173,25 @@ __device__ __forceinline__ void lds_dma4(const void *src, unsigned lds) {
 // A value that is the same in every lane, as a scalar.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// x + the x of the lanes before, in each row of 16 lanes: DPP row_shr by 1, 2, 4 and 8, 0 from outside
+// the row.
+__device__ __forceinline__ int row_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    return x;
+}
+
+// .. and in the whole wave: the last lanes of rows 0 and 2 into the row behind (row_bcast:15), that of
+// the first half into the second (row_bcast:31).
+__device__ __forceinline__ int wave_sums(int x) {
+    x = row_sums(x);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
 __device__ __forceinline__ unsigned lds_addr(const void *p) {
     return (unsigned) (uintptr_t) (const __attribute__((address_space(3))) void *) p;
 }

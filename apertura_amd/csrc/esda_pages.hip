@@ -161,16 +161,6 @@ __device__ __forceinline__ void carry_out(const Params &p) {
     }
 }
 
-// x + the x of the lanes before, in each row of 16 lanes: DPP row_shr by 1, 2, 4 and 8, 0 from outside
-// the row.
-__device__ __forceinline__ int row_sums(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    return x;
-}
-
 // Exclusive sum over the threads of a workgroup of kOneGroup, and the total.  (These kernels are one
 // workgroup, whose time is the latency of its steps and of its code's fetches.)
 struct Scan {
@@ -181,9 +171,7 @@ __device__ __forceinline__ Scan scan(int x) {
     static_assert(W == 16, "a wave's sums: a lane of a row each");
     __shared__ int of[W];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    int in = row_sums(x);
-    in += __builtin_amdgcn_update_dpp(0, in, 0x142, 0xa, 0xf, false);  // row_bcast:15, rows 1 and 3
-    in += __builtin_amdgcn_update_dpp(0, in, 0x143, 0xc, 0xf, false);  // row_bcast:31, rows 2 and 3
+    const int in = wave_sums(x);
     __syncthreads();  // (the last call's sums are read)
     if (lane == 63) of[wave] = in;
     __syncthreads();

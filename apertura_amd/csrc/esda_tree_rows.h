@@ -31,6 +31,61 @@ __device__ __forceinline__ int tree_keys(const TreeParams &p, int len, int &firs
     return len >= 0 && len <= most ? len - first + p.Sq : 0;
 }
 
+// tree_unit where sequences are several: piece g of the batch's, sequences 64 k + lane for k < K by each
+// lane.  (Every workgroup does this before its first load: up to 64 sequences by themselves.)
+template <int K>
+__device__ __forceinline__ TreeUnit tree_unit_of(const TreeParams &p, int g, int lane, TreeUnit t) {
+    using namespace esda_tree_plan;
+    int len[K], n[K], first, sum = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int s = 64 * k + lane, n = p.length[min(s, p.B - 1)];
+        len[k] = s < p.B ? n : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        n[k] = blocks_of(tree_keys(p, len[k], first));
+        sum += n[k];
+    }
+    int chunk = p.forced;
+    if (!p.forced) {
+        auto total = [](int x) { return __builtin_amdgcn_readlane(wave_sums(x), 63); };
+        sum = total(sum);
+#pragma unroll 1
+        for (int i = 0; i <= kTries; ++i) {
+            chunk = chunk_of(sum, p.share, p.B, p.least, i);
+            int count = 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (64 * k + lane < p.B) count += pieces_of(n[k], chunk, p.splits);
+            if (total(count) <= p.share) break;
+        }
+    }
+    int before = 0;  // pieces of the sequences of the rounds before
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (64 * k >= p.B) break;
+        const bool mine = 64 * k + lane < p.B;
+        const int count = mine ? pieces_of(n[k], chunk, p.splits) : 0;
+        const int upto = before + wave_sums(count), from = upto - count;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(from <= g && g < upto);
+        if (who) {
+            const int l = __builtin_ctzll(who);
+            t.there = 1;
+            t.b = 64 * k + l;
+            t.base = __builtin_amdgcn_readlane(from, l);
+            t.len = __builtin_amdgcn_readlane(len[k], l);
+            t.pieces = __builtin_amdgcn_readlane(count, l);
+            t.keys = tree_keys(p, t.len, t.first);
+            t.piece = g - t.base;
+            piece_keys(t.piece, t.pieces, chunk, t.keys, &t.j0, &t.j1);
+            return t;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return t;
+}
+
 // Unit u as a wave: the pieces that the batch's lengths make, and which of them it is.
 __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, unsigned u, int lane) {
     using namespace esda_tree_plan;
@@ -50,65 +105,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, unsigned u, i
         piece_keys(g, t.pieces, chunk, t.keys, &t.j0, &t.j1);
         return t;
     }
-    constexpr int K = 4;  // sequences a lane: 64 k + lane
-    int len[K], n[K], first, sum = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int s = 64 * k + lane, n = p.length[min(s, p.B - 1)];
-        len[k] = s < p.B ? n : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        n[k] = blocks_of(tree_keys(p, len[k], first));
-        sum += n[k];
-    }
-    int chunk = p.forced;
-    if (!p.forced) {
-        auto total = [](int x) {
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-            return uniform(x);
-        };
-        sum = total(sum);
-        for (int i = 0; i <= kTries; ++i) {
-            chunk = chunk_of(sum, p.share, p.B, p.least, i);
-            int count = 0;
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (64 * k + lane < p.B) count += pieces_of(n[k], chunk, p.splits);
-            if (total(count) <= p.share) break;
-        }
-    }
-    int before = 0;  // pieces of the sequences of the rounds before
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (64 * k >= p.B) break;
-        const bool mine = 64 * k + lane < p.B;
-        const int count = mine ? pieces_of(n[k], chunk, p.splits) : 0;
-        int upto = count;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
-        }
-        upto += before;
-        const int from = upto - count;
-        const unsigned long long who = __builtin_amdgcn_ballot_w64(from <= g && g < upto);
-        if (who) {
-            const int l = __builtin_ctzll(who);
-            t.there = 1;
-            t.b = 64 * k + l;
-            t.base = __builtin_amdgcn_readlane(from, l);
-            t.len = __builtin_amdgcn_readlane(len[k], l);
-            t.pieces = __builtin_amdgcn_readlane(count, l);
-            t.keys = tree_keys(p, t.len, t.first);
-            t.piece = g - t.base;
-            piece_keys(t.piece, t.pieces, chunk, t.keys, &t.j0, &t.j1);
-            return t;
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
-    }
-    return t;
+    return p.B <= 64 ? tree_unit_of<1>(p, g, lane, t) : tree_unit_of<4>(p, g, lane, t);
 }
 
 // Sequence b's nodes as a wave: lane i < 64 gets node i's path (bit j: node j is above it, or is it; 0: no
