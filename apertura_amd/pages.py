@@ -30,15 +30,16 @@ def _pool(pool: torch.Tensor) -> Pool:
     return Pool(pool.data_ptr(), planes, heads, dim, 0, pool.stride(0), pool.stride(1), pool.stride(2))
 
 
-def _int_list(name: str, t: torch.Tensor, device: torch.device, n: int | None = None) -> int:
-    """The entries of a list on the device."""
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous int32 list on {device}")
-    if t.shape[0] > MAX_ENTRIES:
-        raise ValueError(f"{name} names {t.shape[0]} slots; a call names at most {MAX_ENTRIES}")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{name} has {t.shape[0]} entries, the other lists {n}")
-    return t.shape[0]
+def _int_list(name: str, t: torch.Tensor, index: int, n: int | None = None) -> int:
+    """The entries of a list on device `index`."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be a contiguous int32 list on cuda:{index}")
+    k = t.numel()
+    if k > MAX_ENTRIES:
+        raise ValueError(f"{name} names {k} slots; a call names at most {MAX_ENTRIES}")
+    if n is not None and k != n:
+        raise ValueError(f"{name} has {k} entries, the other lists {n}")
+    return k
 
 
 def _table_stride(table: torch.Tensor) -> int:
@@ -82,7 +83,7 @@ class PagedCache:
                       "workspace": workspace})
         self.pools, self.table, self.length, self.refs = list(pools), table, length, refs
         self.slots, self.max_pages, self.num_pages, self.page_rows = S, P, N, R
-        self.device = table.device
+        self.device, self._index = table.device, table.device.index
         c = Pages(num_pages=N, page_rows=R, slots=S, max_pages=P, table_stride=stride, table=table.data_ptr(),
                   refs=refs.data_ptr(), length=length.data_ptr(), num_pools=len(pools))
         for i, p in enumerate(pools):
@@ -103,61 +104,59 @@ class PagedCache:
         return cls(pools, torch.full((slots, max_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(slots, dtype=torch.int32, device=device))
 
-    def _on_device(self) -> None:
-        if torch._C._cuda_getDevice() != self.device.index:
+    def _stream(self, stream) -> int:
+        """The launch's HIP stream; the cache has to be on the current device."""
+        if torch._C._cuda_getDevice() != self._index:
             raise ValueError(f"the cache is on {self.device}; the current device is cuda:{torch.cuda.current_device()}")
+        return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else int(stream.cuda_stream)
 
     def reserve(self, slots: torch.Tensor, rows: torch.Tensor, stream=None) -> None:
         """Pages for rows up to rows[i] (exclusive) of slot slots[i]."""
-        n = _int_list("slots", slots, self.device)
-        _int_list("rows", rows, self.device, n)
-        self._on_device()
-        rc = self._lib.esda_pages_reserve(self._ref, slots.data_ptr(), rows.data_ptr(), n, _stream_ptr(stream))
+        n = _int_list("slots", slots, self._index)
+        _int_list("rows", rows, self._index, n)
+        rc = self._lib.esda_pages_reserve(self._ref, slots.data_ptr(), rows.data_ptr(), n, self._stream(stream))
         if rc:
             check(rc)
         _used_on(stream, slots, rows)
 
     def free(self, slots: torch.Tensor, stream=None) -> None:
         """The slots give up their pages and hold no rows."""
-        n = _int_list("slots", slots, self.device)
-        self._on_device()
-        rc = self._lib.esda_pages_free(self._ref, slots.data_ptr(), n, _stream_ptr(stream))
+        n = _int_list("slots", slots, self._index)
+        rc = self._lib.esda_pages_free(self._ref, slots.data_ptr(), n, self._stream(stream))
         if rc:
             check(rc)
         _used_on(stream, slots)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, rows: torch.Tensor | None = None, stream=None) -> None:
         """Slot dst[i] becomes the first rows[i] rows of slot src[i] (None: all of them)."""
-        n = _int_list("src", src, self.device)
-        _int_list("dst", dst, self.device, n)
+        n = _int_list("src", src, self._index)
+        _int_list("dst", dst, self._index, n)
         if rows is not None:
-            _int_list("rows", rows, self.device, n)
-        self._on_device()
+            _int_list("rows", rows, self._index, n)
         rc = self._lib.esda_pages_fork(self._ref, src.data_ptr(), dst.data_ptr(), None if rows is None else rows.data_ptr(), n,
-                                       _stream_ptr(stream))
+                                       self._stream(stream))
         if rc:
             check(rc)
         _used_on(stream, src, dst, rows)
 
     def compact(self, stream=None) -> None:
         """The pages in use move to the front of the pools."""
-        self._on_device()
-        rc = self._lib.esda_pages_compact(self._ref, _stream_ptr(stream))
+        rc = self._lib.esda_pages_compact(self._ref, self._stream(stream))
         if rc:
             check(rc)
 
     def commit(self, accept: torch.Tensor, count: torch.Tensor, stream=None) -> None:
         """The rows of the accepted nodes accept[s][:count[s]] (rising) of a step of drafted tokens become the
         slots' next rows (esda_tree_commit).  accept [slots, A], count [slots] int32."""
-        if accept.dtype != torch.int32 or accept.dim() != 2 or accept.shape[0] != self.slots or \
-                (accept.shape[1] > 1 and accept.stride(1) != 1) or accept.device != self.device:
+        S, A = accept.shape if accept.dim() == 2 else (-1, 0)
+        if accept.dtype is not torch.int32 or S != self.slots or (A > 1 and accept.stride(1) != 1) or \
+                accept.get_device() != self._index:
             raise ValueError(f"accept must be int32 [{self.slots}, most accepted] with dense rows on {self.device}")
-        if count.dtype != torch.int32 or count.shape != (self.slots,) or not count.is_contiguous() or count.device != self.device:
+        if count.dtype is not torch.int32 or count.dim() != 1 or count.numel() != S or not count.is_contiguous() or \
+                count.get_device() != self._index:
             raise ValueError(f"count must be contiguous int32 [{self.slots}] on {self.device}")
-        self._on_device()
-        A = accept.shape[1]
-        rc = self._lib.esda_tree_commit(self._ref, accept.data_ptr(), accept.stride(0) if self.slots > 1 else A, A,
-                                        count.data_ptr(), _stream_ptr(stream))
+        rc = self._lib.esda_tree_commit(self._ref, accept.data_ptr(), accept.stride(0) if S > 1 else A, A, count.data_ptr(),
+                                        self._stream(stream))
         if rc:
             check(rc)
         _used_on(stream, accept, count)

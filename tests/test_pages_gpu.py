@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from _pages_model import Model
+from apertura_amd._lib import EsdaError
 from apertura_amd.pages import PagedCache, pages_read, pages_write
 
 pytestmark = pytest.mark.gpu
@@ -389,6 +390,29 @@ def test_pages_past_32_bit_offsets():
     assert refs.sum().item() == 7
     assert torch.equal(pages_read(pool, table[:1], _ints([0]), 42), want)
     assert torch.equal(pages_read(pool, table[1:2], _ints([0]), 40), want[:, :, :, :40])
+
+
+def test_wrong_lists_are_refused():
+    b = _filled(POOLS[1], 20, 16, 4, 4, [20, 33])
+    c, two, one = b.cache, _ints([0, 1]), _ints([1])
+    many, accept, count = torch.zeros(1025, dtype=torch.int32, device=DEV), torch.zeros((4, 3), dtype=torch.int32, device=DEV), _ints([0] * 4)
+    for bad in (two.long(), two.cpu(), two.view(1, 2), _ints([0, 0, 1, 1])[::2], many):
+        for call in (lambda: c.free(bad), lambda: c.reserve(bad, bad), lambda: c.fork(bad, bad), lambda: c.fork(two, bad),
+                     lambda: c.reserve(two, bad), lambda: c.fork(two, two, bad)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: c.reserve(two, one), lambda: c.fork(two, one), lambda: c.fork(two, two, one)):
+        with pytest.raises(ValueError):
+            call()
+    for bad in (accept.long(), accept.cpu(), accept[:3], accept[0], accept.t().contiguous().t()):
+        with pytest.raises(ValueError):
+            c.commit(bad, count)
+    for bad in (count.long(), count.cpu(), count[:3], count.view(2, 2), _ints([0] * 8)[::2]):
+        with pytest.raises(ValueError):
+            c.commit(accept, bad)
+    with pytest.raises(EsdaError):
+        c.commit(accept[:, :0], count)
+    b.check()
 
 
 def test_a_stream_of_its_own():
