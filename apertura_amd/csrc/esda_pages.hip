@@ -8,9 +8,10 @@
 // entries compete for free pages, write a list of moves, and a grid of waves carries it out.  The copies
 // are bound by memory (a copy of 1 GiB moves 5.1 TB/s here): 4,095 rows of 16 heads x 256, K and V, into
 // 32-row pages, 134 MB in 22 us; 32,767 rows of 4 x 512 out of 16-row pages, 268 MB in 56; 473 MB of
-// moving pages in 86.  Calls of few bytes are bound by their launches, 3 .. 5 us each: reserve_kernel 3.0
-// for 4 entries and 5.3 for 32, which wait for their slots' lengths, tables and free pages one after the
-// other, the commit of 32 sequences' paths on 48 planes (20 MB) 8.3.
+// moving pages in 84.  Calls of few bytes are bound by their launches, 2.4 .. 7 us each: reserve_kernel 2.4
+// for 4 entries and 3.5 for 32, which wait for their slots' lengths, tables and free pages one after the
+// other, the commit of 32 sequences' paths on 48 planes (20 MB) 8.6.  Of such kernels the code's own fetches
+// are a part: loads that are under way together and little code count, unrolled loops do not pay.
 
 #include <hip/hip_runtime.h>
 

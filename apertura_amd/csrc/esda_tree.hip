@@ -9,12 +9,12 @@
 //
 // A launch of pieces (one kv head, one sequence, a share of its keys) and one that merges them.  Few query
 // rows a kv head take runs (tree_run_kernel), bound by memory: 32 sequences of 1,024 .. 8,192 rows of 128
-// dims, K and V of 8 heads in 16-row pages, 608 MB read in 102 us (6.0 TB/s; a read of a large buffer
-// reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 133 (6.2).  More take query tiles
+// dims, K and V of 8 heads in 16-row pages, 608 MB read in 101 us (6.0 TB/s; a read of a large buffer
+// reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 132 (6.3).  More take query tiles
 // (prefill_kernel with TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes
-// over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 150 us with the merge
-// (0.87 PFLOP/s), the matrix pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
-// 3.7 us each by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
+// over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 147 us with the merge
+// (0.89 PFLOP/s; esda_prefill's tiles over the same linear rows are 1 .. 4% faster), the matrix pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
+// 3.4 us each by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
 
 #include <hip/hip_runtime.h>
 
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
 // saw no key.  A workgroup takes 256 / GR lanes of 4 dims, and its GR groups of threads the pieces in
 // turn, U of them in flight, each against its own maximum; the groups meet in LDS.  Few rows take many
 // groups (launch_step), which cover the loads' latency; many rows are bound by the partials' bytes (4,032
-// rows of 512 dims, 67 MB in 12.5 us, 5.4 TB/s).
+// rows of 512 dims, 67 MB in 12.4 us, 5.4 TB/s; eight of a lane in flight were no faster).
 template <int D, int GR>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     constexpr int U = 4, LANES = 256 / GR;
