@@ -13,8 +13,9 @@
 // reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 132 (6.3).  More take query tiles
 // (prefill_kernel with TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes
 // over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 147 us with the merge
-// (0.89 PFLOP/s; esda_prefill's tiles over the same rows, linear, 1 .. 5% less), the matrix pipes busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and
-// 3.4 us each by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
+// (0.89 PFLOP/s; esda_prefill's tiles over the same rows, linear, take 1 .. 5% less), the matrix pipes busy
+// for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and 3.4 us each
+// by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
 
 #include <hip/hip_runtime.h>
 
