@@ -971,9 +971,12 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         const long long gr0 = (long long) tile * QT + br + li;
         if (gr0 >= nq || (ODD && KH && kh)) continue;
         if constexpr (TREE) {
-            if (paths[position_of(gr0, p.G)] == 0ull) {  // no node: nothing seen
+            if (paths[position_of(gr0, p.G)] == 0ull) {  // no node: nothing seen (its q may be anything, and m infinite)
                 lb[nb] = 0.0f;
-                if (nb < QB) l[nb < QB ? nb : 0] = 0.0f;
+                if (nb < QB) {
+                    m[nb < QB ? nb : 0] = -INFINITY;
+                    l[nb < QB ? nb : 0] = 0.0f;
+                }
 #pragma unroll
                 for (int dt = 0; dt < DW; ++dt) acc[nb][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }

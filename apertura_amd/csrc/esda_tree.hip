@@ -106,8 +106,9 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
     };
     const size_t part = (size_t) tree_part(p, t);
     auto finish = [&](int r, int d, f32x4 o, float m, float l) {  // dims d .. d + 3 of query row r
-        if (paths[r / p.G] == 0ull) {  // no node: nothing seen
+        if (paths[r / p.G] == 0ull) {  // no node: nothing seen (its q may be anything, and m infinite)
             o = 0.0f;
+            m = -INFINITY;
             l = 0.0f;
         }
         if (p.splits == 1) {
