@@ -613,7 +613,20 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
             ESDA_WAIT_VM(0);
             return;
         }
+        tr.none = __builtin_amdgcn_ballot_w64(path == 0ull);
     }
+    // TREE: rows of stage s that no node sees may hold anything, with a weight of 0: zeros instead (0 x inf is
+    // NaN).  By the wave whose DMAs they are, once these have landed.
+    auto clear_unseen = [&](int s) {
+        if constexpr (TREE) {
+            const int jst = j0 + s * kStageKeys + 16 * (wave / (NW / 2)), row = tu.first + jst;
+            unsigned rows = tr.unseen(jst);
+            if (holes && row < tu.len && tr.page_of(row >> p.shift) < 0) rows = 0xffffu;
+#pragma unroll
+            for (int t = 0; t < KPW; ++t)
+                if ((rows >> (vrow[t] & 15)) & 1) *reinterpret_cast<u32x4 *>(vslot(s) + ldso[t] + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        }
+    };
     auto shift = [&]() {
         if constexpr (DOCS) {
 #pragma unroll
@@ -638,6 +651,11 @@ __global__ __launch_bounds__(64 * NW, D == 128 && NW == 4 ? 2 : 1) void prefill_
         // The iteration's stages s0 .. s0+SPI-1 landed (this wave's loads; the barrier covers
         // the other waves') and every wave is done with the previous iteration
         ESDA_WAIT_VM(0);
+        if constexpr (TREE) {
+            const int row = tu.first + j0 + s0 * kStageKeys;
+            if (__builtin_expect(holes || row < tr.low || row + SPI * kStageKeys > tu.len, 0))
+                for (int s = s0; s < min(s0 + SPI, nst); ++s) clear_unseen(s);
+        }
         lds_barrier();
         if constexpr (PARTS) {
             // rows past the prefix repeat its last key: with a weight of 0, but 0 x inf is NaN

@@ -20,11 +20,13 @@ namespace esda_stream {
 //                        every wave calls it for its stages in order, before their loads
 //   row(j, k, v)         where row j lies, for stages that are not dense
 //   Stage::end           rows of the stage from it on have no weight
-//   begun()              called once by every wave after its first loads
+//   kUnseen, unseen(jst) whether, and which, rows jst .. jst + 15 have no weight for any query (bits)
+//   begun()              called once by every wave after its first loads, before it asks for unseen rows
 //   appended(wave, lane) called once by every wave after its last stage
 // A run of linear or ring rows, the last one maybe new: rows [j0, j1) of a kv head's nvis visible ones.
 template <int D, bool SH>
 struct RunOf {
+    static constexpr bool kUnseen = false;
     uint16_t *k, *v;               // the cache rows of the kv head
     const uint16_t *k_new, *v_new; // the new token's rows (the last visible row), or null
     int G, j0, j1, nvis, first, cap, newrow;
@@ -57,6 +59,14 @@ struct RunOf {
             }
     }
 };
+
+// Rows of a stage that have a weight of 0 for every query: those from row `last` on repeat the run's last one
+// or hold anything, and unseen ones do, too.  They are zeros in LDS, row r at rows + off(r): 0 x inf is NaN.
+template <int D, class Layout, class Run>
+__device__ __forceinline__ void clear_unseen(const Run &x, unsigned char *rows, int jst, int last, int lane) {
+    for (unsigned todo = (x.unseen(jst) | 0xffffu << min(last, 16)) & 0xffffu; todo; todo &= todo - 1)
+        if (lane < D / 8) *reinterpret_cast<u32x4 *>(rows + Layout::off(__builtin_ctz(todo)) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+}
 
 // The log2-domain scores of a stage's raw products s (rows jst + 4 lg .. of query row 16 g + li), -inf for
 // rows without weight: by score(x, j) one at a time, or by score(s, jst, end, g) together.
@@ -163,8 +173,12 @@ __device__ __forceinline__ void attend_run(unsigned char *lds, Run &x, Query &&q
         }
         asm volatile("" ::: "memory");
         // Rows past the run repeat its last one, with a weight of 0; but 0 x inf is NaN.
-        for (int r = max(0, end - (x.j0 + 16 * st)); r < 16; ++r)
-            if (lane < D / 8) *reinterpret_cast<u32x4 *>(slot + (SH ? 0 : L::HB) + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (Run::kUnseen) {
+            clear_unseen<D, L>(x, slot + (SH ? 0 : L::HB), x.j0 + 16 * st, max(0, end - (x.j0 + 16 * st)), lane);
+        } else {
+            for (int r = max(0, end - (x.j0 + 16 * st)); r < 16; ++r)
+                if (lane < D / 8) *reinterpret_cast<u32x4 *>(slot + (SH ? 0 : L::HB) + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        }
         asm volatile("" ::: "memory");
         // Every K read of the stage, then the products, then every V read, which lands during the
         // softmax.  The scores of few rows go through several sums (a chain of D / 32 products waits for
@@ -369,8 +383,12 @@ __device__ __forceinline__ void attend_groups(unsigned char *lds, Run &x, Query 
             unsigned char *const kb = slot + wave * L::HB, *const vb = SH ? kb : kb + SUB * L::HB;
             const int jst = x.j0 + L::ROWS * i + 16 * wave;
             // Rows past the run repeat its last one or hold anything, with a weight of 0; but 0 x inf is NaN.
-            for (int r = max(0, end - jst); r < 16; ++r)
-                if (lane < D / 8) *reinterpret_cast<u32x4 *>(vb + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+            if constexpr (Run::kUnseen) {
+                clear_unseen<D, L>(x, vb, jst, max(0, end - jst), lane);
+            } else {
+                for (int r = max(0, end - jst); r < 16; ++r)
+                    if (lane < D / 8) *reinterpret_cast<u32x4 *>(vb + L::off(r) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+            }
             asm volatile("" ::: "memory");
             f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // (in four sums, as attend_run's, the step took as long)
 #pragma unroll

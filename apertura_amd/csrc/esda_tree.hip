@@ -37,12 +37,13 @@
 
 namespace {
 
-// A run's rows (esda_tree_rows.h) with what is to be done once its first loads are under way.
+// A run's rows (esda_tree_rows.h) with what is to be done once its first loads are under way, which says
+// which nodes are none.
 template <int D, bool SH, class Begin>
 struct BegunRows : TreeRows<D, SH> {
     Begin &begin;
     __device__ __forceinline__ BegunRows(const TreeParams &p, const TreeUnit &t, int ids, Begin &f) : TreeRows<D, SH>(p, t, ids), begin(f) {}
-    __device__ __forceinline__ void begun() const { begin(); }
+    __device__ __forceinline__ void begun() { this->none = begin(); }
 };
 
 // 16 NG query rows of a (sequence, kv head) over one piece of its keys, in a run (esda_stream.h): four waves
@@ -89,6 +90,7 @@ __global__ __launch_bounds__(256, 1) void tree_run_kernel(TreeParams p) {
             lowest[g] = p.window > 0 ? t.len + __popcll(sees[g]) - p.window : 0;
         }
         if (reports) tree_report(p, t, ok);
+        return __builtin_amdgcn_ballot_w64(path == 0ull);  // the nodes that are none
     };
     BegunRows<D, SH, decltype(begin)> x(p, t, ids, begin);
     x.G = min(rows - r0, 16 * NG);

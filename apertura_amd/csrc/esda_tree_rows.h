@@ -158,6 +158,7 @@ __device__ __forceinline__ int tree_ids(const TreeParams &p, int lane) {
 // The rows of one (sequence, kv head) as esda_stream.h's runs take them.
 template <int D, bool SH>
 struct TreeRows {
+    static constexpr bool kUnseen = true;
     uint16_t *k, *v;                // the kv head in page 0
     const uint16_t *k_new, *v_new;  // its rows of the nodes
     const int *table;               // of the sequence; null: page `page0` alone
@@ -166,6 +167,8 @@ struct TreeRows {
     int len, first, new_stride, N, P, shift, page0;
     int ids, of;                    // lane i: page 64 of + i of the table
     int page;                       // of the last stage
+    int low;                        // committed rows before it are seen by no node
+    unsigned long long none;        // bit i: node i is none, or past the last (said after the first loads)
 
     // ids0: the first 64 entries of the table (tree_ids), or anything
     __device__ __forceinline__ TreeRows(const TreeParams &p, const TreeUnit &w, int ids0) {
@@ -185,6 +188,8 @@ struct TreeRows {
         shift = p.shift;
         page0 = p.linear ? b : 0;
         G = page = 0;
+        low = p.window > 0 ? max(0, w.len + 1 - p.window) : 0;
+        none = 0ull;
         j0 = w.j0;
         j1 = w.j1;
         ids = p.linear ? page0 : (unsigned) ids0 < (unsigned) N ? ids0 : -1;  // (linear: every row in entry 0)
@@ -228,6 +233,13 @@ struct TreeRows {
         const long long at = r < len ? page * page_stride + (long long) (r & ((1 << shift) - 1)) * D : (long long) (r - len) * new_stride;
         kr = (r < len ? k : k_new) + at;
         if constexpr (!SH) vr = (r < len ? v : v_new) + at;
+    }
+    // Those of rows jst .. jst + 15 that no node sees, but for the rows of a page that is none.
+    __device__ __forceinline__ unsigned unseen(int jst) const {
+        const int row = first + jst, i = row - len;  // (i > -16: some row is a node's)
+        unsigned rows = row < low ? (1u << min(low - row, 16)) - 1u : 0u;
+        if (i > -16) rows |= i >= 64 ? 0xffffu : i >= 0 ? (unsigned) ~(~none >> i) : (unsigned) (none << -i);
+        return rows & 0xffffu;
     }
     __device__ __forceinline__ void begun() const {}
     __device__ __forceinline__ void appended(int, int) const {}

@@ -46,3 +46,48 @@ def test_queries_of_no_node(form, split_rows):
         out = tree_decode(c.step, **dict(c.args(), q=q))
         assert not bool(out[none].any() | out[none].isnan().any()), bad
         assert torch.equal(out, want), bad
+
+
+@pytest.mark.parametrize("split_rows", [0, 32])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window", [0, 64])
+def test_rows_that_nobody_sees(form, window, split_rows):
+    """Rows of nodes that are none, rows before every window and rows of a page that is none enter with a weight
+    of 0 and nothing of theirs: NaN and infinities there cost no bit of a row that does not see them."""
+    c = _case(*form, split_rows=split_rows, window=max(window, form[4]) if window else 0)
+    none = _none(c)
+    # (an entry of the table that is no page; page 0 is nobody's)
+    used = set(c.table[c.table >= 0].tolist())
+    if 0 in used:
+        free = next(i for i in range(c.pool.shape[1]) if i not in used)
+        c.pool[:, free] = c.pool[:, 0]
+        c.table[c.table == 0] = free
+    c.table[0, 42] = -1  # rows 672 .. 687 of 700
+    c.pool[:, 0] = 0.0
+    clean = c.full.nan_to_num(nan=0.5)
+    want = None
+    for bad in (1.0, float("nan"), float("inf"), -float("inf")):
+        c.full.copy_(clean)
+        if bad != 1.0:  # before the windows, behind the last rows, pages of nobody
+            c.pool[:, 0] = bad
+            for b, n in enumerate(c.lengths):
+                for r in range(max(0, n - c.window + 1) if c.window else 0):
+                    if int(c.table[b, r // 16]) >= 0:
+                        c.pool[:, int(c.table[b, r // 16]), :, r % 16] = bad
+        kn, vn = c.kn.clone(), None if c.shared else c.vn.clone()
+        for x in (kn, vn):
+            if x is not None:
+                x[none] = bad
+        out = tree_decode(c.step, **dict(c.args(), k_new=kn, v_new=vn))
+        assert bool(torch.isfinite(out).all())
+        want = out if want is None else want
+        assert torch.equal(out, want), bad
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_steps_repeat_themselves(form):
+    """Whichever workgroup ends first, the sums are taken in the same order."""
+    c = _case(*form)
+    want = tree_decode(c.step, **c.args())
+    for _ in range(5):
+        assert torch.equal(tree_decode(c.step, **c.args()), want)
