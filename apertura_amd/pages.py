@@ -55,7 +55,12 @@ class PagedCache:
     the K or the V of a layer; layers of another head shape are another pool).  table [slots, most pages]
     int32 (-1: no page), length [slots] int32, refs [pages] int32: the table entries that hold each page
     (left out: counted here).  The tensors are the caller's and are changed in place; every method is
-    launched on the current stream, or ``stream``, and reads nothing back (``left_out`` does)."""
+    launched on the current stream, or ``stream``, and reads nothing back (``left_out`` does).
+
+    A workspace that is not given is cleared here, and references are counted, on the current stream.  The
+    first call on another stream goes behind that, and the memory of workspace, table, lengths and
+    references is not handed out again before that stream is through.  (A call that is being captured does
+    neither: whoever replays the graph orders it and keeps the cache.)"""
 
     def __init__(self, pools: list[torch.Tensor], table: torch.Tensor, length: torch.Tensor,
                  refs: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
@@ -96,6 +101,11 @@ class PagedCache:
         self.workspace = workspace
         c.workspace, c.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         self._cache, self._ref, self._lib = c, ctypes.byref(c), L
+        self._streams = {torch._C._cuda_getCurrentRawStream(self._index)}  # ordered behind what was done here
+        self._made = None
+        if not torch.cuda.is_current_stream_capturing():
+            self._made = torch.cuda.Event()
+            self._made.record()
 
     @classmethod
     def empty(cls, pools: list[torch.Tensor], slots: int, max_pages: int) -> "PagedCache":
@@ -108,7 +118,20 @@ class PagedCache:
         """The launch's HIP stream; the cache has to be on the current device."""
         if torch._C._cuda_getDevice() != self._index:
             raise ValueError(f"the cache is on {self.device}; the current device is cuda:{torch.cuda.current_device()}")
-        return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else int(stream.cuda_stream)
+        raw = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else int(stream.cuda_stream)
+        if raw not in self._streams:
+            self._first_call_on(torch.cuda.current_stream() if stream is None else stream, raw)
+        return raw
+
+    def _first_call_on(self, stream, raw: int) -> None:
+        """(Once a stream: a block of memory remembers the streams it is used on.)"""
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self._made is not None:
+            stream.wait_event(self._made)
+        _used_on(stream, self.workspace, self.table, self.length, self.refs)
+        self._streams.add(raw)
 
     def reserve(self, slots: torch.Tensor, rows: torch.Tensor, stream=None) -> None:
         """Pages for rows up to rows[i] (exclusive) of slot slots[i]."""
@@ -163,6 +186,7 @@ class PagedCache:
 
     def left_out(self, stream=None) -> int:
         """What the calls left out since the last time (waits for the stream)."""
+        self._stream(stream)
         return pages_status(self.workspace, stream)
 
 
