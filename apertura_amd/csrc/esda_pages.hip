@@ -584,6 +584,7 @@ __global__ __launch_bounds__(256) void commit_kernel(CommitParams p) {
             else add(&p.head->left_out, 1);
         }
     }
+    if (p.num_pools == 0) return;  // (lengths alone)
     unsigned g = blockIdx.x % p.groups;
     int k = 0;
     for (; k + 1 < p.num_pools; ++k) {
