@@ -660,7 +660,8 @@ const char *check_pools(const esda_pages *c, int page_rows) {
     for (int i = 0; i < c->num_pools; ++i) {
         if (const char *why = check_pool(c->pools[i], c->num_pages, page_rows)) return why;
         for (int j = 0; j < i; ++j)
-            if (c->pools[i].data == c->pools[j].data) return "two pools are the same memory";
+            if (!apart(blocks_of(c->pools[i], c->num_pages, page_rows), blocks_of(c->pools[j], c->num_pages, page_rows)))
+                return "two pools overlap, or lie between one another with strides that do not show otherwise";
     }
     return nullptr;
 }

@@ -475,6 +475,12 @@ int esda_tree_decode(const esda_tree_desc *d, const esda_tree_args *a, void *str
         if (out.meets(x)) return refuse("out must not overlap q, the new rows or the pages");
     for (const Range &x : {k_new, v_new})
         if (x.meets(k_pages) || x.meets(v_pages)) return refuse("the new rows must not overlap the pages");
+    if (!shared) {
+        auto plane = [&](const void *at) {
+            return esda_page_view::Blocks{at, {1, d->num_pages, d->num_kv_heads}, {0, d->page_stride, d->head_stride}, (long long) d->page_rows * d->head_dim};
+        };
+        if (!esda_page_view::apart(plane(a->k_pages), plane(a->v_pages))) return refuse("k_pages and v_pages must not overlap");
+    }
     if (!a->workspace || a->workspace_bytes < pl.bytes || !aligned(a->workspace, 16))
         return fail(ESDA_ERR_WORKSPACE, "esda_tree_decode: workspace missing or smaller than esda_tree_workspace_size");
     rc = esda_detail::check_device();

@@ -60,7 +60,8 @@ typedef struct esda_pages {
     int32_t *length;      /* [slots], device memory                     */
     int32_t num_pools;    /* 0 .. ESDA_MAX_POOLS                        */
     int32_t pad;          /* 0                                          */
-    esda_pool pools[ESDA_MAX_POOLS]; /* one table for all of them       */
+    esda_pool pools[ESDA_MAX_POOLS]; /* one table for all of them; they must not overlap, but may lie
+                                        between one another where strides that both have show it */
     void *workspace;      /* esda_pages_workspace_size bytes, 16-byte aligned; zeroed once */
     size_t workspace_bytes;
 } esda_pages;

@@ -59,7 +59,7 @@ typedef struct esda_tree_args {
     const void *k_new;     /* [B, nodes, Hkv, D] bf16                                */
     const void *v_new;     /* the same; ignored when kv_shared                       */
     void *k_pages;         /* a plane of a pool, or a linear cache                   */
-    void *v_pages;         /* another; must equal k_pages when kv_shared             */
+    void *v_pages;         /* another, that does not overlap it; must equal k_pages when kv_shared */
     const int32_t *table;  /* [B][max_pages] int32, device memory (linear: NULL)     */
     const int32_t *length; /* [B] int32, device memory: committed rows               */
     const int32_t *parent; /* [B, nodes] int32, device memory, or NULL: a chain      */
