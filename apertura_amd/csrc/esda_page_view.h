@@ -89,6 +89,7 @@ inline bool meet(const void *a, long long na, const void *b, long long nb) {
 inline Blocks blocks_of(const esda_pool &p, int num_pages, int page_rows) {
     return {p.data, {p.planes, num_pages, p.num_kv_heads}, {p.plane_stride, p.page_stride, p.head_stride}, (long long) page_rows * p.head_dim};
 }
+inline Blocks bytes_at(const void *at, size_t bytes) { return {at, {1, 1, 1}, {0, 0, 0}, (long long) (bytes + 1) / 2}; }
 
 // What is wrong with a pool of pages of page_rows rows, or null.
 inline const char *check_pool(const esda_pool &p, int num_pages, int page_rows) {

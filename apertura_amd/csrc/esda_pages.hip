@@ -666,6 +666,16 @@ const char *check_pools(const esda_pages *c, int page_rows) {
     return nullptr;
 }
 
+// .. with a workspace of which a call uses `bytes`, beside checked pools.  (Lists: in ints.)
+const char *check_workspace(const esda_pages *c, size_t bytes) {
+    auto holds = [&](const void *list, long long ints) { return list && meet(c->workspace, (long long) bytes / 2, list, 2 * ints); };
+    if (holds(c->table, (c->slots - 1) * c->table_stride + c->max_pages) || holds(c->refs, c->num_pages) || holds(c->length, c->slots))
+        return "the workspace must not overlap table, refs or length";
+    for (int i = 0; i < c->num_pools; ++i)
+        if (!apart(bytes_at(c->workspace, bytes), blocks_of(c->pools[i], c->num_pages, c->page_rows))) return "the workspace must not overlap a pool";
+    return nullptr;
+}
+
 // Fills the kernels' parameters; an error code where the cache is none.
 int page_params(const char *call, const esda_pages *c, Params *p) {
     if (!c) return refuse(call, "null cache");
@@ -676,6 +686,7 @@ int page_params(const char *call, const esda_pages *c, Params *p) {
     const Layout l = layout(c->num_pages, c->slots, c->max_pages);
     if (!c->workspace || c->workspace_bytes < l.bytes || !aligned(c->workspace, 16))
         return fail(ESDA_ERR_WORKSPACE, std::string(call) + ": workspace missing or smaller than esda_pages_workspace_size");
+    if (const char *why = check_workspace(c, l.bytes)) return refuse(call, why);
     char *const ws = static_cast<char *>(c->workspace);
     *p = Params{};
     p->N = c->num_pages;
@@ -866,6 +877,7 @@ int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_
         return refuse(call, "accept and count must be 4-byte aligned device memory");
     if (!c->workspace || c->workspace_bytes < zeroed(c->slots) || !aligned(c->workspace, 16))
         return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: workspace missing or smaller than esda_pages_workspace_size");
+    if (const char *why = check_workspace(c, zeroed(c->slots))) return refuse(call, why);
     CommitParams p{};
     p.N = c->num_pages;
     p.linear = linear;

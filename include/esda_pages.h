@@ -62,7 +62,8 @@ typedef struct esda_pages {
     int32_t pad;          /* 0                                          */
     esda_pool pools[ESDA_MAX_POOLS]; /* one table for all of them; they must not overlap, but may lie
                                         between one another where strides that both have show it */
-    void *workspace;      /* esda_pages_workspace_size bytes, 16-byte aligned; zeroed once */
+    void *workspace;      /* esda_pages_workspace_size bytes, 16-byte aligned; zeroed once; must not
+                             overlap the pools, table, refs or length */
     size_t workspace_bytes;
 } esda_pages;
 

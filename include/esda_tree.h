@@ -65,7 +65,8 @@ typedef struct esda_tree_args {
     const int32_t *parent; /* [B, nodes] int32, device memory, or NULL: a chain      */
     void *out;             /* [B, nodes, Hq, D] bf16; must not overlap q, the new rows or the pages, nor
                               the new rows the pages                                 */
-    void *workspace;       /* esda_tree_workspace_size bytes, 16-byte aligned; first 256 zeroed once */
+    void *workspace;       /* esda_tree_workspace_size bytes, 16-byte aligned; first 256 zeroed once;
+                              must not overlap the other tensors                     */
     size_t workspace_bytes;
 } esda_tree_args;
 

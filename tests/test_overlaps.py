@@ -75,6 +75,19 @@ def test_pools_beside_and_between_one_another_are_taken(pools):
         assert code == 4 and "workspace" in why, name  # past the pools' checks
 
 
+@pytest.mark.parametrize("at", [0, 8 * 1000, 2 * ONE - 16, -16])
+def test_workspaces_over_a_pool_are_refused(at):
+    for name, (code, why) in _calls([_pool(4 * ONE), _pool(0)], workspace=AT + at, workspace_bytes=1 << 30).items():
+        assert code == 1 and "overlap a pool" in why, name
+
+
+@pytest.mark.parametrize("what", ["table", "refs", "length"])
+def test_workspaces_over_the_lists_are_refused(what):
+    for name, (code, why) in _calls([_pool(0)], workspace_bytes=1 << 30, **{what: AT - (1 << 24) + 16}).items():
+        if name != "commit" or what != "refs":
+            assert code == 1 and "overlap table, refs or length" in why, name
+
+
 def _tree(k, v, step, **kw):
     d = step.desc()
     ws = tree_workspace_bytes(step)
@@ -105,6 +118,16 @@ def test_planes_that_overlap_are_refused(k, v, kw):
 def test_planes_beside_and_between_one_another_are_taken(k, v, kw):
     code, why, *_ = _tree(k, v, _step(**kw))
     assert code == 4 and "workspace" in why
+
+
+@pytest.mark.parametrize("what", ["q", "k_new", "v_new", "k_pages", "v_pages", "table", "length", "parent", "out"])
+def test_step_workspaces_over_a_tensor_are_refused(what):
+    step, base = _step(split_rows=32), 1 << 28
+    ws = tree_workspace_bytes(step)
+    at = dict(q=0, k_new=1, v_new=2, k_pages=3, v_pages=4, table=5, length=6, out=7, parent=8)
+    for place in (16 - ws, 0):
+        code, why, *_ = _tree(0, base // 2, step, parent=AT + 8 * base, workspace=AT + at[what] * base + place, workspace_bytes=ws)
+        assert code == 1 and "the workspace must not overlap" in why, place
 
 
 def test_apart_against_the_elements(tmp_path):
