@@ -48,7 +48,67 @@ def _table_stride(table: torch.Tensor) -> int:
     return table.stride(0) if table.shape[0] > 1 else table.shape[1]
 
 
-class PagedCache:
+class CacheCalls:
+    """What PagedCache and tree.LinearCache have in common: the description that their calls take, the streams
+    they are launched on, and the accepted rows of a step of drafted tokens."""
+
+    def _set_up(self, c: Pages, workspace: torch.Tensor | None) -> None:
+        need = ctypes.c_size_t(0)
+        L = lib()
+        check(L.esda_pages_workspace_size(ctypes.byref(c), ctypes.byref(need)))
+        if workspace is None:
+            workspace = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
+        self.workspace = workspace
+        c.workspace, c.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        self._cache, self._ref, self._lib = c, ctypes.byref(c), L
+        self._streams = {torch._C._cuda_getCurrentRawStream(self._index)}  # ordered behind what was done here
+        self._made = None
+        if not torch.cuda.is_current_stream_capturing():
+            self._made = torch.cuda.Event()
+            self._made.record()
+
+    def _stream(self, stream) -> int:
+        """The launch's HIP stream; the cache has to be on the current device."""
+        if torch._C._cuda_getDevice() != self._index:
+            raise ValueError(f"the cache is on {self.device}; the current device is cuda:{torch.cuda.current_device()}")
+        raw = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else int(stream.cuda_stream)
+        if raw not in self._streams:
+            self._first_call_on(torch.cuda.current_stream() if stream is None else stream, raw)
+        return raw
+
+    def _first_call_on(self, stream, raw: int) -> None:
+        """(Once a stream: a block of memory remembers the streams it is used on.)"""
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self._made is not None:
+            stream.wait_event(self._made)
+        _used_on(stream, self.workspace, self.length, *self._lists)
+        self._streams.add(raw)
+
+    def commit(self, accept: torch.Tensor, count: torch.Tensor, stream=None) -> None:
+        """The rows of the accepted nodes accept[s][:count[s]] (rising) of a step of drafted tokens become the
+        slots' next rows (esda_tree_commit).  accept [slots, A], count [slots] int32."""
+        S, A = accept.shape if accept.dim() == 2 else (-1, 0)
+        if accept.dtype is not torch.int32 or S != self.slots or (A > 1 and accept.stride(1) != 1) or \
+                accept.get_device() != self._index:
+            raise ValueError(f"accept must be int32 [{self.slots}, most accepted] with dense rows on {self.device}")
+        if count.dtype is not torch.int32 or count.dim() != 1 or count.numel() != S or not count.is_contiguous() or \
+                count.get_device() != self._index:
+            raise ValueError(f"count must be contiguous int32 [{self.slots}] on {self.device}")
+        rc = self._lib.esda_tree_commit(self._ref, accept.data_ptr(), accept.stride(0) if S > 1 else A, A, count.data_ptr(),
+                                        self._stream(stream))
+        if rc:
+            check(rc)
+        _used_on(stream, accept, count)
+
+    def left_out(self, stream=None) -> int:
+        """What the calls left out since the last time (waits for the stream)."""
+        self._stream(stream)
+        return pages_status(self.workspace, stream)
+
+
+class PagedCache(CacheCalls):
     """K / V rows of many sequences in pages (esda_pages).
 
     pools: bf16 views [planes, pages, kv heads, page rows, head_dim] that one table serves (a plane is
@@ -93,19 +153,8 @@ class PagedCache:
                   refs=refs.data_ptr(), length=length.data_ptr(), num_pools=len(pools))
         for i, p in enumerate(pools):
             c.pools[i] = _pool(p)
-        need = ctypes.c_size_t(0)
-        L = lib()
-        check(L.esda_pages_workspace_size(ctypes.byref(c), ctypes.byref(need)))
-        if workspace is None:
-            workspace = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
-        self.workspace = workspace
-        c.workspace, c.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        self._cache, self._ref, self._lib = c, ctypes.byref(c), L
-        self._streams = {torch._C._cuda_getCurrentRawStream(self._index)}  # ordered behind what was done here
-        self._made = None
-        if not torch.cuda.is_current_stream_capturing():
-            self._made = torch.cuda.Event()
-            self._made.record()
+        self._lists = (table, refs)
+        self._set_up(c, workspace)
 
     @classmethod
     def empty(cls, pools: list[torch.Tensor], slots: int, max_pages: int) -> "PagedCache":
@@ -113,25 +162,6 @@ class PagedCache:
         device = pools[0].device
         return cls(pools, torch.full((slots, max_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(slots, dtype=torch.int32, device=device))
-
-    def _stream(self, stream) -> int:
-        """The launch's HIP stream; the cache has to be on the current device."""
-        if torch._C._cuda_getDevice() != self._index:
-            raise ValueError(f"the cache is on {self.device}; the current device is cuda:{torch.cuda.current_device()}")
-        raw = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else int(stream.cuda_stream)
-        if raw not in self._streams:
-            self._first_call_on(torch.cuda.current_stream() if stream is None else stream, raw)
-        return raw
-
-    def _first_call_on(self, stream, raw: int) -> None:
-        """(Once a stream: a block of memory remembers the streams it is used on.)"""
-        with torch.cuda.stream(stream):
-            if torch.cuda.is_current_stream_capturing():
-                return
-        if self._made is not None:
-            stream.wait_event(self._made)
-        _used_on(stream, self.workspace, self.table, self.length, self.refs)
-        self._streams.add(raw)
 
     def reserve(self, slots: torch.Tensor, rows: torch.Tensor, stream=None) -> None:
         """Pages for rows up to rows[i] (exclusive) of slot slots[i]."""
@@ -167,27 +197,6 @@ class PagedCache:
         rc = self._lib.esda_pages_compact(self._ref, self._stream(stream))
         if rc:
             check(rc)
-
-    def commit(self, accept: torch.Tensor, count: torch.Tensor, stream=None) -> None:
-        """The rows of the accepted nodes accept[s][:count[s]] (rising) of a step of drafted tokens become the
-        slots' next rows (esda_tree_commit).  accept [slots, A], count [slots] int32."""
-        S, A = accept.shape if accept.dim() == 2 else (-1, 0)
-        if accept.dtype is not torch.int32 or S != self.slots or (A > 1 and accept.stride(1) != 1) or \
-                accept.get_device() != self._index:
-            raise ValueError(f"accept must be int32 [{self.slots}, most accepted] with dense rows on {self.device}")
-        if count.dtype is not torch.int32 or count.dim() != 1 or count.numel() != S or not count.is_contiguous() or \
-                count.get_device() != self._index:
-            raise ValueError(f"count must be contiguous int32 [{self.slots}] on {self.device}")
-        rc = self._lib.esda_tree_commit(self._ref, accept.data_ptr(), accept.stride(0) if S > 1 else A, A, count.data_ptr(),
-                                        self._stream(stream))
-        if rc:
-            check(rc)
-        _used_on(stream, accept, count)
-
-    def left_out(self, stream=None) -> int:
-        """What the calls left out since the last time (waits for the stream)."""
-        self._stream(stream)
-        return pages_status(self.workspace, stream)
 
 
 def pages_status(workspace: torch.Tensor, stream=None) -> int:

@@ -11,9 +11,9 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import TreeArgs, TreeDesc, check, check_int32, lib
+from ._lib import MAX_POOLS, Pages, TreeArgs, TreeDesc, check, check_int32, lib
 from .decode import _dev_ptr, _on, _same_device, _stream_ptr, _used_on
-from .pages import _table_stride
+from .pages import CacheCalls, _check_pool, _pool, _table_stride
 
 
 @dataclass
@@ -146,7 +146,7 @@ def tree_decode(step: TreeStep, q: torch.Tensor, k_new: torch.Tensor, v_new: tor
                 parent: torch.Tensor | None = None, out: torch.Tensor | None = None,
                 workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Append the nodes' rows behind the committed ones and attend; out [B, nodes, Hq, D] bf16 (see
-    TreeCall).  The lengths stay; PagedCache.commit moves them on."""
+    TreeCall).  The lengths stay; PagedCache.commit, or LinearCache.commit, moves them on."""
     if workspace is None:
         with _on(stream):
             workspace = new_tree_workspace(step, q.device)
@@ -154,3 +154,31 @@ def tree_decode(step: TreeStep, q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     out = call(stream)
     _used_on(stream, out, call.workspace)
     return out
+
+
+class LinearCache(CacheCalls):
+    """Linear K / V rows of B sequences, for the accepted rows of steps of drafted tokens (TreeStep.for_cache):
+    commit and left_out are as PagedCache's.
+
+    caches: bf16 views [planes, B, Hkv, cap, D] (a plane is the K or the V of a layer; layers of another head
+    shape are another entry), length [B] int32: committed rows.  The tensors are the caller's and are changed
+    in place.  Streams, and a workspace that is not given, are as PagedCache's."""
+
+    def __init__(self, caches: list[torch.Tensor], length: torch.Tensor, workspace: torch.Tensor | None = None):
+        if not 1 <= len(caches) <= MAX_POOLS:
+            raise ValueError(f"1 .. {MAX_POOLS} caches of other head shapes")
+        if caches[0].dim() != 5:
+            raise ValueError("a cache is [planes, B, Hkv, cap, D]")
+        B, cap = caches[0].shape[1], caches[0].shape[3]
+        for i, x in enumerate(caches):
+            _check_pool(f"cache {i}", x, B, cap)
+        if length.dtype != torch.int32 or length.shape != (B,) or not length.is_contiguous():
+            raise ValueError("length must be contiguous int32 [B]")
+        check_int32(num_pages=B, page_rows=cap)
+        _same_device({**{f"cache {i}": x for i, x in enumerate(caches)}, "length": length, "workspace": workspace})
+        self.caches, self.length, self.slots, self.cap = list(caches), length, B, cap
+        self.device, self._index, self._lists = length.device, length.device.index, ()
+        c = Pages(num_pages=B, page_rows=cap, slots=B, max_pages=1, length=length.data_ptr(), num_pools=len(caches))
+        for i, x in enumerate(caches):
+            c.pools[i] = _pool(x)
+        self._set_up(c, workspace)
