@@ -846,7 +846,10 @@ int esda_pages_status(void *workspace, int32_t *left_out, void *stream) {
     const char *call = "esda_pages_status";
     if (!workspace || !aligned(workspace, 16) || !left_out) return refuse(call, "null or unaligned argument");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipError_t e = hipMemcpyAsync(left_out, workspace, sizeof(int32_t), hipMemcpyDeviceToHost, st);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(st, &capture);
+    if (e == hipSuccess && capture != hipStreamCaptureStatusNone) return refuse(call, "waits for the stream, and cannot be captured");
+    if (e == hipSuccess) e = hipMemcpyAsync(left_out, workspace, sizeof(int32_t), hipMemcpyDeviceToHost, st);
     if (e == hipSuccess) e = hipMemsetAsync(workspace, 0, sizeof(int32_t), st);
     if (e == hipSuccess) e = hipStreamSynchronize(st);
     return e == hipSuccess ? ESDA_OK : fail(ESDA_ERR_HIP, std::string(call) + ": " + hipGetErrorString(e));

@@ -94,7 +94,7 @@ int esda_pages_fork(const esda_pages *cache, const int32_t *src, const int32_t *
 int esda_pages_compact(const esda_pages *cache, void *stream);
 
 /* Reads (synchronously) and clears the status word of a workspace: what the calls on it left out
- * since the last time. */
+ * since the last time.  Not for a stream that is being captured. */
 int esda_pages_status(void *workspace, int32_t *left_out, void *stream);
 
 /* ------------------------------------------------------------ rows in and out

@@ -3,6 +3,7 @@ its memory kept until that stream is through."""
 import pytest
 import torch
 
+from apertura_amd._lib import EsdaError
 from apertura_amd.pages import PagedCache
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +91,24 @@ def test_a_capture_on_a_stream_of_its_own():
         cache.reserve(_ints([1]), _ints([1]))
         cache.free(_ints([1]))
         assert cache.left_out() == 0
+
+
+def test_left_out_is_not_captured():
+    """The count is read at once: a capture refuses it, and goes on."""
+    pool = torch.randn((1, 8, 1, 16, 128), device=DEV).to(BF)
+    cache = PagedCache.empty([pool], 3, 2)
+    slots, rows = _ints([0, 9]), _ints([20, 20])
+    cache.reserve(slots, rows)
+    assert cache.left_out() == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.free(slots)
+        with pytest.raises(EsdaError) as refused:
+            cache.left_out()
+        cache.reserve(slots, rows)
+    assert refused.value.code == 1 and "captured" in str(refused.value)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert cache.table.tolist() == [[0, 1], [-1, -1], [-1, -1]]
+        assert cache.left_out() == 2 and cache.left_out() == 0
