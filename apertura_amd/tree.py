@@ -127,7 +127,7 @@ class TreeCall:
         bf = torch.bfloat16
         self._keep = (q, k_new, v_new, k_pages, v_pages, length, table, parent)
         self.step, self.out, self.workspace = step, out, workspace
-        self._desc = d
+        self._desc, self._index = d, q.device.index
         self._args = TreeArgs(_dev_ptr(q, bf), _dev_ptr(k_new, bf), None if step.kv_shared else _dev_ptr(v_new, bf),
                               _dev_ptr(k_pages, bf), _dev_ptr(vp, bf), _dev_ptr(table), _dev_ptr(length), _dev_ptr(parent),
                               _dev_ptr(out, bf), _dev_ptr(workspace), workspace.numel() * workspace.element_size())
@@ -135,6 +135,8 @@ class TreeCall:
         self._pd, self._pa = ctypes.byref(self._desc), ctypes.byref(self._args)
 
     def __call__(self, stream=None) -> torch.Tensor:
+        if torch._C._cuda_getDevice() != self._index:
+            raise ValueError(f"the step's tensors are on cuda:{self._index}; the current device is another")
         rc = self._fn(self._pd, self._pa, _stream_ptr(stream))
         if rc:
             check(rc)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from _attn64 import check
-from apertura_amd.tree import tree_decode
+from apertura_amd.tree import TreeCall, tree_decode
 from test_tree_gpu import Case, random_parents
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +91,17 @@ def test_steps_repeat_themselves(form):
     want = tree_decode(c.step, **c.args())
     for _ in range(5):
         assert torch.equal(tree_decode(c.step, **c.args()), want)
+
+
+def test_calls_with_another_current_device_are_refused(monkeypatch):
+    """A launch goes to the current device's stream, where the tensors are not."""
+    c = _case(*FORMS[0])
+    call = TreeCall(c.step, **c.args())
+    want = call().clone()
+    call.out.fill_(7.0)
+    with monkeypatch.context() as m:
+        m.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+        with pytest.raises(ValueError):
+            call()
+    assert bool((call.out == 7.0).all())
+    assert torch.equal(call(), want)
