@@ -878,9 +878,6 @@ int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_
         return refuse(call, "max_accept must be 1 .. 64, accept_stride at least that");
     if (!accept || !count || !aligned(accept, 4) || !aligned(count, 4))
         return refuse(call, "accept and count must be 4-byte aligned device memory");
-    if (!c->workspace || c->workspace_bytes < zeroed(c->slots) || !aligned(c->workspace, 16))
-        return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: workspace missing or smaller than esda_pages_workspace_size");
-    if (const char *why = check_workspace(c, zeroed(c->slots))) return refuse(call, why);
     CommitParams p{};
     p.N = c->num_pages;
     p.linear = linear;
@@ -905,6 +902,9 @@ int esda_tree_commit(const esda_pages *c, const int32_t *accept, int64_t accept_
     groups = std::max(1LL, groups);
     if (groups * c->slots > 1LL << 23) return refuse(call, "too many slots, planes and heads");
     p.groups = (unsigned) groups;
+    if (!c->workspace || c->workspace_bytes < zeroed(c->slots) || !aligned(c->workspace, 16))
+        return fail(ESDA_ERR_WORKSPACE, "esda_tree_commit: workspace missing or smaller than esda_pages_workspace_size");
+    if (const char *why = check_workspace(c, zeroed(c->slots))) return refuse(call, why);
     const int rc = esda_detail::check_device();
     if (rc) return rc;
     hipLaunchKernelGGL(commit_kernel, dim3((unsigned) (groups * c->slots)), dim3(256), 0, static_cast<hipStream_t>(stream), p);

@@ -36,6 +36,7 @@
 extern "C" {
 #endif
 
+/* batch * nodes * num_q_heads * head_dim must be below 2^30. */
 typedef struct esda_tree_desc {
     int32_t batch;        /* 1 .. 256                                               */
     int32_t nodes;        /* 1 .. 64                                                */
@@ -50,7 +51,8 @@ typedef struct esda_tree_desc {
     int64_t table_stride; /* ints; >= max_pages                                     */
     int64_t page_stride;  /* elements: (page, kvh, row, d) at page*page_stride + kvh*head_stride + row*head_dim + d */
     int64_t head_stride;  /* both multiples of 8; blocks of page_rows * head_dim elements must not overlap */
-    int32_t split_rows;   /* rows per split (0: from the lengths, on the device; multiple of 32) */
+    int32_t split_rows;   /* rows per split (0: from the lengths, on the device; multiple of 32, of
+                             which a sequence's room holds at most 4096)            */
     float scale;          /* softmax scale, positive                                */
 } esda_tree_desc;
 
@@ -77,7 +79,9 @@ int esda_tree_decode(const esda_tree_desc *desc, const esda_tree_args *args, voi
  * becomes row length[s] + accept[s][i] for i < count[s], and length[s] grows by count[s].
  * accept: [slots][max_accept], accept_stride ints apart, and count: [slots], device memory; a slot's
  * entries rise and lie in 0 .. 63.  A slot with another list, a count outside 0 .. max_accept or rows
- * that lie in no page is left as it was and counted.  max_accept: 1 .. 64.
+ * that lie in no page is left as it was and counted.  max_accept: 1 .. 64.  Workgroups of 4096 elements
+ * of a row of every plane and head: slots * (planes * num_kv_heads * head_dim / 4096, up, over the pools)
+ * at most 2^23.
  * cache->table NULL: linear caches, slot s in page s (num_pages == slots, max_pages 1, page_rows any
  * 1 .. 2^30); refs is not used.  The workspace is esda_pages.h's, zeroed once. */
 int esda_tree_commit(const esda_pages *cache, const int32_t *accept, int64_t accept_stride, int32_t max_accept,
