@@ -6,12 +6,14 @@
 // What to do is decided on the device, from the table and the references, so that a serving loop never
 // waits for it on the host: small kernels of a workgroup per list entry, or of one workgroup where
 // entries compete for free pages, write a list of moves, and a grid of waves carries it out.  The copies
-// are bound by memory (a copy of 1 GiB moves 5.1 TB/s here): 4,095 rows of 16 heads x 256, K and V, into
-// 32-row pages, 134 MB in 22 us; 32,767 rows of 4 x 512 out of 16-row pages, 268 MB in 56; 473 MB of
-// moving pages in 84.  Calls of few bytes are bound by their launches, 2.4 .. 7 us each: reserve_kernel 2.4
-// for 4 entries and 3.5 for 32, which wait for their slots' lengths, tables and free pages one after the
-// other, the commit of 32 sequences' paths on 48 planes (20 MB) 8.6.  Of such kernels the code's own fetches
-// are a part: loads that are under way together and little code count, unrolled loops do not pay.
+// are bound by memory (a copy of 1 GiB moves 5.1 TB/s here).  Calls among others, on inputs that change: 4,095
+// rows of 16 heads x 256, K and V, into 32-row pages, 134 MB in 22 us (6.1 TB/s: the rows come partly out of
+// the Infinity Cache); 32,767 rows of 4 x 512 out of 16-row pages, 268 MB in 56; 473 MB of moving pages in 94 ..
+// 99.  Calls of few bytes are bound by their launches; kernels by themselves, on the same inputs each time,
+// take 2.4 .. 8 us: reserve_kernel 2.5 for 4 entries and 3.6 for 32, which wait for their slots' lengths, tables
+// and free pages one after the other, the commit of 32 sequences' paths on 48 planes (20 MB) 8.0.  Of such
+// kernels the code's own fetches are a part: loads that are under way together and little code count, unrolled
+// loops do not pay.
 
 #include <hip/hip_runtime.h>
 
@@ -91,11 +93,11 @@ __device__ __forceinline__ bool named_before(const int *list, int i, int t) {
 }
 
 // `chunks` 16-byte pieces by the lanes of a wave, eight loads in flight each.  LOADED / STORED: past the
-// caches.  Pages are written so: nothing reads them soon, and they push out what is (a prompt's 4095 rows of
-// 16 heads x 256, K and V, 134 MB, 32.0 us with plain stores, 23.4); rows that are read out are used next,
-// and written plainly (32,767 of 4 x 512, 268 MB, 45.6 us, 54.1 past the caches).  Pages that move are not
-// read again (16 slots' pool, 473 MB: 104.8 us plain, 101.8 with such stores, 98.3 with such loads too);
-// those that are forked are, by the next child.
+// caches.  Pages are written so: nothing reads them soon, and they push out what is (calls as above: a prompt's
+// 134 MB 22 us, with plain stores 30.5).  Rows that are read out are used next, and written plainly (268 MB: 56
+// us, and 53 past the caches; 65 and 73 where the GPU is waited for after each call).  Pages that move are not
+// read again (473 MB: 94 .. 99 us, 99 .. 100 with such stores alone, 104 .. 105 with neither); those that are
+// forked are, by the next child.
 template <bool LOADED, bool STORED>
 __device__ __forceinline__ void wave_copy(uint16_t *dst, const uint16_t *src, int chunks, int lane) {
     constexpr int U = 8;

@@ -5,17 +5,18 @@
 // over the committed rows within node i's window and the nodes on its path.  A path is 64 bits, bit j for
 // node j; a wave works them out with a node to a lane, doubling the paths' length in each of six rounds,
 // and a node's depth is the number of its bits.  Only stages that hold nodes, the window's edge or a page
-// that is none look at them; the others are plain attention.
+// that is none look at them; the others are plain attention.  Rows that no node sees (of nodes that are none,
+// before the window, of such a page) may hold anything: they are zeros in LDS.
 //
 // A launch of pieces (one kv head, one sequence, a share of its keys) and one that merges them.  Few query
 // rows a kv head take runs (tree_run_kernel), bound by memory: 32 sequences of 1,024 .. 8,192 rows of 128
-// dims, K and V of 8 heads in 16-row pages, 608 MB read in 101 us (6.0 TB/s; a read of a large buffer
+// dims, K and V of 8 heads in 16-row pages, 608 MB read in 102 us (6.0 TB/s; a read of a large buffer
 // reaches 7.2), 8 of 5 nodes each over 16 heads of 256 dims, 831 MB, 132 (6.3).  More take query tiles
 // (prefill_kernel with TreeParams), bound by the matrix instructions and the softmax in turn: 2 x 63 nodes
-// over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 147 us with the merge
-// (0.89 PFLOP/s; esda_prefill's tiles over the same rows, linear, take 1 .. 5% less), the matrix pipes busy
-// for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.0 and 3.4 us each
-// by itself, 10.8 together: the length and the table's first entries, the rows, the waves' sum.
+// over 16,384 and 15,347 rows of 4 heads of 512 dims, K = V, 131 GFLOP in 146 us with the merge, called over
+// and over (0.90 PFLOP/s; esda_prefill's tiles over the same rows, linear, take 1 .. 5% less), the matrix pipes
+// busy for 0.46 of the tiles' cycles.  One token over 1,000 rows is two dependent launches, 8.2 and 3.5 us
+// each by itself, 11.0 together: the length and the table's first entries, the rows, the waves' sum.
 
 #include <hip/hip_runtime.h>
 

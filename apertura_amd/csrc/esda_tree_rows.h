@@ -309,6 +309,7 @@ __device__ __forceinline__ void tree_row_again(const TreeRows<D, SH> &x, const u
 #pragma unroll
         for (int i = 32; i >= 1; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
         const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        // (rounded to bf16, as the weights of the products are)
         const float w = seen ? (float) (__bf16) __builtin_amdgcn_exp2f(s - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
         float sum = w;
 #pragma unroll

@@ -22,7 +22,9 @@
  * counted (esda_pages_status); one of length 0 whose nodes are all none is a batch's padding: it needs no
  * pages and gives 0.  Pages of the nodes' rows belong to one sequence.  Calls that overlap need
  * workspaces of their own.  A value of k or v that is not finite reaches only the queries that see
- * its row. */
+ * its row, and what q holds where there is no node none.
+ * Scores, maxima and sums are fp32; a weight enters the sum of the weights and that of the values rounded to
+ * bf16. */
 #ifndef APERTURA_ESDA_TREE_H
 #define APERTURA_ESDA_TREE_H
 
