@@ -404,7 +404,7 @@ int esda_tree_decode(const esda_tree_desc *d, const esda_tree_args *a, void *str
     if (!a->workspace || a->workspace_bytes < pl.bytes || !aligned(a->workspace, 16))
         return fail(ESDA_ERR_WORKSPACE, "esda_tree_decode: workspace missing or smaller than esda_tree_workspace_size");
     const Range workspace{a->workspace, (long long) pl.bytes / 2}, lists[] = {
-        {a->length, 2LL * d->batch}, {a->parent, 2LL * d->batch * d->nodes}, {a->table, 2 * ((d->batch - 1) * d->table_stride + d->max_pages)}};
+        {a->length, 2LL * d->batch}, {a->parent, 2LL * d->batch * d->nodes}, {a->table, a->table ? 2 * ((d->batch - 1) * d->table_stride + d->max_pages) : 0}};
     for (const Range &x : {Range{a->q, out.n}, out, k_new, v_new, k_pages, v_pages, lists[0], lists[1], lists[2]})
         if (x.at && workspace.meets(x)) return refuse("the workspace must not overlap the tensors");
     rc = esda_detail::check_device();
