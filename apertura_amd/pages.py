@@ -200,7 +200,8 @@ class PagedCache(CacheCalls):
 
 
 def pages_status(workspace: torch.Tensor, stream=None) -> int:
-    """Reads (synchronously) and clears the status word of a workspace of esda_pages.h or esda_tree.h."""
+    """Reads (synchronously, so not in a capture) and clears the status word of a workspace of esda_pages.h or
+    esda_tree.h."""
     n = ctypes.c_int32(0)
     _same_device({"workspace": workspace})
     check(lib().esda_pages_status(workspace.data_ptr(), ctypes.byref(n), _stream_ptr(stream)))

@@ -87,7 +87,7 @@ class TreeCall:
     q [B, nodes, Hq, D], k_new and v_new [B, nodes, Hkv, D]; k_pages, v_pages: planes [pages, Hkv, page
     rows, D] (linear: [B, Hkv, cap, D]); length [B] int32: committed rows; parent [B, nodes] int32 (None: a
     chain): -1 on the committed rows, j < i on node j, anything else no node.  A workspace that is not
-    given is cleared here, on the current stream."""
+    given is cleared here, on the current stream: calls on another one go behind that."""
 
     def __init__(self, step: TreeStep, q, k_new, v_new, k_pages, v_pages, length, table=None, parent=None, out=None,
                  workspace=None):
